@@ -840,6 +840,74 @@ int kt_hip_dec_embed_argmax(int dev, const uint64_t* part_dev, int64_t nparts, c
                             int32_t* r_dev, int32_t* token_dev, int32_t* step_dev, void* stream);
 
 /* ---------------------------------------------------------------------------------------------------------------
+ * The int8 decoder's attention over paged KV caches, for many sequences at once (no counterpart in the reference, whose
+ * decoder serves one sequence from contiguous caches; with 8 bits the integers are those of kt_hip_dec_rope_kv and
+ * kt_hip_dec_attention above).
+ *
+ * A batch is `seqs` sequences with `tokens` new rows among them: sequence b's rows are row_start[b] .. row_start[b+1] - 1
+ * (row_start: seqs + 1 non-decreasing int32; a sequence may have none), and kv_len[b] its positions with the new rows
+ * counted, so its rows are at the positions from kv_len[b] - rows on. Position j lies in slot j % page of page
+ * table[b * max_pages + j / page]. All three arrays are device memory, read by the kernels alone: a captured call replays
+ * on what they then hold. Rows that no sequence has are left as they were. A table entry outside [0, pages) names no
+ * page: what is written there is dropped, and attention leaves its positions out (a window's pages can be given back).
+ * Values outside these rules (a row_start that decreases, a kv_len below the sequence's rows) reach no memory outside the
+ * given arrays; a row at a position below 0 or not below max_pages * page is zeros in every output.
+ *
+ * A pool (K or V) holds pages x nkv parts of kt_hip_dec_page_bytes(page, hd, bits) bytes, 16-byte aligned: page in
+ * {16, 32, 64, 128, 256} slots, hd 64 or 128, bits 8 or 4. Values stand in chunks of 16: a K chunk is 16 neighbouring
+ * dimensions of one slot, [slot][hd / 16]; a V chunk one dimension's 16 neighbouring slots, [slot / 16][hd]. With 8 bits a
+ * chunk is its 16 int8 values. With 4 bits it is 8 bytes, byte 4 h + r holding code 8 h + r in its low half and code
+ * 8 h + 4 + r in its high half, and a part ends with its slots' multipliers (page bytes): a row x of hd values is held as
+ * m = ceil(8 max |x| / 7) and the codes c = clamp(round_half_away(8 x / m), +-7) (0 when m is 0), and stands for c m / 8.
+ *
+ * max_pages * page <= KT_PAGED_MAX_POS; tokens * nh, and 2 * seqs * nh below 2^31. Pointers and strides (in elements) of
+ * int8 rows are multiples of 16.
+ * ------------------------------------------------------------------------------------------------------------- */
+#define KT_PAGED_MAX_POS 524288
+/* Bytes of one kv head's part of a page in one pool; 0 for a page, hd or bits outside the above. */
+size_t kt_hip_dec_page_bytes(int64_t page, int64_t hd, int bits);
+/* The new rows' RoPE (kt_hip_dec_rope_kv's rule and tables, cos / sin of max_pos positions; 8-byte aligned): row t of
+ * qkv_dev (stride qkv_stride; q heads, k heads, v heads; read only) gives its rotated q heads at q_dev + t * q_stride and
+ * its rotated k and its v in its position's slot. A row whose position is not below max_pos is as one outside the table:
+ * zeros in q_dev, nothing written. Two rows of a call may not share a slot's block of 16 (sequences that share pages
+ * share whole pages that no row of the call is in). */
+int kt_hip_dec_rope_kv_paged(int dev, const int8_t* qkv_dev, int64_t tokens, int64_t qkv_stride,
+                             const int32_t* row_start_dev, const int32_t* kv_len_dev, const int32_t* table_dev,
+                             int64_t seqs, int64_t max_pages, int64_t nh, int64_t nkv, int64_t hd,
+                             const int16_t* cos_dev, const int16_t* sin_dev, int64_t max_pos, int8_t* q_dev,
+                             int64_t q_stride, void* kpool_dev, void* vpool_dev, int64_t pages, int64_t page, int bits,
+                             void* stream);
+/* The pages back as contiguous rows: position j < min(kv_len[b], max_pos, max_pages * page) of every sequence to
+ * k_dev / v_dev [seqs][max_pos][nkv][hd] int8 (with seqs = 1 the caches of kt_hip_dec_attention); positions past those
+ * are left as they were. With 4 bits the values are clamp(round_half_away(c m / 8), +-127); a position without a page is
+ * zeros. */
+int kt_hip_dec_kv_read_paged(int dev, const void* kpool_dev, const void* vpool_dev, int64_t pages, int64_t page,
+                             int bits, const int32_t* kv_len_dev, const int32_t* table_dev, int64_t seqs,
+                             int64_t max_pages, int64_t nkv, int64_t hd, int8_t* k_dev, int8_t* v_dev, int64_t max_pos,
+                             void* stream);
+/* Causal GQA attention of the new rows (chunks and single tokens alike) over their sequences' pages, rows of q_dev as
+ * kt_hip_dec_rope_kv_paged leaves them, after the call that wrote the rows' own k and v. A row at p sees the positions
+ * j <= p that have a page and, with window >= 1, are within it (j > p - window) or among the first `sinks`; window = 0
+ * sees all. s_j = q . k_j (4 bits: (m_j (q . c_j) + 4) >> 3), e_j = exp_tab[(max s - s_j + 64) >> 7] with entries clamped
+ * to [0, 2^15] and 0 past the 1024th, o = clamp(round_half_away(sum e_j v_j / sum e_j)), 0 where the sum of e is 0.
+ * ws_dev: kt_hip_dec_attention_paged_workspace bytes of scratch, 16-byte aligned, needing no contents; calls that may
+ * overlap need one each. */
+size_t kt_hip_dec_attention_paged_workspace(int64_t tokens, int64_t seqs, int64_t max_pages, int64_t page, int64_t nh,
+                                            int64_t nkv, int64_t hd);
+int kt_hip_dec_attention_paged(int dev, const int8_t* q_dev, int64_t tokens, int64_t q_stride,
+                               const int32_t* row_start_dev, const int32_t* kv_len_dev, const int32_t* table_dev,
+                               int64_t seqs, int64_t max_pages, int64_t nh, int64_t nkv, int64_t hd,
+                               const int32_t* exp_tab_dev, int64_t window, int64_t sinks, const void* kpool_dev,
+                               const void* vpool_dev, int64_t pages, int64_t page, int bits, int8_t* o_dev,
+                               int64_t o_stride, void* ws_dev, size_t ws_bytes, void* stream);
+/* The greedy choice of a batch: token_dev[r] = the first index of the maximum of the n int32 logits at logits_dev +
+ * r * stride (argmax_codes, generate.rs:48-56, per row). ws_dev: kt_hip_dec_argmax_rows_workspace bytes, 8-byte aligned,
+ * needing no contents. */
+size_t kt_hip_dec_argmax_rows_workspace(int64_t rows, int64_t n);
+int kt_hip_dec_argmax_rows(int dev, const int32_t* logits_dev, int64_t rows, int64_t n, int64_t stride,
+                           int32_t* token_dev, void* ws_dev, size_t ws_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------------------------------
  * Synthetic workload generators (host only, no GPU): the benchmark configs' integer samplers on the reference LCG
  * (apps/kt-demo/src/main.rs:19-22), multithreaded over the host cores. No counterpart in the reference.
  * ------------------------------------------------------------------------------------------------------------- */

@@ -55,6 +55,7 @@ class Scale(C.Structure):
 
 _P = C.c_void_p
 _SZ = C.c_size_t
+_L64 = C.c_int64
 
 
 def _declare(L: C.CDLL) -> None:
@@ -126,6 +127,10 @@ def _declare(L: C.CDLL) -> None:
         "kt_dec_rmsnorm_rows": (None, [_P, _SZ, _SZ, _P]),
         "kt_dec_rope_row": (None, [_P, _SZ, _SZ, _SZ, _P, _P]),
         "kt_dec_attend": (None, [_P, _P, _P, _SZ, _SZ, _SZ, _SZ, _P, _P, _P]),
+        "kt_pg_rope_append": (None, [_P, _P, _L64, _L64, _P, _P, _L64, _P, _L64]),
+        "kt_pg_read": (None, [_P, _P, _P, _L64]),
+        "kt_pg_attend": (None, [_P, _P, _L64, _L64, _P, _L64, _L64, _P, _L64]),
+        "kt_pg_argmax": (None, [_P, _L64, _L64, _L64, _P]),
         "kt_conv2d_i8w16": (None, [_P, _SZ, _SZ, _SZ, _P, _SZ, _SZ, _SZ, _SZ, _SZ, _P, _P, _P, _P, _P, _SZ]),
         "kt_mlp_gelu": (C.c_int, [_P, _SZ, _SZ, _SZ, _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ]),
         "kt_rd_synthetic": (_P, [C.c_uint64, _SZ, _SZ, _SZ, _SZ, _SZ, _SZ, _SZ, C.c_double, C.c_double, _SZ]),
@@ -752,6 +757,58 @@ def dec_generate(shape: dict, arrays: dict, prompt, max_new: int, batched: bool 
     if r:
         raise ValueError("dec_generate: shape beyond the oracle's bounds")
     return toks, logits
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# The W12 decoder's paged KV caches (kt_oracle_paged.c)
+
+
+class Paged(C.Structure):
+    """kt_pg of kt_oracle_paged.c."""
+
+    _fields_ = [(n, C.c_int64) for n in ("tokens", "seqs", "max_pages", "pages", "page", "nkv", "hd", "bits")] + [
+        (n, C.c_void_p) for n in ("row_start", "kv_len", "table", "k", "v")]
+
+
+def paged(tokens: int, row_start, kv_len, table, k, v, page: int, nkv: int, hd: int, bits: int):
+    """A Paged over numpy arrays: table seqs x max_pages int32, k / v uint8 pools of pages (written in place)."""
+    row_start, kv_len, table = _c(row_start, np.int32), _c(kv_len, np.int32), _c(table, np.int32)
+    per = page * hd if bits == 8 else page * (hd // 2 + 1)
+    assert k.dtype == v.dtype == np.uint8 and k.flags.c_contiguous and v.flags.c_contiguous
+    assert k.size == v.size and k.size % (nkv * per) == 0 and row_start.size == kv_len.size + 1
+    P = Paged(tokens, kv_len.size, table.shape[1], k.size // (nkv * per), page, nkv, hd, bits, row_start.ctypes.data,
+              kv_len.ctypes.data, table.ctypes.data, k.ctypes.data, v.ctypes.data)
+    P.keep = (row_start, kv_len, table, k, v)
+    return P
+
+
+def paged_append(P: Paged, qkv, nh: int, cos_t, sin_t, q) -> None:
+    """RoPE of the rows' q heads into q (tokens x at least nh hd, in place) and k / v into P's pools."""
+    qkv, cos_t, sin_t = _c(qkv, np.int8), _c(cos_t, np.int16), _c(sin_t, np.int16)
+    assert q.dtype == np.int8 and q.flags.c_contiguous
+    lib().kt_pg_rope_append(C.byref(P), _ptr(qkv), qkv.shape[1], nh, _ptr(cos_t), _ptr(sin_t), cos_t.shape[0], _ptr(q),
+                            q.shape[1])
+
+
+def paged_read(P: Paged, k, v) -> None:
+    """Every sequence's positions into k / v (seqs x max_pos x nkv x hd int8, in place)."""
+    assert k.dtype == v.dtype == np.int8 and k.flags.c_contiguous and v.flags.c_contiguous
+    lib().kt_pg_read(C.byref(P), _ptr(k), _ptr(v), k.shape[1])
+
+
+def paged_attend(P: Paged, q, nh: int, exp_tab, o, window: int = 0, sinks: int = 0) -> None:
+    """The rows' attention into o (tokens x at least nh hd int8, in place)."""
+    q, exp_tab = _c(q, np.int8), _c(exp_tab, np.int32)
+    assert o.dtype == np.int8 and o.flags.c_contiguous
+    lib().kt_pg_attend(C.byref(P), _ptr(q), q.shape[1], nh, _ptr(exp_tab), window, sinks, _ptr(o), o.shape[1])
+
+
+def argmax_rows(logits, n: int) -> np.ndarray:
+    """The first maximum of the first n values of each row."""
+    logits = _c(logits, np.int32)
+    t = np.empty(logits.shape[0], dtype=np.int32)
+    lib().kt_pg_argmax(_ptr(logits), logits.shape[0], n, logits.shape[1], _ptr(t))
+    return t
 
 
 # ---------------------------------------------------------------------------------------------------------------

@@ -1,0 +1,153 @@
+"""The paged decoder (tritify_amd.paged.PagedDecoder) against DecoderModel, which runs one sequence from contiguous caches and
+is itself checked against the oracle (tests/test_gpu_decoder.py): the same tokens and logits for every sequence, whatever it
+shares its passes with. With 4-bit pages, where no contiguous decoder exists, a batch against its sequences alone."""
+import sys
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+CFG = dict(d=128, ffn=256, nh=4, nkv=2, hd=64, layers=2, vocab=1000)
+
+
+def say(*a):
+    print(*a, file=sys.stderr, flush=True)
+
+
+@pytest.fixture(scope="module")
+def model(torch_dev):
+    from tritify_amd import workloads as W
+    from tritify_amd.decoder import DecoderModel
+
+    m = DecoderModel(CFG, 400, 256)
+    for l in range(CFG["layers"]):
+        m.set_layer(l, *W.decoder_layer_codes(l, CFG, 500))
+    m.set_embedding(*W.decoder_embedding_codes(CFG, 500))
+    m.set_tables(*W.rope_tables(400, CFG["hd"]), W.exp_table(), W.silu_table())
+    return m
+
+
+def prompts(lens):
+    from tritify_amd import workloads as W
+
+    return [W.decoder_prompt(600 + i, n, CFG["vocab"]) for i, n in enumerate(lens)]
+
+
+@pytest.mark.parametrize("page,chunk", [(16, 256), (64, 50), (16, 7)])
+def test_generate_equals_the_contiguous_decoder(model, page, chunk):
+    from tritify_amd.paged import PagedDecoder
+
+    ps = prompts([37, 1, 100, 16, 250, 5])
+    say(f"case: paged generate, page {page}, passes of {chunk} rows")
+    want = np.array([model.generate(p, 12)[0] for p in ps])
+    d = PagedDecoder(model, 60 * 16 // page + 10, page, max_rows=256)
+    free = len(d.free)
+    assert np.array_equal(d.generate(ps, 12, chunk), want)
+    assert len(d.free) == free and sorted(d.free) == list(range(free)) and not d.seq
+
+
+def test_sequences_come_and_go(model, torch_dev):
+    """Sequences that join and leave between passes, prompts beside single tokens: logits of every pass as the contiguous
+    decoder records them."""
+    from tritify_amd.paged import PagedDecoder
+
+    ps = prompts([20, 64, 3, 90])
+    ref = [model.generate(p, 10) for p in ps]
+    d = PagedDecoder(model, 40, max_rows=256)
+    made = {}
+
+    def go(work):
+        t = d.run([(made[i]["id"], x) for i, x in work])
+        for r, (i, _) in enumerate(work):
+            n = made[i]["n"]
+            assert np.array_equal(d.logits[r].cpu().numpy(), ref[i][1][n]), (i, n)
+            made[i]["n"], made[i]["t"] = n + 1, t[r:r + 1]
+            assert int(t[r]) == ref[i][0][n]
+
+    def join(i):
+        made[i] = dict(id=d.add(), n=0)
+        return (i, ps[i])
+
+    def on(*ii):
+        return [(i, made[i]["t"]) for i in ii]
+
+    go([join(0)])
+    go([join(1)] + on(0))
+    go(on(0, 1))
+    go(on(1) + [join(2), join(3)] + on(0))
+    d.release(made[1]["id"])
+    for _ in range(4):
+        go(on(3, 0, 2))
+    k, v = d.read(made[3]["id"], 1)
+    assert k.shape == (d.length(made[3]["id"]), 2, 64) and d.length(made[3]["id"]) == 94
+    model.generate(ps[3], 5)  # leaves the same positions in its own caches
+    n = 400 * 2 * 64
+    assert torch_dev.equal(k.reshape(-1), model.kc[n:n + k.numel()]) and torch_dev.equal(v.reshape(-1), model.vc[n:n + v.numel()])
+
+
+@pytest.mark.parametrize("bits,window,sinks", [(4, 0, 0), (8, 40, 4), (4, 33, 0), (4, 20, 18)])
+def test_a_batch_equals_its_sequences_alone(model, bits, window, sinks):
+    """And in other chunks; with a window, the pages that it leaves behind are free again on the way."""
+    from tritify_amd.paged import PagedDecoder
+
+    ps = prompts([37, 1, 120, 16])
+    say(f"case: paged generate alone and together, bits={bits} window={window} sinks={sinks}")
+    mk = lambda pages: PagedDecoder(model, pages, bits=bits, max_rows=200, window=window, sinks=sinks)  # noqa: E731
+    want = np.concatenate([mk(30).generate([p], 20, 11) for p in ps])
+    assert np.array_equal(mk(60).generate(ps, 20), want)
+    if window:
+        d = mk(8)  # 8 pages of 16: the 140 positions of the longest need 9
+        assert np.array_equal(d.generate([ps[2]], 20, 11), want[2:3])
+        assert sorted(d.free) == list(range(8))
+
+
+def test_refusals_leave_the_decoder_as_it_was(model):
+    from tritify_amd.paged import PagedDecoder
+
+    d = PagedDecoder(model, 6, max_seqs=2, max_rows=100)
+    a, b = d.add(), d.add()
+    d.run([(a, [1, 2, 3])])
+    for bad in ([], [(a, [])], [(a, [1]), (a, [2])], [(99, [1])], [(a, [1000])], [(a, [-1])], [(a, [1] * 101)],
+                [(a, [1] * 94), (b, [1] * 6)], [(a, [0] * 98)], [(a, [1]), (b, [1]), (d.add(), [1])]):
+        with pytest.raises(ValueError):
+            d.run(bad)
+        assert d.length(a) == 3 and len(d.free) == 5 and d.length(b) == 0
+    with pytest.raises(ValueError):
+        d.generate([[1], []], 2)
+    for kw in (dict(max_rows=0), dict(max_seqs=0), dict(window=-1), dict(page=20), dict(bits=3)):
+        with pytest.raises(ValueError):
+            PagedDecoder(model, 6, **kw)
+
+
+def test_captured_decode_steps(model, torch_dev):
+    """A decode step of a batch as one graph: the tables and lengths move on the device arrays between the replays."""
+    from tritify_amd.paged import PagedDecoder
+
+    torch = torch_dev
+    ps = prompts([37, 5, 100])
+    want = np.array([model.generate(p, 9)[0] for p in ps])
+    d = PagedDecoder(model, 40, max_rows=256)
+    ids = [d.add() for _ in ps]
+    tok = d.run(list(zip(ids, ps)))
+    got = [tok.cpu().numpy()]
+    d._reserve([(s, d.length(s) + 8) for s in ids])
+    b = d.batch(ids, [1, 1, 1])
+    x, out = tok.clone(), torch.empty_like(tok)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(s):
+        d.forward(x, b, None, out, s)  # the shape's workspace; the positions are written again by the first replay
+        torch.cuda.synchronize()
+        g.capture_begin()
+        d.forward(x, b, None, out, s)
+        g.capture_end()
+    torch.cuda.synchronize()
+    for step in range(8):
+        g.replay()
+        torch.cuda.synchronize()
+        got.append(out.cpu().numpy())
+        x.copy_(out)
+        b.kv_len.add_(1)
+        torch.cuda.synchronize()
+    assert np.array_equal(np.array(got).T, want)

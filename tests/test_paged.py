@@ -1,0 +1,138 @@
+"""The paged caches' rules on the CPU: the oracle's paged functions against the contiguous decoder's (kt_dec_rope_row,
+kt_dec_attend) and against closed forms, and the arguments that the C ABI refuses before any device work."""
+import numpy as np
+import pytest
+
+from oracle import oracle as O
+from paged_cases import Case, exp_table, part_bytes, rope_tables
+
+
+@pytest.mark.parametrize("page", [16, 64, 256])
+def test_eight_bits_are_the_contiguous_decoder(page):
+    nh, nkv, hd, L = 4, 2, 64, 83
+    c = Case(1, [(L, L), (3, 40)], nh, nkv, hd, page, 8)
+    cos, sin = rope_tables(200, hd)
+    q, k, v = c.append(cos, sin)
+    c.q, c.k, c.v = q, k, v
+    o = c.attend()
+    ck, cv = (np.zeros((L, nkv, hd), dtype=np.int8) for _ in range(2))
+    for p in range(L):
+        row = O.dec_rope(c.qkv[p, : (nh + nkv) * hd], nh + nkv, hd, p, cos, sin).reshape(-1, hd)
+        ck[p], cv[p] = row[nh:], c.qkv[p, (nh + nkv) * hd:].reshape(nkv, hd)
+        assert np.array_equal(q[p].reshape(nh, hd), row[:nh])
+        for h in range(nh):
+            want = O.dec_attend(row[h], ck, cv, p, nkv, h // 2, hd, c.exp)
+            assert np.array_equal(o[p, h * hd:(h + 1) * hd], want), (p, h)
+    rk, rv = (np.full((2, L + 5, nkv, hd), 9, dtype=np.int8) for _ in range(2))
+    O.paged_read(c.oracle(), rk, rv)
+    assert np.array_equal(rk[0, :L], ck) and np.array_equal(rv[0, :L], cv)
+    assert (rk[0, L:] == 9).all() and (rv[1, 40:] == 9).all()
+
+
+def test_four_bits_hold_what_they_say():
+    """Rows whose largest magnitude is at most 7 and even multiples of it survive the 4 bits; every other value is off by
+    half a multiplier step at most (m / 16), and by the rounding of the read (1 / 2)."""
+    hd, nkv, page = 64, 1, 16
+    cos, sin = np.full((16, 32), 16384, dtype=np.int16), np.zeros((16, 32), dtype=np.int16)
+    for top in (0, 1, 2, 3, 5, 7, 8, 33, 127, 128):
+        c = Case(2, [(16, 16)], 1, nkv, hd, page, 4)
+        x = c.g.integers(-top, min(top, 127) + 1, size=(16, 3 * hd))
+        x[:, hd] = x[:, 2 * hd] = -top
+        c.qkv = x.astype(np.int8)
+        q, c.k, c.v = c.append(cos, sin)
+        k, v = (np.zeros((1, 16, nkv, hd), dtype=np.int8) for _ in range(2))
+        O.paged_read(c.oracle(), k, v)
+        for got, sent in ((k, np.clip(x[:, hd:2 * hd], -127, 127)), (v, x[:, 2 * hd:])):
+            m = -(-8 * np.abs(sent).max(axis=1) // 7)
+            off = np.abs(got[0, :, 0].astype(int) - sent)
+            assert (16 * off <= (m + 16)[:, None]).all(), top
+            if top in (0, 1, 2, 3, 7):  # m / 8 is 0, 1/4, 3/8, 1/2 or 1: 8 x / m is exact or rounds back
+                assert (16 * off <= m[:, None]).all() and off.max() <= (0 if top != 2 else 1)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_window_equals_pages_left_out(bits):
+    """A window without sinks is the attention of a table whose older pages are gone, where the window ends at a page."""
+    c = Case(3, [(1, 16 * 9)], 4, 2, 64, 16, bits)
+    o = c.attend(window=32)
+    c.table[0, :7] = [-1, 99, c.pages, -5, 2 ** 30, -1, -1]
+    assert np.array_equal(c.attend(), o)
+    c.table[0, :] = -1
+    assert (c.attend() == 0).all()
+
+
+def _lib():
+    from tritify_amd import backend as B
+
+    return B.lib()
+
+
+@pytest.mark.parametrize("page,hd,bits,want", [(16, 64, 8, 1024), (16, 64, 4, 528), (256, 128, 8, 32768), (256, 128, 4, 16640),
+                                               (32, 128, 4, 2080), (8, 64, 8, 0), (48, 64, 8, 0), (512, 64, 8, 0), (16, 32, 8, 0),
+                                               (16, 96, 4, 0), (16, 64, 2, 0), (0, 64, 8, 0), (-16, 64, 8, 0)])
+def test_page_bytes(page, hd, bits, want):
+    assert _lib().kt_hip_dec_page_bytes(page, hd, bits) == want
+    if want:
+        assert part_bytes(page, hd, bits) == want
+
+
+P = 1 << 20  # an aligned address that no call here dereferences
+APPEND = dict(dev=0, qkv=P, tokens=3, qkv_stride=512, row_start=P, kv_len=P, table=P, seqs=2, max_pages=4, nh=4, nkv=2, hd=64,
+              cos=P, sin=P, max_pos=64, q=P, q_stride=256, k=P, v=P, pages=8, page=16, bits=8, stream=None)
+READ = dict(dev=0, k=P, v=P, pages=8, page=16, bits=8, kv_len=P, table=P, seqs=2, max_pages=4, nkv=2, hd=64, ko=P, vo=P,
+            max_pos=64, stream=None)
+ATTEND = dict(dev=0, q=P, tokens=3, q_stride=256, row_start=P, kv_len=P, table=P, seqs=2, max_pages=4, nh=4, nkv=2, hd=64, exp=P,
+              window=0, sinks=0, k=P, v=P, pages=8, page=16, bits=8, o=P, o_stride=256, ws=P, ws_bytes=1 << 40, stream=None)
+ARGMAX = dict(dev=0, logits=P, rows=3, n=1000, stride=1000, token=P, ws=P, ws_bytes=1 << 40, stream=None)
+GEOMETRY = [dict(page=24), dict(page=0), dict(hd=32), dict(hd=256), dict(bits=16), dict(seqs=-1), dict(max_pages=0),
+            dict(max_pages=524288 // 16 + 1), dict(nkv=0), dict(pages=-1), dict(pages=1 << 31), dict(k=P + 8), dict(v=None),
+            dict(kv_len=None), dict(table=None)]
+HEADS = [dict(nh=5), dict(nh=0), dict(tokens=-1), dict(tokens=1 << 30), dict(seqs=1 << 29), dict(row_start=None)]
+REFUSED = (
+    [("kt_hip_dec_rope_kv_paged", APPEND, x) for x in GEOMETRY + HEADS + [
+        dict(qkv_stride=511), dict(qkv_stride=520), dict(q_stride=240), dict(q_stride=264), dict(qkv=P + 4), dict(q=None),
+        dict(cos=P + 4), dict(sin=None), dict(max_pos=-1), dict(max_pos=1 << 31)]]
+    + [("kt_hip_dec_kv_read_paged", READ, x) for x in GEOMETRY + [
+        dict(ko=None), dict(vo=P + 1), dict(max_pos=-1), dict(seqs=1 << 29, max_pos=1 << 20, max_pages=1 << 14)]]
+    + [("kt_hip_dec_attention_paged", ATTEND, x) for x in GEOMETRY + HEADS + [
+        dict(q_stride=240), dict(q_stride=257), dict(o_stride=128), dict(o_stride=260), dict(q=None), dict(o=P + 8), dict(exp=None),
+        dict(window=-1), dict(sinks=-1), dict(ws=None), dict(ws=P + 4), dict(ws_bytes=0)]]
+    + [("kt_hip_dec_argmax_rows", ARGMAX, x) for x in [
+        dict(rows=-1), dict(rows=65536), dict(n=0), dict(n=1 << 31), dict(stride=999), dict(logits=None), dict(token=None),
+        dict(ws=None), dict(ws=P + 4), dict(ws_bytes=0)]]
+)
+
+
+@pytest.mark.parametrize("name,args,change", REFUSED, ids=[f"{n[11:]}-{'-'.join(f'{k}={v}' for k, v in x.items())}" for n, _, x in REFUSED])
+def test_refused_before_any_device_work(name, args, change):
+    assert getattr(_lib(), name)(*{**args, **change}.values()) == 1  # hipErrorInvalidValue
+
+
+def test_empty_calls_do_nothing():
+    L = _lib()
+    for empty in (dict(tokens=0), dict(seqs=0)):
+        assert L.kt_hip_dec_rope_kv_paged(*{**APPEND, **empty, "qkv": None, "q": None}.values()) == 0
+        assert L.kt_hip_dec_attention_paged(*{**ATTEND, **empty, "q": None, "o": None}.values()) == 0
+    assert L.kt_hip_dec_kv_read_paged(*{**READ, "seqs": 0, "ko": None}.values()) == 0
+    assert L.kt_hip_dec_kv_read_paged(*{**READ, "max_pos": 0, "ko": None}.values()) == 0
+    assert L.kt_hip_dec_argmax_rows(*{**ARGMAX, "rows": 0, "logits": None}.values()) == 0
+
+
+def test_workspaces_of_refused_shapes_are_zero():
+    from tritify_amd import backend as B
+
+    L = _lib()
+    assert L.kt_hip_dec_attention_paged_workspace(1, 1, 4, 16, 4, 2, 64) > 0
+    for bad in ((-1, 1, 4, 16, 4, 2, 64), (1, 1, 0, 16, 4, 2, 64), (1, 1, 4, 17, 4, 2, 64), (1, 1, 4, 16, 4, 3, 64), (1, 1, 4, 16, 4, 2, 48)):
+        assert L.kt_hip_dec_attention_paged_workspace(*bad) == 0
+    assert L.kt_hip_dec_argmax_rows_workspace(1, 0) == 0
+    with pytest.raises(ValueError):
+        B.dec_argmax_rows_workspace(70000, 5)
+
+
+def test_first_maximum_of_ties():
+    x = np.zeros((3, 9), dtype=np.int32)
+    x[1, [3, 5]] = 4
+    x[2] = -(2 ** 31)
+    assert O.argmax_rows(x, 9).tolist() == [0, 3, 0] and O.argmax_rows(x, 3).tolist() == [0, 0, 0]
+    assert exp_table(64)[0] == 32768

@@ -110,6 +110,15 @@ def _declare(L: C.CDLL) -> None:
         "kt_hip_w12_linear_add_o": (_I, [_I, _P, _P, _P, _I64, _I64, _P, _P, _P, _P, _P, _P, _P]),
         "kt_hip_dec_argmax_part": (_I, [_I, _P, _I64, _P, _I64, _P, _P, _P, _I64, _P]),
         "kt_hip_dec_embed_argmax": (_I, [_I, _P, _I64, _P, _I64, _P, _P, _P, _P]),
+        "kt_hip_dec_page_bytes": (_SZ, [_I64, _I64, _I]),
+        "kt_hip_dec_rope_kv_paged": (_I, [_I, _P, _I64, _I64, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _I64, _P,
+                                          _I64, _P, _P, _I64, _I64, _I, _P]),
+        "kt_hip_dec_kv_read_paged": (_I, [_I, _P, _P, _I64, _I64, _I, _P, _P, _I64, _I64, _I64, _I64, _P, _P, _I64, _P]),
+        "kt_hip_dec_attention_paged_workspace": (_SZ, [_I64] * 7),
+        "kt_hip_dec_attention_paged": (_I, [_I, _P, _I64, _I64, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _I64, _I64,
+                                            _P, _P, _I64, _I64, _I, _P, _I64, _P, _SZ, _P]),
+        "kt_hip_dec_argmax_rows_workspace": (_SZ, [_I64, _I64]),
+        "kt_hip_dec_argmax_rows": (_I, [_I, _P, _I64, _I64, _I64, _P, _P, _SZ, _P]),
         "kt_hip_w12_linear_norm": (_I, [_I, _P, _P, _P, _I64, _I64, _I64, _P, _P, _I, _P, _P]),
         "kt_hip_w12_swiglu_norm": (_I, [_I, _P, _P, _P, _I64, _I64, _I64, _P, _P, _P, _I, _P, _I64, _P]),
         "kt_hip_quant_linear_workspace": (_SZ, [_I64, _I64, _I64, _P]),
@@ -1049,3 +1058,23 @@ def ref_merge_rows(rows_dev, rs_dev, tokens: int, dim: int, ws_dev, ws_bytes: in
                    dev: int = 0) -> None:
     check(lib().kt_hip_ref_merge_rows(dev, _ptr(rows_dev), _ptr(rs_dev), tokens, dim, _ptr(ws_dev), ws_bytes,
                                       _ptr(out_dev), _ptr(os_dev), _stream(stream)), "ref merge rows")
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# the greedy choice of a batch (the paged caches themselves: tritify_amd/paged.py)
+
+
+def dec_argmax_rows_workspace(rows: int, n: int) -> int:
+    """Bytes of scratch that dec_argmax_rows of rows x n logits needs."""
+    b = lib().kt_hip_dec_argmax_rows_workspace(rows, n)
+    if b == 0:
+        raise ValueError(f"dec_argmax_rows: {rows} rows of {n} logits")
+    return b
+
+
+def dec_argmax_rows(logits_dev, rows: int, n: int, token_dev, ws_dev, stride: int | None = None, stream=None,
+                    dev: int = 0) -> None:
+    """token_dev[r] = the first index of the maximum of row r's n int32 logits (rows `stride` apart, n by default)."""
+    check(lib().kt_hip_dec_argmax_rows(dev, _ptr(logits_dev), rows, n, n if stride is None else stride,
+                                       _ptr(token_dev), _ptr(ws_dev), ws_dev.numel() * ws_dev.element_size(),
+                                       _stream(stream)), "dec argmax rows")

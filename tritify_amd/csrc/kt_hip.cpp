@@ -13,6 +13,7 @@
 #include <limits.h>
 #include <string.h>
 
+#include <algorithm>
 #include <atomic>
 #include <map>
 #include <mutex>
@@ -1029,6 +1030,118 @@ int kt_hip_dec_embed_argmax(int dev, const uint64_t* part_dev, int64_t nparts, c
     KT_TRY(hipSetDevice(dev));
     return (int)kt::launch_dec_embed_argmax(part_dev, (int)nparts, emb_dev, (int)d, r_dev, token_dev, step_dev,
                                             (hipStream_t)stream);
+}
+
+// The geometry that every call on paged caches checks: {page, hd, bits} of the layout, heads and batch within the kernels'
+// 32-bit counts. Device arrays are only dereferenced on the device.
+static bool paged_ok(int64_t tokens, int64_t seqs, int64_t max_pages, int64_t nh, int64_t nkv, int64_t hd,
+                     int64_t pages, int64_t page, int bits) {
+    return kt_hip_dec_page_bytes(page, hd, bits) != 0 && nkv >= 1 && nh >= nkv && nh % nkv == 0 && nh <= 65535 &&
+           tokens >= 0 && seqs >= 0 && tokens <= INT_MAX / nh && tokens <= 1 << 30 && seqs <= INT_MAX / (2 * nh) && max_pages >= 1 &&
+           max_pages <= KT_PAGED_MAX_POS / page && pages >= 0 && pages <= INT_MAX;
+}
+
+static bool aligned_to(const void* p, size_t n) { return p != nullptr && (uintptr_t)p % n == 0; }
+
+static kt::Paged paged_args(const int32_t* row_start, const int32_t* kv_len, const int32_t* table, const void* k,
+                            const void* v, int64_t tokens, int64_t seqs, int64_t max_pages, int64_t pages, int64_t page,
+                            int64_t nkv, int64_t hd, int bits) {
+    int sh = 4;
+    while ((1 << sh) < page) sh++;
+    return {row_start, kv_len, table, (uint8_t*)k, (uint8_t*)v, (int)tokens, (int)seqs, (int)max_pages, (int)pages, sh,
+            (int)nkv, kt::paged_part((int)page, (int)hd, bits)};
+}
+
+size_t kt_hip_dec_page_bytes(int64_t page, int64_t hd, int bits) {
+    if ((page != 16 && page != 32 && page != 64 && page != 128 && page != 256) || (hd != 64 && hd != 128) ||
+        (bits != 8 && bits != 4))
+        return 0;
+    return (size_t)kt::paged_part((int)page, (int)hd, bits);
+}
+
+int kt_hip_dec_rope_kv_paged(int dev, const int8_t* qkv_dev, int64_t tokens, int64_t qkv_stride,
+                             const int32_t* row_start_dev, const int32_t* kv_len_dev, const int32_t* table_dev,
+                             int64_t seqs, int64_t max_pages, int64_t nh, int64_t nkv, int64_t hd,
+                             const int16_t* cos_dev, const int16_t* sin_dev, int64_t max_pos, int8_t* q_dev,
+                             int64_t q_stride, void* kpool_dev, void* vpool_dev, int64_t pages, int64_t page, int bits,
+                             void* stream) {
+    if (!paged_ok(tokens, seqs, max_pages, nh, nkv, hd, pages, page, bits) || max_pos < 0 || max_pos > INT_MAX ||
+        qkv_stride < (nh + 2 * nkv) * hd || qkv_stride % 16 || q_stride < nh * hd || q_stride % 16)
+        return (int)hipErrorInvalidValue;
+    if (tokens == 0 || seqs == 0) return 0;
+    if (!row_start_dev || !kv_len_dev || !table_dev || !aligned_to(qkv_dev, 16) || !aligned_to(q_dev, 16) ||
+        (max_pos > 0 && (!aligned_to(cos_dev, 8) || !aligned_to(sin_dev, 8))) ||
+        (pages > 0 && (!aligned_to(kpool_dev, 16) || !aligned_to(vpool_dev, 16))))
+        return (int)hipErrorInvalidValue;
+    KT_TRY(hipSetDevice(dev));
+    return (int)kt::launch_pg_append(paged_args(row_start_dev, kv_len_dev, table_dev, kpool_dev, vpool_dev, tokens,
+                                                seqs, max_pages, pages, page, nkv, hd, bits),
+                                     (int)hd, bits, qkv_dev, qkv_stride, (int)nh, cos_dev, sin_dev, (int)max_pos, q_dev,
+                                     q_stride, (hipStream_t)stream);
+}
+
+int kt_hip_dec_kv_read_paged(int dev, const void* kpool_dev, const void* vpool_dev, int64_t pages, int64_t page,
+                             int bits, const int32_t* kv_len_dev, const int32_t* table_dev, int64_t seqs,
+                             int64_t max_pages, int64_t nkv, int64_t hd, int8_t* k_dev, int8_t* v_dev, int64_t max_pos,
+                             void* stream) {
+    if (!paged_ok(0, seqs, max_pages, nkv, nkv, hd, pages, page, bits) || max_pos < 0 ||
+        (max_pos > 0 && seqs > INT_MAX / ((std::min(max_pos, max_pages * page) + 15) / 16)))
+        return (int)hipErrorInvalidValue;
+    if (seqs == 0 || max_pos == 0) return 0;
+    if (!kv_len_dev || !table_dev || !aligned_to(k_dev, 16) || !aligned_to(v_dev, 16) ||
+        (pages > 0 && (!aligned_to(kpool_dev, 16) || !aligned_to(vpool_dev, 16))))
+        return (int)hipErrorInvalidValue;
+    KT_TRY(hipSetDevice(dev));
+    return (int)kt::launch_pg_read(paged_args(nullptr, kv_len_dev, table_dev, kpool_dev, vpool_dev, 0, seqs, max_pages,
+                                              pages, page, nkv, hd, bits),
+                                   (int)hd, bits, k_dev, v_dev, max_pos, (hipStream_t)stream);
+}
+
+size_t kt_hip_dec_attention_paged_workspace(int64_t tokens, int64_t seqs, int64_t max_pages, int64_t page, int64_t nh,
+                                            int64_t nkv, int64_t hd) {
+    if (!paged_ok(tokens, seqs, max_pages, nh, nkv, hd, 0, page, 8)) return 0;
+    return kt::pg_attend_workspace((int)tokens, (int)seqs, max_pages * page, (int)nh, (int)nkv, (int)hd);
+}
+
+int kt_hip_dec_attention_paged(int dev, const int8_t* q_dev, int64_t tokens, int64_t q_stride,
+                               const int32_t* row_start_dev, const int32_t* kv_len_dev, const int32_t* table_dev,
+                               int64_t seqs, int64_t max_pages, int64_t nh, int64_t nkv, int64_t hd,
+                               const int32_t* exp_tab_dev, int64_t window, int64_t sinks, const void* kpool_dev,
+                               const void* vpool_dev, int64_t pages, int64_t page, int bits, int8_t* o_dev,
+                               int64_t o_stride, void* ws_dev, size_t ws_bytes, void* stream) {
+    if (!paged_ok(tokens, seqs, max_pages, nh, nkv, hd, pages, page, bits) || window < 0 || sinks < 0 ||
+        q_stride < nh * hd || q_stride % 16 || o_stride < nh * hd || o_stride % 16)
+        return (int)hipErrorInvalidValue;
+    if (tokens == 0 || seqs == 0) return 0;
+    if (!row_start_dev || !kv_len_dev || !table_dev || !exp_tab_dev || !aligned_to(q_dev, 16) ||
+        !aligned_to(o_dev, 16) || !aligned_to(ws_dev, 16) ||
+        (pages > 0 && (!aligned_to(kpool_dev, 16) || !aligned_to(vpool_dev, 16))) ||
+        ws_bytes < kt_hip_dec_attention_paged_workspace(tokens, seqs, max_pages, page, nh, nkv, hd))
+        return (int)hipErrorInvalidValue;
+    // past the longest table a window or sink changes nothing
+    const int64_t most = KT_PAGED_MAX_POS;
+    KT_TRY(hipSetDevice(dev));
+    return (int)kt::launch_pg_attend(paged_args(row_start_dev, kv_len_dev, table_dev, kpool_dev, vpool_dev, tokens,
+                                                seqs, max_pages, pages, page, nkv, hd, bits),
+                                     (int)hd, bits, q_dev, q_stride, (int)nh, exp_tab_dev,
+                                     (int)(window < most ? window : 0), (int)std::min(sinks, most), o_dev, o_stride,
+                                     ws_dev, (hipStream_t)stream);
+}
+
+size_t kt_hip_dec_argmax_rows_workspace(int64_t rows, int64_t n) {
+    if (rows < 0 || n < 1 || rows > 65535 || n > INT_MAX) return 0;
+    return std::max<size_t>(256, (size_t)rows * (size_t)kt::pg_argmax_parts(rows, n) * 8);
+}
+
+int kt_hip_dec_argmax_rows(int dev, const int32_t* logits_dev, int64_t rows, int64_t n, int64_t stride,
+                           int32_t* token_dev, void* ws_dev, size_t ws_bytes, void* stream) {
+    if (rows < 0 || rows > 65535 || n < 1 || n > INT_MAX || stride < n) return (int)hipErrorInvalidValue;
+    if (rows == 0) return 0;
+    if (!logits_dev || !token_dev || !aligned_to(ws_dev, 8) || ws_bytes < kt_hip_dec_argmax_rows_workspace(rows, n))
+        return (int)hipErrorInvalidValue;
+    KT_TRY(hipSetDevice(dev));
+    return (int)kt::launch_pg_argmax(logits_dev, (int)rows, (int)n, stride, token_dev, (uint64_t*)ws_dev,
+                                     (hipStream_t)stream);
 }
 
 int kt_hip_probe_mfma(int dev, const int8_t* a_dev, const int8_t* b_dev, int32_t* c32_dev, int32_t* c16_dev,

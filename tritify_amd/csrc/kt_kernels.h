@@ -80,6 +80,25 @@ hipError_t launch_dec_argmax_part(const int32_t* logits, int n, uint64_t* part, 
                                   const int32_t* step, int32_t* pos, int advance, hipStream_t s);
 hipError_t launch_dec_embed_argmax(const uint64_t* part, int nparts, const int16_t* emb, int d, int32_t* r,
                                    int32_t* token, int32_t* step, hipStream_t s);
+// Paged KV caches (kt_hip_dec_*_paged): the batch's descriptors and the pools.
+struct Paged {
+    const int32_t *row_start, *kv_len, *table;
+    uint8_t *k, *v;
+    int tokens, seqs, max_pages, pages, page_sh, nkv;
+    int part;  // bytes of a kv head's part of a page
+};
+inline int paged_part(int page, int hd, int bits) { return bits == 8 ? page * hd : page * (hd / 2 + 1); }
+hipError_t launch_pg_append(const Paged& a, int hd, int bits, const int8_t* qkv, int64_t stride, int nh,
+                            const int16_t* cosT, const int16_t* sinT, int max_pos, int8_t* q, int64_t q_stride,
+                            hipStream_t s);
+hipError_t launch_pg_read(const Paged& a, int hd, int bits, int8_t* k, int8_t* v, int64_t max_pos, hipStream_t s);
+hipError_t launch_pg_attend(const Paged& a, int hd, int bits, const int8_t* q, int64_t q_stride, int nh,
+                            const int32_t* exp_tab, int window, int sinks, int8_t* o, int64_t o_stride, void* ws,
+                            hipStream_t s);
+size_t pg_attend_workspace(int tokens, int seqs, int64_t max_pos, int nh, int nkv, int hd);
+int pg_argmax_parts(int64_t rows, int64_t n);
+hipError_t launch_pg_argmax(const int32_t* logits, int rows, int n, int64_t stride, int32_t* token, uint64_t* part,
+                            hipStream_t s);
 hipError_t launch_w12_swiglu(const int8_t* x, const int8_t* lo, const uint8_t* nib, int M, int F, int kp,
                              const int32_t* mant, const int32_t* shift, const int16_t* silu, int h_shift, int8_t* y,
                              int ystride, hipStream_t s);

@@ -1,0 +1,320 @@
+// The int8 decoder's paged KV caches on gfx950: the new rows' RoPE with the write of k and v to their pages (8 bits, or
+// quantised to 4), the read back, and the greedy choice of a batch's rows. The attention is kt_paged_attn.hip. The rules
+// and the layout of the pools are stated with kt_hip_dec_*_paged in include/kt_hip.h; the decoder these serve is the one of
+// kt_decoder.hip (DecoderModel, crates/01-engine/kt-core/src/model.rs:168-188, 290-353), for many sequences at once.
+
+#include <algorithm>
+#include <hip/hip_runtime.h>
+#include <limits.h>
+#include <stdint.h>
+
+#include "kt_paged.h"
+#include "kt_w12_core.h"
+
+namespace kt {
+
+namespace {
+
+__device__ __forceinline__ int rope_round(int v) {  // clamp(round_half_away(v / 2^14)), |v| < 2^30
+    int q = ((v < 0 ? -v : v) + (1 << 13)) >> 14;
+    q = q > 127 ? 127 : q;
+    return v < 0 ? -q : q;
+}
+
+__device__ __forceinline__ int byte_of(int w, int i) { return (int)(int8_t)(w >> (8 * i)); }
+
+// The multiplier of a row whose largest magnitude is `top` (0 .. 128): ceil(8 top / 7), at most 147.
+__device__ __forceinline__ int mult4(int top) { return (8 * top + 6) / 7; }
+
+// 2^20 / (2 m) rounded up: n / (2 m) = (n inv) >> 20 for 0 <= n <= 2195 (n inv / 2^20 exceeds n / (2 m) by less than
+// n / 2^20 < 1 / 294 <= 1 / (2 m), and n inv < 2^31 from m = 2 on, the least multiplier of a row that is not zeros).
+__device__ __forceinline__ int mult4_inv(int m) { return m ? ((1 << 20) + 2 * m - 1) / (2 * m) : 0; }
+
+// clamp(round_half_away(8 x / m), +-7): floor((16 |x| + m) / (2 m)); 0 where m is 0 (x is then too).
+__device__ __forceinline__ int code4(int x, int m, int inv) {
+    const int a = x < 0 ? -x : x;
+    int c = ((16 * a + m) * inv) >> 20;
+    c = c > 7 ? 7 : c;
+    return x < 0 ? -c : c;
+}
+
+// clamp(round_half_away(c m / 8)).
+__device__ __forceinline__ int value4(int c, int m) {
+    const int t = c * m;
+    int q = ((t < 0 ? -t : t) + 4) >> 3;
+    q = q > 127 ? 127 : q;
+    return t < 0 ? -q : q;
+}
+
+// One CTA per (block of 16 positions that a sequence's rows reach, kv head): it rotates the q heads of the group and the k
+// head of the rows in the block, four pairs a thread, stages k and v in LDS and writes the block's bytes. The block is the
+// unit because V's chunk is 16 positions of a dimension, in 4 bits with two positions to a byte: whole blocks go out as
+// 16-byte (8-byte) stores, and one that only some of its rows belong to is written byte by byte (4 bits: read, merged and
+// written back by its only owner).
+template <int HD, int BITS>
+__global__ __launch_bounds__(256) void pg_append_kernel(Paged a, const int8_t* __restrict__ qkv, int64_t stride, int nh,
+                                                        const int16_t* __restrict__ cosT,
+                                                        const int16_t* __restrict__ sinT, int max_pos,
+                                                        int8_t* __restrict__ q, int64_t q_stride) {
+    constexpr int HH = HD / 2, CH = HD / 16;
+    __shared__ __attribute__((aligned(16))) int8_t sKV[2][16][HD];
+    __shared__ int sM[2][16];
+    const int tid = threadIdx.x, g = blockIdx.y, rep = nh / a.nkv;
+    int first = 0;
+    const int b = pg_tile_seq(a, (int)blockIdx.x, 1, 16, 2, &first);
+    if (b < 0) return;
+    const PgRows s = pg_rows(a, b);
+    const int blk = (s.p0 >> 4) + ((int)blockIdx.x - first);
+    const int lo = max(16 * blk, s.p0), hi = min(16 * blk + 16, s.p0 + s.n);
+    if (lo >= hi) return;
+    // the rows whose position the tables and the caches have
+    const int cap = min(max_pos, a.max_pages << a.page_sh), vlo = max(lo, 0), vhi = min(hi, cap);
+    const int items = (hi - lo) * (rep + 1) * (HH / 4);
+    for (int i = tid; i < items; i += 256) {
+        const int c = i % (HH / 4), r = i / (HH / 4) / (rep + 1), hv = i / (HH / 4) - r * (rep + 1), p = lo + r;
+        const size_t t = (size_t)(s.t0 + (p - s.p0));
+        const bool live = p >= vlo && p < vhi;
+        int x = 0, y = 0;
+        if (live) {
+            const int8_t* src = qkv + t * stride + (hv < rep ? g * rep + hv : nh + g) * HD + 4 * c;
+            const int xa = *reinterpret_cast<const int*>(src), xb = *reinterpret_cast<const int*>(src + HH);
+            const v2i C = *reinterpret_cast<const v2i*>(cosT + (size_t)p * HH + 4 * c);
+            const v2i S = *reinterpret_cast<const v2i*>(sinT + (size_t)p * HH + 4 * c);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int cc = (int)(int16_t)(C[e >> 1] >> (16 * (e & 1))), ss = (int)(int16_t)(S[e >> 1] >> (16 * (e & 1)));
+                const int u = byte_of(xa, e), w = byte_of(xb, e);
+                x |= (rope_round(u * cc - w * ss) & 255) << (8 * e);
+                y |= (rope_round(w * cc + u * ss) & 255) << (8 * e);
+            }
+        }
+        if (hv < rep) {
+            int8_t* to = q + t * q_stride + (g * rep + hv) * HD + 4 * c;
+            *reinterpret_cast<int*>(to) = x;
+            *reinterpret_cast<int*>(to + HH) = y;
+        } else if (live) {
+            *reinterpret_cast<int*>(&sKV[0][p & 15][4 * c]) = x;
+            *reinterpret_cast<int*>(&sKV[0][p & 15][4 * c + HH]) = y;
+        }
+    }
+    if (vlo >= vhi) return;
+    const int id = pg_page(a, b, blk);
+    if (id < 0) return;
+    for (int i = tid; i < (vhi - vlo) * CH; i += 256) {
+        const int p = vlo + i / CH, c = i % CH;
+        const int8_t* src = qkv + (size_t)(s.t0 + (p - s.p0)) * stride + (nh + a.nkv + g) * HD + 16 * c;
+        *reinterpret_cast<v4i*>(&sKV[1][p & 15][16 * c]) = *reinterpret_cast<const v4i*>(src);
+    }
+    __syncthreads();
+    const int r0 = vlo & 15, r1 = vhi - 16 * blk;  // the block's rows r0 .. r1 - 1
+    const size_t part = ((size_t)id * a.nkv + g) * (size_t)a.part;
+    const int slot = (16 * blk) & ((1 << a.page_sh) - 1);
+    if constexpr (BITS == 8) {
+        uint8_t* kd = a.k + part + slot * HD;
+        uint8_t* vd = a.v + part + slot * HD;
+        for (int i = tid; i < 16 * CH; i += 256) {
+            const int r = i / CH, c = i % CH;
+            if (r >= r0 && r < r1) *reinterpret_cast<v4i*>(kd + r * HD + 16 * c) = *reinterpret_cast<const v4i*>(&sKV[0][r][16 * c]);
+        }
+        for (int d = tid; d < HD; d += 256) {
+            if (r1 - r0 == 16) {
+                v4i w = {0, 0, 0, 0};
+#pragma unroll
+                for (int r = 0; r < 16; r++) w[r >> 2] |= (int)(uint8_t)sKV[1][r][d] << (8 * (r & 3));
+                *reinterpret_cast<v4i*>(vd + 16 * d) = w;
+            } else {
+                for (int r = r0; r < r1; r++) vd[16 * d + r] = (uint8_t)sKV[1][r][d];
+            }
+        }
+    } else {
+        {  // 8 threads a row: its largest magnitude
+            const int w = tid >> 7, r = (tid >> 3) & 15, e = tid & 7;
+            int top = 0;
+            if (r >= r0 && r < r1)
+                for (int d = e; d < HD; d += 8) {
+                    const int x = sKV[w][r][d], m = x < 0 ? -x : x;
+                    top = m > top ? m : top;
+                }
+#pragma unroll
+            for (int d = 4; d >= 1; d >>= 1) top = max(top, __shfl_xor(top, d));
+            if (e == 0 && r >= r0 && r < r1) {
+                const int m = mult4(top);
+                sM[w][r] = m;
+                (w ? a.v : a.k)[part + (size_t)(HH << a.page_sh) + slot + r] = (uint8_t)m;
+            }
+        }
+        __syncthreads();
+        uint8_t* kd = a.k + part + slot * HH;
+        uint8_t* vd = a.v + part + slot * HH;
+        for (int i = tid; i < 16 * CH; i += 256) {
+            const int r = i / CH, c = i % CH;
+            if (r < r0 || r >= r1) continue;
+            const int m = sM[0][r], inv = mult4_inv(m);
+            v2i w = {0, 0};
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+                w[e >> 3] |= (code4(sKV[0][r][16 * c + e], m, inv) & 15) << (8 * (e & 3) + 4 * ((e >> 2) & 1));
+            *reinterpret_cast<v2i*>(kd + r * HH + 8 * c) = w;
+        }
+        for (int d = tid; d < HD; d += 256) {
+            v2i w = {0, 0};
+            if (r1 - r0 < 16) w = *reinterpret_cast<const v2i*>(vd + 8 * d);
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                if (r < r0 || r >= r1) continue;
+                const int sh = 8 * (r & 3) + 4 * ((r >> 2) & 1), m = sM[1][r];
+                w[r >> 3] = (w[r >> 3] & ~(15 << sh)) | ((code4(sKV[1][r][d], m, mult4_inv(m)) & 15) << sh);
+            }
+            *reinterpret_cast<v2i*>(vd + 8 * d) = w;
+        }
+    }
+}
+
+// One CTA per block of 16 positions of a sequence, all its kv heads: K's chunks as they stand, V four dimensions a thread
+// (their 16 positions are four chunks side by side), so that 16 threads write one position's row.
+template <int HD, int BITS>
+__global__ __launch_bounds__(256) void pg_read_kernel(Paged a, int8_t* __restrict__ k, int8_t* __restrict__ v,
+                                                      int64_t max_pos, int nblk) {
+    constexpr int HH = HD / 2, CH = HD / 16;
+    const int b = (int)blockIdx.x / nblk, blk = (int)blockIdx.x - b * nblk;
+    int end = min(pg_len(a, b), a.max_pages << a.page_sh);
+    end = (int64_t)end < max_pos ? end : (int)max_pos;
+    const int n = min(16, end - 16 * blk);
+    if (n <= 0) return;
+    const int id = pg_page(a, b, blk), slot = (16 * blk) & ((1 << a.page_sh) - 1);
+    const int8_t* kp = reinterpret_cast<const int8_t*>(a.k) + (size_t)(id < 0 ? 0 : id) * a.nkv * a.part;
+    const int8_t* vp = reinterpret_cast<const int8_t*>(a.v) + (size_t)(id < 0 ? 0 : id) * a.nkv * a.part;
+    const size_t out = ((size_t)b * max_pos + 16 * blk) * a.nkv * HD;
+    for (int i = threadIdx.x; i < n * a.nkv * CH; i += 256) {
+        const int c = i % CH, g = i / CH % a.nkv, r = i / CH / a.nkv;
+        v4i w = {0, 0, 0, 0};
+        if (id >= 0) {
+            const int8_t* pg = kp + (size_t)g * a.part;
+            if constexpr (BITS == 8) {
+                w = *reinterpret_cast<const v4i*>(pg + (slot + r) * HD + 16 * c);
+            } else {
+                const v2i x = *reinterpret_cast<const v2i*>(pg + (slot + r) * HH + 8 * c);
+                const int m = (uint8_t)pg[(HH << a.page_sh) + slot + r];
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const int code = (x[e >> 3] << (28 - 8 * (e & 3) - 4 * ((e >> 2) & 1))) >> 28;
+                    w[e >> 2] |= (value4(code, m) & 255) << (8 * (e & 3));
+                }
+            }
+        }
+        *reinterpret_cast<v4i*>(k + out + ((size_t)r * a.nkv + g) * HD + 16 * c) = w;
+    }
+    for (int i = threadIdx.x; i < a.nkv * (HD / 4); i += 256) {
+        const int d = 4 * (i % (HD / 4)), g = i / (HD / 4);
+        int w[16];
+#pragma unroll
+        for (int r = 0; r < 16; r++) w[r] = 0;
+        if (id >= 0) {
+            const int8_t* pg = vp + (size_t)g * a.part;
+            v4i m4 = {0, 0, 0, 0};
+            if constexpr (BITS == 4) m4 = *reinterpret_cast<const v4i*>(pg + (HH << a.page_sh) + slot);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if constexpr (BITS == 8) {
+                    const v4i x = *reinterpret_cast<const v4i*>(pg + slot * HD + 16 * (d + e));
+#pragma unroll
+                    for (int r = 0; r < 16; r++) w[r] |= (byte_of(x[r >> 2], r & 3) & 255) << (8 * e);
+                } else {
+                    const v2i x = *reinterpret_cast<const v2i*>(pg + slot * HH + 8 * (d + e));
+#pragma unroll
+                    for (int r = 0; r < 16; r++) {
+                        const int code = (x[r >> 3] << (28 - 8 * (r & 3) - 4 * ((r >> 2) & 1))) >> 28;
+                        w[r] |= (value4(code, (m4[r >> 2] >> (8 * (r & 3))) & 255) & 255) << (8 * e);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 16; r++)
+            if (r < n) *reinterpret_cast<int*>(v + out + ((size_t)r * a.nkv + g) * HD + d) = w[r];
+    }
+}
+
+// The greedy choice. A key is (value, then the lower index) in 64 bits, the largest key the first maximum:
+// ((v ^ 2^31) << 32) | (2^32 - 1 - i).
+__device__ __forceinline__ uint64_t block_max_key(uint64_t best, uint64_t* s_key) {
+    best = (uint64_t)wave_max_i64((int64_t)(best ^ (1ull << 63))) ^ (1ull << 63);
+    if ((threadIdx.x & 63) == 0) s_key[threadIdx.x >> 6] = best;
+    __syncthreads();
+    best = s_key[0];
+#pragma unroll
+    for (int q = 1; q < 4; q++) best = s_key[q] > best ? s_key[q] : best;
+    return best;
+}
+
+// Grid (parts, rows): the best key of a part of a row; with one part a row, its index is the answer.
+__global__ __launch_bounds__(256) void pg_argmax_kernel(const int32_t* __restrict__ logits, int n, int64_t stride,
+                                                        int per, uint64_t* __restrict__ part,
+                                                        int32_t* __restrict__ token) {
+    __shared__ uint64_t s_key[4];
+    const int32_t* x = logits + (size_t)blockIdx.y * stride;
+    const uint32_t i0 = blockIdx.x * (uint32_t)per, i1 = min(i0 + (uint32_t)per, (uint32_t)n);
+    uint64_t best = 0;
+#pragma unroll 8
+    for (uint32_t i = i0 + threadIdx.x; i < i1; i += 256) {
+        const uint64_t key = ((uint64_t)((uint32_t)x[i] ^ 0x80000000u) << 32) | (0xFFFFFFFFu - i);
+        best = key > best ? key : best;
+    }
+    best = block_max_key(best, s_key);
+    if (threadIdx.x == 0) {
+        if (gridDim.x == 1) token[blockIdx.y] = (int32_t)(0xFFFFFFFFu - (uint32_t)best);
+        else part[(size_t)blockIdx.y * gridDim.x + blockIdx.x] = best;
+    }
+}
+
+__global__ __launch_bounds__(256) void pg_argmax_join_kernel(const uint64_t* __restrict__ part, int parts,
+                                                             int32_t* __restrict__ token) {
+    __shared__ uint64_t s_key[4];
+    uint64_t best = 0;
+    for (int i = threadIdx.x; i < parts; i += 256) {
+        const uint64_t key = part[(size_t)blockIdx.x * parts + i];
+        best = key > best ? key : best;
+    }
+    best = block_max_key(best, s_key);
+    if (threadIdx.x == 0) token[blockIdx.x] = (int32_t)(0xFFFFFFFFu - (uint32_t)best);
+}
+
+}  // namespace
+
+hipError_t launch_pg_append(const Paged& a, int hd, int bits, const int8_t* qkv, int64_t stride, int nh,
+                            const int16_t* cosT, const int16_t* sinT, int max_pos, int8_t* q, int64_t q_stride,
+                            hipStream_t s) {
+    const dim3 grid((unsigned)(a.tokens / 16 + 2 * a.seqs), (unsigned)a.nkv);
+    auto go = [&](auto kern) {
+        kern<<<grid, dim3(256), 0, s>>>(a, qkv, stride, nh, cosT, sinT, max_pos, q, q_stride);
+        return hipGetLastError();
+    };
+    if (hd == 64) return bits == 8 ? go(pg_append_kernel<64, 8>) : go(pg_append_kernel<64, 4>);
+    return bits == 8 ? go(pg_append_kernel<128, 8>) : go(pg_append_kernel<128, 4>);
+}
+
+hipError_t launch_pg_read(const Paged& a, int hd, int bits, int8_t* k, int8_t* v, int64_t max_pos, hipStream_t s) {
+    const int nblk = (int)((std::min<int64_t>(max_pos, (int64_t)a.max_pages << a.page_sh) + 15) / 16);
+    auto go = [&](auto kern) {
+        kern<<<dim3((unsigned)(a.seqs * nblk)), dim3(256), 0, s>>>(a, k, v, max_pos, nblk);
+        return hipGetLastError();
+    };
+    if (hd == 64) return bits == 8 ? go(pg_read_kernel<64, 8>) : go(pg_read_kernel<64, 4>);
+    return bits == 8 ? go(pg_read_kernel<128, 8>) : go(pg_read_kernel<128, 4>);
+}
+
+int pg_argmax_parts(int64_t rows, int64_t n) {
+    return (int)std::max<int64_t>(1, std::min((n + 4095) / 4096, (2048 + rows - 1) / std::max<int64_t>(rows, 1)));
+}
+
+hipError_t launch_pg_argmax(const int32_t* logits, int rows, int n, int64_t stride, int32_t* token, uint64_t* part,
+                            hipStream_t s) {
+    const int parts = pg_argmax_parts(rows, n), per = (int)(((int64_t)n + parts - 1) / parts);
+    pg_argmax_kernel<<<dim3((unsigned)parts, (unsigned)rows), dim3(256), 0, s>>>(logits, n, stride, per, part, token);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || parts == 1) return e;
+    pg_argmax_join_kernel<<<dim3((unsigned)rows), dim3(256), 0, s>>>(part, parts, token);
+    return hipGetLastError();
+}
+
+}  // namespace kt
