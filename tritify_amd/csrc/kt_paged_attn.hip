@@ -1,4 +1,5 @@
-// Attention of a ragged batch's new rows over paged KV caches on gfx950 (kt_hip_dec_attention_paged).
+// Attention of a ragged batch's new rows over paged KV caches on gfx950 (kt_hip_dec_attention_paged, stated in
+// include/kt_hip.h): chunks, whole prompts and single tokens by one kernel.
 
 #include <algorithm>
 #include <hip/hip_runtime.h>
@@ -12,116 +13,409 @@ namespace kt {
 
 namespace {
 
-// clamp(round_half_away(a / b)), b > 0.
-__device__ __forceinline__ int div_round_q8(int64_t a, int64_t b) {
-    const uint64_t m = a < 0 ? 0 - (uint64_t)a : (uint64_t)a;
-    uint64_t q = (2 * m + (uint64_t)b) / (2 * (uint64_t)b);
-    q = q > 127 ? 127 : q;
-    return a < 0 ? -(int)q : (int)q;
-}
+struct PgAttend {
+    const int8_t* q;
+    int8_t* o;
+    int64_t q_stride, o_stride;
+    const int32_t* exp_tab;
+    int rep, window, sinks, splits;
+    int32_t* wmax;   // [tile][kv head][split][column]
+    int64_t* wsum;   // [tile][kv head][split][column group, 16 dimensions][register][lane], then the weights' sums
+};
 
-// One CTA per (row, q head): the scores of 256 positions at a time, one a thread, their maximum; then the scores again,
-// the weights to LDS and the weighted sum of v, a thread per (dimension, share of the positions).
+enum { PG_WHOLE = 0, PG_MAX = 1, PG_SUMS = 2 };
+
+// What a wave holds of 64 positions (four blocks of 16) of one kv head. K: lane l has dimensions 16 (l / 16) .. of 64 from
+// position 16 (l / 4 % 4) + 4 t + l % 4 in k[t][.]: as the A operand of a 16x16x64 product its 16 rows give lane l the
+// scores of positions 16 (l / 16) + 4 t + r in register r. So a lane's 16 scores of the four products are one block's 16
+// positions in order, which is the layout of a B operand of the product with V, whose chunks (16 positions of a dimension)
+// are loaded as they stand.
 template <int HD, int BITS>
-__global__ __launch_bounds__(256) void pg_attend_row_kernel(Paged a, const int8_t* __restrict__ q, int64_t q_stride,
-                                                            int nh, const int32_t* __restrict__ exp_tab, int window,
-                                                            int sinks, int8_t* __restrict__ o, int64_t o_stride) {
-    constexpr int HH = HD / 2, SH = 256 / HD;
-    __shared__ __attribute__((aligned(16))) int8_t sQ[HD];
-    __shared__ int sE[256], sMul[256], sRed[8];
-    __shared__ const int8_t* sV[256];
-    __shared__ int64_t sDen[4], sSum[SH][HD];
-    const int t = (int)blockIdx.x / nh, h = (int)blockIdx.x - t * nh, g = h / (nh / a.nkv), tid = threadIdx.x;
+struct PgTile {
+    v4i k[4][HD / 64];
+    v4i v[HD / 16];
+    v4i km, vm;
+};
+
+template <int HD, int BITS, int MT, int W, int MODE>
+__global__ __launch_bounds__(64 * W) void pg_attend_kernel(Paged a, PgAttend p) {
+    constexpr int HH = HD / 2, KC = HD / 64, DT = HD / 16, ND = BITS == 8 ? 2 : 3, COLS = 16 * MT;
+    constexpr int ROWB = BITS == 8 ? HD : HH, CHB = BITS == 8 ? 16 : 8;
+    constexpr bool MAXP = MODE != PG_SUMS, SUMP = MODE != PG_MAX;
+    __shared__ int64_t sSum[SUMP ? MT * DT * 4 * 64 : 1];
+    __shared__ int64_t sDen[COLS];
+    __shared__ int sMax[W][COLS];
+    __shared__ uint16_t sE[1026];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l16 = lane & 15, gq = lane >> 4, kb = (lane >> 2) & 3;
+    const int split = (int)blockIdx.y;
+    // the kv head fastest: CTAs go to the XCDs in turn, so an XCD's L2 holds the heads congruent to it
+    const int tile = (int)(gridDim.x / a.nkv) - 1 - (int)blockIdx.x / a.nkv, g = (int)blockIdx.x % a.nkv;
     int first = 0;
-    const int b = pg_tile_seq(a, t, 1, 1, 0, &first);
+    const int b = pg_tile_seq(a, tile, p.rep, COLS, 1, &first);
     if (b < 0) return;
     const PgRows s = pg_rows(a, b);
-    if (t < s.t0 || t >= s.t0 + s.n) return;
-    const int p = s.p0 + (t - s.t0);
-    int8_t* to = o + (size_t)t * o_stride + h * HD;
-    if (p < 0 || p >= a.max_pages << a.page_sh) {
-        if (tid < HD) to[tid] = 0;
+    const int m0 = (tile - first) * COLS, mrows = s.n * p.rep;  // m: row i, head r of the group as i rep + r
+    if (m0 >= mrows) return;
+    const int cols = min(COLS, mrows - m0), nmt = (cols + 15) / 16;
+    const int cap = a.max_pages << a.page_sh, nblk = cap >> 4;
+    const int pmin = s.p0 + m0 / p.rep, pmax = min(s.p0 + (m0 + cols - 1) / p.rep, cap - 1);
+    // the tiles of 64 positions: those of the sinks, then those of the window
+    const int ntile = pmax < 0 || a.pages == 0 ? 0 : pmax / 64 + 1;
+    int nsink = 0, w0 = 0;
+    if (p.window) {
+        nsink = min((min(p.sinks, pmax + 1) + 63) / 64, ntile);
+        w0 = max(nsink, (max(pmin, 0) - min(p.window - 1, max(pmin, 0))) / 64);
+    }
+    const int total = nsink + max(0, ntile - w0);
+    auto tile_at = [&](int i) { return i < nsink ? i : i - nsink + w0; };
+
+    if constexpr (SUMP) {
+        for (int i = tid; i < 1025; i += 64 * W) {
+            const int e = i < 1024 ? min(max(p.exp_tab[i], 0), 32768) : 0;
+            // 8 bits: the two balanced base-256 digits of -e (2^15 itself has none, -2^15 does); 4 bits: e
+            sE[i] = BITS == 8 ? (uint16_t)((0x8080 - e) ^ 0x8080) : (uint16_t)e;
+        }
+        for (int i = tid; i < MT * DT * 4 * 64; i += 64 * W) sSum[i] = 0;
+        if (tid < COLS) sDen[tid] = 0;
+    }
+
+    // the columns' rows and positions, and their q as B operands
+    int pos[MT];
+    v4i q[MT][KC];
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++) {
+        const int m = m0 + min(16 * mt + l16, cols - 1), i = m / p.rep, r = m - i * p.rep;
+        pos[mt] = 16 * mt + l16 < cols && s.p0 + i < cap ? s.p0 + i : -1;
+        const int8_t* qr = p.q + (size_t)(s.t0 + i) * p.q_stride + (g * p.rep + r) * HD + 16 * gq;
+#pragma unroll
+        for (int c = 0; c < KC; c++) q[mt][c] = *reinterpret_cast<const v4i*>(qr + 64 * c);
+    }
+
+    // page ids of the tile's blocks kb (K) and gq (V and the multipliers)
+    struct Ids {
+        int k, v;
+    };
+    auto page_ids = [&](int T) {
+        const int bk = min(4 * T + kb, nblk - 1), bv = min(4 * T + gq, nblk - 1);
+        const int32_t* tab = a.table + (size_t)b * a.max_pages;
+        return Ids{tab[bk >> (a.page_sh - 4)], tab[bv >> (a.page_sh - 4)]};
+    };
+    auto slot_of = [&](int blk) { return (blk << 4) & ((1 << a.page_sh) - 1); };
+    auto part_of = [&](int id) { return ((size_t)((unsigned)id < (unsigned)a.pages ? id : 0) * a.nkv + g) * (size_t)a.part; };
+    auto load_k = [&](int T, Ids id, PgTile<HD, BITS>& x) {
+        const uint8_t* at = a.k + part_of(id.k) + (size_t)((slot_of(min(4 * T + kb, nblk - 1)) + (lane & 3)) * ROWB + gq * CHB);
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int c = 0; c < KC; c++) {
+                if constexpr (BITS == 8) {
+                    x.k[t][c] = *reinterpret_cast<const v4i*>(at + 4 * t * ROWB + 64 * c);
+                } else {
+                    const v2i y = *reinterpret_cast<const v2i*>(at + 4 * t * ROWB + 32 * c);
+                    x.k[t][c].x = y.x, x.k[t][c].y = y.y;
+                }
+            }
+        if constexpr (BITS == 4)
+            x.km = *reinterpret_cast<const v4i*>(a.k + part_of(id.v) + (size_t)((HH << a.page_sh) + slot_of(min(4 * T + gq, nblk - 1))));
+    };
+    auto load_v = [&](int T, Ids id, PgTile<HD, BITS>& x) {
+        const int slot = slot_of(min(4 * T + gq, nblk - 1));
+        const uint8_t* at = a.v + part_of(id.v) + (size_t)(slot * ROWB + l16 * CHB);
+#pragma unroll
+        for (int d = 0; d < DT; d++) {
+            if constexpr (BITS == 8) {
+                x.v[d] = *reinterpret_cast<const v4i*>(at + 16 * CHB * d);
+            } else {
+                const v2i y = *reinterpret_cast<const v2i*>(at + 16 * CHB * d);
+                x.v[d].x = y.x, x.v[d].y = y.y;
+            }
+        }
+        if constexpr (BITS == 4)
+            x.vm = *reinterpret_cast<const v4i*>(a.v + part_of(id.v) + (size_t)((HH << a.page_sh) + slot));
+    };
+    // 4 bits: 16 times the 16 codes of a chunk, in order (byte 4 h + r: code 8 h + r low, code 8 h + 4 + r high)
+    auto widen = [](v4i x) {
+        constexpr int M = (int)0xF0F0F0F0;
+        return v4i{(x.x << 4) & M, x.x & M, (x.y << 4) & M, x.y & M};
+    };
+    // the scores of column group mt: register r of s[t] is position 16 gq + 4 t + r of the tile
+    auto scores = [&](const PgTile<HD, BITS>& x, int mt, v4i (&sc)[4]) {
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            sc[t] = v4i{0, 0, 0, 0};
+#pragma unroll
+            for (int c = 0; c < KC; c++) sc[t] = mfma16(BITS == 8 ? x.k[t][c] : widen(x.k[t][c]), q[mt][c], sc[t]);
+            if constexpr (BITS == 4) {
+#pragma unroll
+                for (int r = 0; r < 4; r++)  // (m (q . c) + 4) >> 3 of 16 (q . c)
+                    sc[t][r] = (__mul24(sc[t][r], (x.km[t] >> (8 * r)) & 255) + 64) >> 7;
+            }
+        }
+    };
+    auto sees = [&](int j, int pp) { return j <= pp && (p.window == 0 || j > pp - p.window || j < p.sinks); };
+    // whether every column sees every position of the tile (uniform)
+    auto full = [&](int T, bool ok) {
+        return __all(ok) && 64 * T + 63 <= pmin && (p.window == 0 || 64 * T > pmax - p.window || 64 * T + 63 < p.sinks);
+    };
+    auto page_ok = [&](int T, Ids id) { return (unsigned)id.v < (unsigned)a.pages && 4 * T + gq < nblk; };
+
+    const int step = p.splits * W, start = split * W + w;
+    int mx[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++) mx[mt] = INT_MIN;
+    if constexpr (MAXP) {
+        PgTile<HD, BITS> x;
+        Ids id = {0, 0};
+        if (start < total) id = page_ids(tile_at(start)), load_k(tile_at(start), id, x);
+        for (int i = start; i < total; i += step) {
+            const int T = tile_at(i);
+            const bool ok = page_ok(T, id);
+            PgTile<HD, BITS> nx;
+            Ids nid = id;
+            if (i + step < total) nid = page_ids(tile_at(i + step)), load_k(tile_at(i + step), nid, nx);
+            const bool all = full(T, ok);
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++) {
+                if (mt >= nmt) break;
+                v4i sc[4];
+                scores(x, mt, sc);
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        if (all || (ok && sees(64 * T + 16 * gq + 4 * t + r, pos[mt]))) mx[mt] = max(mx[mt], sc[t][r]);
+            }
+            x = nx, id = nid;
+        }
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++) {
+            mx[mt] = max(mx[mt], __shfl_xor(mx[mt], 16));
+            mx[mt] = max(mx[mt], __shfl_xor(mx[mt], 32));
+            if (gq == 0) sMax[w][16 * mt + l16] = mx[mt];
+        }
+    }
+    __syncthreads();
+    const size_t unit = ((size_t)tile * a.nkv + g) * p.splits;  // of the workspace's parts
+    if constexpr (MODE == PG_MAX) {
+        if (tid < COLS) {
+            int m = sMax[0][tid];
+#pragma unroll
+            for (int i = 1; i < W; i++) m = max(m, sMax[i][tid]);
+            p.wmax[(unit + split) * COLS + tid] = m;
+        }
         return;
     }
-    if (tid < HD) sQ[tid] = q[(size_t)t * q_stride + h * HD + tid];
-    __syncthreads();
-    auto score = [&](int j, int& sc) {
-        if (j > p || (window && j <= p - window && j >= sinks)) return false;
-        const int id = pg_page(a, b, j >> 4);
-        if (id < 0) return false;
-        const size_t part = ((size_t)id * a.nkv + g) * (size_t)a.part;
-        const int slot = j & ((1 << a.page_sh) - 1);
-        const int8_t* k = reinterpret_cast<const int8_t*>(a.k) + part;
-        sc = 0;
-        if constexpr (BITS == 8) {
-            for (int d = 0; d < HD; d++) sc += sQ[d] * k[slot * HD + d];
-        } else {
-            for (int d = 0; d < HD; d++) {
-                const int x = (uint8_t)k[slot * HH + d / 16 * 8 + d % 16 / 8 * 4 + d % 4];
-                sc += sQ[d] * ((d % 8 >= 4 ? x << 24 : x << 28) >> 28);
+    if constexpr (MODE == PG_WHOLE) {
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+            for (int i = 0; i < W; i++) mx[mt] = max(mx[mt], sMax[i][16 * mt + l16]);
+    }
+    if constexpr (MODE == PG_SUMS) {
+        for (int i = 0; i < p.splits; i++)
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++) mx[mt] = max(mx[mt], p.wmax[(unit + i) * COLS + 16 * mt + l16]);
+    }
+    if constexpr (SUMP) {
+        v4i acc[MT][DT][ND];
+        int den[MT][2];
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++) {
+            mx[mt] = (mx[mt] == INT_MIN ? 0 : mx[mt]) + 64;  // of a column that sees nothing every weight is masked
+            den[mt][0] = den[mt][1] = 0;
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int n = 0; n < ND; n++) acc[mt][d][n] = v4i{0, 0, 0, 0};
+        }
+        PgTile<HD, BITS> x;
+        Ids id = {0, 0};
+        const int last = start < total ? start + (total - 1 - start) / step * step : -1;  // from the end: its K is nearest
+        if (last >= 0) id = page_ids(tile_at(last)), load_k(tile_at(last), id, x);
+        for (int i = last; i >= start; i -= step) {
+            const int T = tile_at(i);
+            const bool ok = page_ok(T, id), all = full(T, ok);
+            load_v(T, id, x);
+            PgTile<HD, BITS> nx;
+            Ids nid = id;
+            if (i - step >= start) nid = page_ids(tile_at(i - step)), load_k(tile_at(i - step), nid, nx);
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++) {
+                if (mt >= nmt) break;
+                v4i sc[4], P[ND];
+                scores(x, mt, sc);
+                auto weights = [&](bool masked) {
+#pragma unroll
+                    for (int t = 0; t < 4; t++) {
+                        uint32_t e[4];
+#pragma unroll
+                        for (int r = 0; r < 4; r++) {
+                            uint32_t ix = min((uint32_t)(mx[mt] - sc[t][r]) >> 7, 1024u);
+                            if (masked) ix = ok && sees(64 * T + 16 * gq + 4 * t + r, pos[mt]) ? ix : 1024u;
+                            e[r] = sE[ix];
+                            if constexpr (BITS == 4) {  // the digits of e m
+                                den[mt][0] += (int)e[r];
+                                e[r] = (__umul24(e[r], ((uint32_t)x.vm[t] >> (8 * r)) & 255) + 0x808080) ^ 0x808080;
+                            }
+                        }
+                        const uint32_t e01 = __builtin_amdgcn_perm(e[1], e[0], 0x05010400), e23 = __builtin_amdgcn_perm(e[3], e[2], 0x05010400);
+                        P[0][t] = (int)__builtin_amdgcn_perm(e23, e01, 0x05040100);
+                        P[1][t] = (int)__builtin_amdgcn_perm(e23, e01, 0x07060302);
+                        if constexpr (BITS == 4)
+                            P[ND - 1][t] = (int)__builtin_amdgcn_perm(__builtin_amdgcn_perm(e[3], e[2], 0x0c0c0602), __builtin_amdgcn_perm(e[1], e[0], 0x0c0c0602), 0x05040100);
+                        if constexpr (BITS == 8) {
+                            den[mt][0] = __builtin_amdgcn_sdot4(P[0][t], 0x01010101, den[mt][0], false);
+                            den[mt][1] = __builtin_amdgcn_sdot4(P[1][t], 0x01010101, den[mt][1], false);
+                        }
+                    }
+                };
+                if (all) weights(false);
+                else weights(true);
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int n = 0; n < ND; n++) acc[mt][d][n] = mfma16(BITS == 8 ? x.v[d] : widen(x.v[d]), P[n], acc[mt][d][n]);
             }
-            sc = (sc * (uint8_t)k[(HH << a.page_sh) + slot] + 4) >> 3;
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int c = 0; c < KC; c++) x.k[t][c] = nx.k[t][c];
+            x.km = nx.km;
+            id = nid;
         }
-        sV[tid] = reinterpret_cast<const int8_t*>(a.v) + part;
-        return true;
-    };
-    int mx = INT_MIN;
-    for (int j = tid; j <= p; j += 256) {
-        int sc;
-        if (score(j, sc)) mx = max(mx, sc);
-    }
-    mx = wave_max_i32(mx);
-    if ((tid & 63) == 0) sRed[tid >> 6] = mx;
-    __syncthreads();
-    mx = max(max(sRed[0], sRed[1]), max(sRed[2], sRed[3]));
-    int64_t den = 0, sum = 0;
-    const int d = tid % HD, sh = tid / HD;
-    for (int j0 = 0; j0 <= p; j0 += 256) {
-        __syncthreads();
-        int sc, e = 0;
-        if (score(j0 + tid, sc)) {
-            const int i = (mx - sc + 64) >> 7;
-            e = i < 1024 ? min(max(exp_tab[i], 0), 32768) : 0;
+        // the waves' sums: register r of lane l is dimension 16 d + 4 (l / 16) + r of column l % 16
+        if (start < total) {
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++) {
+                if (mt >= nmt) break;
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        int64_t v = (int64_t)acc[mt][d][0][r] + ((int64_t)acc[mt][d][1][r] << 8);
+                        if constexpr (BITS == 4) v += (int64_t)acc[mt][d][ND - 1][r] << 16;
+                        atomicAdd(reinterpret_cast<unsigned long long*>(&sSum[((mt * DT + d) * 4 + r) * 64 + lane]), (unsigned long long)v);
+                    }
+                const int64_t dn = BITS == 8 ? (int64_t)den[mt][0] + ((int64_t)den[mt][1] << 8) : (int64_t)den[mt][0];
+                atomicAdd(reinterpret_cast<unsigned long long*>(&sDen[16 * mt + l16]), (unsigned long long)dn);
+            }
         }
-        sE[tid] = e;
-        den += e;
         __syncthreads();
-        for (int i = sh; i < 256; i += SH) {
-            if (sE[i] == 0) continue;
-            const int slot = (j0 + i) & ((1 << a.page_sh) - 1);
-            if constexpr (BITS == 8) {
-                sum += sE[i] * sV[i][(slot >> 4) * 16 * HD + 16 * d + (slot & 15)];
-            } else {
-                const int r = slot & 15, x = (uint8_t)sV[i][(slot >> 4) * 8 * HD + 8 * d + (r >> 3) * 4 + (r & 3)];
-                sum += (int64_t)(sE[i] * (uint8_t)sV[i][(HH << a.page_sh) + slot]) * ((r & 4 ? x << 24 : x << 28) >> 28);
+        for (int it = tid; it < nmt * DT * 64; it += 64 * W) {
+            const int mt = it / (DT * 64), d = it / 64 % DT, col = 16 * mt + (it & 15);
+            int64_t v[4];
+#pragma unroll
+            for (int r = 0; r < 4; r++) v[r] = sSum[((mt * DT + d) * 4 + r) * 64 + (it & 63)];
+            if constexpr (MODE == PG_SUMS) {
+                int64_t* to = p.wsum + (unit + split) * (size_t)(COLS * (HD + 1));
+#pragma unroll
+                for (int r = 0; r < 4; r++) to[((mt * DT + d) * 4 + r) * 64 + (it & 63)] = v[r];
+                if (d == 0 && (it & 63) < 16) to[COLS * HD + col] = sDen[col];
+            } else if (col < cols) {
+                const int i = (m0 + col) / p.rep, r0 = m0 + col - i * p.rep, pp = s.p0 + i;
+                const int64_t dn = BITS == 8 ? -sDen[col] : 128 * sDen[col];
+                uint32_t out = 0;
+                if (pp >= 0 && pp < cap && dn > 0)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) out |= (uint32_t)(uint8_t)div_round_q8(BITS == 8 ? -v[r] : v[r], dn) << (8 * r);
+                *reinterpret_cast<uint32_t*>(p.o + (size_t)(s.t0 + i) * p.o_stride + (g * p.rep + r0) * HD + 16 * d + 4 * ((it & 63) >> 4)) = out;
             }
         }
     }
-    den = (int64_t)wave_sum_u64((uint64_t)den);
-    if ((tid & 63) == 0) sDen[tid >> 6] = den;
-    sSum[sh][d] = sum;
-    __syncthreads();
-    if (tid < HD) {
-        int64_t top = 0;
-        for (int i = 0; i < SH; i++) top += sSum[i][tid];
-        den = (sDen[0] + sDen[1] + sDen[2] + sDen[3]) * (BITS == 8 ? 1 : 8);
-        to[tid] = den ? (int8_t)div_round_q8(top, den) : 0;
+}
+
+// The splits' sums joined: one CTA per (tile, kv head, 16 columns).
+template <int HD, int BITS, int MT>
+__global__ __launch_bounds__(256) void pg_join_kernel(Paged a, PgAttend p) {
+    constexpr int DT = HD / 16, COLS = 16 * MT;
+    const int tile = (int)blockIdx.x / a.nkv, g = (int)blockIdx.x % a.nkv, mt = blockIdx.y;
+    int first = 0;
+    const int b = pg_tile_seq(a, tile, p.rep, COLS, 1, &first);
+    if (b < 0) return;
+    const PgRows s = pg_rows(a, b);
+    const int m0 = (tile - first) * COLS, cols = min(COLS, s.n * p.rep - m0), cap = a.max_pages << a.page_sh;
+    if (16 * mt >= cols) return;
+    const int64_t* from = p.wsum + ((size_t)tile * a.nkv + g) * p.splits * (size_t)(COLS * (HD + 1));
+    for (int it = threadIdx.x; it < DT * 64; it += 256) {
+        const int d = it / 64, lane = it & 63, col = 16 * mt + (lane & 15);
+        if (col >= cols) continue;
+        int64_t v[4] = {0, 0, 0, 0}, dn = 0;
+#pragma unroll 4
+        for (int i = 0; i < p.splits; i++) {
+            const int64_t* x = from + (size_t)i * (COLS * (HD + 1));
+#pragma unroll
+            for (int r = 0; r < 4; r++) v[r] += x[((mt * DT + d) * 4 + r) * 64 + lane];
+            dn += x[COLS * HD + col];
+        }
+        const int i = (m0 + col) / p.rep, r0 = m0 + col - i * p.rep, pp = s.p0 + i;
+        dn = BITS == 8 ? -dn : 128 * dn;
+        uint32_t out = 0;
+        if (pp >= 0 && pp < cap && dn > 0)
+#pragma unroll
+            for (int r = 0; r < 4; r++) out |= (uint32_t)(uint8_t)div_round_q8(BITS == 8 ? -v[r] : v[r], dn) << (8 * r);
+        *reinterpret_cast<uint32_t*>(p.o + (size_t)(s.t0 + i) * p.o_stride + (g * p.rep + r0) * HD + 16 * d + 4 * (lane >> 4)) = out;
     }
+}
+
+struct Plan {
+    int mt, w, tiles, splits;
+};
+
+Plan plan(int tokens, int seqs, int64_t max_pos, int nh, int nkv, int hd) {
+    const int rep = nh / nkv;
+    const int64_t each = ((int64_t)tokens * rep + seqs - 1) / std::max(seqs, 1);
+    Plan x;
+    x.mt = each <= 16 ? 1 : (hd == 64 ? 4 : 2);
+    x.w = 8;
+    const int64_t tiles = (int64_t)tokens * rep / (16 * x.mt) + seqs;
+    x.tiles = (int)tiles;
+    const int64_t ctas = std::min<int64_t>(tiles, tokens) * nkv, work = (max_pos + 63) / 64;
+    x.splits = (int)std::max<int64_t>(1, std::min<int64_t>((512 + ctas - 1) / ctas, work / (2 * x.w)));
+    if (ctas >= 256) x.splits = 1;
+    return x;
+}
+
+size_t ws_max_bytes(const Plan& x, int nkv) {
+    return ((size_t)x.tiles * nkv * x.splits * 16 * x.mt * 4 + 255) / 256 * 256;
 }
 
 }  // namespace
 
-size_t pg_attend_workspace(int, int, int64_t, int, int, int) { return 256; }
+size_t pg_attend_workspace(int tokens, int seqs, int64_t max_pos, int nh, int nkv, int hd) {
+    const Plan x = plan(tokens, seqs, max_pos, nh, nkv, hd);
+    if (x.splits == 1) return 256;
+    return ws_max_bytes(x, nkv) + (size_t)x.tiles * nkv * x.splits * 16 * x.mt * (hd + 1) * 8;
+}
+
+template <int HD, int BITS, int MT, int W>
+static hipError_t attend(const Paged& a, PgAttend p, const Plan& x, hipStream_t s) {
+    const dim3 grid((unsigned)(x.tiles * a.nkv), (unsigned)x.splits), block(64 * W);
+    if (x.splits == 1) {
+        pg_attend_kernel<HD, BITS, MT, W, PG_WHOLE><<<grid, block, 0, s>>>(a, p);
+        return hipGetLastError();
+    }
+    pg_attend_kernel<HD, BITS, MT, W, PG_MAX><<<grid, block, 0, s>>>(a, p);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    pg_attend_kernel<HD, BITS, MT, W, PG_SUMS><<<grid, block, 0, s>>>(a, p);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+    pg_join_kernel<HD, BITS, MT><<<dim3((unsigned)(x.tiles * a.nkv), MT), dim3(256), 0, s>>>(a, p);
+    return hipGetLastError();
+}
 
 hipError_t launch_pg_attend(const Paged& a, int hd, int bits, const int8_t* q, int64_t q_stride, int nh,
-                            const int32_t* exp_tab, int window, int sinks, int8_t* o, int64_t o_stride, void*,
+                            const int32_t* exp_tab, int window, int sinks, int8_t* o, int64_t o_stride, void* ws,
                             hipStream_t s) {
-    auto go = [&](auto kern) {
-        kern<<<dim3((unsigned)(a.tokens * nh)), dim3(256), 0, s>>>(a, q, q_stride, nh, exp_tab, window, sinks, o, o_stride);
-        return hipGetLastError();
-    };
-    if (hd == 64) return bits == 8 ? go(pg_attend_row_kernel<64, 8>) : go(pg_attend_row_kernel<64, 4>);
-    return bits == 8 ? go(pg_attend_row_kernel<128, 8>) : go(pg_attend_row_kernel<128, 4>);
+    const Plan x = plan(a.tokens, a.seqs, (int64_t)a.max_pages << a.page_sh, nh, a.nkv, hd);
+    const PgAttend p = {q, o, q_stride, o_stride, exp_tab, nh / a.nkv, window, sinks, x.splits, (int32_t*)ws,
+                        (int64_t*)((char*)ws + ws_max_bytes(x, a.nkv))};
+    if (hd == 64) {
+        if (x.mt == 1) return bits == 8 ? attend<64, 8, 1, 8>(a, p, x, s) : attend<64, 4, 1, 8>(a, p, x, s);
+        return bits == 8 ? attend<64, 8, 4, 8>(a, p, x, s) : attend<64, 4, 4, 8>(a, p, x, s);
+    }
+    if (x.mt == 1) return bits == 8 ? attend<128, 8, 1, 8>(a, p, x, s) : attend<128, 4, 1, 8>(a, p, x, s);
+    return bits == 8 ? attend<128, 8, 2, 8>(a, p, x, s) : attend<128, 4, 2, 8>(a, p, x, s);
 }
 
 }  // namespace kt
