@@ -23,6 +23,7 @@ struct PgAttend {
     int64_t* wsum;   // [tile][kv head][split][column group, 16 dimensions][register][lane], then the weights' sums
 };
 
+constexpr int PG_W = 8;  // waves of a CTA
 enum { PG_WHOLE = 0, PG_MAX = 1, PG_SUMS = 2 };
 
 // What a wave holds of 64 positions (four blocks of 16) of one kv head. K: lane l has dimensions 16 (l / 16) .. of 64 from
@@ -164,29 +165,50 @@ __global__ __launch_bounds__(64 * W) void pg_attend_kernel(Paged a, PgAttend p) 
     int mx[MT];
 #pragma unroll
     for (int mt = 0; mt < MT; mt++) mx[mt] = INT_MIN;
+    // Tiles start, start + step, ... go through a ring of tiles in registers. A tile's page ids are read a round of the ring
+    // before its loads are issued, and those a round before they are used: a wave waits for neither.
+    const int mine = start < total ? (total - 1 - start) / step + 1 : 0;
     if constexpr (MAXP) {
-        PgTile<HD, BITS> x;
-        Ids id = {0, 0};
-        if (start < total) id = page_ids(tile_at(start)), load_k(tile_at(start), id, x);
-        for (int i = start; i < total; i += step) {
-            const int T = tile_at(i);
-            const bool ok = page_ok(T, id);
-            PgTile<HD, BITS> nx;
-            Ids nid = id;
-            if (i + step < total) nid = page_ids(tile_at(i + step)), load_k(tile_at(i + step), nid, nx);
-            const bool all = full(T, ok);
+        constexpr int NB = MT == 1 ? 4 : 2;
+        PgTile<HD, BITS> x[NB];
+        Ids id[NB], nid[NB];
+        auto at = [&](int n) { return tile_at(start + n * step); };
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++) {
-                if (mt >= nmt) break;
-                v4i sc[4];
-                scores(x, mt, sc);
+        for (int u = 0; u < NB; u++) {
+            id[u] = nid[u] = Ids{0, 0};
+            if (u < mine) id[u] = page_ids(at(u));
+            if (u + NB < mine) nid[u] = page_ids(at(u + NB));
+        }
 #pragma unroll
-                for (int t = 0; t < 4; t++)
+        for (int u = 0; u < NB; u++)
+            if (u < mine) load_k(at(u), id[u], x[u]);
+        for (int n0 = 0; n0 < mine; n0 += NB) {
 #pragma unroll
-                    for (int r = 0; r < 4; r++)
-                        if (all || (ok && sees(64 * T + 16 * gq + 4 * t + r, pos[mt]))) mx[mt] = max(mx[mt], sc[t][r]);
+            for (int u = 0; u < NB; u++) {
+                const int n = n0 + u;
+                if (n >= mine) break;
+                const int T = at(n);
+                const bool ok = page_ok(T, id[u]), all = full(T, ok);
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++) {
+                    if (mt >= nmt) break;
+                    v4i sc[4];
+                    scores(x[u], mt, sc);
+                    if (all) {
+#pragma unroll
+                        for (int t = 0; t < 4; t++) mx[mt] = max(max(mx[mt], max(sc[t].x, sc[t].y)), max(sc[t].z, sc[t].w));
+                    } else {
+#pragma unroll
+                        for (int t = 0; t < 4; t++)
+#pragma unroll
+                            for (int r = 0; r < 4; r++)
+                                if (ok && sees(64 * T + 16 * gq + 4 * t + r, pos[mt])) mx[mt] = max(mx[mt], sc[t][r]);
+                    }
+                }
+                if (n + NB < mine) load_k(at(n + NB), nid[u], x[u]);
+                id[u] = nid[u];
+                if (n + 2 * NB < mine) nid[u] = page_ids(at(n + 2 * NB));
             }
-            x = nx, id = nid;
         }
 #pragma unroll
         for (int mt = 0; mt < MT; mt++) {
@@ -229,60 +251,70 @@ __global__ __launch_bounds__(64 * W) void pg_attend_kernel(Paged a, PgAttend p) 
 #pragma unroll
                 for (int n = 0; n < ND; n++) acc[mt][d][n] = v4i{0, 0, 0, 0};
         }
-        PgTile<HD, BITS> x;
-        Ids id = {0, 0};
-        const int last = start < total ? start + (total - 1 - start) / step * step : -1;  // from the end: its K is nearest
-        if (last >= 0) id = page_ids(tile_at(last)), load_k(tile_at(last), id, x);
-        for (int i = last; i >= start; i -= step) {
-            const int T = tile_at(i);
-            const bool ok = page_ok(T, id), all = full(T, ok);
-            load_v(T, id, x);
-            PgTile<HD, BITS> nx;
-            Ids nid = id;
-            if (i - step >= start) nid = page_ids(tile_at(i - step)), load_k(tile_at(i - step), nid, nx);
+        constexpr int NB = MT == 1 ? 2 : 1;
+        PgTile<HD, BITS> x[NB];
+        Ids id[NB], nid[NB];
+        auto at = [&](int n) { return tile_at(start + (mine - 1 - n) * step); };  // from the end: its K is nearest
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++) {
-                if (mt >= nmt) break;
-                v4i sc[4], P[ND];
-                scores(x, mt, sc);
-                auto weights = [&](bool masked) {
+        for (int u = 0; u < NB; u++) {
+            id[u] = nid[u] = Ids{0, 0};
+            if (u < mine) id[u] = page_ids(at(u));
+            if (u + NB < mine) nid[u] = page_ids(at(u + NB));
+        }
 #pragma unroll
-                    for (int t = 0; t < 4; t++) {
-                        uint32_t e[4];
+        for (int u = 0; u < NB; u++)
+            if (u < mine) load_k(at(u), id[u], x[u]), load_v(at(u), id[u], x[u]);
+        for (int n0 = 0; n0 < mine; n0 += NB) {
 #pragma unroll
-                        for (int r = 0; r < 4; r++) {
-                            uint32_t ix = min((uint32_t)(mx[mt] - sc[t][r]) >> 7, 1024u);
-                            if (masked) ix = ok && sees(64 * T + 16 * gq + 4 * t + r, pos[mt]) ? ix : 1024u;
-                            e[r] = sE[ix];
-                            if constexpr (BITS == 4) {  // the digits of e m
-                                den[mt][0] += (int)e[r];
-                                e[r] = (__umul24(e[r], ((uint32_t)x.vm[t] >> (8 * r)) & 255) + 0x808080) ^ 0x808080;
+            for (int u = 0; u < NB; u++) {
+                const int n = n0 + u;
+                if (n >= mine) break;
+                const int T = at(n);
+                const bool ok = page_ok(T, id[u]), all = full(T, ok);
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++) {
+                    if (mt >= nmt) break;
+                    v4i sc[4], P[ND];
+                    scores(x[u], mt, sc);
+                    const v4i vm = x[u].vm;
+                    if (mt == nmt - 1 && n + NB < mine) load_k(at(n + NB), nid[u], x[u]);
+                    auto weights = [&](bool masked) {
+#pragma unroll
+                        for (int t = 0; t < 4; t++) {
+                            uint32_t e[4];
+#pragma unroll
+                            for (int r = 0; r < 4; r++) {
+                                uint32_t ix = min((uint32_t)(mx[mt] - sc[t][r]) >> 7, 1024u);
+                                if (masked) ix = ok && sees(64 * T + 16 * gq + 4 * t + r, pos[mt]) ? ix : 1024u;
+                                e[r] = sE[ix];
+                                if constexpr (BITS == 4) {  // the digits of e m
+                                    den[mt][0] += (int)e[r];
+                                    e[r] = (__umul24(e[r], ((uint32_t)vm[t] >> (8 * r)) & 255) + 0x808080) ^ 0x808080;
+                                }
+                            }
+                            const uint32_t e01 = __builtin_amdgcn_perm(e[1], e[0], 0x05010400), e23 = __builtin_amdgcn_perm(e[3], e[2], 0x05010400);
+                            P[0][t] = (int)__builtin_amdgcn_perm(e23, e01, 0x05040100);
+                            P[1][t] = (int)__builtin_amdgcn_perm(e23, e01, 0x07060302);
+                            if constexpr (BITS == 4)
+                                P[ND - 1][t] = (int)__builtin_amdgcn_perm(__builtin_amdgcn_perm(e[3], e[2], 0x0c0c0602), __builtin_amdgcn_perm(e[1], e[0], 0x0c0c0602), 0x05040100);
+                            if constexpr (BITS == 8) {
+                                den[mt][0] = __builtin_amdgcn_sdot4(P[0][t], 0x01010101, den[mt][0], false);
+                                den[mt][1] = __builtin_amdgcn_sdot4(P[1][t], 0x01010101, den[mt][1], false);
                             }
                         }
-                        const uint32_t e01 = __builtin_amdgcn_perm(e[1], e[0], 0x05010400), e23 = __builtin_amdgcn_perm(e[3], e[2], 0x05010400);
-                        P[0][t] = (int)__builtin_amdgcn_perm(e23, e01, 0x05040100);
-                        P[1][t] = (int)__builtin_amdgcn_perm(e23, e01, 0x07060302);
-                        if constexpr (BITS == 4)
-                            P[ND - 1][t] = (int)__builtin_amdgcn_perm(__builtin_amdgcn_perm(e[3], e[2], 0x0c0c0602), __builtin_amdgcn_perm(e[1], e[0], 0x0c0c0602), 0x05040100);
-                        if constexpr (BITS == 8) {
-                            den[mt][0] = __builtin_amdgcn_sdot4(P[0][t], 0x01010101, den[mt][0], false);
-                            den[mt][1] = __builtin_amdgcn_sdot4(P[1][t], 0x01010101, den[mt][1], false);
-                        }
-                    }
-                };
-                if (all) weights(false);
-                else weights(true);
+                    };
+                    if (all) weights(false);
+                    else weights(true);
 #pragma unroll
-                for (int d = 0; d < DT; d++)
+                    for (int d = 0; d < DT; d++)
 #pragma unroll
-                    for (int n = 0; n < ND; n++) acc[mt][d][n] = mfma16(BITS == 8 ? x.v[d] : widen(x.v[d]), P[n], acc[mt][d][n]);
+                        for (int k = 0; k < ND; k++)
+                            acc[mt][d][k] = mfma16(BITS == 8 ? x[u].v[d] : widen(x[u].v[d]), P[k], acc[mt][d][k]);
+                }
+                if (n + NB < mine) load_v(at(n + NB), nid[u], x[u]);
+                id[u] = nid[u];
+                if (n + 2 * NB < mine) nid[u] = page_ids(at(n + 2 * NB));
             }
-#pragma unroll
-            for (int t = 0; t < 4; t++)
-#pragma unroll
-                for (int c = 0; c < KC; c++) x.k[t][c] = nx.k[t][c];
-            x.km = nx.km;
-            id = nid;
         }
         // the waves' sums: register r of lane l is dimension 16 d + 4 (l / 16) + r of column l % 16
         if (start < total) {
@@ -325,10 +357,11 @@ __global__ __launch_bounds__(64 * W) void pg_attend_kernel(Paged a, PgAttend p) 
     }
 }
 
-// The splits' sums joined: one CTA per (tile, kv head, 16 columns).
+// The splits' sums joined: one CTA per (tile, kv head, 16 columns, 64 dimensions), four shares of the splits side by side.
 template <int HD, int BITS, int MT>
-__global__ __launch_bounds__(256) void pg_join_kernel(Paged a, PgAttend p) {
+__global__ __launch_bounds__(1024) void pg_join_kernel(Paged a, PgAttend p) {
     constexpr int DT = HD / 16, COLS = 16 * MT;
+    __shared__ int64_t sV[4][4][256], sD[4][256];
     const int tile = (int)blockIdx.x / a.nkv, g = (int)blockIdx.x % a.nkv, mt = blockIdx.y;
     int first = 0;
     const int b = pg_tile_seq(a, tile, p.rep, COLS, 1, &first);
@@ -337,41 +370,51 @@ __global__ __launch_bounds__(256) void pg_join_kernel(Paged a, PgAttend p) {
     const int m0 = (tile - first) * COLS, cols = min(COLS, s.n * p.rep - m0), cap = a.max_pages << a.page_sh;
     if (16 * mt >= cols) return;
     const int64_t* from = p.wsum + ((size_t)tile * a.nkv + g) * p.splits * (size_t)(COLS * (HD + 1));
-    for (int it = threadIdx.x; it < DT * 64; it += 256) {
-        const int d = it / 64, lane = it & 63, col = 16 * mt + (lane & 15);
-        if (col >= cols) continue;
-        int64_t v[4] = {0, 0, 0, 0}, dn = 0;
-#pragma unroll 4
-        for (int i = 0; i < p.splits; i++) {
+    const int it = threadIdx.x & 255, share = threadIdx.x >> 8;
+    const int d = 4 * blockIdx.z + it / 64, lane = it & 63, col = 16 * mt + (lane & 15);
+    int64_t v[4] = {0, 0, 0, 0}, dn = 0;
+    if (col < cols) {
+#pragma unroll 8
+        for (int i = share; i < p.splits; i += 4) {
             const int64_t* x = from + (size_t)i * (COLS * (HD + 1));
 #pragma unroll
             for (int r = 0; r < 4; r++) v[r] += x[((mt * DT + d) * 4 + r) * 64 + lane];
             dn += x[COLS * HD + col];
         }
-        const int i = (m0 + col) / p.rep, r0 = m0 + col - i * p.rep, pp = s.p0 + i;
-        dn = BITS == 8 ? -dn : 128 * dn;
-        uint32_t out = 0;
-        if (pp >= 0 && pp < cap && dn > 0)
-#pragma unroll
-            for (int r = 0; r < 4; r++) out |= (uint32_t)(uint8_t)div_round_q8(BITS == 8 ? -v[r] : v[r], dn) << (8 * r);
-        *reinterpret_cast<uint32_t*>(p.o + (size_t)(s.t0 + i) * p.o_stride + (g * p.rep + r0) * HD + 16 * d + 4 * (lane >> 4)) = out;
     }
+#pragma unroll
+    for (int r = 0; r < 4; r++) sV[share][r][it] = v[r];
+    sD[share][it] = dn;
+    __syncthreads();
+    if (share || col >= cols) return;
+    for (int k = 1; k < 4; k++) {
+#pragma unroll
+        for (int r = 0; r < 4; r++) v[r] += sV[k][r][it];
+        dn += sD[k][it];
+    }
+    const int i = (m0 + col) / p.rep, r0 = m0 + col - i * p.rep, pp = s.p0 + i;
+    dn = BITS == 8 ? -dn : 128 * dn;
+    uint32_t out = 0;
+    if (pp >= 0 && pp < cap && dn > 0)
+#pragma unroll
+        for (int r = 0; r < 4; r++) out |= (uint32_t)(uint8_t)div_round_q8(BITS == 8 ? -v[r] : v[r], dn) << (8 * r);
+    *reinterpret_cast<uint32_t*>(p.o + (size_t)(s.t0 + i) * p.o_stride + (g * p.rep + r0) * HD + 16 * d + 4 * (lane >> 4)) = out;
 }
 
 struct Plan {
-    int mt, w, tiles, splits;
+    int mt, tiles, splits;
 };
 
-Plan plan(int tokens, int seqs, int64_t max_pos, int nh, int nkv, int hd) {
+Plan plan(int tokens, int seqs, int64_t max_pos, int nh, int nkv, int hd, int bits) {
     const int rep = nh / nkv;
     const int64_t each = ((int64_t)tokens * rep + seqs - 1) / std::max(seqs, 1);
     Plan x;
-    x.mt = each <= 16 ? 1 : (hd == 64 ? 4 : 2);
-    x.w = 8;
+    // as many columns as the registers hold beside a tile: a wave's loads serve them all
+    x.mt = each <= 16 ? 1 : (hd == 64 ? 4 : 2) / (bits == 8 ? 1 : 2);
     const int64_t tiles = (int64_t)tokens * rep / (16 * x.mt) + seqs;
     x.tiles = (int)tiles;
     const int64_t ctas = std::min<int64_t>(tiles, tokens) * nkv, work = (max_pos + 63) / 64;
-    x.splits = (int)std::max<int64_t>(1, std::min<int64_t>((512 + ctas - 1) / ctas, work / (2 * x.w)));
+    x.splits = (int)std::max<int64_t>(1, std::min<int64_t>((512 + ctas - 1) / ctas, work / (2 * PG_W)));
     if (ctas >= 256) x.splits = 1;
     return x;
 }
@@ -380,42 +423,47 @@ size_t ws_max_bytes(const Plan& x, int nkv) {
     return ((size_t)x.tiles * nkv * x.splits * 16 * x.mt * 4 + 255) / 256 * 256;
 }
 
-}  // namespace
-
-size_t pg_attend_workspace(int tokens, int seqs, int64_t max_pos, int nh, int nkv, int hd) {
-    const Plan x = plan(tokens, seqs, max_pos, nh, nkv, hd);
+size_t ws_bytes(const Plan& x, int nkv, int hd) {
     if (x.splits == 1) return 256;
     return ws_max_bytes(x, nkv) + (size_t)x.tiles * nkv * x.splits * 16 * x.mt * (hd + 1) * 8;
 }
 
-template <int HD, int BITS, int MT, int W>
-static hipError_t attend(const Paged& a, PgAttend p, const Plan& x, hipStream_t s) {
-    const dim3 grid((unsigned)(x.tiles * a.nkv), (unsigned)x.splits), block(64 * W);
+template <int HD, int BITS, int MT>
+hipError_t attend(const Paged& a, const PgAttend& p, const Plan& x, hipStream_t s) {
+    const dim3 grid((unsigned)(x.tiles * a.nkv), (unsigned)x.splits), block(64 * PG_W);
     if (x.splits == 1) {
-        pg_attend_kernel<HD, BITS, MT, W, PG_WHOLE><<<grid, block, 0, s>>>(a, p);
+        pg_attend_kernel<HD, BITS, MT, PG_W, PG_WHOLE><<<grid, block, 0, s>>>(a, p);
         return hipGetLastError();
     }
-    pg_attend_kernel<HD, BITS, MT, W, PG_MAX><<<grid, block, 0, s>>>(a, p);
+    pg_attend_kernel<HD, BITS, MT, PG_W, PG_MAX><<<grid, block, 0, s>>>(a, p);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    pg_attend_kernel<HD, BITS, MT, W, PG_SUMS><<<grid, block, 0, s>>>(a, p);
+    pg_attend_kernel<HD, BITS, MT, PG_W, PG_SUMS><<<grid, block, 0, s>>>(a, p);
     if ((e = hipGetLastError()) != hipSuccess) return e;
-    pg_join_kernel<HD, BITS, MT><<<dim3((unsigned)(x.tiles * a.nkv), MT), dim3(256), 0, s>>>(a, p);
+    pg_join_kernel<HD, BITS, MT><<<dim3((unsigned)(x.tiles * a.nkv), MT, HD / 64), dim3(1024), 0, s>>>(a, p);
     return hipGetLastError();
+}
+
+}  // namespace
+
+// bits is not known here: the layout's larger need
+size_t pg_attend_workspace(int tokens, int seqs, int64_t max_pos, int nh, int nkv, int hd) {
+    return std::max(ws_bytes(plan(tokens, seqs, max_pos, nh, nkv, hd, 8), nkv, hd),
+                    ws_bytes(plan(tokens, seqs, max_pos, nh, nkv, hd, 4), nkv, hd));
 }
 
 hipError_t launch_pg_attend(const Paged& a, int hd, int bits, const int8_t* q, int64_t q_stride, int nh,
                             const int32_t* exp_tab, int window, int sinks, int8_t* o, int64_t o_stride, void* ws,
                             hipStream_t s) {
-    const Plan x = plan(a.tokens, a.seqs, (int64_t)a.max_pages << a.page_sh, nh, a.nkv, hd);
+    const Plan x = plan(a.tokens, a.seqs, (int64_t)a.max_pages << a.page_sh, nh, a.nkv, hd, bits);
     const PgAttend p = {q, o, q_stride, o_stride, exp_tab, nh / a.nkv, window, sinks, x.splits, (int32_t*)ws,
                         (int64_t*)((char*)ws + ws_max_bytes(x, a.nkv))};
     if (hd == 64) {
-        if (x.mt == 1) return bits == 8 ? attend<64, 8, 1, 8>(a, p, x, s) : attend<64, 4, 1, 8>(a, p, x, s);
-        return bits == 8 ? attend<64, 8, 4, 8>(a, p, x, s) : attend<64, 4, 4, 8>(a, p, x, s);
+        if (x.mt == 1) return bits == 8 ? attend<64, 8, 1>(a, p, x, s) : attend<64, 4, 1>(a, p, x, s);
+        return bits == 8 ? attend<64, 8, 4>(a, p, x, s) : attend<64, 4, 2>(a, p, x, s);
     }
-    if (x.mt == 1) return bits == 8 ? attend<128, 8, 1, 8>(a, p, x, s) : attend<128, 4, 1, 8>(a, p, x, s);
-    return bits == 8 ? attend<128, 8, 2, 8>(a, p, x, s) : attend<128, 4, 2, 8>(a, p, x, s);
+    if (x.mt == 1) return bits == 8 ? attend<128, 8, 1>(a, p, x, s) : attend<128, 4, 1>(a, p, x, s);
+    return attend<128, 8, 2>(a, p, x, s);
 }
 
 }  // namespace kt
