@@ -21,11 +21,13 @@ struct PgAttend {
     int64_t q_stride, o_stride;
     const int32_t* exp_tab;
     int rep, window, sinks, splits;
-    int32_t* wmax;   // [tile][kv head][split][column]
-    int64_t* wsum;   // [tile][kv head][split][column group, 16 dimensions][register][lane], then the weights' sums
+    int keep;       // bytes of LDS for scores kept between the passes (PG_KEEP)
+    int32_t* wmax;  // [tile][kv head][split][column]
+    unsigned long long* wsum;  // [tile][kv head][column group, 16 dimensions][register][lane], then the weights' sums
+    unsigned* wcnt;            // [tile][kv head]
 };
 
-enum { PG_WHOLE = 0, PG_MAX = 1, PG_SUMS = 2 };
+enum { PG_WHOLE = 0, PG_MAX = 1, PG_SUMS = 2, PG_KEEP = 3 };
 
 // What a wave holds of a tile, 64 positions (four blocks of 16) of one kv head.
 //
@@ -45,10 +47,14 @@ struct PgChunk<4> {
 };
 
 template <int HD, int BITS>
-struct PgTile {
-    typedef typename PgChunk<BITS>::T Chunk;
-    Chunk raw[HD / 16], v[HD / 16];
-    v4i km, vm;  // 4 bits: the multipliers of block l / 16
+struct PgK {
+    typename PgChunk<BITS>::T raw[HD / 16];
+    v4i m;  // 4 bits: the multipliers of block l / 16
+};
+template <int HD, int BITS>
+struct PgV {
+    typename PgChunk<BITS>::T v[HD / 16];
+    v4i m;
 };
 
 // The swizzle of a row's chunks in the wave's LDS (row r of block n), by which the lanes that one LDS cycle serves (8 of 16
@@ -72,13 +78,17 @@ __device__ __forceinline__ void pg_store(int8_t* to, const int64_t (&v)[4], int6
 }
 
 template <int HD, int BITS, int MT, int WM, int WP, int MODE>
-__global__ __launch_bounds__(64 * WM * WP) void pg_attend_kernel(Paged a, PgAttend p) {
+#ifndef PG_EU
+#define PG_EU 2
+#endif
+__global__ __launch_bounds__(64 * WM * WP) __attribute__((amdgpu_waves_per_eu(PG_EU))) void pg_attend_kernel(Paged a, PgAttend p) {
     constexpr int HH = HD / 2, KC = HD / 64, DT = HD / 16, ND = BITS == 8 ? 2 : 3;
     constexpr int W = WM * WP, NT = 64 * W, CW = 16 * MT, COLS = CW * WM;  // threads; columns of a wave and of the CTA
     constexpr int NMAX = COLS * WP > NT ? WP : NT / COLS;
     constexpr int ROWB = BITS == 8 ? HD : HH, CHB = BITS == 8 ? 16 : 8;  // bytes of a K row of a slot, of a chunk
-    typedef PgTile<HD, BITS> Tile;
-    typedef typename Tile::Chunk Chunk;
+    typedef PgK<HD, BITS> Tile;
+    typedef PgV<HD, BITS> VTile;
+    typedef typename PgChunk<BITS>::T Chunk;
     constexpr bool MAXP = MODE != PG_SUMS, SUMP = MODE != PG_MAX;
     __shared__ int64_t sSum[SUMP && WP > 1 ? WM * MT * DT * 4 * 64 : 1];
     __shared__ int64_t sDen[SUMP ? COLS : 1];
@@ -87,19 +97,28 @@ __global__ __launch_bounds__(64 * WM * WP) void pg_attend_kernel(Paged a, PgAtte
     __shared__ __attribute__((aligned(16))) int8_t sK[W][64 * ROWB];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = w / WP, wp = w % WP, l16 = lane & 15, gq = lane >> 4, kb = (lane >> 2) & 3;
+    extern __shared__ __attribute__((aligned(16))) int sS[];  // PG_KEEP: the scores of each wave's first tiles
     const int split = (int)blockIdx.y;
     int et[(1024 + NT - 1) / NT];
     if constexpr (SUMP) {  // the table is on its way while the batch is looked up
 #pragma unroll
         for (int i = 0; i < (1024 + NT - 1) / NT; i++) et[i] = p.exp_tab[min(tid + i * NT, 1023)];
     }
-    // the kv head fastest: CTAs go to the XCDs in turn, so an XCD's L2 holds the heads congruent to it
-    const int tile = (int)(gridDim.x / a.nkv) - 1 - (int)blockIdx.x / a.nkv, g = (int)blockIdx.x % a.nkv;
-    int first = 0;
-    const int b = pg_tile_seq(a, tile, p.rep, COLS, 1, &first);
+    // The kv head fastest: CTAs go to the XCDs in turn, so an XCD's L2 holds the heads congruent to it. Numbers 0 .. seqs - 1
+    // are the sequences' first tiles, the rest their further ones (from the last: of a prompt's, those see the most), and a
+    // kind that may be empty comes last: single tokens have no further tiles, and CTAs that leave at once between others
+    // would leave the XCDs different numbers of those that stay (256 of them on 256 CUs took two rounds).
+    const int ntiles = (int)gridDim.x / a.nkv, g = (int)blockIdx.x % a.nkv, order = (int)blockIdx.x / a.nkv;
+    const int tile = WM * MT == 1 ? order : ntiles - 1 - order;
+    int b = tile, nth = 0;
+    if (tile >= a.seqs) {
+        int first = 0;
+        b = pg_tile_seq(a, tile - a.seqs, p.rep, COLS, 0, &first);
+        nth = tile - a.seqs - first + 1;
+    }
     if (b < 0) return;
     const PgRows s = pg_rows(a, b);
-    const int mc = (tile - first) * COLS, mrows = s.n * p.rep;  // m: row i, head r of the group as i rep + r
+    const int mc = nth * COLS, mrows = s.n * p.rep;  // m: row i, head r of the group as i rep + r
     if (mc >= mrows) return;
     const int m0 = mc + wm * CW, cols = max(0, min(CW, mrows - m0)), nmt = (cols + 15) / 16;  // this wave's columns
     const int cap = a.max_pages << a.page_sh, nblk = cap >> 4;
@@ -153,13 +172,13 @@ __global__ __launch_bounds__(64 * WM * WP) void pg_attend_kernel(Paged a, PgAtte
         const uint8_t* at = kbase + part_of(id) + (uint32_t)(slot_of(T) * ROWB);
 #pragma unroll
         for (int i = 0; i < DT; i++) x.raw[i] = *reinterpret_cast<const Chunk*>(at + 16 * CHB * i);
-        if constexpr (BITS == 4) x.km = *reinterpret_cast<const v4i*>(kmult + part_of(id) + (uint32_t)slot_of(T));
+        if constexpr (BITS == 4) x.m = *reinterpret_cast<const v4i*>(kmult + part_of(id) + (uint32_t)slot_of(T));
     };
-    auto load_v = [&](int T, int id, Tile& x) {
+    auto load_v = [&](int T, int id, VTile& x) {
         const uint8_t* at = vbase + part_of(id) + (uint32_t)(slot_of(T) * ROWB);
 #pragma unroll
         for (int d = 0; d < DT; d++) x.v[d] = *reinterpret_cast<const Chunk*>(at + 16 * CHB * d);
-        if constexpr (BITS == 4) x.vm = *reinterpret_cast<const v4i*>(vmult + part_of(id) + (uint32_t)slot_of(T));
+        if constexpr (BITS == 4) x.m = *reinterpret_cast<const v4i*>(vmult + part_of(id) + (uint32_t)slot_of(T));
     };
     int8_t* const sk = sK[w];
     auto turn_k = [&](const Tile& x, Chunk (&k)[4][KC]) {
@@ -216,11 +235,22 @@ __global__ __launch_bounds__(64 * WM * WP) void pg_attend_kernel(Paged a, PgAtte
     // Tiles start, start + step, ... go through a ring of tiles in registers. A tile's page ids are read a round of the ring
     // before its loads are issued, and those a round before they are used: a wave waits for neither.
     const int mine = start < total ? (total - 1 - start) / step + 1 : 0;
+    // PG_KEEP: as many of the wave's tiles as the LDS holds keep their scores, a column's 16 bytes at a time (lanes side by
+    // side); the others' are formed again from K, last tile first: its K is nearest.
+    const int kept = MODE == PG_KEEP ? min(mine, p.keep / (256 * WP * max(cols, 1))) : 0;
+    auto kept_place = [&](int n, int t) { return reinterpret_cast<v4i*>(sS) + (((n * WP + wp) * 4 + t) * 4 + gq) * cols + l16; };
+    auto keep_at = [&](int n, const v4i (&sc)[4]) {
+#pragma unroll
+        for (int t = 0; t < 4; t++) *kept_place(n, t) = sc[t];
+    };
+    constexpr int NV = MODE == PG_KEEP && HD == 64 ? 4 : 1;  // V's ring over the kept tiles, begun before the maximum is known
+    VTile xv[NV];
+    int idv[NV], nidv[NV];
+    auto at = [&](int n) { return tile_at(start + n * step); };
     if constexpr (MAXP) {
         constexpr int NB = MT * HD <= 64 ? 4 : 2;
         Tile x[NB];
         int id[NB], nid[NB];
-        auto at = [&](int n) { return tile_at(start + n * step); };
 #pragma unroll
         for (int u = 0; u < NB; u++) {
             id[u] = nid[u] = 0;
@@ -230,6 +260,14 @@ __global__ __launch_bounds__(64 * WM * WP) void pg_attend_kernel(Paged a, PgAtte
 #pragma unroll
         for (int u = 0; u < NB; u++)
             if (u < mine) load_k(at(u), id[u], x[u]);
+        if constexpr (MODE == PG_KEEP) {
+#pragma unroll
+            for (int u = 0; u < NV; u++) {
+                idv[u] = id[u], nidv[u] = 0;
+                if (u < kept) load_v(at(u), idv[u], xv[u]);
+                if (u + NV < kept) nidv[u] = page_id(at(u + NV));
+            }
+        }
         for (int n0 = 0; n0 < mine; n0 += NB) {
 #pragma unroll
             for (int u = 0; u < NB; u++) {
@@ -239,20 +277,26 @@ __global__ __launch_bounds__(64 * WM * WP) void pg_attend_kernel(Paged a, PgAtte
                 const bool ok = page_ok(T, id[u]), all = full(T, ok);
                 Chunk k[4][KC];
                 turn_k(x[u], k);
-                const v4i km = x[u].km;
+                const v4i km = x[u].m;
                 if (n + NB < mine) load_k(at(n + NB), nid[u], x[u]);
                 id[u] = nid[u];
                 if (n + 2 * NB < mine) nid[u] = page_id(at(n + 2 * NB));
+                if (all) {
 #pragma unroll
-                for (int mt = 0; mt < MT; mt++) {
-                    if (mt >= nmt) break;
-                    v4i sc[4];
-                    scores(k, km, mt, sc);
-                    if (all) {
+                    for (int mt = 0; mt < MT; mt++) {
+                        v4i sc[4];
+                        scores(k, km, mt, sc);
+                        if (MODE == PG_KEEP && n < kept && l16 < cols) keep_at(n, sc);
 #pragma unroll
                         for (int t = 0; t < 4; t++) mx[mt] = max(max(mx[mt], max(sc[t].x, sc[t].y)), max(sc[t].z, sc[t].w));
-                    } else {
-                        asm volatile("");  // keeps the masks out of the other tiles' path
+                    }
+                } else {
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++) {
+                        if (mt >= nmt) break;
+                        v4i sc[4];
+                        scores(k, km, mt, sc);
+                        if (MODE == PG_KEEP && n < kept && l16 < cols) keep_at(n, sc);
 #pragma unroll
                         for (int t = 0; t < 4; t++)
 #pragma unroll
@@ -270,11 +314,11 @@ __global__ __launch_bounds__(64 * WM * WP) void pg_attend_kernel(Paged a, PgAtte
                 if (gq == 0) sMax[wp][wm * CW + 16 * mt + l16] = mx[mt];
         }
     }
-    const size_t unit = ((size_t)tile * a.nkv + g) * p.splits;  // of the workspace's parts
+    const size_t unit = (size_t)tile * a.nkv + g;  // of the workspace's parts
     if constexpr (MODE == PG_SUMS) {  // the splits' maxima, each column's dealt to threads
         int m = INT_MIN;
         if (tid < NMAX * COLS)
-            for (int i = tid / COLS; i < p.splits; i += NMAX) m = max(m, p.wmax[(unit + i) * COLS + tid % COLS]);
+            for (int i = tid / COLS; i < p.splits; i += NMAX) m = max(m, p.wmax[(unit * p.splits + i) * COLS + tid % COLS]);
         if (tid < NMAX * COLS) sMax[tid / COLS][tid % COLS] = m;
     }
     __syncthreads();
@@ -283,8 +327,11 @@ __global__ __launch_bounds__(64 * WM * WP) void pg_attend_kernel(Paged a, PgAtte
             int m = sMax[0][c];
 #pragma unroll
             for (int i = 1; i < WP; i++) m = max(m, sMax[i][c]);
-            p.wmax[(unit + split) * COLS + c] = m;
+            p.wmax[(unit * p.splits + split) * COLS + c] = m;
         }
+        // and what the sums are added to starts from zero, each split clearing its share
+        for (int i = split * NT + tid; i < COLS * (HD + 1); i += p.splits * NT) p.wsum[unit * (size_t)(COLS * (HD + 1)) + i] = 0;
+        if (split == 0 && tid == 0) p.wcnt[unit] = 0;
         return;
     }
     if constexpr (MODE == PG_SUMS || WP > 1) {
@@ -305,72 +352,109 @@ __global__ __launch_bounds__(64 * WM * WP) void pg_attend_kernel(Paged a, PgAtte
 #pragma unroll
                 for (int n = 0; n < ND; n++) acc[mt][d][n] = v4i{0, 0, 0, 0};
         }
-        constexpr int NB = MT * HD <= 64 ? 2 : 1;
-        Tile x[NB];
-        int id[NB], nid[NB];
-        auto at = [&](int n) { return tile_at(start + (mine - 1 - n) * step); };  // from the end: its K is nearest
+        auto weights = [&](auto masked, int T, bool ok, v4i vm, int mt, const v4i (&sc)[4], v4i (&P)[ND]) {
 #pragma unroll
-        for (int u = 0; u < NB; u++) {
-            id[u] = nid[u] = 0;
-            if (u < mine) id[u] = page_id(at(u));
-            if (u + NB < mine) nid[u] = page_id(at(u + NB));
-        }
+            for (int t = 0; t < 4; t++) {
+                uint32_t e[4];
 #pragma unroll
-        for (int u = 0; u < NB; u++)
-            if (u < mine) load_k(at(u), id[u], x[u]), load_v(at(u), id[u], x[u]);
-        for (int n0 = 0; n0 < mine; n0 += NB) {
+                for (int r = 0; r < 4; r++) {
+                    uint32_t ix = min((uint32_t)(mx[mt] - sc[t][r]) >> 7, 1024u);
+                    if constexpr (masked) ix = ok & sees(64 * T + 16 * gq + 4 * t + r, pos[mt]) ? ix : 1024u;
+                    e[r] = sE[ix];
+                    if constexpr (BITS == 4) {  // the digits of e m
+                        den[mt][0] += (int)e[r];
+                        e[r] = (__umul24(e[r], ((uint32_t)vm[t] >> (8 * r)) & 255) + 0x808080) ^ 0x808080;
+                    }
+                }
+                const uint32_t e01 = __builtin_amdgcn_perm(e[1], e[0], 0x05010400), e23 = __builtin_amdgcn_perm(e[3], e[2], 0x05010400);
+                P[0][t] = (int)__builtin_amdgcn_perm(e23, e01, 0x05040100);
+                P[1][t] = (int)__builtin_amdgcn_perm(e23, e01, 0x07060302);
+                if constexpr (BITS == 4)
+                    P[ND - 1][t] = (int)__builtin_amdgcn_perm(__builtin_amdgcn_perm(e[3], e[2], 0x0c0c0602), __builtin_amdgcn_perm(e[1], e[0], 0x0c0c0602), 0x05040100);
+                if constexpr (BITS == 8) {
+                    den[mt][0] = __builtin_amdgcn_sdot4(P[0][t], 0x01010101, den[mt][0], false);
+                    den[mt][1] = __builtin_amdgcn_sdot4(P[1][t], 0x01010101, den[mt][1], false);
+                }
+            }
+        };
+        auto add_v = [&](const VTile& x, int mt, const v4i (&P)[ND]) {
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int e = 0; e < ND; e++) acc[mt][d][e] = mfma16(widen(x.v[d]), P[e], acc[mt][d][e]);
+        };
+        {
+            constexpr int NB = MT * HD <= 64 && MODE != PG_KEEP ? 2 : 1;
+            Tile x[NB];
+            VTile y[NB];
+            int id[NB], nid[NB];
+            const int left = mine - kept;
+            auto back = [&](int n) { return at(mine - 1 - n); };
 #pragma unroll
             for (int u = 0; u < NB; u++) {
-                const int n = n0 + u;
-                if (n >= mine) break;
-                const int T = at(n);
-                const bool ok = page_ok(T, id[u]), all = full(T, ok);
-                Chunk k[4][KC];
-                turn_k(x[u], k);
-                const v4i km = x[u].km, vm = x[u].vm;
-                if (n + NB < mine) load_k(at(n + NB), nid[u], x[u]);
+                id[u] = nid[u] = 0;
+                if (u < left) id[u] = page_id(back(u));
+                if (u + NB < left) nid[u] = page_id(back(u + NB));
+            }
 #pragma unroll
-                for (int mt = 0; mt < MT; mt++) {
-                    if (mt >= nmt) break;
-                    v4i sc[4], P[ND];
-                    scores(k, km, mt, sc);
-                    auto weights = [&](auto masked) {
-                        if constexpr (masked) asm volatile("");  // keeps the masks out of the other tiles' path
+            for (int u = 0; u < NB; u++)
+                if (u < left) load_k(back(u), id[u], x[u]), load_v(back(u), id[u], y[u]);
+            for (int n0 = 0; n0 < left; n0 += NB) {
 #pragma unroll
-                        for (int t = 0; t < 4; t++) {
-                            uint32_t e[4];
+                for (int u = 0; u < NB; u++) {
+                    const int n = n0 + u;
+                    if (n >= left) break;
+                    const int T = back(n);
+                    const bool ok = page_ok(T, id[u]), all = full(T, ok);
+                    Chunk k[4][KC];
+                    turn_k(x[u], k);
+                    const v4i km = x[u].m;
+                    if (n + NB < left) load_k(back(n + NB), nid[u], x[u]);
+                    if (BITS == 8 && all && nmt == MT) {  // one straight block: a group's lookups under the next one's products
+                        v4i sc[MT][4], P[MT][ND];
 #pragma unroll
-                            for (int r = 0; r < 4; r++) {
-                                uint32_t ix = min((uint32_t)(mx[mt] - sc[t][r]) >> 7, 1024u);
-                                if constexpr (masked) ix = ok & sees(64 * T + 16 * gq + 4 * t + r, pos[mt]) ? ix : 1024u;
-                                e[r] = sE[ix];
-                                if constexpr (BITS == 4) {  // the digits of e m
-                                    den[mt][0] += (int)e[r];
-                                    e[r] = (__umul24(e[r], ((uint32_t)vm[t] >> (8 * r)) & 255) + 0x808080) ^ 0x808080;
-                                }
-                            }
-                            const uint32_t e01 = __builtin_amdgcn_perm(e[1], e[0], 0x05010400), e23 = __builtin_amdgcn_perm(e[3], e[2], 0x05010400);
-                            P[0][t] = (int)__builtin_amdgcn_perm(e23, e01, 0x05040100);
-                            P[1][t] = (int)__builtin_amdgcn_perm(e23, e01, 0x07060302);
-                            if constexpr (BITS == 4)
-                                P[ND - 1][t] = (int)__builtin_amdgcn_perm(__builtin_amdgcn_perm(e[3], e[2], 0x0c0c0602), __builtin_amdgcn_perm(e[1], e[0], 0x0c0c0602), 0x05040100);
-                            if constexpr (BITS == 8) {
-                                den[mt][0] = __builtin_amdgcn_sdot4(P[0][t], 0x01010101, den[mt][0], false);
-                                den[mt][1] = __builtin_amdgcn_sdot4(P[1][t], 0x01010101, den[mt][1], false);
-                            }
+                        for (int mt = 0; mt < MT; mt++) scores(k, km, mt, sc[mt]);
+#pragma unroll
+                        for (int mt = 0; mt < MT; mt++) weights(std::false_type(), T, ok, y[u].m, mt, sc[mt], P[mt]);
+#pragma unroll
+                        for (int mt = 0; mt < MT; mt++) add_v(y[u], mt, P[mt]);
+                    } else {
+#pragma unroll
+                        for (int mt = 0; mt < MT; mt++) {
+                            if (mt >= nmt) break;
+                            v4i sc[4], P[ND];
+                            scores(k, km, mt, sc);
+                            if (BITS == 4 && all) weights(std::false_type(), T, ok, y[u].m, mt, sc, P);
+                            else weights(std::true_type(), T, ok, y[u].m, mt, sc, P);
+                            add_v(y[u], mt, P);
                         }
-                    };
-                    if (all) weights(std::false_type());
-                    else weights(std::true_type());
-#pragma unroll
-                    for (int d = 0; d < DT; d++)
-#pragma unroll
-                        for (int e = 0; e < ND; e++)
-                            acc[mt][d][e] = mfma16(widen(x[u].v[d]), P[e], acc[mt][d][e]);
+                    }
+                    if (n + NB < left) load_v(back(n + NB), nid[u], y[u]);
+                    id[u] = nid[u];
+                    if (n + 2 * NB < left) nid[u] = page_id(back(n + 2 * NB));
                 }
-                if (n + NB < mine) load_v(at(n + NB), nid[u], x[u]);
-                id[u] = nid[u];
-                if (n + 2 * NB < mine) nid[u] = page_id(at(n + 2 * NB));
+            }
+        }
+        if constexpr (MODE == PG_KEEP) {
+            for (int n0 = 0; n0 < kept; n0 += NV) {
+#pragma unroll
+                for (int u = 0; u < NV; u++) {
+                    const int n = n0 + u;
+                    if (n >= kept) break;
+                    const int T = at(n);
+                    const bool ok = page_ok(T, idv[u]), all = full(T, ok);
+                    v4i sc[4] = {}, P[ND];
+                    if (l16 < cols) {
+#pragma unroll
+                        for (int t = 0; t < 4; t++) sc[t] = *kept_place(n, t);
+                    }
+                    if (all) weights(std::false_type(), T, ok, xv[u].m, 0, sc, P);
+                    else weights(std::true_type(), T, ok, xv[u].m, 0, sc, P);
+                    add_v(xv[u], 0, P);
+                    if (n + NV < kept) load_v(at(n + NV), nidv[u], xv[u]);
+                    idv[u] = nidv[u];
+                    if (n + 2 * NV < kept) nidv[u] = page_id(at(n + 2 * NV));
+                }
             }
         }
         // register r of lane l is dimension 16 d + 4 (l / 16) + r of column l % 16
@@ -380,20 +464,28 @@ __global__ __launch_bounds__(64 * WM * WP) void pg_attend_kernel(Paged a, PgAtte
             return v;
         };
         auto den_of = [&](int mt) { return BITS == 8 ? (int64_t)den[mt][0] + ((int64_t)den[mt][1] << 8) : (int64_t)den[mt][0]; };
-        int64_t* const to = p.wsum + ((unit + split) * WM) * (size_t)(CW * (HD + 1));
-        // four dimensions of column c of wave group gm: to the output, or to this split's part of the workspace
-        auto give = [&](int gm, int mt, int d, int ln, const int64_t (&v)[4], int64_t dn) {
-            const int c = 16 * mt + (ln & 15), m = mc + gm * CW + c;
-            if constexpr (MODE == PG_SUMS) {
-                int64_t* x = to + (size_t)gm * (CW * (HD + 1));
-#pragma unroll
-                for (int r = 0; r < 4; r++) x[((mt * DT + d) * 4 + r) * 64 + ln] = v[r];
-                if (d == 0 && ln < 16) x[CW * HD + c] = dn;
-            } else if (m < mrows) {
-                const int i = m / p.rep, r0 = m - i * p.rep, pp = s.p0 + i;
+        unsigned long long* const sum = p.wsum + unit * (size_t)(COLS * (HD + 1));
+        auto place = [&](int cg, int d, int r, int ln) { return sum + ((cg * DT + d) * 4 + r) * 64 + ln; };
+        auto put = [&](int cg, int d, int ln, const int64_t (&v)[4], int64_t dn) {
+            const int m = mc + 16 * cg + (ln & 15), i = m / p.rep, r0 = m - i * p.rep, pp = s.p0 + i;
+            if (m < mrows)
                 pg_store<BITS>(p.o + (size_t)(s.t0 + i) * p.o_stride + (g * p.rep + r0) * HD + 16 * d + 4 * (ln >> 4), v, dn, pp >= 0 && pp < cap);
+        };
+        // four dimensions of a column (lane ln of 16 columns cg): to the output, or added to the other splits'
+        auto give = [&](int cg, int d, int ln, const int64_t (&v)[4], int64_t dn) {
+            if constexpr (MODE == PG_SUMS) {
+                if (mc + 16 * cg + (ln & 15) < mrows) {
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        (void)__hip_atomic_fetch_add(place(cg, d, r, ln), (unsigned long long)v[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    if (d == 0 && ln < 16)
+                        (void)__hip_atomic_fetch_add(sum + COLS * HD + 16 * cg + ln, (unsigned long long)dn, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                }
+            } else {
+                put(cg, d, ln, v, dn);
             }
         };
+        const int groups = min((mrows - mc + 15) / 16, COLS / 16);
         if constexpr (WP == 1) {
 #pragma unroll
             for (int mt = 0; mt < MT; mt++) {
@@ -404,7 +496,7 @@ __global__ __launch_bounds__(64 * WM * WP) void pg_attend_kernel(Paged a, PgAtte
 #pragma unroll
                 for (int d = 0; d < DT; d++) {
                     const int64_t v[4] = {total_of(mt, d, 0), total_of(mt, d, 1), total_of(mt, d, 2), total_of(mt, d, 3)};
-                    give(wm, mt, d, lane, v, dn);
+                    give(wm * MT + mt, d, lane, v, dn);
                 }
             }
         } else {
@@ -422,56 +514,25 @@ __global__ __launch_bounds__(64 * WM * WP) void pg_attend_kernel(Paged a, PgAtte
                 }
             }
             __syncthreads();
-            const int groups = min((mrows - mc + 15) / 16, COLS / 16);
             for (int it = tid; it < groups * DT * 64; it += NT) {
                 const int cg = it / (DT * 64), d = it / 64 % DT, ln = it & 63;
                 int64_t v[4];
 #pragma unroll
                 for (int r = 0; r < 4; r++) v[r] = sSum[((cg * DT + d) * 4 + r) * 64 + ln];
-                give(cg / MT, cg % MT, d, ln, v, sDen[16 * cg + (ln & 15)]);
+                give(cg, d, ln, v, sDen[16 * cg + (ln & 15)]);
+            }
+        }
+        if constexpr (MODE == PG_SUMS) {  // the tile's last CTA has every split's sums
+            if (!split_last(p.wcnt + unit)) return;
+            for (int it = tid; it < groups * DT * 64; it += NT) {
+                const int cg = it / (DT * 64), d = it / 64 % DT, ln = it & 63;
+                int64_t v[4];
+#pragma unroll
+                for (int r = 0; r < 4; r++) v[r] = (int64_t)__hip_atomic_load(place(cg, d, r, ln), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                put(cg, d, ln, v, (int64_t)__hip_atomic_load(sum + COLS * HD + 16 * cg + (ln & 15), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
             }
         }
     }
-}
-
-// The splits' sums joined: one CTA per (tile, kv head, 16 columns, 16 dimensions), the splits dealt to its waves.
-template <int HD, int BITS, int MT, int WM>
-__global__ __launch_bounds__(512) void pg_join_kernel(Paged a, PgAttend p) {
-    constexpr int CW = 16 * MT, COLS = CW * WM, DT = HD / 16;
-    __shared__ int64_t sV[8][5][64];
-    const int tile = (int)blockIdx.x / a.nkv, g = (int)blockIdx.x % a.nkv, cg = blockIdx.y, d = blockIdx.z;
-    const int lane = threadIdx.x & 63, share = threadIdx.x >> 6, shares = blockDim.x >> 6;
-    int first = 0;
-    const int b = pg_tile_seq(a, tile, p.rep, COLS, 1, &first);
-    if (b < 0) return;
-    const PgRows s = pg_rows(a, b);
-    const int m = (tile - first) * COLS + 16 * cg + (lane & 15), mrows = s.n * p.rep;
-    if (m - (lane & 15) >= mrows) return;
-    const size_t part = CW * (HD + 1);
-    const int64_t* from = p.wsum + (((size_t)tile * a.nkv + g) * p.splits * WM + cg / MT) * part;
-    int64_t v[4] = {0, 0, 0, 0}, dn = 0;
-    if (m < mrows) {
-#pragma unroll 8
-        for (int i = share; i < p.splits; i += shares) {
-            const int64_t* x = from + (size_t)i * (WM * part);
-#pragma unroll
-            for (int r = 0; r < 4; r++) v[r] += x[(((cg % MT) * DT + d) * 4 + r) * 64 + lane];
-            dn += x[CW * HD + 16 * (cg % MT) + (lane & 15)];
-        }
-    }
-#pragma unroll
-    for (int r = 0; r < 4; r++) sV[share][r][lane] = v[r];
-    sV[share][4][lane] = dn;
-    __syncthreads();
-    if (share || m >= mrows) return;
-    for (int k = 1; k < shares; k++) {
-#pragma unroll
-        for (int r = 0; r < 4; r++) v[r] += sV[k][r][lane];
-        dn += sV[k][4][lane];
-    }
-    const int i = m / p.rep, r0 = m - i * p.rep, pp = s.p0 + i;
-    pg_store<BITS>(p.o + (size_t)(s.t0 + i) * p.o_stride + (g * p.rep + r0) * HD + 16 * d + 4 * (lane >> 4), v, dn,
-                   pp >= 0 && pp < a.max_pages << a.page_sh);
 }
 
 struct Plan {
@@ -485,7 +546,7 @@ Plan plan(int tokens, int seqs, int64_t max_pos, int nh, int nkv, int hd, int bi
     const int64_t each = ((int64_t)tokens * rep + seqs - 1) / std::max(seqs, 1);
     Plan x;
     if (each <= 16) x.mt = x.wm = 1, x.wp = 8;
-    else x.mt = hd == 64 ? 2 : 1, x.wm = tune("PGT_WM", 4), x.wp = 8 / x.wm;
+    else x.mt = hd == 64 ? 2 : 1, x.wm = tune("PGT_WM", 4), x.wp = tune("PGT_WP", 2);
     const int64_t cols = 16 * x.mt * x.wm, tiles = (int64_t)tokens * rep / cols + seqs;
     x.tiles = (int)tiles;
     const int64_t ctas = std::min<int64_t>(tiles, tokens) * nkv, work = (max_pos + 63) / 64;
@@ -495,30 +556,33 @@ Plan plan(int tokens, int seqs, int64_t max_pos, int nh, int nkv, int hd, int bi
     return x;
 }
 
-size_t ws_max_bytes(const Plan& x, int nkv) {
-    return ((size_t)x.tiles * nkv * x.splits * 16 * x.mt * x.wm * 4 + 255) / 256 * 256;
-}
+// The workspace's parts: the splits' maxima, the sums, the counts of arrived splits.
+struct Parts {
+    size_t sum, cnt, bytes;
+};
 
-size_t ws_bytes(const Plan& x, int nkv, int hd) {
-    if (x.splits == 1) return 256;
-    return ws_max_bytes(x, nkv) + (size_t)x.tiles * nkv * x.splits * 16 * x.mt * x.wm * (hd + 1) * 8;
+Parts parts(const Plan& x, int nkv, int hd) {
+    if (x.splits == 1) return {0, 0, 256};
+    const size_t units = (size_t)x.tiles * nkv, cols = 16 * x.mt * x.wm;
+    const size_t sum = (units * x.splits * cols * 4 + 255) / 256 * 256, cnt = sum + units * cols * (hd + 1) * 8;
+    return {sum, cnt, cnt + (units * 4 + 255) / 256 * 256};
 }
 
 template <int HD, int BITS, int MT, int WM, int WP>
-hipError_t attend(const Paged& a, const PgAttend& p, const Plan& x, hipStream_t s) {
+hipError_t attend(const Paged& a, PgAttend p, const Plan& x, hipStream_t s) {
     const dim3 grid((unsigned)(x.tiles * a.nkv), (unsigned)x.splits), block(64 * WM * WP);
     if (x.splits == 1) {
-        pg_attend_kernel<HD, BITS, MT, WM, WP, PG_WHOLE><<<grid, block, 0, s>>>(a, p);
+        if constexpr (MT == 1 && WM == 1) {
+            pg_attend_kernel<HD, BITS, MT, WM, WP, PG_KEEP><<<grid, block, (size_t)p.keep, s>>>(a, p);
+        } else {
+            pg_attend_kernel<HD, BITS, MT, WM, WP, PG_WHOLE><<<grid, block, 0, s>>>(a, p);
+        }
         return hipGetLastError();
     }
     pg_attend_kernel<HD, BITS, MT, WM, WP, PG_MAX><<<grid, block, 0, s>>>(a, p);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     pg_attend_kernel<HD, BITS, MT, WM, WP, PG_SUMS><<<grid, block, 0, s>>>(a, p);
-    if ((e = hipGetLastError()) != hipSuccess) return e;
-    int shares = 1;
-    while (shares < 8 && 2 * shares <= x.splits) shares *= 2;
-    pg_join_kernel<HD, BITS, MT, WM><<<dim3((unsigned)(x.tiles * a.nkv), MT * WM, HD / 16), dim3(64 * shares), 0, s>>>(a, p);
     return hipGetLastError();
 }
 
@@ -526,26 +590,33 @@ template <int HD, int BITS>
 hipError_t attend_by(const Paged& a, const PgAttend& p, const Plan& x, hipStream_t s) {
     constexpr int MT = HD == 64 ? 2 : 1;
     if (x.mt == 1 && x.wm == 1) return attend<HD, BITS, 1, 1, 8>(a, p, x, s);
-    if (x.wm == 1) return attend<HD, BITS, MT, 1, 8>(a, p, x, s);
-    if (x.wm == 2) return attend<HD, BITS, MT, 2, 4>(a, p, x, s);
-    if (x.wm == 4) return attend<HD, BITS, MT, 4, 2>(a, p, x, s);
-    return attend<HD, BITS, MT, 8, 1>(a, p, x, s);
+    if (x.wm == 1 && x.wp == 4) return attend<HD, BITS, MT, 1, 4>(a, p, x, s);
+    if (x.wm == 2 && x.wp == 2) return attend<HD, BITS, MT, 2, 2>(a, p, x, s);
+    if (x.wm == 4 && x.wp == 1) return attend<HD, BITS, MT, 4, 1>(a, p, x, s);
+    if (x.wm == 2 && x.wp == 4) return attend<HD, BITS, MT, 2, 4>(a, p, x, s);
+    return attend<HD, BITS, MT, 4, 2>(a, p, x, s);
 }
 
 }  // namespace
 
 // bits is not known here: the layout's larger need
 size_t pg_attend_workspace(int tokens, int seqs, int64_t max_pos, int nh, int nkv, int hd) {
-    return std::max(ws_bytes(plan(tokens, seqs, max_pos, nh, nkv, hd, 8), nkv, hd),
-                    ws_bytes(plan(tokens, seqs, max_pos, nh, nkv, hd, 4), nkv, hd));
+    return std::max(parts(plan(tokens, seqs, max_pos, nh, nkv, hd, 8), nkv, hd).bytes,
+                    parts(plan(tokens, seqs, max_pos, nh, nkv, hd, 4), nkv, hd).bytes);
 }
 
 hipError_t launch_pg_attend(const Paged& a, int hd, int bits, const int8_t* q, int64_t q_stride, int nh,
                             const int32_t* exp_tab, int window, int sinks, int8_t* o, int64_t o_stride, void* ws,
                             hipStream_t s) {
-    const Plan x = plan(a.tokens, a.seqs, (int64_t)a.max_pages << a.page_sh, nh, a.nkv, hd, bits);
-    const PgAttend p = {q, o, q_stride, o_stride, exp_tab, nh / a.nkv, window, sinks, x.splits, (int32_t*)ws,
-                        (int64_t*)((char*)ws + ws_max_bytes(x, a.nkv))};
+    const int64_t max_pos = (int64_t)a.max_pages << a.page_sh;
+    const Plan x = plan(a.tokens, a.seqs, max_pos, nh, a.nkv, hd, bits);
+    const Parts w = parts(x, a.nkv, hd);
+    const int rep = nh / a.nkv, cols = a.tokens > a.seqs ? 16 : std::min(rep, 16);
+    // kept scores: 256 bytes a column and tile, as far as a CTA's LDS (160 KB) goes beside its static arrays
+    const int64_t room = 163840 - 12288 - 8 * 64 * (bits == 8 ? hd : hd / 2) - hd * 128;
+    const int64_t keep = std::min<int64_t>((max_pos / 64 + x.wp) / x.wp * x.wp * cols * 256, tune("PGT_KEEP", (int)room));
+    const PgAttend p = {q, o, q_stride, o_stride, exp_tab, rep, window, sinks, x.splits, (int)keep, (int32_t*)ws,
+                        (unsigned long long*)((char*)ws + w.sum), (unsigned*)((char*)ws + w.cnt)};
     if (hd == 64) return bits == 8 ? attend_by<64, 8>(a, p, x, s) : attend_by<64, 4>(a, p, x, s);
     return bits == 8 ? attend_by<128, 8>(a, p, x, s) : attend_by<128, 4>(a, p, x, s);
 }
