@@ -888,7 +888,7 @@ int kt_hip_dec_kv_read_paged(int dev, const void* kpool_dev, const void* vpool_d
 /* Causal GQA attention of the new rows (chunks and single tokens alike) over their sequences' pages, rows of q_dev as
  * kt_hip_dec_rope_kv_paged leaves them, after the call that wrote the rows' own k and v. A row at p sees the positions
  * j <= p that have a page and, with window >= 1, are within it (j > p - window) or among the first `sinks`; window = 0
- * sees all. s_j = q . k_j (4 bits: (m_j (q . c_j) + 4) >> 3), e_j = exp_tab[(max s - s_j + 64) >> 7] with entries clamped
+ * sees all. s_j = q . k_j (q of -128, which RoPE never gives, as -127; 4 bits: (m_j (q . c_j) + 4) >> 3), e_j = exp_tab[(max s - s_j + 64) >> 7] with entries clamped
  * to [0, 2^15] and 0 past the 1024th, o = clamp(round_half_away(sum e_j v_j / sum e_j)), 0 where the sum of e is 0.
  * ws_dev: kt_hip_dec_attention_paged_workspace bytes of scratch, 16-byte aligned, needing no contents; calls that may
  * overlap need one each. */

@@ -160,7 +160,7 @@ void kt_pg_attend(const kt_pg* P, const int8_t* q, int64_t q_stride, int64_t nh,
                     e[j] = INT64_MIN;
                     if (!pk || (window && j <= p - window && j >= sinks)) continue;
                     int64_t s = 0;
-                    for (int64_t d = 0; d < hd; d++) s += (int64_t)qr[d] * get_code(P, pk, 0, j % P->page, d);
+                    for (int64_t d = 0; d < hd; d++) s += clampv(qr[d], -127, 127) * get_code(P, pk, 0, j % P->page, d);
                     if (P->bits == 4) {
                         s = s * get_mult(P, pk, j % P->page) + 4;
                         s = s >= 0 ? s / 8 : -((-s + 7) / 8); /* floor */

@@ -15,6 +15,8 @@ namespace kt {
 
 namespace {
 
+typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+
 struct PgAttend {
     const int8_t* q;
     int8_t* o;
@@ -22,7 +24,7 @@ struct PgAttend {
     const int32_t* exp_tab;
     int rep, window, sinks, splits;
     int keep;       // bytes of LDS for scores kept between the passes (PG_KEEP)
-    int32_t* wmax;  // [tile][kv head][split][column]
+    int32_t* wlow;  // [tile][kv head][split][column]: the least negated scores
     unsigned long long* wsum;  // [tile][kv head][column group, 16 dimensions][register][lane], then the weights' sums
     unsigned* wcnt;            // [tile][kv head]
 };
@@ -57,6 +59,18 @@ struct PgV {
     v4i m;
 };
 
+// -x of 16 int8 values, -128 taken as -127. A byte of sign h and low bits lo: 2^7 - lo takes no borrow from its neighbours and
+// reaches 2^7 where lo is 0, that is for 0 and -128.
+__device__ __forceinline__ v4i negate8(v4i x) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t u = (uint32_t)x[i], h = u & 0x80808080u, t = 0x80808080u - (u & 0x7F7F7F7Fu);
+        const uint32_t z = t & 0x80808080u, least = h & z;
+        x[i] = (int)((t & 0x7F7F7F7Fu) | (~(h | z) & 0x80808080u) | (least - (least >> 7)));
+    }
+    return x;
+}
+
 // The swizzle of a row's chunks in the wave's LDS (row r of block n), by which the lanes that one LDS cycle serves (8 of 16
 // bytes, 16 of 8: rows 4 t .. 4 t + 3 of two or four blocks) read different banks.
 template <int HD, int BITS>
@@ -66,14 +80,25 @@ __device__ __forceinline__ int pg_swz(int n, int r) {
 }
 
 // Four neighbouring dimensions of an output row: clamp(round_half_away(sum e v / sum e)) of what the digits add up to (8
-// bits: both negated; 4 bits: v as 16 codes times 1/8 of a multiplier), zeros where nothing was seen.
+// bits: both negated; 4 bits: v as 16 codes times 1/8 of a multiplier), zeros where nothing was seen. The quotients
+// floor((2 |a| + b) / (2 b)) are double estimates by one reciprocal (within one of the exact quotient, which is below 2^8 past
+// the first test) and the exact remainders.
 template <int BITS>
 __device__ __forceinline__ void pg_store(int8_t* to, const int64_t (&v)[4], int64_t dn, bool live) {
-    dn = BITS == 8 ? -dn : 128 * dn;
+    const uint64_t b = (uint64_t)(BITS == 8 ? -dn : 128 * dn), d = 2 * b;
+    const double rd = 1.0 / (double)d;
     uint32_t out = 0;
-    if (live && dn > 0)
+    if (live && (int64_t)b > 0)
 #pragma unroll
-        for (int r = 0; r < 4; r++) out |= (uint32_t)(uint8_t)div_round_q8(BITS == 8 ? -v[r] : v[r], dn) << (8 * r);
+        for (int r = 0; r < 4; r++) {
+            const int64_t a = BITS == 8 ? -v[r] : v[r];
+            const uint64_t m = a < 0 ? 0 - (uint64_t)a : (uint64_t)a, n = 2 * m + b;
+            int q = (int)((double)n * rd);
+            const int64_t rem = (int64_t)(n - (uint64_t)(uint32_t)q * d);
+            q += rem < 0 ? -1 : (rem >= (int64_t)d ? 1 : 0);
+            q = m >= 128 * b || q > 127 ? 127 : q;
+            out |= (uint32_t)(uint8_t)(a < 0 ? -q : q) << (8 * r);
+        }
     *reinterpret_cast<uint32_t*>(to) = out;
 }
 
@@ -92,7 +117,7 @@ __global__ __launch_bounds__(64 * WM * WP) __attribute__((amdgpu_waves_per_eu(PG
     constexpr bool MAXP = MODE != PG_SUMS, SUMP = MODE != PG_MAX;
     __shared__ int64_t sSum[SUMP && WP > 1 ? WM * MT * DT * 4 * 64 : 1];
     __shared__ int64_t sDen[SUMP ? COLS : 1];
-    __shared__ int sMax[NMAX][COLS];
+    __shared__ int sLow[NMAX][COLS];
     __shared__ uint16_t sE[1026];
     __shared__ __attribute__((aligned(16))) int8_t sK[W][64 * ROWB];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -136,7 +161,7 @@ __global__ __launch_bounds__(64 * WM * WP) __attribute__((amdgpu_waves_per_eu(PG
     const uint8_t *const kbase = a.k + (size_t)g * a.part + l16 * CHB, *const vbase = a.v + (size_t)g * a.part + l16 * CHB;
     const uint8_t *const kmult = a.k + (size_t)g * a.part + (HH << a.page_sh), *const vmult = a.v + (size_t)g * a.part + (HH << a.page_sh);
 
-    // the columns' rows and positions, and their q as B operands
+    // the columns' rows and positions, and their negated q as B operands
     int pos[MT];
     v4i q[MT][KC];
 #pragma unroll
@@ -145,7 +170,7 @@ __global__ __launch_bounds__(64 * WM * WP) __attribute__((amdgpu_waves_per_eu(PG
         pos[mt] = 16 * mt + l16 < cols && s.p0 + i < cap ? s.p0 + i : -1;
         const int8_t* qr = p.q + (size_t)(s.t0 + i) * p.q_stride + (g * p.rep + r) * HD + 16 * gq;
 #pragma unroll
-        for (int c = 0; c < KC; c++) q[mt][c] = *reinterpret_cast<const v4i*>(qr + 64 * c);
+        for (int c = 0; c < KC; c++) q[mt][c] = negate8(*reinterpret_cast<const v4i*>(qr + 64 * c));
     }
     if constexpr (SUMP) {
 #pragma unroll
@@ -207,7 +232,7 @@ __global__ __launch_bounds__(64 * WM * WP) __attribute__((amdgpu_waves_per_eu(PG
             return v4i{(x.x << 4) & M, x.x & M, (x.y << 4) & M, x.y & M};
         }
     };
-    // the scores of column group mt: register r of s[t] is position 16 gq + 4 t + r of the tile
+    // the negated scores of column group mt: register r of sc[t] is position 16 gq + 4 t + r of the tile
     auto scores = [&](const Chunk (&k)[4][KC], v4i km, int mt, v4i (&sc)[4]) {
 #pragma unroll
         for (int t = 0; t < 4; t++) {
@@ -216,8 +241,8 @@ __global__ __launch_bounds__(64 * WM * WP) __attribute__((amdgpu_waves_per_eu(PG
             for (int c = 0; c < KC; c++) sc[t] = mfma16(widen(k[t][c]), q[mt][c], sc[t]);
             if constexpr (BITS == 4) {
 #pragma unroll
-                for (int r = 0; r < 4; r++)  // (m (q . c) + 4) >> 3 of 16 (q . c)
-                    sc[t][r] = (__mul24(sc[t][r], (km[t] >> (8 * r)) & 255) + 64) >> 7;
+                for (int r = 0; r < 4; r++)  // -((m (q . c) + 4) >> 3) of -16 (q . c)
+                    sc[t][r] = (__mul24(sc[t][r], (km[t] >> (8 * r)) & 255) + 63) >> 7;
             }
         }
     };
@@ -229,9 +254,9 @@ __global__ __launch_bounds__(64 * WM * WP) __attribute__((amdgpu_waves_per_eu(PG
     auto page_ok = [&](int T, int id) { return (unsigned)id < (unsigned)a.pages && 4 * T + gq < nblk; };
 
     const int step = p.splits * WP, start = split * WP + wp;
-    int mx[MT];
+    int low[MT];  // the least negated score of the columns
 #pragma unroll
-    for (int mt = 0; mt < MT; mt++) mx[mt] = INT_MIN;
+    for (int mt = 0; mt < MT; mt++) low[mt] = INT_MAX;
     // Tiles start, start + step, ... go through a ring of tiles in registers. A tile's page ids are read a round of the ring
     // before its loads are issued, and those a round before they are used: a wave waits for neither.
     const int mine = start < total ? (total - 1 - start) / step + 1 : 0;
@@ -288,7 +313,7 @@ __global__ __launch_bounds__(64 * WM * WP) __attribute__((amdgpu_waves_per_eu(PG
                         scores(k, km, mt, sc);
                         if (MODE == PG_KEEP && n < kept && l16 < cols) keep_at(n, sc);
 #pragma unroll
-                        for (int t = 0; t < 4; t++) mx[mt] = max(max(mx[mt], max(sc[t].x, sc[t].y)), max(sc[t].z, sc[t].w));
+                        for (int t = 0; t < 4; t++) low[mt] = min(min(low[mt], min(sc[t].x, sc[t].y)), min(sc[t].z, sc[t].w));
                     }
                 } else {
 #pragma unroll
@@ -301,33 +326,33 @@ __global__ __launch_bounds__(64 * WM * WP) __attribute__((amdgpu_waves_per_eu(PG
                         for (int t = 0; t < 4; t++)
 #pragma unroll
                             for (int r = 0; r < 4; r++)
-                                mx[mt] = max(mx[mt], ok & sees(64 * T + 16 * gq + 4 * t + r, pos[mt]) ? sc[t][r] : INT_MIN);
+                                low[mt] = min(low[mt], ok & sees(64 * T + 16 * gq + 4 * t + r, pos[mt]) ? sc[t][r] : INT_MAX);
                     }
                 }
             }
         }
 #pragma unroll
         for (int mt = 0; mt < MT; mt++) {
-            mx[mt] = max(mx[mt], __shfl_xor(mx[mt], 16));
-            mx[mt] = max(mx[mt], __shfl_xor(mx[mt], 32));
+            low[mt] = min(low[mt], __shfl_xor(low[mt], 16));
+            low[mt] = min(low[mt], __shfl_xor(low[mt], 32));
             if (WP > 1 || MODE == PG_MAX)
-                if (gq == 0) sMax[wp][wm * CW + 16 * mt + l16] = mx[mt];
+                if (gq == 0) sLow[wp][wm * CW + 16 * mt + l16] = low[mt];
         }
     }
     const size_t unit = (size_t)tile * a.nkv + g;  // of the workspace's parts
-    if constexpr (MODE == PG_SUMS) {  // the splits' maxima, each column's dealt to threads
-        int m = INT_MIN;
+    if constexpr (MODE == PG_SUMS) {  // the splits' least, each column's dealt to threads
+        int m = INT_MAX;
         if (tid < NMAX * COLS)
-            for (int i = tid / COLS; i < p.splits; i += NMAX) m = max(m, p.wmax[(unit * p.splits + i) * COLS + tid % COLS]);
-        if (tid < NMAX * COLS) sMax[tid / COLS][tid % COLS] = m;
+            for (int i = tid / COLS; i < p.splits; i += NMAX) m = min(m, p.wlow[(unit * p.splits + i) * COLS + tid % COLS]);
+        if (tid < NMAX * COLS) sLow[tid / COLS][tid % COLS] = m;
     }
     __syncthreads();
     if constexpr (MODE == PG_MAX) {
         for (int c = tid; c < COLS; c += NT) {
-            int m = sMax[0][c];
+            int m = sLow[0][c];
 #pragma unroll
-            for (int i = 1; i < WP; i++) m = max(m, sMax[i][c]);
-            p.wmax[(unit * p.splits + split) * COLS + c] = m;
+            for (int i = 1; i < WP; i++) m = min(m, sLow[i][c]);
+            p.wlow[(unit * p.splits + split) * COLS + c] = m;
         }
         // and what the sums are added to starts from zero, each split clearing its share
         for (int i = split * NT + tid; i < COLS * (HD + 1); i += p.splits * NT) p.wsum[unit * (size_t)(COLS * (HD + 1)) + i] = 0;
@@ -338,43 +363,79 @@ __global__ __launch_bounds__(64 * WM * WP) __attribute__((amdgpu_waves_per_eu(PG
 #pragma unroll
         for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-            for (int i = 0; i < (MODE == PG_SUMS ? NMAX : WP); i++) mx[mt] = max(mx[mt], sMax[i][wm * CW + 16 * mt + l16]);
+            for (int i = 0; i < (MODE == PG_SUMS ? NMAX : WP); i++) low[mt] = min(low[mt], sLow[i][wm * CW + 16 * mt + l16]);
     }
     if constexpr (SUMP) {
         v4i acc[MT][DT][ND];
-        int den[MT][2];
+        int den[MT][2], top[MT];
 #pragma unroll
         for (int mt = 0; mt < MT; mt++) {
-            mx[mt] = (mx[mt] == INT_MIN ? 0 : mx[mt]) + 64;  // of a column that sees nothing every weight is masked
+            // 2 (max + 64); of a column that sees nothing every weight is masked
+            top[mt] = 128 - 2 * (low[mt] == INT_MAX ? 0 : low[mt]);
             den[mt][0] = den[mt][1] = 0;
 #pragma unroll
             for (int d = 0; d < DT; d++)
 #pragma unroll
                 for (int n = 0; n < ND; n++) acc[mt][d][n] = v4i{0, 0, 0, 0};
         }
-        auto weights = [&](auto masked, int T, bool ok, v4i vm, int mt, const v4i (&sc)[4], v4i (&P)[ND]) {
+        // The weights' digits as B operands, from y = 2 (max - s + 64): the table index is y >> 8, bytes 1 and 2 of y (|s| is
+        // at most 2^21, so y < 2^24 wherever the column sees the position; of other columns any index below 2^16 will do).
+        auto weights = [&](auto masked, int T, bool ok, v4i vm, int mt, const v4i (&y)[4], v4i (&P)[ND]) {
 #pragma unroll
             for (int t = 0; t < 4; t++) {
-                uint32_t e[4];
+                uint32_t u[4];
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    uint32_t ix = min((uint32_t)(mx[mt] - sc[t][r]) >> 7, 1024u);
-                    if constexpr (masked) ix = ok & sees(64 * T + 16 * gq + 4 * t + r, pos[mt]) ? ix : 1024u;
-                    e[r] = sE[ix];
-                    if constexpr (BITS == 4) {  // the digits of e m
-                        den[mt][0] += (int)e[r];
-                        e[r] = (__umul24(e[r], ((uint32_t)vm[t] >> (8 * r)) & 255) + 0x808080) ^ 0x808080;
-                    }
+                    u[r] = (uint32_t)y[t][r];
+                    if constexpr (masked) u[r] = ok & sees(64 * T + 16 * gq + 4 * t + r, pos[mt]) ? u[r] : 0x00FFFFFFu;
                 }
-                const uint32_t e01 = __builtin_amdgcn_perm(e[1], e[0], 0x05010400), e23 = __builtin_amdgcn_perm(e[3], e[2], 0x05010400);
-                P[0][t] = (int)__builtin_amdgcn_perm(e23, e01, 0x05040100);
-                P[1][t] = (int)__builtin_amdgcn_perm(e23, e01, 0x07060302);
-                if constexpr (BITS == 4)
-                    P[ND - 1][t] = (int)__builtin_amdgcn_perm(__builtin_amdgcn_perm(e[3], e[2], 0x0c0c0602), __builtin_amdgcn_perm(e[1], e[0], 0x0c0c0602), 0x05040100);
+                us2 e[2];
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const uint32_t ix = __builtin_bit_cast(uint32_t, __builtin_elementwise_min(
+                        __builtin_bit_cast(us2, __builtin_amdgcn_perm(u[2 * h + 1], u[2 * h], 0x06050201)), us2{1024, 1024}));
+                    e[h] = us2{sE[ix & 0xFFFF], sE[ix >> 16]};
+                }
                 if constexpr (BITS == 8) {
+                    const uint32_t e01 = __builtin_bit_cast(uint32_t, e[0]), e23 = __builtin_bit_cast(uint32_t, e[1]);
+                    P[0][t] = (int)__builtin_amdgcn_perm(e23, e01, 0x06040200);
+                    P[1][t] = (int)__builtin_amdgcn_perm(e23, e01, 0x07050301);
                     den[mt][0] = __builtin_amdgcn_sdot4(P[0][t], 0x01010101, den[mt][0], false);
                     den[mt][1] = __builtin_amdgcn_sdot4(P[1][t], 0x01010101, den[mt][1], false);
+                } else {
+                    uint32_t f[4];
+#pragma unroll
+                    for (int r = 0; r < 4; r++)  // the balanced digits of e m
+                        f[r] = (__umul24((uint32_t)e[r >> 1][r & 1], ((uint32_t)vm[t] >> (8 * r)) & 255) + 0x808080) ^ 0x808080;
+                    const uint32_t f01 = __builtin_amdgcn_perm(f[1], f[0], 0x05010400), f23 = __builtin_amdgcn_perm(f[3], f[2], 0x05010400);
+                    P[0][t] = (int)__builtin_amdgcn_perm(f23, f01, 0x05040100);
+                    P[1][t] = (int)__builtin_amdgcn_perm(f23, f01, 0x07060302);
+                    P[ND - 1][t] = (int)__builtin_amdgcn_perm(__builtin_amdgcn_perm(f[3], f[2], 0x0c0c0602), __builtin_amdgcn_perm(f[1], f[0], 0x0c0c0602), 0x05040100);
+                    den[mt][0] = (int)__builtin_amdgcn_udot2(e[0], us2{1, 1}, (uint32_t)den[mt][0], false);
+                    den[mt][0] = (int)__builtin_amdgcn_udot2(e[1], us2{1, 1}, (uint32_t)den[mt][0], false);
                 }
+            }
+        };
+        // y of the negated scores: 2 (-s) + 2 (max + 64). 8 bits: the product taken twice over, on top of the latter.
+        auto lift = [&](int mt, const v4i (&sc)[4], v4i (&y)[4]) {
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) y[t][r] = (int)((uint32_t)sc[t][r] * 2 + (uint32_t)top[mt]);
+        };
+        auto lifted = [&](const Chunk (&k)[4][KC], v4i km, int mt, v4i (&y)[4]) {
+            if constexpr (BITS == 8) {
+                const v4i top4 = {top[mt], top[mt], top[mt], top[mt]};
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    y[t] = top4;
+#pragma unroll
+                    for (int c = 0; c < 2 * KC; c++) y[t] = mfma16(k[t][c >> 1], q[mt][c >> 1], y[t]);
+                }
+            } else {
+                v4i sc[4];
+                scores(k, km, mt, sc);
+                lift(mt, sc, y);
             }
         };
         auto add_v = [&](const VTile& x, int mt, const v4i (&P)[ND]) {
@@ -413,7 +474,7 @@ __global__ __launch_bounds__(64 * WM * WP) __attribute__((amdgpu_waves_per_eu(PG
                     if (BITS == 8 && all && nmt == MT) {  // one straight block: a group's lookups under the next one's products
                         v4i sc[MT][4], P[MT][ND];
 #pragma unroll
-                        for (int mt = 0; mt < MT; mt++) scores(k, km, mt, sc[mt]);
+                        for (int mt = 0; mt < MT; mt++) lifted(k, km, mt, sc[mt]);
 #pragma unroll
                         for (int mt = 0; mt < MT; mt++) weights(std::false_type(), T, ok, y[u].m, mt, sc[mt], P[mt]);
 #pragma unroll
@@ -423,7 +484,7 @@ __global__ __launch_bounds__(64 * WM * WP) __attribute__((amdgpu_waves_per_eu(PG
                         for (int mt = 0; mt < MT; mt++) {
                             if (mt >= nmt) break;
                             v4i sc[4], P[ND];
-                            scores(k, km, mt, sc);
+                            lifted(k, km, mt, sc);
                             if (BITS == 4 && all) weights(std::false_type(), T, ok, y[u].m, mt, sc, P);
                             else weights(std::true_type(), T, ok, y[u].m, mt, sc, P);
                             add_v(y[u], mt, P);
@@ -443,13 +504,14 @@ __global__ __launch_bounds__(64 * WM * WP) __attribute__((amdgpu_waves_per_eu(PG
                     if (n >= kept) break;
                     const int T = at(n);
                     const bool ok = page_ok(T, idv[u]), all = full(T, ok);
-                    v4i sc[4] = {}, P[ND];
+                    v4i sc[4] = {}, y[4], P[ND];
                     if (l16 < cols) {
 #pragma unroll
                         for (int t = 0; t < 4; t++) sc[t] = *kept_place(n, t);
                     }
-                    if (all) weights(std::false_type(), T, ok, xv[u].m, 0, sc, P);
-                    else weights(std::true_type(), T, ok, xv[u].m, 0, sc, P);
+                    lift(0, sc, y);
+                    if (all) weights(std::false_type(), T, ok, xv[u].m, 0, y, P);
+                    else weights(std::true_type(), T, ok, xv[u].m, 0, y, P);
                     add_v(xv[u], 0, P);
                     if (n + NV < kept) load_v(at(n + NV), nidv[u], xv[u]);
                     idv[u] = nidv[u];
