@@ -1076,5 +1076,5 @@ def dec_argmax_rows(logits_dev, rows: int, n: int, token_dev, ws_dev, stride: in
                     dev: int = 0) -> None:
     """token_dev[r] = the first index of the maximum of row r's n int32 logits (rows `stride` apart, n by default)."""
     check(lib().kt_hip_dec_argmax_rows(dev, _ptr(logits_dev), rows, n, n if stride is None else stride,
-                                       _ptr(token_dev), _ptr(ws_dev), ws_dev.numel() * ws_dev.element_size(),
+                                       _ptr(token_dev), _ptr(ws_dev), ws_dev.nbytes,
                                        _stream(stream)), "dec argmax rows")

@@ -58,7 +58,7 @@ __global__ __launch_bounds__(256) void pg_append_kernel(Paged a, const int8_t* _
                                                         int8_t* __restrict__ q, int64_t q_stride) {
     constexpr int HH = HD / 2, CH = HD / 16;
     __shared__ __attribute__((aligned(16))) int8_t sKV[2][16][HD];
-    __shared__ int sM[2][16];
+    __shared__ int sM[2][16], sInv[2][16];
     const int tid = threadIdx.x, g = blockIdx.y, rep = nh / a.nkv;
     int first = 0;
     const int b = pg_tile_seq(a, (int)blockIdx.x, 1, 16, 2, &first);
@@ -140,6 +140,7 @@ __global__ __launch_bounds__(256) void pg_append_kernel(Paged a, const int8_t* _
             if (e == 0 && r >= r0 && r < r1) {
                 const int m = mult4(top);
                 sM[w][r] = m;
+                sInv[w][r] = mult4_inv(m);
                 (w ? a.v : a.k)[part + (size_t)(HH << a.page_sh) + slot + r] = (uint8_t)m;
             }
         }
@@ -149,7 +150,7 @@ __global__ __launch_bounds__(256) void pg_append_kernel(Paged a, const int8_t* _
         for (int i = tid; i < 16 * CH; i += 256) {
             const int r = i / CH, c = i % CH;
             if (r < r0 || r >= r1) continue;
-            const int m = sM[0][r], inv = mult4_inv(m);
+            const int m = sM[0][r], inv = sInv[0][r];
             v2i w = {0, 0};
 #pragma unroll
             for (int e = 0; e < 16; e++)
@@ -162,8 +163,8 @@ __global__ __launch_bounds__(256) void pg_append_kernel(Paged a, const int8_t* _
 #pragma unroll
             for (int r = 0; r < 16; r++) {
                 if (r < r0 || r >= r1) continue;
-                const int sh = 8 * (r & 3) + 4 * ((r >> 2) & 1), m = sM[1][r];
-                w[r >> 3] = (w[r >> 3] & ~(15 << sh)) | ((code4(sKV[1][r][d], m, mult4_inv(m)) & 15) << sh);
+                const int sh = 8 * (r & 3) + 4 * ((r >> 2) & 1);
+                w[r >> 3] = (w[r >> 3] & ~(15 << sh)) | ((code4(sKV[1][r][d], sM[1][r], sInv[1][r]) & 15) << sh);
             }
             *reinterpret_cast<v2i*>(vd + 8 * d) = w;
         }

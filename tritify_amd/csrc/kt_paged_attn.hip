@@ -15,6 +15,12 @@ namespace kt {
 
 namespace {
 
+#ifndef PG_EU1
+#define PG_EU1 3
+#endif
+#ifndef PG_NB1
+#define PG_NB1 1
+#endif
 typedef unsigned short us2 __attribute__((ext_vector_type(2)));
 
 struct PgAttend {
@@ -102,11 +108,11 @@ __device__ __forceinline__ void pg_store(int8_t* to, const int64_t (&v)[4], int6
     *reinterpret_cast<uint32_t*>(to) = out;
 }
 
+// Waves a SIMD is meant to hold: registers for 2, or lean ones for 4.
+constexpr int pg_eu(int hd, int mt, int wp) { return wp == 8 ? 2 : (hd * mt == 64 ? PG_EU1 : 2); }
+
 template <int HD, int BITS, int MT, int WM, int WP, int MODE>
-#ifndef PG_EU
-#define PG_EU 2
-#endif
-__global__ __launch_bounds__(64 * WM * WP) __attribute__((amdgpu_waves_per_eu(PG_EU))) void pg_attend_kernel(Paged a, PgAttend p) {
+__global__ __launch_bounds__(64 * WM * WP) __attribute__((amdgpu_waves_per_eu(pg_eu(HD, MT, WP)))) void pg_attend_kernel(Paged a, PgAttend p) {
     constexpr int HH = HD / 2, KC = HD / 64, DT = HD / 16, ND = BITS == 8 ? 2 : 3;
     constexpr int W = WM * WP, NT = 64 * W, CW = 16 * MT, COLS = CW * WM;  // threads; columns of a wave and of the CTA
     constexpr int NMAX = COLS * WP > NT ? WP : NT / COLS;
@@ -134,7 +140,7 @@ __global__ __launch_bounds__(64 * WM * WP) __attribute__((amdgpu_waves_per_eu(PG
     // kind that may be empty comes last: single tokens have no further tiles, and CTAs that leave at once between others
     // would leave the XCDs different numbers of those that stay (256 of them on 256 CUs took two rounds).
     const int ntiles = (int)gridDim.x / a.nkv, g = (int)blockIdx.x % a.nkv, order = (int)blockIdx.x / a.nkv;
-    const int tile = WM * MT == 1 ? order : ntiles - 1 - order;
+    const int tile = WP == 8 ? order : ntiles - 1 - order;
     int b = tile, nth = 0;
     if (tile >= a.seqs) {
         int first = 0;
@@ -158,7 +164,7 @@ __global__ __launch_bounds__(64 * WM * WP) __attribute__((amdgpu_waves_per_eu(PG
     const int total = nsink + max(0, ntile - w0);
     auto tile_at = [&](int i) { return i < nsink ? i : i - nsink + w0; };
 
-    const uint8_t *const kbase = a.k + (size_t)g * a.part + l16 * CHB, *const vbase = a.v + (size_t)g * a.part + l16 * CHB;
+    const uint8_t *const kbase = a.k + (size_t)g * a.part, *const vbase = a.v + (size_t)g * a.part;
     const uint8_t *const kmult = a.k + (size_t)g * a.part + (HH << a.page_sh), *const vmult = a.v + (size_t)g * a.part + (HH << a.page_sh);
 
     // the columns' rows and positions, and their negated q as B operands
@@ -194,13 +200,13 @@ __global__ __launch_bounds__(64 * WM * WP) __attribute__((amdgpu_waves_per_eu(PG
     auto part_of = [&](int id) { return (uint64_t)((unsigned)id < (unsigned)a.pages ? (uint32_t)id : 0u) * stride; };
     auto slot_of = [&](int T) { return (block_of(T) << 4) & ((1 << a.page_sh) - 1); };
     auto load_k = [&](int T, int id, Tile& x) {
-        const uint8_t* at = kbase + part_of(id) + (uint32_t)(slot_of(T) * ROWB);
+        const uint8_t* at = kbase + (part_of(id) + (uint32_t)(slot_of(T) * ROWB + l16 * CHB));
 #pragma unroll
         for (int i = 0; i < DT; i++) x.raw[i] = *reinterpret_cast<const Chunk*>(at + 16 * CHB * i);
         if constexpr (BITS == 4) x.m = *reinterpret_cast<const v4i*>(kmult + part_of(id) + (uint32_t)slot_of(T));
     };
     auto load_v = [&](int T, int id, VTile& x) {
-        const uint8_t* at = vbase + part_of(id) + (uint32_t)(slot_of(T) * ROWB);
+        const uint8_t* at = vbase + (part_of(id) + (uint32_t)(slot_of(T) * ROWB + l16 * CHB));
 #pragma unroll
         for (int d = 0; d < DT; d++) x.v[d] = *reinterpret_cast<const Chunk*>(at + 16 * CHB * d);
         if constexpr (BITS == 4) x.m = *reinterpret_cast<const v4i*>(vmult + part_of(id) + (uint32_t)slot_of(T));
@@ -268,12 +274,22 @@ __global__ __launch_bounds__(64 * WM * WP) __attribute__((amdgpu_waves_per_eu(PG
 #pragma unroll
         for (int t = 0; t < 4; t++) *kept_place(n, t) = sc[t];
     };
-    constexpr int NV = MODE == PG_KEEP && HD == 64 ? 4 : 1;  // V's ring over the kept tiles, begun before the maximum is known
+    // V's ring over the kept tiles; at hd 64 there are registers to begin it before the maximum is known
+    constexpr int NV = MODE == PG_KEEP && HD == 64 ? 4 : 1;
+    constexpr bool EARLY = MODE == PG_KEEP && HD == 64;
     VTile xv[NV];
     int idv[NV], nidv[NV];
     auto at = [&](int n) { return tile_at(start + n * step); };
+    auto begin_v = [&]() {
+#pragma unroll
+        for (int u = 0; u < NV; u++) {
+            idv[u] = nidv[u] = 0;
+            if (u < kept) idv[u] = page_id(at(u)), load_v(at(u), idv[u], xv[u]);
+            if (u + NV < kept) nidv[u] = page_id(at(u + NV));
+        }
+    };
     if constexpr (MAXP) {
-        constexpr int NB = MT * HD <= 64 ? 4 : 2;
+        constexpr int NB = WP == 8 ? (HD == 64 ? 4 : 2) : PG_NB1;
         Tile x[NB];
         int id[NB], nid[NB];
 #pragma unroll
@@ -285,14 +301,7 @@ __global__ __launch_bounds__(64 * WM * WP) __attribute__((amdgpu_waves_per_eu(PG
 #pragma unroll
         for (int u = 0; u < NB; u++)
             if (u < mine) load_k(at(u), id[u], x[u]);
-        if constexpr (MODE == PG_KEEP) {
-#pragma unroll
-            for (int u = 0; u < NV; u++) {
-                idv[u] = id[u], nidv[u] = 0;
-                if (u < kept) load_v(at(u), idv[u], xv[u]);
-                if (u + NV < kept) nidv[u] = page_id(at(u + NV));
-            }
-        }
+        if constexpr (EARLY) begin_v();
         for (int n0 = 0; n0 < mine; n0 += NB) {
 #pragma unroll
             for (int u = 0; u < NB; u++) {
@@ -416,7 +425,7 @@ __global__ __launch_bounds__(64 * WM * WP) __attribute__((amdgpu_waves_per_eu(PG
                 }
             }
         };
-        // y of the negated scores: 2 (-s) + 2 (max + 64). 8 bits: the product taken twice over, on top of the latter.
+        // y of the negated scores: 2 (-s) + 2 (max + 64); where the products are short, taken twice over on top of the latter.
         auto lift = [&](int mt, const v4i (&sc)[4], v4i (&y)[4]) {
 #pragma unroll
             for (int t = 0; t < 4; t++)
@@ -424,7 +433,7 @@ __global__ __launch_bounds__(64 * WM * WP) __attribute__((amdgpu_waves_per_eu(PG
                 for (int r = 0; r < 4; r++) y[t][r] = (int)((uint32_t)sc[t][r] * 2 + (uint32_t)top[mt]);
         };
         auto lifted = [&](const Chunk (&k)[4][KC], v4i km, int mt, v4i (&y)[4]) {
-            if constexpr (BITS == 8) {
+            if constexpr (BITS == 8 && HD == 64) {
                 const v4i top4 = {top[mt], top[mt], top[mt], top[mt]};
 #pragma unroll
                 for (int t = 0; t < 4; t++) {
@@ -445,7 +454,7 @@ __global__ __launch_bounds__(64 * WM * WP) __attribute__((amdgpu_waves_per_eu(PG
                 for (int e = 0; e < ND; e++) acc[mt][d][e] = mfma16(widen(x.v[d]), P[e], acc[mt][d][e]);
         };
         {
-            constexpr int NB = MT * HD <= 64 && MODE != PG_KEEP ? 2 : 1;
+            constexpr int NB = WP == 8 && HD == 64 && MODE != PG_KEEP ? 2 : 1;
             Tile x[NB];
             VTile y[NB];
             int id[NB], nid[NB];
@@ -471,7 +480,7 @@ __global__ __launch_bounds__(64 * WM * WP) __attribute__((amdgpu_waves_per_eu(PG
                     turn_k(x[u], k);
                     const v4i km = x[u].m;
                     if (n + NB < left) load_k(back(n + NB), nid[u], x[u]);
-                    if (BITS == 8 && all && nmt == MT) {  // one straight block: a group's lookups under the next one's products
+                    if (BITS == 8 && MT == 2 && all && nmt == MT) {  // one straight block: a group's lookups under the next one's products
                         v4i sc[MT][4], P[MT][ND];
 #pragma unroll
                         for (int mt = 0; mt < MT; mt++) lifted(k, km, mt, sc[mt]);
@@ -485,7 +494,7 @@ __global__ __launch_bounds__(64 * WM * WP) __attribute__((amdgpu_waves_per_eu(PG
                             if (mt >= nmt) break;
                             v4i sc[4], P[ND];
                             lifted(k, km, mt, sc);
-                            if (BITS == 4 && all) weights(std::false_type(), T, ok, y[u].m, mt, sc, P);
+                            if ((BITS == 4 || MT == 1) && all) weights(std::false_type(), T, ok, y[u].m, mt, sc, P);
                             else weights(std::true_type(), T, ok, y[u].m, mt, sc, P);
                             add_v(y[u], mt, P);
                         }
@@ -497,6 +506,7 @@ __global__ __launch_bounds__(64 * WM * WP) __attribute__((amdgpu_waves_per_eu(PG
             }
         }
         if constexpr (MODE == PG_KEEP) {
+            if constexpr (!EARLY) begin_v();
             for (int n0 = 0; n0 < kept; n0 += NV) {
 #pragma unroll
                 for (int u = 0; u < NV; u++) {
@@ -608,7 +618,7 @@ Plan plan(int tokens, int seqs, int64_t max_pos, int nh, int nkv, int hd, int bi
     const int64_t each = ((int64_t)tokens * rep + seqs - 1) / std::max(seqs, 1);
     Plan x;
     if (each <= 16) x.mt = x.wm = 1, x.wp = 8;
-    else x.mt = hd == 64 ? 2 : 1, x.wm = tune("PGT_WM", 4), x.wp = tune("PGT_WP", 2);
+    else x.mt = tune("PGT_MT", hd == 64 ? 2 : 1), x.wm = tune("PGT_WM", 4), x.wp = tune("PGT_WP", 2);
     const int64_t cols = 16 * x.mt * x.wm, tiles = (int64_t)tokens * rep / cols + seqs;
     x.tiles = (int)tiles;
     const int64_t ctas = std::min<int64_t>(tiles, tokens) * nkv, work = (max_pos + 63) / 64;
@@ -634,7 +644,7 @@ template <int HD, int BITS, int MT, int WM, int WP>
 hipError_t attend(const Paged& a, PgAttend p, const Plan& x, hipStream_t s) {
     const dim3 grid((unsigned)(x.tiles * a.nkv), (unsigned)x.splits), block(64 * WM * WP);
     if (x.splits == 1) {
-        if constexpr (MT == 1 && WM == 1) {
+        if constexpr (WP == 8) {
             pg_attend_kernel<HD, BITS, MT, WM, WP, PG_KEEP><<<grid, block, (size_t)p.keep, s>>>(a, p);
         } else {
             pg_attend_kernel<HD, BITS, MT, WM, WP, PG_WHOLE><<<grid, block, 0, s>>>(a, p);
@@ -651,12 +661,17 @@ hipError_t attend(const Paged& a, PgAttend p, const Plan& x, hipStream_t s) {
 template <int HD, int BITS>
 hipError_t attend_by(const Paged& a, const PgAttend& p, const Plan& x, hipStream_t s) {
     constexpr int MT = HD == 64 ? 2 : 1;
-    if (x.mt == 1 && x.wm == 1) return attend<HD, BITS, 1, 1, 8>(a, p, x, s);
+    if (x.wp == 8) return attend<HD, BITS, 1, 1, 8>(a, p, x, s);
+    if (x.mt == 1) {
+    if (x.wm == 1 && x.wp == 4) return attend<HD, BITS, 1, 1, 4>(a, p, x, s);
+    if (x.wm == 2 && x.wp == 2) return attend<HD, BITS, 1, 2, 2>(a, p, x, s);
+    if (x.wm == 4 && x.wp == 2) return attend<HD, BITS, 1, 4, 2>(a, p, x, s);
+    if (x.wm == 2 && x.wp == 4) return attend<HD, BITS, 1, 2, 4>(a, p, x, s);
+    return attend<HD, BITS, 1, 4, 1>(a, p, x, s);
+    }
     if (x.wm == 1 && x.wp == 4) return attend<HD, BITS, MT, 1, 4>(a, p, x, s);
     if (x.wm == 2 && x.wp == 2) return attend<HD, BITS, MT, 2, 2>(a, p, x, s);
-    if (x.wm == 4 && x.wp == 1) return attend<HD, BITS, MT, 4, 1>(a, p, x, s);
-    if (x.wm == 2 && x.wp == 4) return attend<HD, BITS, MT, 2, 4>(a, p, x, s);
-    return attend<HD, BITS, MT, 4, 2>(a, p, x, s);
+    return attend<HD, BITS, MT, 4, 1>(a, p, x, s);
 }
 
 }  // namespace

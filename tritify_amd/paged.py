@@ -24,10 +24,10 @@ def page_bytes(page: int, hd: int, bits: int = 8) -> int:
     return n
 
 
-def _need(t, what: str, dtype: str, device, shape=None) -> None:
-    if str(t.dtype) != "torch." + dtype or t.device != device or not t.is_contiguous():
+def _need(t, what: str, dtype, device, shape=None) -> None:
+    if t.dtype != dtype or t.device != device or not t.is_contiguous():
         raise ValueError(f"{what}: a contiguous {dtype} tensor on {device} is needed")
-    if shape is not None and tuple(t.shape) != shape:
+    if shape is not None and t.shape != shape:
         raise ValueError(f"{what}: shape {tuple(t.shape)}, {shape} is needed")
 
 
@@ -37,15 +37,17 @@ class PagedBatch:
     kernels run, so a captured call follows what is copied into them."""
 
     def __init__(self, row_start, kv_len, table, tokens: int):
+        import torch
+
         dv = table.device
         if dv.type != "cuda":
             raise ValueError("PagedBatch: the tensors live on the GPU")
         if table.dim() != 2 or not 0 <= tokens <= 1 << 30:
             raise ValueError("PagedBatch: table is seqs x max_pages, tokens a count of rows")
         self.seqs, self.max_pages, self.tokens, self.device = table.shape[0], table.shape[1], int(tokens), dv
-        _need(table, "table", "int32", dv)
-        _need(row_start, "row_start", "int32", dv, (self.seqs + 1,))
-        _need(kv_len, "kv_len", "int32", dv, (self.seqs,))
+        _need(table, "table", torch.int32, dv)
+        _need(row_start, "row_start", torch.int32, dv, (self.seqs + 1,))
+        _need(kv_len, "kv_len", torch.int32, dv, (self.seqs,))
         self.row_start, self.kv_len, self.table = row_start, kv_len, table
         self.ptrs = (row_start.data_ptr(), kv_len.data_ptr(), table.data_ptr())
 
@@ -63,11 +65,13 @@ class PagedKV:
             raise ValueError("PagedKV: pages >= 0 and nkv >= 1")
         self.pages, self.page, self.nkv, self.hd, self.bits, self.dev = pages, page, nkv, hd, bits, dev
         self.device = torch.device("cuda", dev)
+        self._i8, self._i16, self._i32 = torch.int8, torch.int16, torch.int32
         shape = (pages, nkv, part)
         self.k = torch.zeros(shape, dtype=torch.int8, device=self.device) if k is None else k
         self.v = torch.zeros(shape, dtype=torch.int8, device=self.device) if v is None else v
-        _need(self.k, "k", "int8", self.device, shape)
-        _need(self.v, "v", "int8", self.device, shape)
+        _need(self.k, "k", torch.int8, self.device, shape)
+        _need(self.v, "v", torch.int8, self.device, shape)
+        self._pools = (self.k.data_ptr(), self.v.data_ptr(), pages, page, bits)  # as every call passes them
 
     def _batch(self, batch: PagedBatch) -> None:
         if batch.device != self.device:
@@ -75,47 +79,44 @@ class PagedKV:
         if not 1 <= batch.max_pages <= MAX_POS // self.page:
             raise ValueError(f"a table of {batch.max_pages} pages of {self.page}: 1 to {MAX_POS} positions")
 
-    def _rows(self, t, what: str, batch: PagedBatch, width: int) -> int:
-        """The stride of `t`, whose rows hold at least `width` int8 values for every row of the batch."""
-        if t.dim() != 2 or str(t.dtype) != "torch.int8" or t.device != self.device:
+    def _rows(self, t, what: str, batch: PagedBatch, width: int) -> tuple[int, int]:
+        """The address and stride of `t`, whose rows hold at least `width` int8 values for every row of the batch."""
+        if t.dtype != self._i8 or t.device != self.device or t.dim() != 2:
             raise ValueError(f"{what}: an int8 matrix on {self.device} is needed")
-        rows, cols = t.shape
-        stride = t.stride(0) if rows > 1 else max(t.stride(0), cols)
-        if rows < batch.tokens or cols < width or (cols > 1 and t.stride(1) != 1) or stride < cols:
+        (rows, cols), (stride, by), at = t.shape, t.stride(), t.data_ptr()
+        if rows <= 1 and stride < cols:
+            stride = cols
+        if rows < batch.tokens or cols < width or (by != 1 and cols > 1) or stride < cols:
             raise ValueError(f"{what}: {tuple(t.shape)} with strides {t.stride()}: {batch.tokens} rows of {width} side by side")
-        if stride % 16 or t.data_ptr() % 16:
+        if stride % 16 or at % 16:
             raise ValueError(f"{what}: rows must start at multiples of 16 bytes")
-        return stride
+        return at, stride
 
     def append(self, qkv, batch: PagedBatch, nh: int, cos, sin, q, stream=None) -> None:
         """The rows of qkv (q heads, k heads, v heads; read only): their rotated q heads to q, their rotated k and their v
         to the pages. cos / sin: int16 tables of max_pos x hd / 2 at 2^14."""
         self._batch(batch)
         hd, nkv = self.hd, self.nkv
-        if cos.dim() != 2:
-            raise ValueError("cos: max_pos x hd / 2")
-        shape = (cos.shape[0], hd // 2)
-        _need(cos, "cos", "int16", self.device, shape)
-        _need(sin, "sin", "int16", self.device, shape)
-        s_in, s_q = self._rows(qkv, "qkv", batch, (nh + 2 * nkv) * hd), self._rows(q, "q", batch, nh * hd)
+        n = cos.shape[0] if cos.dim() == 2 else -1
+        _need(cos, "cos", self._i16, self.device, (n, hd // 2))
+        _need(sin, "sin", self._i16, self.device, (n, hd // 2))
+        at, stride = self._rows(qkv, "qkv", batch, (nh + 2 * nkv) * hd)
+        to, q_stride = self._rows(q, "q", batch, nh * hd)
         B.check(B.lib().kt_hip_dec_rope_kv_paged(
-            self.dev, qkv.data_ptr(), batch.tokens, s_in, *batch.ptrs, batch.seqs, batch.max_pages, nh, nkv, hd,
-            cos.data_ptr(), sin.data_ptr(), shape[0], q.data_ptr(), s_q, self.k.data_ptr(), self.v.data_ptr(), self.pages,
-            self.page, self.bits, B._stream(stream)), "dec rope + paged append")
+            self.dev, at, batch.tokens, stride, *batch.ptrs, batch.seqs, batch.max_pages, nh, nkv, hd, cos.data_ptr(),
+            sin.data_ptr(), n, to, q_stride, *self._pools, B._stream(stream)), "dec rope + paged append")
 
     def read(self, batch: PagedBatch, k, v, stream=None) -> None:
         """Every sequence's positions as contiguous rows: k / v seqs x max_pos x nkv x hd int8, positions from
         min(kv_len, max_pos) on left as they are."""
         self._batch(batch)
-        if k.dim() != 4:
-            raise ValueError("k: seqs x max_pos x nkv x hd")
-        shape = (batch.seqs, k.shape[1], self.nkv, self.hd)
-        _need(k, "k", "int8", self.device, shape)
-        _need(v, "v", "int8", self.device, shape)
+        n = k.shape[1] if k.dim() == 4 else -1
+        shape = (batch.seqs, n, self.nkv, self.hd)
+        _need(k, "k", self._i8, self.device, shape)
+        _need(v, "v", self._i8, self.device, shape)
         B.check(B.lib().kt_hip_dec_kv_read_paged(
-            self.dev, self.k.data_ptr(), self.v.data_ptr(), self.pages, self.page, self.bits, batch.ptrs[1],
-            batch.ptrs[2], batch.seqs, batch.max_pages, self.nkv, self.hd, k.data_ptr(), v.data_ptr(), shape[1],
-            B._stream(stream)), "dec paged read")
+            self.dev, *self._pools, batch.ptrs[1], batch.ptrs[2], batch.seqs, batch.max_pages, self.nkv, self.hd,
+            k.data_ptr(), v.data_ptr(), n, B._stream(stream)), "dec paged read")
 
     def workspace_bytes(self, batch: PagedBatch, nh: int) -> int:
         """Scratch bytes of attend for `nh` q heads over this batch's shape."""
@@ -137,14 +138,15 @@ class PagedKV:
         """The rows' attention over their sequences' pages (after the append of the rows' own k and v), q and o rows of
         nh * hd. window >= 1: a row at p sees positions past p - window and the first `sinks`; 0: all up to its own."""
         self._batch(batch)
-        _need(exp_tab, "exp_tab", "int32", self.device, (1024,))
+        _need(exp_tab, "exp_tab", self._i32, self.device, (1024,))
         if ws.device != self.device or not ws.is_contiguous():
             raise ValueError(f"ws: a contiguous tensor on {self.device} is needed")
-        s_q, s_o = self._rows(q, "q", batch, nh * self.hd), self._rows(o, "o", batch, nh * self.hd)
+        at, q_stride = self._rows(q, "q", batch, nh * self.hd)
+        to, o_stride = self._rows(o, "o", batch, nh * self.hd)
         B.check(B.lib().kt_hip_dec_attention_paged(
-            self.dev, q.data_ptr(), batch.tokens, s_q, *batch.ptrs, batch.seqs, batch.max_pages, nh, self.nkv, self.hd,
-            exp_tab.data_ptr(), window, sinks, self.k.data_ptr(), self.v.data_ptr(), self.pages, self.page, self.bits,
-            o.data_ptr(), s_o, ws.data_ptr(), ws.numel() * ws.element_size(), B._stream(stream)), "dec paged attention")
+            self.dev, at, batch.tokens, q_stride, *batch.ptrs, batch.seqs, batch.max_pages, nh, self.nkv, self.hd,
+            exp_tab.data_ptr(), window, sinks, *self._pools, to, o_stride, ws.data_ptr(), ws.nbytes, B._stream(stream)),
+            "dec paged attention")
 
 
 class PagedDecoder:
