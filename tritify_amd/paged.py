@@ -230,7 +230,9 @@ class PagedDecoder:
     def batch(self, seqs: list, rows: list) -> PagedBatch:
         """The batch of `rows` new rows for each of `seqs`, whose positions are reserved."""
         torch = self.torch
-        table = np.full((len(seqs), self.max_pages), -1, dtype=np.int32)
+        # as wide as the longest needs, to a power of two: the attention divides its work by the table's width
+        need = max([1] + [len(self.seq[s]["pages"]) for s in seqs])
+        table = np.full((len(seqs), min(self.max_pages, 1 << (need - 1).bit_length())), -1, dtype=np.int32)
         for i, s in enumerate(seqs):
             table[i, : len(self.seq[s]["pages"])] = self.seq[s]["pages"]
         start = np.concatenate([[0], np.cumsum(rows)]).astype(np.int32)
