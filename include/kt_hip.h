@@ -860,7 +860,7 @@ int kt_hip_dec_embed_argmax(int dev, const uint64_t* part_dev, int64_t nparts, c
  * 8 h + 4 + r in its high half, and a part ends with its slots' multipliers (page bytes): a row x of hd values is held as
  * m = ceil(8 max |x| / 7) and the codes c = clamp(round_half_away(8 x / m), +-7) (0 when m is 0), and stands for c m / 8.
  *
- * max_pages * page <= KT_PAGED_MAX_POS; tokens * nh, and 2 * seqs * nh below 2^31. Pointers and strides (in elements) of
+ * max_pages * page <= KT_PAGED_MAX_POS; nh <= 4096; tokens * nh and 2 * seqs * nh below 2^31. Pointers and strides (in elements) of
  * int8 rows are multiples of 16.
  * ------------------------------------------------------------------------------------------------------------- */
 #define KT_PAGED_MAX_POS 524288

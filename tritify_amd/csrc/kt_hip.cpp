@@ -1036,7 +1036,7 @@ int kt_hip_dec_embed_argmax(int dev, const uint64_t* part_dev, int64_t nparts, c
 // 32-bit counts. Device arrays are only dereferenced on the device.
 static bool paged_ok(int64_t tokens, int64_t seqs, int64_t max_pages, int64_t nh, int64_t nkv, int64_t hd,
                      int64_t pages, int64_t page, int bits) {
-    return kt_hip_dec_page_bytes(page, hd, bits) != 0 && nkv >= 1 && nh >= nkv && nh % nkv == 0 && nh <= 65535 &&
+    return kt_hip_dec_page_bytes(page, hd, bits) != 0 && nkv >= 1 && nh >= nkv && nh % nkv == 0 && nh <= 4096 &&
            tokens >= 0 && seqs >= 0 && tokens <= INT_MAX / nh && tokens <= 1 << 30 && seqs <= INT_MAX / (2 * nh) && max_pages >= 1 &&
            max_pages <= KT_PAGED_MAX_POS / page && pages >= 0 && pages <= INT_MAX;
 }

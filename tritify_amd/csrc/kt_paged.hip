@@ -48,11 +48,10 @@ __device__ __forceinline__ int value4(int c, int m) {
 
 // One CTA per (block of 16 positions that a sequence's rows reach, kv head): it rotates the q heads of the group and the k
 // head of the rows in the block, four pairs a thread, stages k and v in LDS and writes the block's bytes. The block is the
-// unit because V's chunk is 16 positions of a dimension, in 4 bits with two positions to a byte: whole blocks go out as
-// 16-byte (8-byte) stores, and one that only some of its rows belong to is written byte by byte (4 bits: read, merged and
-// written back by its only owner).
-template <int HD, int BITS>
-__global__ __launch_bounds__(256) void pg_append_kernel(Paged a, const int8_t* __restrict__ qkv, int64_t stride, int nh,
+// unit because V's chunk is 16 positions of a dimension, in 4 bits with two positions to a byte: what rows fill goes out in
+// dwords, what only some of them belong to byte by byte (4 bits: read, merged and written back by its only owner).
+template <int HD, int BITS, int NT>
+__global__ __launch_bounds__(NT) void pg_append_kernel(Paged a, const int8_t* __restrict__ qkv, int64_t stride, int nh,
                                                         const int16_t* __restrict__ cosT,
                                                         const int16_t* __restrict__ sinT, int max_pos,
                                                         int8_t* __restrict__ q, int64_t q_stride) {
@@ -69,9 +68,16 @@ __global__ __launch_bounds__(256) void pg_append_kernel(Paged a, const int8_t* _
     if (lo >= hi) return;
     // the rows whose position the tables and the caches have
     const int cap = min(max_pos, a.max_pages << a.page_sh), vlo = max(lo, 0), vhi = min(hi, cap);
+    for (int i = tid; i < (vhi - vlo) * CH; i += NT) {
+        const int p = vlo + i / CH, c = i % CH;
+        const int8_t* src = qkv + (size_t)(s.t0 + (p - s.p0)) * stride + (nh + a.nkv + g) * HD + 16 * c;
+        *reinterpret_cast<v4i*>(&sKV[1][p & 15][16 * c]) = *reinterpret_cast<const v4i*>(src);
+    }
     const int items = (hi - lo) * (rep + 1) * (HH / 4);
-    for (int i = tid; i < items; i += 256) {
-        const int c = i % (HH / 4), r = i / (HH / 4) / (rep + 1), hv = i / (HH / 4) - r * (rep + 1), p = lo + r;
+    const uint32_t inv = 0xFFFFFFFFu / (uint32_t)(rep + 1) + 1;  // x / (rep + 1) = x inv >> 32 while x (rep + 1) < 2^32
+    for (int i = tid; i < items; i += NT) {
+        const int c = i % (HH / 4), x4 = i / (HH / 4), r = (int)__umulhi((uint32_t)x4, inv);
+        const int hv = x4 - r * (rep + 1), p = lo + r;
         const size_t t = (size_t)(s.t0 + (p - s.p0));
         const bool live = p >= vlo && p < vhi;
         int x = 0, y = 0;
@@ -100,11 +106,6 @@ __global__ __launch_bounds__(256) void pg_append_kernel(Paged a, const int8_t* _
     if (vlo >= vhi) return;
     const int id = pg_page(a, b, blk);
     if (id < 0) return;
-    for (int i = tid; i < (vhi - vlo) * CH; i += 256) {
-        const int p = vlo + i / CH, c = i % CH;
-        const int8_t* src = qkv + (size_t)(s.t0 + (p - s.p0)) * stride + (nh + a.nkv + g) * HD + 16 * c;
-        *reinterpret_cast<v4i*>(&sKV[1][p & 15][16 * c]) = *reinterpret_cast<const v4i*>(src);
-    }
     __syncthreads();
     const int r0 = vlo & 15, r1 = vhi - 16 * blk;  // the block's rows r0 .. r1 - 1
     const size_t part = ((size_t)id * a.nkv + g) * (size_t)a.part;
@@ -112,32 +113,32 @@ __global__ __launch_bounds__(256) void pg_append_kernel(Paged a, const int8_t* _
     if constexpr (BITS == 8) {
         uint8_t* kd = a.k + part + slot * HD;
         uint8_t* vd = a.v + part + slot * HD;
-        for (int i = tid; i < 16 * CH; i += 256) {
-            const int r = i / CH, c = i % CH;
-            if (r >= r0 && r < r1) *reinterpret_cast<v4i*>(kd + r * HD + 16 * c) = *reinterpret_cast<const v4i*>(&sKV[0][r][16 * c]);
-        }
-        for (int d = tid; d < HD; d += 256) {
-            if (r1 - r0 == 16) {
-                v4i w = {0, 0, 0, 0};
+        for (int i = tid; i < 16 * CH + 4 * HD; i += NT) {
+            if (i < 16 * CH) {  // a chunk of K
+                const int r = i / CH, c = i % CH;
+                if (r >= r0 && r < r1) *reinterpret_cast<v4i*>(kd + r * HD + 16 * c) = *reinterpret_cast<const v4i*>(&sKV[0][r][16 * c]);
+            } else {  // four positions of a dimension of V
+                const int d = (i - 16 * CH) >> 2, r = 4 * ((i - 16 * CH) & 3);
+                if (r >= r0 && r + 4 <= r1) {
+                    uint32_t w = 0;
 #pragma unroll
-                for (int r = 0; r < 16; r++) w[r >> 2] |= (int)(uint8_t)sKV[1][r][d] << (8 * (r & 3));
-                *reinterpret_cast<v4i*>(vd + 16 * d) = w;
-            } else {
-                for (int r = r0; r < r1; r++) vd[16 * d + r] = (uint8_t)sKV[1][r][d];
+                    for (int e = 0; e < 4; e++) w |= (uint32_t)(uint8_t)sKV[1][r + e][d] << (8 * e);
+                    *reinterpret_cast<uint32_t*>(vd + 16 * d + r) = w;
+                } else {
+                    for (int e = max(r, r0); e < min(r + 4, r1); e++) vd[16 * d + e] = (uint8_t)sKV[1][e][d];
+                }
             }
         }
     } else {
-        {  // 8 threads a row: its largest magnitude
-            const int w = tid >> 7, r = (tid >> 3) & 15, e = tid & 7;
+        constexpr int RT = HD / 4;  // threads of a row: its largest magnitude, four values each
+        for (int i = tid; i < 32 * RT; i += NT) {
+            const int w = i / (16 * RT), r = i / RT % 16, x = *reinterpret_cast<const int*>(&sKV[w][r][4 * (i % RT)]);
             int top = 0;
-            if (r >= r0 && r < r1)
-                for (int d = e; d < HD; d += 8) {
-                    const int x = sKV[w][r][d], m = x < 0 ? -x : x;
-                    top = m > top ? m : top;
-                }
 #pragma unroll
-            for (int d = 4; d >= 1; d >>= 1) top = max(top, __shfl_xor(top, d));
-            if (e == 0 && r >= r0 && r < r1) {
+            for (int e = 0; e < 4; e++) top = max(top, max(byte_of(x, e), -byte_of(x, e)));
+#pragma unroll
+            for (int o = RT / 2; o >= 1; o >>= 1) top = max(top, __shfl_xor(top, o));
+            if (i % RT == 0 && r >= r0 && r < r1) {
                 const int m = mult4(top);
                 sM[w][r] = m;
                 sInv[w][r] = mult4_inv(m);
@@ -147,55 +148,56 @@ __global__ __launch_bounds__(256) void pg_append_kernel(Paged a, const int8_t* _
         __syncthreads();
         uint8_t* kd = a.k + part + slot * HH;
         uint8_t* vd = a.v + part + slot * HH;
-        for (int i = tid; i < 16 * CH; i += 256) {
-            const int r = i / CH, c = i % CH;
-            if (r < r0 || r >= r1) continue;
-            const int m = sM[0][r], inv = sInv[0][r];
-            v2i w = {0, 0};
-#pragma unroll
-            for (int e = 0; e < 16; e++)
-                w[e >> 3] |= (code4(sKV[0][r][16 * c + e], m, inv) & 15) << (8 * (e & 3) + 4 * ((e >> 2) & 1));
-            *reinterpret_cast<v2i*>(kd + r * HH + 8 * c) = w;
-        }
-        for (int d = tid; d < HD; d += 256) {
-            v2i w = {0, 0};
-            if (r1 - r0 < 16) w = *reinterpret_cast<const v2i*>(vd + 8 * d);
-#pragma unroll
-            for (int r = 0; r < 16; r++) {
+        for (int i = tid; i < 32 * CH + 2 * HD; i += NT) {  // half a chunk, 8 codes, each
+            uint32_t w = 0;
+            if (i < 32 * CH) {
+                const int r = i / (2 * CH), x = i % (2 * CH);
                 if (r < r0 || r >= r1) continue;
-                const int sh = 8 * (r & 3) + 4 * ((r >> 2) & 1);
-                w[r >> 3] = (w[r >> 3] & ~(15 << sh)) | ((code4(sKV[1][r][d], sM[1][r], sInv[1][r]) & 15) << sh);
+                const int m = sM[0][r], inv = sInv[0][r];
+#pragma unroll
+                for (int e = 0; e < 8; e++) w |= (uint32_t)(code4(sKV[0][r][8 * x + e], m, inv) & 15) << (8 * (e & 3) + 4 * (e >> 2));
+                *reinterpret_cast<uint32_t*>(kd + r * HH + 4 * x) = w;
+            } else {
+                const int d = (i - 32 * CH) >> 1, r = 8 * ((i - 32 * CH) & 1);
+                if (r >= r1 || r + 8 <= r0) continue;
+                uint32_t* to = reinterpret_cast<uint32_t*>(vd + 8 * d + (r >> 1));
+                if (r < r0 || r + 8 > r1) w = *to;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    if (r + e < r0 || r + e >= r1) continue;
+                    const int sh = 8 * (e & 3) + 4 * (e >> 2);
+                    w = (w & ~(15u << sh)) | ((uint32_t)(code4(sKV[1][r + e][d], sM[1][r + e], sInv[1][r + e]) & 15) << sh);
+                }
+                *to = w;
             }
-            *reinterpret_cast<v2i*>(vd + 8 * d) = w;
         }
     }
 }
 
-// One CTA per block of 16 positions of a sequence, all its kv heads: K's chunks as they stand, V four dimensions a thread
-// (their 16 positions are four chunks side by side), so that 16 threads write one position's row.
+// One CTA per (block of 16 positions of a sequence, kv head), 2 HD threads: the first HD move K's chunks, the others take four
+// dimensions by four positions of V each (the chunks hold positions side by side, the rows dimensions).
 template <int HD, int BITS>
-__global__ __launch_bounds__(256) void pg_read_kernel(Paged a, int8_t* __restrict__ k, int8_t* __restrict__ v,
-                                                      int64_t max_pos, int nblk) {
+__global__ __launch_bounds__(2 * HD) void pg_read_kernel(Paged a, int8_t* __restrict__ k, int8_t* __restrict__ v,
+                                                         int64_t max_pos, int nblk) {
     constexpr int HH = HD / 2, CH = HD / 16;
-    const int b = (int)blockIdx.x / nblk, blk = (int)blockIdx.x - b * nblk;
+    const int b = (int)blockIdx.x / nblk, blk = (int)blockIdx.x - b * nblk, g = blockIdx.y;
     int end = min(pg_len(a, b), a.max_pages << a.page_sh);
     end = (int64_t)end < max_pos ? end : (int)max_pos;
     const int n = min(16, end - 16 * blk);
     if (n <= 0) return;
     const int id = pg_page(a, b, blk), slot = (16 * blk) & ((1 << a.page_sh) - 1);
-    const int8_t* kp = reinterpret_cast<const int8_t*>(a.k) + (size_t)(id < 0 ? 0 : id) * a.nkv * a.part;
-    const int8_t* vp = reinterpret_cast<const int8_t*>(a.v) + (size_t)(id < 0 ? 0 : id) * a.nkv * a.part;
-    const size_t out = ((size_t)b * max_pos + 16 * blk) * a.nkv * HD;
-    for (int i = threadIdx.x; i < n * a.nkv * CH; i += 256) {
-        const int c = i % CH, g = i / CH % a.nkv, r = i / CH / a.nkv;
+    const size_t part = ((size_t)(id < 0 ? 0 : id) * a.nkv + g) * (size_t)a.part, mult = part + (size_t)(HH << a.page_sh) + slot;
+    const size_t out = (((size_t)b * max_pos + 16 * blk) * a.nkv + g) * HD, row = (size_t)a.nkv * HD;
+    if (threadIdx.x < HD) {
+        const int c = threadIdx.x % CH, r = threadIdx.x / CH;
+        if (r >= n) return;
         v4i w = {0, 0, 0, 0};
         if (id >= 0) {
-            const int8_t* pg = kp + (size_t)g * a.part;
             if constexpr (BITS == 8) {
-                w = *reinterpret_cast<const v4i*>(pg + (slot + r) * HD + 16 * c);
+                w = *reinterpret_cast<const v4i*>(a.k + part + (slot + r) * HD + 16 * c);
             } else {
-                const v2i x = *reinterpret_cast<const v2i*>(pg + (slot + r) * HH + 8 * c);
-                const int m = (uint8_t)pg[(HH << a.page_sh) + slot + r];
+                const v2i x = *reinterpret_cast<const v2i*>(a.k + part + (slot + r) * HH + 8 * c);
+                const int m = a.k[mult + r];
 #pragma unroll
                 for (int e = 0; e < 16; e++) {
                     const int code = (x[e >> 3] << (28 - 8 * (e & 3) - 4 * ((e >> 2) & 1))) >> 28;
@@ -203,37 +205,31 @@ __global__ __launch_bounds__(256) void pg_read_kernel(Paged a, int8_t* __restric
                 }
             }
         }
-        *reinterpret_cast<v4i*>(k + out + ((size_t)r * a.nkv + g) * HD + 16 * c) = w;
+        *reinterpret_cast<v4i*>(k + out + r * row + 16 * c) = w;
+        return;
     }
-    for (int i = threadIdx.x; i < a.nkv * (HD / 4); i += 256) {
-        const int d = 4 * (i % (HD / 4)), g = i / (HD / 4);
-        int w[16];
+    const int d = 4 * ((threadIdx.x - HD) % (HD / 4)), t = (threadIdx.x - HD) / (HD / 4);  // positions 4 t .. 4 t + 3
+    if (4 * t >= n) return;
+    int w[4] = {0, 0, 0, 0};
+    if (id >= 0) {
+        int m = 0;
+        if constexpr (BITS == 4) m = *reinterpret_cast<const int*>(a.v + mult + 4 * t);
 #pragma unroll
-        for (int r = 0; r < 16; r++) w[r] = 0;
-        if (id >= 0) {
-            const int8_t* pg = vp + (size_t)g * a.part;
-            v4i m4 = {0, 0, 0, 0};
-            if constexpr (BITS == 4) m4 = *reinterpret_cast<const v4i*>(pg + (HH << a.page_sh) + slot);
+        for (int e = 0; e < 4; e++) {
+            if constexpr (BITS == 8) {
+                const int x = *reinterpret_cast<const int*>(a.v + part + slot * HD + 16 * (d + e) + 4 * t);
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                if constexpr (BITS == 8) {
-                    const v4i x = *reinterpret_cast<const v4i*>(pg + slot * HD + 16 * (d + e));
+                for (int r = 0; r < 4; r++) w[r] |= (byte_of(x, r) & 255) << (8 * e);
+            } else {
+                const int x = *reinterpret_cast<const int*>(a.v + part + slot * HH + 8 * (d + e) + 4 * (t >> 1)) << (4 - 4 * (t & 1));
 #pragma unroll
-                    for (int r = 0; r < 16; r++) w[r] |= (byte_of(x[r >> 2], r & 3) & 255) << (8 * e);
-                } else {
-                    const v2i x = *reinterpret_cast<const v2i*>(pg + slot * HH + 8 * (d + e));
-#pragma unroll
-                    for (int r = 0; r < 16; r++) {
-                        const int code = (x[r >> 3] << (28 - 8 * (r & 3) - 4 * ((r >> 2) & 1))) >> 28;
-                        w[r] |= (value4(code, (m4[r >> 2] >> (8 * (r & 3))) & 255) & 255) << (8 * e);
-                    }
-                }
+                for (int r = 0; r < 4; r++) w[r] |= (value4((x << (24 - 8 * r)) >> 28, (m >> (8 * r)) & 255) & 255) << (8 * e);
             }
         }
-#pragma unroll
-        for (int r = 0; r < 16; r++)
-            if (r < n) *reinterpret_cast<int*>(v + out + ((size_t)r * a.nkv + g) * HD + d) = w[r];
     }
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+        if (4 * t + r < n) *reinterpret_cast<int*>(v + out + (4 * t + r) * row + d) = w[r];
 }
 
 // The greedy choice. A key is (value, then the lower index) in 64 bits, the largest key the first maximum:
@@ -286,18 +282,24 @@ hipError_t launch_pg_append(const Paged& a, int hd, int bits, const int8_t* qkv,
                             const int16_t* cosT, const int16_t* sinT, int max_pos, int8_t* q, int64_t q_stride,
                             hipStream_t s) {
     const dim3 grid((unsigned)(a.tokens / 16 + 2 * a.seqs), (unsigned)a.nkv);
-    auto go = [&](auto kern) {
-        kern<<<grid, dim3(256), 0, s>>>(a, qkv, stride, nh, cosT, sinT, max_pos, q, q_stride);
+    // blocks that rows fill have work for many threads, a single token's for few
+    const bool many = a.tokens >= 8 * (int64_t)a.seqs;
+    auto go = [&](auto few, auto lots) {
+        if (many) lots<<<grid, dim3(1024), 0, s>>>(a, qkv, stride, nh, cosT, sinT, max_pos, q, q_stride);
+        else few<<<grid, dim3(256), 0, s>>>(a, qkv, stride, nh, cosT, sinT, max_pos, q, q_stride);
         return hipGetLastError();
     };
-    if (hd == 64) return bits == 8 ? go(pg_append_kernel<64, 8>) : go(pg_append_kernel<64, 4>);
-    return bits == 8 ? go(pg_append_kernel<128, 8>) : go(pg_append_kernel<128, 4>);
+    if (hd == 64)
+        return bits == 8 ? go(pg_append_kernel<64, 8, 256>, pg_append_kernel<64, 8, 1024>)
+                         : go(pg_append_kernel<64, 4, 256>, pg_append_kernel<64, 4, 1024>);
+    return bits == 8 ? go(pg_append_kernel<128, 8, 256>, pg_append_kernel<128, 8, 1024>)
+                     : go(pg_append_kernel<128, 4, 256>, pg_append_kernel<128, 4, 1024>);
 }
 
 hipError_t launch_pg_read(const Paged& a, int hd, int bits, int8_t* k, int8_t* v, int64_t max_pos, hipStream_t s) {
     const int nblk = (int)((std::min<int64_t>(max_pos, (int64_t)a.max_pages << a.page_sh) + 15) / 16);
     auto go = [&](auto kern) {
-        kern<<<dim3((unsigned)(a.seqs * nblk)), dim3(256), 0, s>>>(a, k, v, max_pos, nblk);
+        kern<<<dim3((unsigned)(a.seqs * nblk), (unsigned)a.nkv), dim3(2 * hd), 0, s>>>(a, k, v, max_pos, nblk);
         return hipGetLastError();
     };
     if (hd == 64) return bits == 8 ? go(pg_read_kernel<64, 8>) : go(pg_read_kernel<64, 4>);
