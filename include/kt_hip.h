@@ -860,8 +860,8 @@ int kt_hip_dec_embed_argmax(int dev, const uint64_t* part_dev, int64_t nparts, c
  * 8 h + 4 + r in its high half, and a part ends with its slots' multipliers (page bytes): a row x of hd values is held as
  * m = ceil(8 max |x| / 7) and the codes c = clamp(round_half_away(8 x / m), +-7) (0 when m is 0), and stands for c m / 8.
  *
- * max_pages * page <= KT_PAGED_MAX_POS; nh <= 4096; tokens * nh and 2 * seqs * nh below 2^31. Pointers and strides (in elements) of
- * int8 rows are multiples of 16.
+ * max_pages * page <= KT_PAGED_MAX_POS; nh <= 4096; (tokens + 32 seqs) * nh < 2^27. Pointers and strides (in elements) of int8
+ * rows are multiples of 16.
  * ------------------------------------------------------------------------------------------------------------- */
 #define KT_PAGED_MAX_POS 524288
 /* Bytes of one kv head's part of a page in one pool; 0 for a page, hd or bits outside the above. */
@@ -880,7 +880,7 @@ int kt_hip_dec_rope_kv_paged(int dev, const int8_t* qkv_dev, int64_t tokens, int
 /* The pages back as contiguous rows: position j < min(kv_len[b], max_pos, max_pages * page) of every sequence to
  * k_dev / v_dev [seqs][max_pos][nkv][hd] int8 (with seqs = 1 the caches of kt_hip_dec_attention); positions past those
  * are left as they were. With 4 bits the values are clamp(round_half_away(c m / 8), +-127); a position without a page is
- * zeros. */
+ * zeros. seqs times the blocks of 16 positions below min(max_pos, max_pages * page) stays below 2^24. */
 int kt_hip_dec_kv_read_paged(int dev, const void* kpool_dev, const void* vpool_dev, int64_t pages, int64_t page,
                              int bits, const int32_t* kv_len_dev, const int32_t* table_dev, int64_t seqs,
                              int64_t max_pages, int64_t nkv, int64_t hd, int8_t* k_dev, int8_t* v_dev, int64_t max_pos,
@@ -888,8 +888,9 @@ int kt_hip_dec_kv_read_paged(int dev, const void* kpool_dev, const void* vpool_d
 /* Causal GQA attention of the new rows (chunks and single tokens alike) over their sequences' pages, rows of q_dev as
  * kt_hip_dec_rope_kv_paged leaves them, after the call that wrote the rows' own k and v. A row at p sees the positions
  * j <= p that have a page and, with window >= 1, are within it (j > p - window) or among the first `sinks`; window = 0
- * sees all. s_j = q . k_j (q of -128, which RoPE never gives, as -127; 4 bits: (m_j (q . c_j) + 4) >> 3), e_j = exp_tab[(max s - s_j + 64) >> 7] with entries clamped
- * to [0, 2^15] and 0 past the 1024th, o = clamp(round_half_away(sum e_j v_j / sum e_j)), 0 where the sum of e is 0.
+ * sees all. s_j = q . k_j (q of -128, which RoPE never gives, as -127; 4 bits: (m_j (q . c_j) + 4) >> 3),
+ * e_j = exp_tab[(max s - s_j + 64) >> 7] with entries clamped to [0, 2^15] and 0 past the 1024th,
+ * o = clamp(round_half_away(sum e_j v_j / sum e_j)), 0 where the sum of e is 0.
  * ws_dev: kt_hip_dec_attention_paged_workspace bytes of scratch, 16-byte aligned, needing no contents; calls that may
  * overlap need one each. */
 size_t kt_hip_dec_attention_paged_workspace(int64_t tokens, int64_t seqs, int64_t max_pages, int64_t page, int64_t nh,

@@ -94,6 +94,20 @@ def test_attend_many_sequences(torch_dev):
     check_attend(torch_dev, Case(7, [(1, 40 + 3 * i) for i in range(130)], 4, 2, 64, 16, 8))
 
 
+@pytest.mark.parametrize("bits,hd", [(8, 64), (4, 64), (8, 128), (4, 128)])
+@pytest.mark.parametrize("seqs,nkv,window", [(150, 2, 0), (150, 2, 50), (420, 4, 0), (420, 4, 33)])
+def test_attend_more_units_than_cus(torch_dev, seqs, nkv, window, bits, hd):
+    """Single tokens, sequences without rows and chunks, more column tiles than CUs and many times as many."""
+    lens = [(60, 90 + i) if i % 100 == 7 else (int(i % 9 > 0), 1 + (i * 53) % 140) for i in range(seqs)]
+    check_attend(torch_dev, Case(60, lens, 4 * nkv if seqs < 400 else nkv, nkv, hd, 16, bits, behind=2), window, 3)
+
+
+@pytest.mark.parametrize("bits,hd", [(8, 64), (4, 64), (8, 128), (4, 128)])
+@pytest.mark.parametrize("window", [0, 2100])
+def test_attend_chunk_behind_more_than_a_cta_keeps(torch_dev, window, bits, hd):
+    check_attend(torch_dev, Case(61, [(160, 2600), (1, 4100), (3, 4000)], 7, 1, hd, 16, bits), window, 70)
+
+
 @pytest.mark.parametrize("bits", [8, 4])
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (7, 3), (64, 0), (65, 4), (100, 20), (300, 64), (128, 1000), (5000, 4), (2 ** 31 - 1, 2 ** 31 - 1)])
 def test_attend_window(torch_dev, window, sinks, bits):
@@ -171,6 +185,19 @@ def test_append_and_read(torch_dev, nh, nkv, hd, page, bits):
         d.kv.read(d.b, *got)
         same(got[0], want[0], f"read k {max_pos}")
         same(got[1], want[1], f"read v {max_pos}")
+
+
+@pytest.mark.parametrize("bits,hd", [(8, 64), (4, 64), (8, 128), (4, 128)])
+def test_append_many_sequences(torch_dev, bits, hd):
+    """More blocks than the chip takes at once: single tokens and chunks, begun and ended inside blocks."""
+    lens = [(50, 70 + i) if i % 40 == 3 else (int(i % 7 > 0), 1 + (i * 29) % 90) for i in range(130)]
+    c = Case(22, lens, 8, 4, hd, 32, bits, behind=2, pad=16)
+    cos, sin = rope_tables(200, hd)
+    d = Dev(torch_dev, c)
+    q, k, v = c.append(cos, sin, FILL)
+    same(d.append(cos, sin), q, "q")
+    same(d.kv.k, k.view(np.int8), "k pool")
+    same(d.kv.v, v.view(np.int8), "v pool")
 
 
 @pytest.mark.parametrize("bits", [8, 4])

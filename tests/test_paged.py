@@ -103,6 +103,15 @@ REFUSED = (
 )
 
 
+# past a grid's threads, just
+BIG = [dict(tokens=1 << 25, qkv_stride=512), dict(tokens=(1 << 25) - 32, seqs=1), dict(seqs=1 << 20), dict(nh=4098, nkv=2, q_stride=1 << 20)]
+REFUSED += (
+    [("kt_hip_dec_rope_kv_paged", APPEND, {**{k: v for k, v in x.items() if k in APPEND}, **({"qkv_stride": 1 << 20} if "nh" in x else {})}) for x in BIG]
+    + [("kt_hip_dec_attention_paged", ATTEND, {**{k: v for k, v in x.items() if k in ATTEND}, **({"o_stride": 1 << 20} if "nh" in x else {})}) for x in BIG]
+    + [("kt_hip_dec_kv_read_paged", READ, dict(seqs=1 << 20, max_pos=256, max_pages=16)), ("kt_hip_dec_kv_read_paged", READ, dict(seqs=1 << 21))]
+)
+
+
 @pytest.mark.parametrize("name,args,change", REFUSED, ids=[f"{n[11:]}-{'-'.join(f'{k}={v}' for k, v in x.items())}" for n, _, x in REFUSED])
 def test_refused_before_any_device_work(name, args, change):
     assert getattr(_lib(), name)(*{**args, **change}.values()) == 1  # hipErrorInvalidValue

@@ -1033,12 +1033,13 @@ int kt_hip_dec_embed_argmax(int dev, const uint64_t* part_dev, int64_t nparts, c
 }
 
 // The geometry that every call on paged caches checks: {page, hd, bits} of the layout, heads and batch within the kernels'
-// 32-bit counts. Device arrays are only dereferenced on the device.
+// 32-bit counts and a grid's 2^32 threads (16 columns or 16 rows to at most 512 threads, two such blocks a sequence). Device
+// arrays are only dereferenced on the device.
 static bool paged_ok(int64_t tokens, int64_t seqs, int64_t max_pages, int64_t nh, int64_t nkv, int64_t hd,
                      int64_t pages, int64_t page, int bits) {
     return kt_hip_dec_page_bytes(page, hd, bits) != 0 && nkv >= 1 && nh >= nkv && nh % nkv == 0 && nh <= 4096 &&
-           tokens >= 0 && seqs >= 0 && tokens <= INT_MAX / nh && tokens <= 1 << 30 && seqs <= INT_MAX / (2 * nh) && max_pages >= 1 &&
-           max_pages <= KT_PAGED_MAX_POS / page && pages >= 0 && pages <= INT_MAX;
+           tokens >= 0 && seqs >= 0 && tokens < 1 << 27 && seqs < 1 << 22 && (tokens + 32 * seqs) * nh < 1 << 27 &&
+           max_pages >= 1 && max_pages <= KT_PAGED_MAX_POS / page && pages >= 0 && pages <= INT_MAX;
 }
 
 static bool aligned_to(const void* p, size_t n) { return p != nullptr && (uintptr_t)p % n == 0; }
@@ -1085,7 +1086,7 @@ int kt_hip_dec_kv_read_paged(int dev, const void* kpool_dev, const void* vpool_d
                              int64_t max_pages, int64_t nkv, int64_t hd, int8_t* k_dev, int8_t* v_dev, int64_t max_pos,
                              void* stream) {
     if (!paged_ok(0, seqs, max_pages, nkv, nkv, hd, pages, page, bits) || max_pos < 0 ||
-        (max_pos > 0 && seqs > INT_MAX / ((std::min(max_pos, max_pages * page) + 15) / 16)))
+        seqs * ((std::min(max_pos, max_pages * page) + 15) / 16) >= 1 << 24)
         return (int)hipErrorInvalidValue;
     if (seqs == 0 || max_pos == 0) return 0;
     if (!kv_len_dev || !table_dev || !aligned_to(k_dev, 16) || !aligned_to(v_dev, 16) ||
