@@ -282,10 +282,12 @@ hipError_t launch_pg_append(const Paged& a, int hd, int bits, const int8_t* qkv,
                             const int16_t* cosT, const int16_t* sinT, int max_pos, int8_t* q, int64_t q_stride,
                             hipStream_t s) {
     const dim3 grid((unsigned)(a.tokens / 16 + 2 * a.seqs), (unsigned)a.nkv);
-    // blocks that rows fill have work for many threads, a single token's for few
-    const bool many = a.tokens >= 8 * (int64_t)a.seqs;
+    // Few CTAs get more threads each, as long as the chip holds them side by side (two of 1024 a CU, some of them empty). us
+    // with 256 / 1024: 132 single tokens' CTAs 4-bit 5.0 / 4.6, a chunk of 100 rows 5.0 / 4.2, 512 rows 4-bit 6.7 / 5.6, 498 CTAs
+    // 7.2 / 6.8, 520 (hd 128, 4-bit) 13.2 / 10.6; 948 9.8 / 11.1, 1008 (hd 128, 4-bit) 16.0 / 17.1, 1056 of single tokens 4.9 / 7.4.
+    const bool wide = (int64_t)grid.x * grid.y <= 768;
     auto go = [&](auto few, auto lots) {
-        if (many) lots<<<grid, dim3(1024), 0, s>>>(a, qkv, stride, nh, cosT, sinT, max_pos, q, q_stride);
+        if (wide) lots<<<grid, dim3(1024), 0, s>>>(a, qkv, stride, nh, cosT, sinT, max_pos, q, q_stride);
         else few<<<grid, dim3(256), 0, s>>>(a, qkv, stride, nh, cosT, sinT, max_pos, q, q_stride);
         return hipGetLastError();
     };
