@@ -234,30 +234,32 @@ __global__ __launch_bounds__(2 * HD) void pg_read_kernel(Paged a, int8_t* __rest
 
 // The greedy choice. A key is (value, then the lower index) in 64 bits, the largest key the first maximum:
 // ((v ^ 2^31) << 32) | (2^32 - 1 - i).
+template <int NT>
 __device__ __forceinline__ uint64_t block_max_key(uint64_t best, uint64_t* s_key) {
     best = (uint64_t)wave_max_i64((int64_t)(best ^ (1ull << 63))) ^ (1ull << 63);
     if ((threadIdx.x & 63) == 0) s_key[threadIdx.x >> 6] = best;
     __syncthreads();
     best = s_key[0];
 #pragma unroll
-    for (int q = 1; q < 4; q++) best = s_key[q] > best ? s_key[q] : best;
+    for (int q = 1; q < NT / 64; q++) best = s_key[q] > best ? s_key[q] : best;
     return best;
 }
 
 // Grid (parts, rows): the best key of a part of a row; with one part a row, its index is the answer.
-__global__ __launch_bounds__(256) void pg_argmax_kernel(const int32_t* __restrict__ logits, int n, int64_t stride,
+template <int NT>
+__global__ __launch_bounds__(NT) void pg_argmax_kernel(const int32_t* __restrict__ logits, int n, int64_t stride,
                                                         int per, uint64_t* __restrict__ part,
                                                         int32_t* __restrict__ token) {
-    __shared__ uint64_t s_key[4];
+    __shared__ uint64_t s_key[NT / 64];
     const int32_t* x = logits + (size_t)blockIdx.y * stride;
     const uint32_t i0 = blockIdx.x * (uint32_t)per, i1 = min(i0 + (uint32_t)per, (uint32_t)n);
     uint64_t best = 0;
 #pragma unroll 8
-    for (uint32_t i = i0 + threadIdx.x; i < i1; i += 256) {
+    for (uint32_t i = i0 + threadIdx.x; i < i1; i += NT) {
         const uint64_t key = ((uint64_t)((uint32_t)x[i] ^ 0x80000000u) << 32) | (0xFFFFFFFFu - i);
         best = key > best ? key : best;
     }
-    best = block_max_key(best, s_key);
+    best = block_max_key<NT>(best, s_key);
     if (threadIdx.x == 0) {
         if (gridDim.x == 1) token[blockIdx.y] = (int32_t)(0xFFFFFFFFu - (uint32_t)best);
         else part[(size_t)blockIdx.y * gridDim.x + blockIdx.x] = best;
@@ -272,7 +274,7 @@ __global__ __launch_bounds__(256) void pg_argmax_join_kernel(const uint64_t* __r
         const uint64_t key = part[(size_t)blockIdx.x * parts + i];
         best = key > best ? key : best;
     }
-    best = block_max_key(best, s_key);
+    best = block_max_key<256>(best, s_key);
     if (threadIdx.x == 0) token[blockIdx.x] = (int32_t)(0xFFFFFFFFu - (uint32_t)best);
 }
 
@@ -308,14 +310,20 @@ hipError_t launch_pg_read(const Paged& a, int hd, int bits, int8_t* k, int8_t* v
     return bits == 8 ? go(pg_read_kernel<128, 8>) : go(pg_read_kernel<128, 4>);
 }
 
+// One CTA a row saves the second launch, and reads what is left of a long row alone. us a call, one / parts: 1 row of 4097 to 32768
+// 4.4 / 7.2, of 65536 5.1 / 7.2, of 151936 11.8 / 7.3; 64 rows of 65536 6.4 / 7.1, of 151936 17.7 / 11.2. Parts are of 4096 logits,
+// the rows' parts together some 2048 CTAs.
 int pg_argmax_parts(int64_t rows, int64_t n) {
+    if (n <= 65536) return 1;
     return (int)std::max<int64_t>(1, std::min((n + 4095) / 4096, (2048 + rows - 1) / std::max<int64_t>(rows, 1)));
 }
 
 hipError_t launch_pg_argmax(const int32_t* logits, int rows, int n, int64_t stride, int32_t* token, uint64_t* part,
                             hipStream_t s) {
     const int parts = pg_argmax_parts(rows, n), per = (int)(((int64_t)n + parts - 1) / parts);
-    pg_argmax_kernel<<<dim3((unsigned)parts, (unsigned)rows), dim3(256), 0, s>>>(logits, n, stride, per, part, token);
+    const dim3 grid((unsigned)parts, (unsigned)rows);
+    if (parts == 1) pg_argmax_kernel<1024><<<grid, dim3(1024), 0, s>>>(logits, n, stride, per, part, token);
+    else pg_argmax_kernel<256><<<grid, dim3(256), 0, s>>>(logits, n, stride, per, part, token);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || parts == 1) return e;
     pg_argmax_join_kernel<<<dim3((unsigned)rows), dim3(256), 0, s>>>(part, parts, token);
