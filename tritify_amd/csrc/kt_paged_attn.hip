@@ -84,12 +84,13 @@ __device__ __forceinline__ int pg_swz(int n, int r) {
 
 // Four neighbouring dimensions of an output row: clamp(round_half_away(sum e v / sum e)) of what the digits add up to (8
 // bits: both negated; 4 bits: v as 16 codes times 1/8 of a multiplier), zeros where nothing was seen. The quotients
-// floor((2 |a| + b) / (2 b)) are double estimates by one reciprocal (within one of the exact quotient, which is below 2^8 past
-// the first test) and the exact remainders.
+// floor((2 |a| + b) / (2 b)), at most 128 past the first test, are float estimates by one reciprocal (off by less than 2^-13: at
+// most one from the exact quotient) and the exact remainders.
 template <int BITS>
 __device__ __forceinline__ void pg_store(int8_t* to, const int64_t (&v)[4], int64_t dn, bool live) {
     const uint64_t b = (uint64_t)(BITS == 8 ? -dn : 128 * dn), d = 2 * b;
-    const double rd = 1.0 / (double)d;
+    auto f = [](uint64_t x) { return __builtin_fmaf((float)(uint32_t)(x >> 32), 4294967296.0f, (float)(uint32_t)x); };
+    const float rd = __builtin_amdgcn_rcpf(f(d));
     uint32_t out = 0;
     if (live && (int64_t)b > 0)
 #pragma unroll
@@ -98,7 +99,7 @@ __device__ __forceinline__ void pg_store(int8_t* to, const int64_t (&v)[4], int6
             const uint64_t m = a < 0 ? 0 - (uint64_t)a : (uint64_t)a, n = 2 * m + b;
             int q = 127;
             if (m < 128 * b) {
-                q = (int)((double)n * rd);
+                q = (int)(f(n) * rd);
                 const int64_t rem = (int64_t)(n - (uint64_t)(uint32_t)q * d);
                 q += rem < 0 ? -1 : (rem >= (int64_t)d ? 1 : 0);
                 q = q > 127 ? 127 : q;
@@ -237,7 +238,22 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(W == 8 |
             }
         }
     };
-    auto sees = [&](int j) { return (j <= pos) & ((p.window == 0) | (j > pos - p.window) | (j < p.sinks)); };
+    // what the column sees of a tile's block: its positions k <= hi and, with a window, k > lo or k < sink
+    struct Mask {
+        int hi, lo, sink;
+    };
+    auto mask_of = [&](int T, bool ok) {
+        const int from = 64 * T + 16 * gq;
+        return Mask{ok ? pos - from : -1, pos - p.window - from, p.sinks - from};
+    };
+    auto sees = [](auto how, const Mask& m, int k) {
+        if constexpr (how == 0) return true;
+        else if constexpr (how == 1) return k <= m.hi;
+        else return (k <= m.hi) & ((k > m.lo) | (k < m.sink));
+    };
+    typedef std::integral_constant<int, 0> All;  // every position; those up to the column's own; and with a window
+    typedef std::integral_constant<int, 1> Causal;
+    typedef std::integral_constant<int, 2> Window;
     // whether every column sees every position of the tile (uniform)
     auto full = [&](int T, bool ok) {
         return __all(ok) && 64 * T + 63 <= pmin && (p.window == 0 || 64 * T > pmax - p.window || 64 * T + 63 < p.sinks);
@@ -299,14 +315,18 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(W == 8 |
 #pragma unroll
                     for (int t = 0; t < 4; t++) *kept_place(n, t) = sc[t];
                 }
+                auto least = [&](auto how) {
+                    const Mask k = mask_of(T, ok);
 #pragma unroll
-                for (int t = 0; t < 4; t++) {
-                    if (!all) {
+                    for (int t = 0; t < 4; t++) {
 #pragma unroll
-                        for (int r = 0; r < 4; r++) sc[t][r] = ok & sees(64 * T + 16 * gq + 4 * t + r) ? sc[t][r] : INT_MAX;
+                        for (int r = 0; r < 4; r++) sc[t][r] = sees(how, k, 4 * t + r) ? sc[t][r] : INT_MAX;
+                        low = min(min(low, min(sc[t].x, sc[t].y)), min(sc[t].z, sc[t].w));
                     }
-                    low = min(min(low, min(sc[t].x, sc[t].y)), min(sc[t].z, sc[t].w));
-                }
+                };
+                if (all) least(All());
+                else if (p.window == 0) least(Causal());
+                else least(Window());
             }
         }
         low = min(low, __shfl_xor(low, 16));
@@ -357,14 +377,15 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(W == 8 |
         };
         // The weights' digits as B operands: the table index is y >> 8, bytes 1 and 2 of y (|s| is at most 2^21, so y < 2^24
         // wherever the column sees the position; of other columns any index below 2^16 will do).
-        auto weights = [&](auto masked, int T, bool ok, v4i m, const v4i (&y)[4], v4i (&P)[ND]) {
+        auto weights = [&](auto how, int T, bool ok, v4i m, const v4i (&y)[4], v4i (&P)[ND]) {
+            const Mask k = mask_of(T, ok);
 #pragma unroll
             for (int t = 0; t < 4; t++) {
                 uint32_t u[4];
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     u[r] = (uint32_t)y[t][r];
-                    if constexpr (masked) u[r] = ok & sees(64 * T + 16 * gq + 4 * t + r) ? u[r] : 0x00FFFFFFu;
+                    u[r] = sees(how, k, 4 * t + r) ? u[r] : 0x00FFFFFFu;
                 }
                 us2 e[2];
 #pragma unroll
@@ -396,8 +417,9 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(W == 8 |
         };
         auto add_v = [&](int T, bool ok, const Tile& v, const v4i (&y)[4]) {
             v4i P[ND];
-            if (full(T, ok)) weights(std::false_type(), T, ok, v.m, y, P);
-            else weights(std::true_type(), T, ok, v.m, y, P);
+            if (full(T, ok)) weights(All(), T, ok, v.m, y, P);
+            else if (p.window == 0) weights(Causal(), T, ok, v.m, y, P);
+            else weights(Window(), T, ok, v.m, y, P);
 #pragma unroll
             for (int d = 0; d < DT; d++)
 #pragma unroll
@@ -476,9 +498,9 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(W == 8 |
             atomicAdd(reinterpret_cast<unsigned long long*>(&sDen[l16]), (unsigned long long)dn);
         }
         __syncthreads();
+        int8_t* const out = p.o + (size_t)(s.t0 + row) * p.o_stride + head * HD;  // (it % 16 is this thread's l16)
         auto put = [&](int it, const int64_t (&v)[4], int64_t dn) {  // dimensions 16 (it / 64) + 4 (it % 64 / 16) ..
-            const int m = m0 + (it & 15), i = m / p.rep, h = g * p.rep + m - i * p.rep, pp = s.p0 + i;
-            pg_store<BITS>(p.o + (size_t)(s.t0 + i) * p.o_stride + h * HD + 16 * (it >> 6) + 4 * ((it & 63) >> 4), v, dn, pp >= 0 && pp < cap);
+            pg_store<BITS>(out + 16 * (it >> 6) + 4 * ((it & 63) >> 4), v, dn, pos >= 0);
         };
         for (int it = tid; it < DT * 64; it += NT) {
             if ((it & 15) >= cols) continue;
