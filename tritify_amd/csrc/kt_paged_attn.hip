@@ -132,11 +132,10 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(W == 8 |
     }
 
     // The kv head fastest: CTAs go to the XCDs in turn, so an XCD's L2 holds the heads congruent to it. Column tiles 0 .. seqs -
-    // 1 are the sequences' first ones, the rest their further ones (from the last: of a prompt's, those see the most). With
-    // 8 waves a CTA the first ones go first: there single tokens may have no others, and CTAs that leave at once between
-    // those that stay would leave the XCDs different numbers of them (256 on 256 CUs took two rounds: 68 us against 50).
-    const int ntiles = (int)gridDim.x / a.nkv, g = (int)blockIdx.x % a.nkv, order = (int)blockIdx.x / a.nkv;
-    const int tile = W == 8 ? order : ntiles - 1 - order;
+    // 1 are the sequences' first ones, the rest their further ones, from the last (of a prompt's, those see the most). Single
+    // tokens may have first ones alone: CTAs that leave at once between those that stay would leave the XCDs different numbers
+    // of them (numbered sequence by sequence, 256 on 256 CUs took two rounds: 68 us against 50).
+    const int ntiles = (int)gridDim.x / a.nkv, g = (int)blockIdx.x % a.nkv, tile = ntiles - 1 - (int)blockIdx.x / a.nkv;
     int b = tile, nth = 0;
     if (tile >= a.seqs) {
         int first = 0;
@@ -261,7 +260,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(W == 8 |
 
     // PG_KEEP: as many of the wave's tiles as the LDS holds keep their scores, a column's 16 bytes at a time (lanes side by
     // side); the others' are formed again from K, last tile first: its K is nearest. 128 single tokens behind about 6100
-    // positions 53 -> 50 us.
+    // positions 52.1 -> 48.2 us.
     const int kept = MODE == PG_KEEP ? min(mine, p.keep / (256 * W * cols)) : 0;
     auto kept_place = [&](int n, int t) { return reinterpret_cast<v4i*>(sS) + (((n * W + w) * 4 + t) * 4 + gq) * cols + l16; };
     // V's ring over the kept tiles; at hd 64 there are registers to begin it before the maximum is known
@@ -537,12 +536,19 @@ struct Plan {
 
 // From the counts that the host knows. A unit is a column tile of one kv head. Waves: 8 a CTA, one CTA a CU, while the units
 // fit the CUs; else 4, and 2 where that fills the chip by itself (a CTA's waves share its columns, so fewer of them join less).
-// us with 2 / 4 / 8, 14 heads over 2, hd 64: 64 rows behind 4000 positions (56 units) 36.6 / 23.6 / 18.3; 512 behind 4000 (448)
-// 47.1 / 30.6 / 36.8; 1024 alone (896) 15.2 / 12.1 / 27.9; 3 x 1021 alone (2682) 25.4 / 28.2 / 72.5. A wave never has more than
+// us with 2 / 4 / 8, 14 heads over 2, hd 64: 64 rows behind 4000 positions (56 units) 36.6 / 23.2 / 17.5; 512 behind 4000 (448)
+// 47.2 / 31.2 / 37.9; 1024 alone (896) 15.8 / 13.0 / 25.8; 3 x 1021 alone (2682) 26.8 / 30.1 / 68.5. A wave never has more than
 // 65536 positions: its digit sums stay within 2^14 2^16. Splits, where units leave CUs without one: to 128 CTAs, of at least 8
 // tiles; past that the extra launch, the second reading of K and the sums that meet in memory outweigh it. us with 1 / the
-// rule's / twice its splits: one token behind 131000 (2 units) 373 / 19.9 / 19.8, 4 behind 32000 (8) 98 / 19.4 / 24.1, 16 behind
-// 8000 (32) 31.1 / 19.5 / 19.7, 64 (128) 34.4 / 34.4 / 42.1; behind 2000 it gains nothing (12.2 / 11.8).
+// rule's / twice its splits: one token behind 131000 (2 units) 363 / 20.3 / 20.9, 4 behind 32000 (8) 95.5 / 19.8 / 24.2, 16 behind
+// 8000 (32) 30.0 / 20.0 / 19.8, 64 (128) 39.5 / 39.5 / 44.5; below 64 tiles it gains nothing (behind 2000 11.2 / 11.9 with two).
+//
+// Kernel times against the bytes and operations that cannot be left out (4 hd a column and visible position): 128 single tokens
+// behind 6100 positions 48.2 us, 199 MB of K and V at 4.1 TB/s (the loads of ragged lengths end unevenly; a plain read of as much
+// reaches 5.9); one token behind 131000 4-bit positions 7 + 15 us for 17 MB (two launches, 32 tiles a wave and a join each); 1024
+// rows behind 7777 83 us, 0.37 of 2.1 int8 POPS counted once (pass 1 forms the scores a second time, weights take two digits);
+// there matrix units, vector units and LDS are each busy 24, 50 and 57 % of the time and a wave waits for one of them in turn:
+// 4 waves on 64 columns sharing a tile's K and V in LDS (a third of the reads from the L2) took 87 us.
 Plan plan(int64_t tokens, int64_t seqs, int64_t max_pos, int rep, int nkv) {
     const int64_t tiles = seqs + tokens * rep / PG_COLS, steps = max_pos / 64;
     const int64_t units = std::min(tiles, tokens * ((rep + PG_COLS - 1) / PG_COLS)) * nkv;
