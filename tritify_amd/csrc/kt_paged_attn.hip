@@ -82,30 +82,41 @@ __device__ __forceinline__ int pg_swz(int n, int r) {
     else return HD == 64 ? n : ((r >> 1) & 1) | (n << 1);
 }
 
-// Four neighbouring dimensions of an output row: clamp(round_half_away(sum e v / sum e)) of what the digits add up to (8
-// bits: both negated; 4 bits: v as 16 codes times 1/8 of a multiplier), zeros where nothing was seen. The quotients
-// floor((2 |a| + b) / (2 b)), at most 128 past the first test, are float estimates by one reciprocal (off by less than 2^-13: at
-// most one from the exact quotient) and the exact remainders.
+// Four neighbouring dimensions of an output row: clamp(round_half_away(a / b)), a = sum e v and b = sum e as the digits add up (8
+// bits: both negated; 4 bits: v as 16 codes times 1/8 of a multiplier, so 128 sum e), zeros where nothing was seen. The quotient
+// is a float estimate (relative error below 2^-20, so below 2^-12 for |a / b| < 256); where that is within 2^-12 of a half the
+// exact remainder of 2 |a| + b by 2 b says which side.
 template <int BITS>
 __device__ __forceinline__ void pg_store(int8_t* to, const int64_t (&v)[4], int64_t dn, bool live) {
-    const uint64_t b = (uint64_t)(BITS == 8 ? -dn : 128 * dn), d = 2 * b;
+    const int64_t b = BITS == 8 ? -dn : 128 * dn;
     auto f = [](uint64_t x) { return __builtin_fmaf((float)(uint32_t)(x >> 32), 4294967296.0f, (float)(uint32_t)x); };
-    const float rd = __builtin_amdgcn_rcpf(f(d));
     uint32_t out = 0;
-    if (live && (int64_t)b > 0)
+    if (live && b > 0) {
+        const float rb = __builtin_amdgcn_rcpf(f((uint64_t)b));
+        uint64_t m[4];
+        int q[4];
+        bool unsure = false;
 #pragma unroll
         for (int r = 0; r < 4; r++) {
-            const int64_t a = BITS == 8 ? -v[r] : v[r];
-            const uint64_t m = a < 0 ? 0 - (uint64_t)a : (uint64_t)a, n = 2 * m + b;
-            int q = 127;
-            if (m < 128 * b) {
-                q = (int)(f(n) * rd);
-                const int64_t rem = (int64_t)(n - (uint64_t)(uint32_t)q * d);
-                q += rem < 0 ? -1 : (rem >= (int64_t)d ? 1 : 0);
-                q = q > 127 ? 127 : q;
-            }
-            out |= (uint32_t)(uint8_t)(a < 0 ? -q : q) << (8 * r);
+            m[r] = v[r] < 0 ? 0 - (uint64_t)v[r] : (uint64_t)v[r];
+            const float t = f(m[r]) * rb + 0.5f;
+            unsure |= !(__builtin_fabsf(__builtin_amdgcn_fractf(t) - 0.5f) < 0.5f - 0x1p-12f);
+            q[r] = (int)t;
         }
+        if (unsure) {
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const uint64_t n = 2 * m[r] + (uint64_t)b, d = 2 * (uint64_t)b;
+                const int64_t rem = (int64_t)(n - (uint64_t)(uint32_t)q[r] * d);
+                q[r] += rem < 0 ? -1 : (rem >= (int64_t)d ? 1 : 0);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const int x = min(q[r], 127);
+            out |= (uint32_t)(uint8_t)((BITS == 8) != (v[r] < 0) ? -x : x) << (8 * r);
+        }
+    }
     *reinterpret_cast<uint32_t*>(to) = out;
 }
 
@@ -113,22 +124,24 @@ template <int HD, int BITS, int W, int MODE>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(W == 8 || HD == 128 ? 2 : (BITS == 8 ? 4 : 3)))) void pg_attend_kernel(
     Paged a, PgAttend p) {
     constexpr int HH = HD / 2, KC = HD / 64, DT = HD / 16, ND = BITS == 8 ? 2 : 3;
-    constexpr int NT = 64 * W, ET = (1024 + NT - 1) / NT;
+    constexpr int NT = 64 * W, ET = 256 / NT > 1 ? 256 / NT : 1;  // fours of table entries a thread
     constexpr int ROWB = BITS == 8 ? HD : HH, CHB = BITS == 8 ? 16 : 8;  // bytes of a K row of a slot, of a chunk
     constexpr bool MAXP = MODE != PG_SUMS, SUMP = MODE != PG_MAX;
     typedef PgTile<HD, BITS> Tile;
     typedef typename PgChunk<BITS>::T Chunk;
     __shared__ int64_t sSum[SUMP ? DT * 4 * 64 : 1], sDen[PG_COLS];
     __shared__ int sLow[MODE == PG_SUMS ? NT / PG_COLS : W][PG_COLS];
-    __shared__ uint16_t sE[1026];
+    __shared__ __attribute__((aligned(8))) uint16_t sE[1028];
     __shared__ __attribute__((aligned(16))) int8_t sK[W][64 * ROWB];
     extern __shared__ __attribute__((aligned(16))) int sS[];  // PG_KEEP: the scores of each wave's first tiles
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, gq = lane >> 4, kb = (lane >> 2) & 3, split = (int)blockIdx.y;
-    int et[ET];
+    typedef int tab4 __attribute__((ext_vector_type(4), aligned(4)));
+    tab4 et[ET];
     if constexpr (SUMP) {  // the table is on its way while the batch is looked up
 #pragma unroll
-        for (int i = 0; i < ET; i++) et[i] = p.exp_tab[min(tid + i * NT, 1023)];
+        for (int i = 0; i < ET; i++)
+            if (NT <= 256 || tid < 256) et[i] = *reinterpret_cast<const tab4*>(p.exp_tab + 4 * (tid + i * NT));
     }
 
     // The kv head fastest: CTAs go to the XCDs in turn, so an XCD's L2 holds the heads congruent to it. Column tiles 0 .. seqs -
@@ -172,9 +185,15 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(W == 8 |
     if constexpr (SUMP) {
 #pragma unroll
         for (int i = 0; i < ET; i++) {
-            const int e = min(max(et[i], 0), 32768);
-            // 8 bits: the two balanced base-256 digits of -e (2^15 itself has none, -2^15 does); 4 bits: e
-            if (tid + i * NT < 1024) sE[tid + i * NT] = BITS == 8 ? (uint16_t)((0x8080 - e) ^ 0x8080) : (uint16_t)e;
+            uint32_t e[4];
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                e[r] = (uint32_t)min(max(et[i][r], 0), 32768);
+                // 8 bits: the two balanced base-256 digits of -e (2^15 itself has none, -2^15 does); 4 bits: e
+                if constexpr (BITS == 8) e[r] = ((0x8080u - e[r]) ^ 0x8080u) & 0xFFFFu;
+            }
+            if (NT <= 256 || tid < 256)
+                *reinterpret_cast<v2i*>(sE + 4 * (tid + i * NT)) = v2i{(int)(e[0] | e[1] << 16), (int)(e[2] | e[3] << 16)};
         }
         if (tid == 0) sE[1024] = 0;
         for (int i = tid; i < DT * 4 * 64; i += NT) sSum[i] = 0;
