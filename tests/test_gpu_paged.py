@@ -256,7 +256,7 @@ def test_offsets_past_32_bits(torch_dev, bits):
     same(got[1], want[1], "read v")
 
 
-@pytest.mark.parametrize("rows,n", [(1, 1), (1, 2), (3, 97), (1, 4097), (5, 4096), (2, 151936), (64, 5000), (70, 300), (2, 65536), (3, 65537), (1, 1023), (1, 1025), (300, 70000)])
+@pytest.mark.parametrize("rows,n", [(1, 1), (1, 2), (3, 97), (1, 4097), (5, 4096), (2, 151936), (64, 5000), (70, 300), (2, 65536), (3, 65537), (1, 1023), (1, 1025), (300, 70000), (1, 100000), (2, 100001), (255, 101000)])
 def test_argmax_rows(torch_dev, rows, n):
     """Distinct values, ties (the first wins), all equal, both ends of int32, a stride, rows far apart."""
     import tritify_amd as TA
@@ -287,14 +287,14 @@ def test_replayed_graph_follows_its_arrays(torch_dev):
     cos, sin = rope_tables(1000, 64)
     cd, sd = torch.from_numpy(cos).cuda(), torch.from_numpy(sin).cuda()
     k, v = (torch.zeros(3, 64, 2, 64, dtype=torch.int8, device="cuda") for _ in range(2))
-    x = torch.zeros(3, 70000, dtype=torch.int32, device="cuda")
-    t, ws = torch.zeros(3, dtype=torch.int32, device="cuda"), torch.empty(TA.dec_argmax_rows_workspace(3, 70000), dtype=torch.int8, device="cuda")
+    x = torch.zeros(3, 110000, dtype=torch.int32, device="cuda")
+    t, ws = torch.zeros(3, dtype=torch.int32, device="cuda"), torch.empty(TA.dec_argmax_rows_workspace(3, 110000), dtype=torch.int8, device="cuda")
 
     def step(s):
         d.kv.append(d.qkv, d.b, 14, cd, sd, d.q, s)
         d.kv.attend(d.q, d.b, 14, d.exp, d.o, d.ws, 0, 0, s)
         d.kv.read(d.b, k, v, s)
-        TA.dec_argmax_rows(x, 3, 70000, t, ws, stream=s)
+        TA.dec_argmax_rows(x, 3, 110000, t, ws, stream=s)
 
     s = torch.cuda.Stream()
     s.wait_stream(torch.cuda.current_stream())
@@ -311,7 +311,7 @@ def test_replayed_graph_follows_its_arrays(torch_dev):
         say(f"case: replay {i}")
         c.kv_len = np.array([900 - 7 * i, 30 - i, 1 + 100 * i], dtype=np.int32)
         c.qkv = c.rows8(*c.qkv.shape)
-        logits = c.g.integers(-50, 50, size=(3, 70000)).astype(np.int32)
+        logits = c.g.integers(-50, 50, size=(3, 110000)).astype(np.int32)
         d.b.kv_len.copy_(torch.from_numpy(c.kv_len))
         d.qkv.copy_(torch.from_numpy(c.qkv))
         x.copy_(torch.from_numpy(logits))
@@ -329,7 +329,7 @@ def test_replayed_graph_follows_its_arrays(torch_dev):
         n = [min(64, int(L)) for L in c.kv_len]
         for b in range(3):
             same(k[b, :n[b]], want[0][b, :n[b]], f"read {i}")
-        assert t.cpu().numpy().tolist() == O.argmax_rows(logits, 70000).tolist()
+        assert t.cpu().numpy().tolist() == O.argmax_rows(logits, 110000).tolist()
 
 
 def test_two_streams_and_two_captured_graphs(torch_dev):

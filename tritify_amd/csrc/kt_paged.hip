@@ -250,20 +250,43 @@ __device__ __forceinline__ uint64_t block_max_key(uint64_t best, uint64_t* s_key
     return best;
 }
 
+typedef int i32x4 __attribute__((ext_vector_type(4), aligned(4)));
+
 // Grid (parts, rows): the best key of a part of a row; with one part a row, its index is the answer. One pass over the logits:
-// 64 rows of 151936 in 10.1 us with the second launch, 39 MB at 3.9 TB/s.
+// 256 rows of 151936 in 28.8 us, 156 MB at 5.4 TB/s; 64 rows in 10.9 us with the second launch, 39 MB at 3.6 TB/s.
 template <int NT>
 __global__ __launch_bounds__(NT) void pg_argmax_kernel(const int32_t* __restrict__ logits, int n, int64_t stride,
                                                         int per, uint64_t* __restrict__ part,
                                                         int32_t* __restrict__ token) {
     __shared__ uint64_t s_key[NT / 64];
     const int32_t* x = logits + (size_t)blockIdx.y * stride;
-    const uint32_t i0 = blockIdx.x * (uint32_t)per, i1 = min(i0 + (uint32_t)per, (uint32_t)n);
+    const uint32_t i0 = min(blockIdx.x * (uint32_t)per, (uint32_t)n), i1 = min(i0 + (uint32_t)per, (uint32_t)n);
+    // fours of logits (on any boundary of four bytes), then the up to three that are left
+    const uint32_t first = i0 + 4 * threadIdx.x, end = i0 + ((i1 - i0) & ~3u);
+    auto four = [&](uint32_t i) { return *reinterpret_cast<const i32x4*>(x + i); };
+    auto key = [](int v, uint32_t i) { return ((uint64_t)((uint32_t)v ^ 0x80000000u) << 32) | (0xFFFFFFFFu - i); };
+    int top = INT_MIN;
+    uint32_t at = first;  // the first four with the largest value yet
+    constexpr int U = NT == 1024 ? 8 : 4;  // loads in flight; past the end the last four again
+    for (uint32_t i = first; i < end; i += U * 4 * NT) {
+        i32x4 v[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) v[u] = four(min(i + u * 4 * NT, end - 4));
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int m = max(max(v[u].x, v[u].y), max(v[u].z, v[u].w));
+            at = m > top ? min(i + u * 4 * NT, end - 4) : at;
+            top = max(top, m);
+        }
+    }
     uint64_t best = 0;
-#pragma unroll 8
-    for (uint32_t i = i0 + threadIdx.x; i < i1; i += NT) {
-        const uint64_t key = ((uint64_t)((uint32_t)x[i] ^ 0x80000000u) << 32) | (0xFFFFFFFFu - i);
-        best = key > best ? key : best;
+    if (first < end) {
+        const i32x4 v = four(at);
+        best = key(top, at + (v.x == top ? 0 : (v.y == top ? 1 : (v.z == top ? 2 : 3))));
+    }
+    if (end + threadIdx.x < i1) {
+        const uint64_t last = key(x[end + threadIdx.x], end + threadIdx.x);
+        best = last > best ? last : best;
     }
     best = block_max_key<NT>(best, s_key);
     if (threadIdx.x == 0) {
@@ -316,11 +339,12 @@ hipError_t launch_pg_read(const Paged& a, int hd, int bits, int8_t* k, int8_t* v
     return bits == 8 ? go(pg_read_kernel<128, 8>) : go(pg_read_kernel<128, 4>);
 }
 
-// One CTA a row saves the second launch, and reads what is left of a long row alone. us a call, one / parts: 1 row of 4097 to 32768
-// 4.4 / 7.2, of 65536 5.1 / 7.2, of 151936 11.8 / 7.3; 64 rows of 65536 6.4 / 7.1, of 151936 17.7 / 11.2. Parts are of 4096 logits,
+// One CTA a row saves the second launch, and reads what is left of a long row alone. us a call, one / parts: 1 row of 8192 to 65536
+// 4.3 / 7.5, of 100000 5.1 / 7.6, of 151936 8.2 / 7.6, of 300000 13.7 / 7.4; 64 rows of 65536 5.9 / 7.3, of 100000 7.5 / 8.2, of 151936
+// 14.8 / 10.9; 256 rows fill the chip: of 32768 6.9 / 9.4, of 151936 28.8 / 32.5, of 300000 53.7 / 58.8. Parts are of 4096 logits,
 // the rows' parts together some 2048 CTAs.
 int pg_argmax_parts(int64_t rows, int64_t n) {
-    if (n <= 65536) return 1;
+    if (n <= 100000 || rows >= 256) return 1;
     return (int)std::max<int64_t>(1, std::min((n + 4095) / 4096, (2048 + rows - 1) / std::max<int64_t>(rows, 1)));
 }
 
