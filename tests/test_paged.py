@@ -50,6 +50,47 @@ def test_four_bits_hold_what_they_say():
                 assert (16 * off <= m[:, None]).all() and off.max() <= (0 if top != 2 else 1)
 
 
+def unpacked(c, pool, is_v):
+    """Codes [page][kv head][slot][hd] and multipliers [page][kv head][slot] (1 for 8 bits) of a pool."""
+    n, x = c.page * c.hd, pool.reshape(c.pages, c.nkv, -1)
+    if c.bits == 8:
+        codes, m = x.view(np.int8).astype(np.int64), np.ones((c.pages, c.nkv, c.page), dtype=np.int64)
+    else:
+        b, m = x[..., : n // 2].reshape(c.pages, c.nkv, -1, 2, 4).astype(np.int64), x[..., n // 2:].astype(np.int64)
+        codes = np.stack([b & 15, b >> 4], axis=-2).reshape(c.pages, c.nkv, n)
+        codes = np.where(codes > 7, codes - 16, codes)
+    if is_v:
+        return codes.reshape(c.pages, c.nkv, c.page // 16, c.hd, 16).swapaxes(3, 4).reshape(c.pages, c.nkv, c.page, c.hd), m
+    return codes.reshape(c.pages, c.nkv, c.page, c.hd), m
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (20, 3), (1, 50)])
+@pytest.mark.parametrize("bits,hd", [(8, 64), (4, 64), (4, 128)])
+def test_attention_is_the_formula(bits, hd, window, sinks):
+    c = Case(6, [(3, 90), (1, 40)], 4, 2, hd, 32, bits)
+    c.table[0, 1] = -1
+    o = c.attend(window, sinks)
+    (kc, km), (vc, vm) = unpacked(c, c.k, False), unpacked(c, c.v, True)
+    for b, (n, L) in enumerate(c.lens):
+        for i in range(n):
+            p = L - n + i
+            j = np.arange(p + 1)
+            page = c.table[b, j // c.page]
+            see = (page >= 0) & ((window == 0) | (j > p - window) | (j < sinks))
+            j, page = j[see], page[see]
+            for h in range(c.nh):
+                t, g = c.row_start[b] + i, h * c.nkv // c.nh
+                s = kc[page, g, j % c.page] @ np.maximum(c.q[t, h * hd:(h + 1) * hd].astype(np.int64), -127)
+                if bits == 4:
+                    s = (km[page, g, j % c.page] * s + 4) >> 3
+                ix = (s.max() - s + 64) >> 7
+                e = np.where(ix < 1024, c.exp[np.minimum(ix, 1023)].astype(np.int64), 0)
+                num = (e * vm[page, g, j % c.page]) @ vc[page, g, j % c.page]
+                den = e.sum() * (8 if bits == 4 else 1)
+                want = np.sign(num) * np.minimum((2 * np.abs(num) + den) // (2 * den), 127)
+                assert np.array_equal(o[t, h * hd:(h + 1) * hd], want), (b, i, h)
+
+
 @pytest.mark.parametrize("bits", [8, 4])
 def test_window_equals_pages_left_out(bits):
     """A window without sinks is the attention of a table whose older pages are gone, where the window ends at a page."""
