@@ -102,6 +102,20 @@ def test_attend_more_units_than_cus(torch_dev, seqs, nkv, window, bits, hd):
     check_attend(torch_dev, Case(60, lens, 4 * nkv if seqs < 400 else nkv, nkv, hd, 16, bits, behind=2), window, 3)
 
 
+@pytest.mark.parametrize("seqs", [63, 64, 65, 4095, 4097, 9000])
+def test_sequences_are_found_among_many(torch_dev, seqs):
+    """Runs of sequences without rows, at the counts where the search takes another level: append and attention."""
+    lens = [(0, 3) if i % 5 < 3 and i % 70 > 9 else (1 + i % 3 + 20 * (i % 61 == 0), 25 + i % 3) for i in range(seqs)]
+    c = Case(62, lens, 2, 1, 64, 16, 8, behind=3)
+    check_attend(torch_dev, c)
+    cos, sin = rope_tables(30, 64)
+    d = Dev(torch_dev, c)
+    q, k, v = c.append(cos, sin, FILL)
+    same(d.append(cos, sin), q, "q")
+    same(d.kv.k, k.view(np.int8), "k pool")
+    same(d.kv.v, v.view(np.int8), "v pool")
+
+
 @pytest.mark.parametrize("bits,hd", [(8, 64), (4, 64), (8, 128), (4, 128)])
 @pytest.mark.parametrize("window", [0, 2100])
 def test_attend_chunk_behind_more_than_a_cta_keeps(torch_dev, window, bits, hd):

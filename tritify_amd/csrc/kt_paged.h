@@ -4,7 +4,6 @@
 
 #include <stdint.h>
 
-#include "kt_dpp.h"
 #include "kt_kernels.h"
 
 namespace kt {
@@ -33,16 +32,22 @@ __device__ __forceinline__ PgRows pg_rows(const Paged& a, int b) {
 // Tiles of `step` units, sequence b with rows * mul units: its tiles begin at number floor(t0 mul / step) + per b, which
 // leaves it at least floor(rows mul / step) + per of them, so the grid needs no lengths from the host:
 // tokens mul / step + per seqs tiles in all. Returns the last sequence that begins at or before tile `t` and its first tile,
-// -1 where none does. Each lane of a wave looks at every 64th sequence. row_start must not decrease; where it does, some
-// sequence is returned all the same, and its tiles are bounded by its own rows.
+// -1 where none does: the wave probes 64 sequences at even distances and goes on between two of them. row_start must not
+// decrease; where it does, some sequence is returned all the same, and its tiles are bounded by its own rows.
 __device__ __forceinline__ int pg_tile_seq(const Paged& a, int t, int mul, int step, int per, int* first) {
     const int lane = threadIdx.x & 63;
     auto begin = [&](int b) { return (int)((int64_t)pg_start(a, b) * mul / step) + per * b; };
-    int c = 0;
-    for (int b = lane; b < a.seqs; b += 64) c += begin(b) <= t;
-    const int b = wave_sum_i32(c) - 1;
-    if (b >= 0) *first = begin(b);
-    return b;
+    for (int lo = 0, n = a.seqs;;) {
+        const int gap = (n + 63) / 64;
+        const int c = __popcll(__ballot(lane * gap < n && begin(lo + lane * gap) <= t));
+        if (c == 0) return -1;
+        lo += (c - 1) * gap;
+        if (gap == 1) {
+            *first = begin(lo);
+            return lo;
+        }
+        n = min(gap, n - (c - 1) * gap);
+    }
 }
 
 // The page of position block `blk` (16 positions) of sequence b, or -1.

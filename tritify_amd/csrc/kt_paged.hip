@@ -8,6 +8,7 @@
 #include <limits.h>
 #include <stdint.h>
 
+#include "kt_dpp.h"
 #include "kt_paged.h"
 #include "kt_w12_core.h"
 
