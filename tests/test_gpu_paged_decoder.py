@@ -151,3 +151,49 @@ def test_captured_decode_steps(model, torch_dev):
         b.kv_len.add_(1)
         torch.cuda.synchronize()
     assert np.array_equal(np.array(got).T, want)
+
+
+def test_captured_steps_of_two_shapes_and_passes_between(model, torch_dev):
+    """Two captured steps whose batches differ, replayed in turn, with eager passes of other shapes between: the scratch that a
+    graph holds stays its own."""
+    from tritify_amd.paged import PagedDecoder
+
+    torch = torch_dev
+    ps = prompts([37, 5, 100, 250])
+    want = [model.generate(p, 9)[0] for p in ps]
+    d = PagedDecoder(model, 4096, max_rows=512)
+    ids = [d.add() for _ in ps]
+    tok = d.run(list(zip(ids, ps)))
+    d._reserve([(s, d.length(s) + 8) for s in ids])
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    steps = []
+    for part in ([0, 1, 2], [3]):
+        b = d.batch([ids[i] for i in part], [1] * len(part))
+        if part == [3]:  # a table long enough for split passes
+            wide = torch.full((1, 1024), -1, dtype=torch.int32, device="cuda")
+            wide[:, : b.max_pages] = b.table
+            from tritify_amd.paged import PagedBatch
+            b = PagedBatch(b.row_start, b.kv_len, wide, 1)
+        x = tok[part[0]: part[-1] + 1].clone()
+        out, g = torch.empty_like(x), torch.cuda.CUDAGraph()
+        with torch.cuda.stream(s):
+            d.forward(x, b, None, out, s)
+            torch.cuda.synchronize()
+            g.capture_begin()
+            d.forward(x, b, None, out, s)
+            g.capture_end()
+        steps.append((part, b, x, out, g))
+    other = d.add()
+    torch.cuda.synchronize()
+    for n in range(1, 9):
+        for part, b, x, out, g in steps:
+            g.replay()
+            torch.cuda.synchronize()
+            assert out.cpu().numpy().tolist() == [want[i][n] for i in part], (n, part)
+            x.copy_(out)
+            b.kv_len.add_(1)
+            junk = [torch.full((1 << 16,), 0x55, dtype=torch.int8, device="cuda") for _ in range(20)]
+            d.run([(other, [1] * (3 * n))])
+            del junk
+            torch.cuda.synchronize()

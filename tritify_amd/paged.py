@@ -187,7 +187,7 @@ class PagedDecoder:
         self.qkv, self.q, self.o = zeros(R, m.nq), zeros(R, m.nh * m.hd), zeros(R, m.nh * m.hd)
         self.r_last, self.x_last = zeros(max_seqs, m.d, dt=torch.int32), zeros(max_seqs, m.d)
         self.logits = zeros(max_seqs, m.V, dt=torch.int32)
-        self.ws = {}
+        self._ws = []
 
     # sequences -----------------------------------------------------------------------------------------------------
 
@@ -277,18 +277,23 @@ class PagedDecoder:
             return torch.cuda.default_stream(self.device)
         return torch.cuda.ExternalStream(stream, device=self.device) if isinstance(stream, int) else stream
 
+    def _workspaces(self, b: PagedBatch) -> tuple:
+        """Scratch of the attention and of the choice. What a captured pass may hold is kept when a larger one is made."""
+        n, top = self.kv[0].workspace_bytes(b, self.m.nh), B.dec_argmax_rows_workspace(b.seqs, self.m.V)
+        n = -(-n // 256) * 256
+        if not self._ws or self._ws[-1].numel() < n + top:
+            size = max(n + top, 2 * self._ws[-1].numel() if self._ws else 1 << 16)
+            self._ws.append(self.torch.empty(size, dtype=self.torch.int8, device=self.device))
+        return self._ws[-1][:n], self._ws[-1][n:]
+
     def forward(self, tokens_dev, b: PagedBatch, last, out, stream=None) -> None:
         """The layers over the batch's rows, the logits of each sequence's last row (`last`: their indexes, None where
         every sequence has one row) to self.logits, the greedy choice of each to out. Asynchronous on `stream`, which
-        torch's current stream has to be; capturable when self.ws holds the shape's workspace (after a first call)."""
+        torch's current stream has to be; capturable after a call of the batch's shape. Passes of one decoder, captured or
+        not, share its buffers: they follow one another."""
         m, lib, dev, s, P = self.m, B.lib(), self.dev, B._stream(stream), B._ptr
         T, d, ffn, nh, hd, nq = b.tokens, m.d, m.ffn, m.nh, m.hd, m.nq
-        key = (T, b.seqs, b.max_pages)
-        if key not in self.ws:
-            self.ws = {key: (self.kv[0].workspace(b, nh),
-                             self.torch.empty(B.dec_argmax_rows_workspace(b.seqs, m.V), dtype=self.torch.int8,
-                                              device=self.device))}
-        ws, ws_top = self.ws[key]
+        ws, ws_top = self._workspaces(b)
         B.check(lib.kt_hip_dec_embed(dev, P(tokens_dev), T, P(m.emb16), d, P(self.r), s), "dec embed")
         fuse = m.fuse_norm and T <= B.NORM_MAX_M
         for l in range(m.L):
