@@ -119,6 +119,49 @@ def test_refusals_leave_the_decoder_as_it_was(model):
             PagedDecoder(model, 6, **kw)
 
 
+def test_tokens_as_tensors(model, torch_dev):
+    """Host lists, host tensors and tensors of the device of either width are the same; ids outside the vocabulary on the device
+    count as the nearest inside; matrices and floats are refused."""
+    from tritify_amd.paged import PagedDecoder
+
+    torch = torch_dev
+    d = PagedDecoder(model, 64, max_rows=100)
+    got = []
+    for ids in ([0, 7, 999], torch.tensor([0, 7, 999]), torch.tensor([0, 7, 999], dtype=torch.int32),
+                torch.tensor([0, 7, 999], device="cuda"), torch.tensor([-5, 7, 2 ** 40], device="cuda"),
+                torch.tensor([[0, 1], [7, 1], [999, 1]], device="cuda", dtype=torch.int32)[:, 0]):
+        s = d.add()
+        d.run([(s, ids)])
+        got.append(d.logits[0].cpu().numpy())
+        d.release(s)
+    assert all(np.array_equal(g, got[0]) for g in got)
+    s = d.add()
+    for bad in (torch.tensor([[1, 2]], device="cuda"), torch.tensor([1.0], device="cuda"), torch.tensor([1000]), torch.tensor([True])):
+        with pytest.raises(ValueError):
+            d.run([(s, bad)])
+        assert d.length(s) == 0
+
+
+def test_passes_and_reads_on_another_stream(model, torch_dev):
+    from tritify_amd.paged import PagedDecoder
+
+    torch = torch_dev
+    ps = prompts([60, 9])
+    want = [model.generate(p, 4)[0] for p in ps]
+    d, s = PagedDecoder(model, 64, max_rows=100), torch.cuda.Stream()
+    ids = [d.add() for _ in ps]
+    torch.cuda.synchronize()
+    t, got = d.run(list(zip(ids, ps)), stream=s), []
+    for _ in range(3):
+        got.append(t)
+        t = d.run([(ids[0], t[:1]), (ids[1], t[1:])], stream=s)
+    k, _ = d.read(ids[0], 0, stream=s)
+    s.synchronize()
+    assert np.array_equal(torch.stack(got + [t]).cpu().numpy().T, np.array(want))
+    model.generate(ps[0], 4)
+    assert torch.equal(k[:62].reshape(-1), model.kc[: 62 * 2 * 64])
+
+
 def test_captured_decode_steps(model, torch_dev):
     """A decode step of a batch as one graph: the tables and lengths move on the device arrays between the replays."""
     from tritify_amd.paged import PagedDecoder

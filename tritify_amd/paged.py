@@ -4,7 +4,7 @@ single tokens over them, and the greedy choice of a batch, over the C ABI (kt_hi
 The reference decodes one sequence from contiguous caches (crates/01-engine/kt-core/src/model.rs:290-353,
 generate.rs:82-111); `DecoderModel` mirrors that. `PagedKV` holds one layer's pools and offers the operators on them;
 `PagedDecoder` runs a DecoderModel's layers over them for a batch whose sequences come and go. With 8-bit pages every
-sequence gets the integers that DecoderModel gives it alone. torch allocates the buffers and copies; it computes nothing.
+sequence gets the integers that DecoderModel gives it alone. torch allocates the buffers, copies, and bounds token ids; it computes nothing else.
 """
 from __future__ import annotations
 
@@ -195,7 +195,7 @@ class PagedDecoder:
         """A new, empty sequence."""
         s = self._next
         self._next += 1
-        self.seq[s] = dict(len=0, pages=[])
+        self.seq[s] = dict(len=0, pages=[], gone=-(-self.sinks // self.page))
         return s
 
     def release(self, s: int) -> None:
@@ -220,10 +220,10 @@ class PagedDecoder:
         """Pages that the window has left behind, and no sink is in, are free again."""
         e = self.seq[s]
         gone = max(0, e["len"] + 1 - self.window) // self.page  # pages that no later row's window reaches
-        for i in range(-(-self.sinks // self.page), gone):
-            if e["pages"][i] >= 0:
-                self.free.append(e["pages"][i])
-                e["pages"][i] = -1
+        for i in range(e["gone"], gone):
+            self.free.append(e["pages"][i])
+            e["pages"][i] = -1
+        e["gone"] = max(e["gone"], gone)
 
     # a pass --------------------------------------------------------------------------------------------------------
 
@@ -243,7 +243,8 @@ class PagedDecoder:
     def run(self, work: list, stream=None):
         """One pass over (sequence, its new tokens) pairs: prompts, chunks of prompts and single tokens alike. Returns the
         greedy next token of each (int32, on the device); their logits are self.logits[: len(work)]. The tokens may be
-        host integers or an int32 tensor of the device."""
+        host integers, which are checked, or a tensor of the device, whose ids outside the vocabulary count as the nearest
+        one inside. Asynchronous on `stream` (None: the null stream); other streams' work is the caller's to order."""
         torch = self.torch
         seqs = [s for s, _ in work]
         rows = [len(t) for _, t in work]
@@ -252,12 +253,14 @@ class PagedDecoder:
         if min(rows) < 1 or sum(rows) > self.max_rows:
             raise ValueError(f"run: at least one token each, {self.max_rows} in all at most")
         for s, t in work:
-            if not torch.is_tensor(t) and not all(0 <= int(x) < self.m.V for x in t):
+            if torch.is_tensor(t) and (t.dim() != 1 or t.dtype not in (torch.int32, torch.int64)):
+                raise ValueError(f"run: sequence {s}: tokens are a vector of int32 or int64")
+            if not self._on_gpu(t) and not all(0 <= int(x) < self.m.V for x in t):
                 raise ValueError(f"run: sequence {s} has a token outside the vocabulary")
         self._reserve([(s, self.seq[s]["len"] + n) for s, n in zip(seqs, rows)])
         with torch.cuda.stream(self._torch_stream(stream)):
             b = self.batch(seqs, rows)
-            toks = [t.to(device=self.device, dtype=torch.int32) if torch.is_tensor(t) else
+            toks = [t.clamp(0, self.m.V - 1).to(device=self.device, dtype=torch.int32) if self._on_gpu(t) else
                     torch.tensor([int(x) for x in t], dtype=torch.int32, device=self.device) for _, t in work]
             toks = torch.cat(toks) if len(toks) > 1 else toks[0].contiguous()
             last = None
@@ -270,6 +273,9 @@ class PagedDecoder:
             if self.window:
                 self._trim(s)
         return out
+
+    def _on_gpu(self, t) -> bool:
+        return self.torch.is_tensor(t) and t.is_cuda
 
     def _torch_stream(self, stream):
         torch = self.torch
@@ -322,13 +328,14 @@ class PagedDecoder:
         m._gemm("emb", 0, self.x_last, b.seqs, m.V, d, self.logits, B.OUT_I32, s)
         B.dec_argmax_rows(self.logits, b.seqs, m.V, out, ws_top, stream=stream, dev=dev)
 
-    def read(self, s: int, layer: int, max_pos: int | None = None):
+    def read(self, s: int, layer: int, max_pos: int | None = None, stream=None):
         """Sequence s's K and V of a layer as contiguous rows (max_pos x nkv x hd int8, zeros past its length): the caches
-        that DecoderModel continues from."""
+        that DecoderModel continues from. On `stream`, as the passes are."""
         torch = self.torch
         n = self.seq[s]["len"] if max_pos is None else max_pos
-        k, v = (torch.zeros(1, n, self.m.nkv, self.m.hd, dtype=torch.int8, device=self.device) for _ in range(2))
-        self.kv[layer].read(self.batch([s], [0]), k, v)
+        with torch.cuda.stream(self._torch_stream(stream)):
+            k, v = (torch.zeros(1, n, self.m.nkv, self.m.hd, dtype=torch.int8, device=self.device) for _ in range(2))
+            self.kv[layer].read(self.batch([s], [0]), k, v, stream)
         return k[0], v[0]
 
     def generate(self, prompts: list, max_new: int, chunk: int | None = None) -> np.ndarray:
