@@ -563,11 +563,11 @@ struct Plan {
 // 8000 (32) 30.0 / 20.0 / 19.8, 64 (128) 39.5 / 39.5 / 44.5; below 64 tiles it gains nothing (behind 2000 11.2 / 11.9 with two).
 //
 // Kernel times against the bytes and operations that cannot be left out (4 hd a column and visible position): 128 single tokens
-// behind 6100 positions 48.2 us, 199 MB of K and V at 4.1 TB/s (the loads of ragged lengths end unevenly; a plain read of as much
-// reaches 5.9); one token behind 131000 4-bit positions 7 + 15 us for 17 MB (two launches, 32 tiles a wave and a join each); 1024
-// rows behind 7777 83 us, 0.37 of 2.1 int8 POPS counted once (pass 1 forms the scores a second time, weights take two digits);
-// there matrix units, vector units and LDS are each busy 24, 50 and 57 % of the time and a wave waits for one of them in turn:
-// 4 waves on 64 columns sharing a tile's K and V in LDS (a third of the reads from the L2) took 87 us.
+// behind 6100 positions 47.8 us, 199 MB of K and V at 4.2 TB/s (the loads of ragged lengths end unevenly; a plain read of as much
+// reaches 5.9); one token behind 131000 4-bit positions 7 + 15 us for 17 MB (two launches, four tiles a wave each, and a join); 1024
+// rows behind 7777 75 us, 30.4 GOP at 0.40 POPS counted once (the scores are formed three times over, weights take two digits);
+// there matrix units, vector units and LDS are busy 25, 50 and 58 % of the time and a wave waits for one of them in turn: 4 waves
+// on 64 columns sharing a tile's K and V in LDS (a third of the reads from the L2) took 87 us against 84 under the profiler.
 Plan plan(int64_t tokens, int64_t seqs, int64_t max_pos, int rep, int nkv) {
     const int64_t tiles = seqs + tokens * rep / PG_COLS, steps = max_pos / 64;
     const int64_t units = std::min(tiles, tokens * ((rep + PG_COLS - 1) / PG_COLS)) * nkv;
