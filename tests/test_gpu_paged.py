@@ -128,6 +128,13 @@ def test_attend_window(torch_dev, window, sinks, bits):
     check_attend(torch_dev, Case(8, [(1, 1), (1, 900), (30, 700), (70, 70), (150, 1000)], 7, 1, 64, 16, bits), window, sinks)
 
 
+@pytest.mark.parametrize("window,sinks", [(300, 5), (4000, 0), (9000, 700)])
+@pytest.mark.parametrize("bits,hd", [(8, 64), (4, 64), (8, 128), (4, 128)])
+def test_attend_window_in_a_wide_table(torch_dev, window, sinks, bits, hd):
+    """Positions far behind the window: what divides the work is what the window reaches."""
+    check_attend(torch_dev, Case(12, [(1, 20011), (2, 9000), (1, 100)], 7, 1, hd, 64, bits), window, sinks)
+
+
 @pytest.mark.parametrize("bits", [8, 4])
 def test_attend_pages_left_out(torch_dev, bits):
     """Entries outside the pool leave positions out (rows of the batch among them); a sequence without any page is zeros."""

@@ -618,11 +618,14 @@ hipError_t launch_pg_attend(const Paged& a, int hd, int bits, const int8_t* q, i
                             hipStream_t s) {
     const int64_t max_pos = (int64_t)a.max_pages << a.page_sh;
     const int rep = nh / a.nkv;
-    const Plan x = plan(a.tokens, a.seqs, max_pos, rep, a.nkv);
+    // With a window a column tile's positions are fewer than window + sinks + 256 (15 of other rows, two tiles' ends each), whatever
+    // the table's width: fewer splits than the workspace is made for, so no more of it.
+    const int64_t reach = window ? std::min<int64_t>(max_pos, (int64_t)window + sinks + 256) : max_pos;
+    const Plan x = plan(a.tokens, a.seqs, reach, rep, a.nkv);
     const Parts w = parts(x, a.nkv, hd);
     // kept scores: 256 bytes a column and tile, as far as a CTA's LDS (160 KB) goes beside the static arrays (K's 8 tiles, the
     // sums, 4 KB of others)
-    const int64_t cols = a.tokens > a.seqs ? PG_COLS : std::min(rep, PG_COLS), most = (max_pos / 64 + 8) / 8 * 8 * cols * 256;
+    const int64_t cols = a.tokens > a.seqs ? PG_COLS : std::min(rep, PG_COLS), most = (reach / 64 + 8) / 8 * 8 * cols * 256;
     const int64_t room = 163840 - 8 * 64 * (bits == 8 ? hd : hd / 2) - hd * 128 - 4096;
     const PgAttend p = {q, o, q_stride, o_stride, exp_tab, rep, window, sinks, x.splits, (int)std::min(most, room),
                         (int32_t*)ws, (unsigned long long*)((char*)ws + w.sum), (unsigned*)((char*)ws + w.cnt)};
