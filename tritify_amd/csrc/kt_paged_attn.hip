@@ -284,7 +284,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(W == 8 |
     auto kept_place = [&](int n, int t) { return reinterpret_cast<v4i*>(sS) + (((n * W + w) * 4 + t) * 4 + gq) * cols + l16; };
     // V's ring over the kept tiles; at hd 64 there are registers to begin it before the maximum is known
     constexpr bool EARLY = MODE == PG_KEEP && HD == 64;
-    constexpr int NV = EARLY ? 4 : 1;
+    constexpr int NV = EARLY ? 2 : 1;
     Tile xv[NV];
     int idv[NV], nidv[NV];
     auto begin_v = [&]() {
@@ -296,12 +296,14 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(W == 8 |
         }
     };
 
-    // Tiles go through rings in registers. A tile's page ids are read a round of the ring before its loads are issued, and
-    // those a round before they are used: a wave waits for neither. CTAs of 8 waves have a CU to themselves and deep rings,
-    // smaller ones four (hd 128: two) waves a SIMD beside each other.
+    // Tiles go through rings in registers, with 8 waves (one CTA a CU) two of K in pass 1 and two of V for kept scores, else one:
+    // a tile's page ids are read a round of the ring before its loads are issued, and those a round before they are used, so a
+    // wave waits for neither. No more, as every copy of a loop's body is fetched anew by each launch: with four of each and two
+    // in pass 2, 128 single tokens took 48.2 us against 45.5 and one token behind 131000 positions of 4 bits 21.8 against 20.7; a
+    // chunk of 1024 rows behind 7777 takes 83.7 traced.
     int low = INT_MAX;  // the least negated score of the column
     if constexpr (MAXP) {
-        constexpr int NB = W == 8 ? (HD == 64 ? 4 : 2) : 1;
+        constexpr int NB = W == 8 ? 2 : 1;
         Tile x[NB];
         int id[NB], nid[NB];
 #pragma unroll
@@ -444,7 +446,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(W == 8 |
                 for (int e = 0; e < ND; e++) acc[d][e] = mfma16(widen(v.x[d]), P[e], acc[d][e]);
         };
         {
-            constexpr int NB = W == 8 && HD == 64 && MODE != PG_KEEP ? 2 : 1;
+            constexpr int NB = 1;  // (as a loop without the ring's form the compiler's order of it is slower: the chunk above 86.6 us)
             Tile x[NB], v[NB];
             int id[NB], nid[NB];
             const int left = mine - kept;
