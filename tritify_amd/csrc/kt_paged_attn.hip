@@ -279,7 +279,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(W == 8 |
 
     // PG_KEEP: as many of the wave's tiles as the LDS holds keep their scores, a column's 16 bytes at a time (lanes side by
     // side); the others' are formed again from K, last tile first: its K is nearest. 128 single tokens behind about 6100
-    // positions 52.1 -> 48.2 us.
+    // positions 50.3 -> 45.5 us.
     const int kept = MODE == PG_KEEP ? min(mine, p.keep / (256 * W * cols)) : 0;
     auto kept_place = [&](int n, int t) { return reinterpret_cast<v4i*>(sS) + (((n * W + w) * 4 + t) * 4 + gq) * cols + l16; };
     // V's ring over the kept tiles; at hd 64 there are registers to begin it before the maximum is known
@@ -557,17 +557,18 @@ struct Plan {
 
 // From the counts that the host knows. A unit is a column tile of one kv head. Waves: 8 a CTA, one CTA a CU, while the units
 // fit the CUs; else 4, and 2 where that fills the chip by itself (a CTA's waves share its columns, so fewer of them join less).
-// us with 2 / 4 / 8, 14 heads over 2, hd 64: 64 rows behind 4000 positions (56 units) 36.6 / 23.2 / 17.5; 512 behind 4000 (448)
-// 47.2 / 31.2 / 37.9; 1024 alone (896) 15.8 / 13.0 / 25.8; 3 x 1021 alone (2682) 26.8 / 30.1 / 68.5. A wave never has more than
+// us with 2 / 4 / 8, 14 heads over 2, hd 64: 64 rows behind 4000 positions (56 units) 36.0 / 22.7 / 16.5; 512 behind 4000 (448)
+// 45.9 / 30.9 / 35.3; 1024 alone (896) 15.1 / 12.4 / 23.6; 3 x 1021 alone (2682) 25.5 / 29.0 / 63.5. A wave never has more than
 // 65536 positions: its digit sums stay within 2^14 2^16. Splits, where units leave CUs without one: to 128 CTAs, of at least 8
 // tiles; past that the extra launch, the second reading of K and the sums that meet in memory outweigh it. us with 1 / the
-// rule's / twice its splits: one token behind 131000 (2 units) 363 / 20.3 / 20.9, 4 behind 32000 (8) 95.5 / 19.8 / 24.2, 16 behind
-// 8000 (32) 30.0 / 20.0 / 19.8, 64 (128) 39.5 / 39.5 / 44.5; below 64 tiles it gains nothing (behind 2000 11.2 / 11.9 with two).
+// rule's / twice its splits: one token behind 131000 (2 units) 353 / 17.8 / 20.2, 4 behind 32000 (8) 92.5 / 18.1 / 21.1, 16 behind
+// 8000 (32) 28.3 / 17.7 / 20.8, 64 (128) 37.1 / 37.1 / 53.8, one behind 5000 17.8 / 11.0 / 10.8; below 64 tiles it gains nothing
+// (behind 2000 10.1 / 11.1 with two).
 //
 // Kernel times against the bytes and operations that cannot be left out (4 hd a column and visible position): 128 single tokens
-// behind 6100 positions 47.8 us, 199 MB of K and V at 4.2 TB/s (the loads of ragged lengths end unevenly; a plain read of as much
-// reaches 5.9); one token behind 131000 4-bit positions 7 + 15 us for 17 MB (two launches, four tiles a wave each, and a join); 1024
-// rows behind 7777 75 us, 30.4 GOP at 0.40 POPS counted once (the scores are formed three times over, weights take two digits);
+// behind 6100 positions 45.5 us, 199 MB of K and V at 4.4 TB/s (the loads of ragged lengths end unevenly; a plain read of as much
+// reaches 5.9); one token behind 131000 4-bit positions 6 + 14.5 us for 17 MB (two launches, four tiles a wave each, and a join); 1024
+// rows behind 7777 74 us, 30.4 GOP at 0.41 POPS counted once (the scores are formed three times over, weights take two digits);
 // there matrix units, vector units and LDS are busy 25, 50 and 58 % of the time and a wave waits for one of them in turn: 4 waves
 // on 64 columns sharing a tile's K and V in LDS (a third of the reads from the L2) took 87 us against 84 under the profiler.
 Plan plan(int64_t tokens, int64_t seqs, int64_t max_pos, int rep, int nkv) {
