@@ -24,11 +24,10 @@ def page_bytes(page: int, hd: int, bits: int = 8) -> int:
     return n
 
 
-def _need(t, what: str, dtype, device, shape=None) -> None:
-    if t.dtype != dtype or t.device != device or not t.is_contiguous():
-        raise ValueError(f"{what}: a contiguous {dtype} tensor on {device} is needed")
-    if shape is not None and t.shape != shape:
-        raise ValueError(f"{what}: shape {tuple(t.shape)}, {shape} is needed")
+def _need(t, what: str, dtype, dev: int, shape) -> None:
+    if t.dtype is not dtype or t.get_device() != dev or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{what}: a contiguous {dtype} tensor of shape {tuple(shape)} on GPU {dev} is needed, not "
+                         f"{tuple(t.shape)} {t.dtype} on {t.device}")
 
 
 class PagedBatch:
@@ -39,15 +38,14 @@ class PagedBatch:
     def __init__(self, row_start, kv_len, table, tokens: int):
         import torch
 
-        dv = table.device
-        if dv.type != "cuda":
+        if not table.is_cuda:
             raise ValueError("PagedBatch: the tensors live on the GPU")
         if table.dim() != 2 or not 0 <= tokens <= 1 << 30:
             raise ValueError("PagedBatch: table is seqs x max_pages, tokens a count of rows")
-        self.seqs, self.max_pages, self.tokens, self.device = table.shape[0], table.shape[1], int(tokens), dv
-        _need(table, "table", torch.int32, dv)
-        _need(row_start, "row_start", torch.int32, dv, (self.seqs + 1,))
-        _need(kv_len, "kv_len", torch.int32, dv, (self.seqs,))
+        self.seqs, self.max_pages, self.tokens, self.dev = table.shape[0], table.shape[1], int(tokens), table.get_device()
+        _need(table, "table", torch.int32, self.dev, table.shape)
+        _need(row_start, "row_start", torch.int32, self.dev, (self.seqs + 1,))
+        _need(kv_len, "kv_len", torch.int32, self.dev, (self.seqs,))
         self.row_start, self.kv_len, self.table = row_start, kv_len, table
         self.ptrs = (row_start.data_ptr(), kv_len.data_ptr(), table.data_ptr())
 
@@ -69,20 +67,20 @@ class PagedKV:
         shape = (pages, nkv, part)
         self.k = torch.zeros(shape, dtype=torch.int8, device=self.device) if k is None else k
         self.v = torch.zeros(shape, dtype=torch.int8, device=self.device) if v is None else v
-        _need(self.k, "k", torch.int8, self.device, shape)
-        _need(self.v, "v", torch.int8, self.device, shape)
+        _need(self.k, "k", torch.int8, dev, shape)
+        _need(self.v, "v", torch.int8, dev, shape)
         self._pools = (self.k.data_ptr(), self.v.data_ptr(), pages, page, bits)  # as every call passes them
 
     def _batch(self, batch: PagedBatch) -> None:
-        if batch.device != self.device:
-            raise ValueError(f"the batch is on {batch.device}, the pools on {self.device}")
+        if batch.dev != self.dev:
+            raise ValueError(f"the batch is on GPU {batch.dev}, the pools on GPU {self.dev}")
         if not 1 <= batch.max_pages <= MAX_POS // self.page:
             raise ValueError(f"a table of {batch.max_pages} pages of {self.page}: 1 to {MAX_POS} positions")
 
     def _rows(self, t, what: str, batch: PagedBatch, width: int) -> tuple[int, int]:
         """The address and stride of `t`, whose rows hold at least `width` int8 values for every row of the batch."""
-        if t.dtype != self._i8 or t.device != self.device or t.dim() != 2:
-            raise ValueError(f"{what}: an int8 matrix on {self.device} is needed")
+        if t.dtype is not self._i8 or t.get_device() != self.dev or t.dim() != 2:
+            raise ValueError(f"{what}: an int8 matrix on GPU {self.dev} is needed")
         (rows, cols), (stride, by), at = t.shape, t.stride(), t.data_ptr()
         if rows <= 1 and stride < cols:
             stride = cols
@@ -97,9 +95,10 @@ class PagedKV:
         to the pages. cos / sin: int16 tables of max_pos x hd / 2 at 2^14."""
         self._batch(batch)
         hd, nkv = self.hd, self.nkv
-        n = cos.shape[0] if cos.dim() == 2 else -1
-        _need(cos, "cos", self._i16, self.device, (n, hd // 2))
-        _need(sin, "sin", self._i16, self.device, (n, hd // 2))
+        shape = cos.shape
+        n = shape[0] if len(shape) == 2 and shape[1] == hd // 2 else -1
+        _need(cos, "cos", self._i16, self.dev, shape if n >= 0 else (n, hd // 2))
+        _need(sin, "sin", self._i16, self.dev, shape)
         at, stride = self._rows(qkv, "qkv", batch, (nh + 2 * nkv) * hd)
         to, q_stride = self._rows(q, "q", batch, nh * hd)
         B.check(B.lib().kt_hip_dec_rope_kv_paged(
@@ -112,8 +111,8 @@ class PagedKV:
         self._batch(batch)
         n = k.shape[1] if k.dim() == 4 else -1
         shape = (batch.seqs, n, self.nkv, self.hd)
-        _need(k, "k", self._i8, self.device, shape)
-        _need(v, "v", self._i8, self.device, shape)
+        _need(k, "k", self._i8, self.dev, shape)
+        _need(v, "v", self._i8, self.dev, shape)
         B.check(B.lib().kt_hip_dec_kv_read_paged(
             self.dev, *self._pools, batch.ptrs[1], batch.ptrs[2], batch.seqs, batch.max_pages, self.nkv, self.hd,
             k.data_ptr(), v.data_ptr(), n, B._stream(stream)), "dec paged read")
@@ -138,9 +137,9 @@ class PagedKV:
         """The rows' attention over their sequences' pages (after the append of the rows' own k and v), q and o rows of
         nh * hd. window >= 1: a row at p sees positions past p - window and the first `sinks`; 0: all up to its own."""
         self._batch(batch)
-        _need(exp_tab, "exp_tab", self._i32, self.device, (1024,))
-        if ws.device != self.device or not ws.is_contiguous():
-            raise ValueError(f"ws: a contiguous tensor on {self.device} is needed")
+        _need(exp_tab, "exp_tab", self._i32, self.dev, (1024,))
+        if ws.get_device() != self.dev or not ws.is_contiguous():
+            raise ValueError(f"ws: a contiguous tensor on GPU {self.dev} is needed")
         at, q_stride = self._rows(q, "q", batch, nh * self.hd)
         to, o_stride = self._rows(o, "o", batch, nh * self.hd)
         B.check(B.lib().kt_hip_dec_attention_paged(
