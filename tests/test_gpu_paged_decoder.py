@@ -148,9 +148,10 @@ def test_passes_and_reads_on_another_stream(model, torch_dev):
     torch = torch_dev
     ps = prompts([60, 9])
     want = [model.generate(p, 4)[0] for p in ps]
-    d, s = PagedDecoder(model, 64, max_rows=100), torch.cuda.Stream()
+    s = torch.cuda.Stream()
+    torch.cuda._sleep(20_000_000)  # the null stream is behind: a decoder made on it is whole all the same
+    d = PagedDecoder(model, 64, max_rows=100)
     ids = [d.add() for _ in ps]
-    torch.cuda.synchronize()
     t, got = d.run(list(zip(ids, ps)), stream=s), []
     for _ in range(3):
         got.append(t)

@@ -67,6 +67,8 @@ class PagedKV:
         shape = (pages, nkv, part)
         self.k = torch.zeros(shape, dtype=torch.int8, device=self.device) if k is None else k
         self.v = torch.zeros(shape, dtype=torch.int8, device=self.device) if v is None else v
+        if k is None or v is None:  # zeros before any stream writes
+            torch.cuda.current_stream(self.device).synchronize()
         _need(self.k, "k", torch.int8, dev, shape)
         _need(self.v, "v", torch.int8, dev, shape)
         self._pools = (self.k.data_ptr(), self.v.data_ptr(), pages, page, bits)  # as every call passes them
@@ -187,6 +189,7 @@ class PagedDecoder:
         self.r_last, self.x_last = zeros(max_seqs, m.d, dt=torch.int32), zeros(max_seqs, m.d)
         self.logits = zeros(max_seqs, m.V, dt=torch.int32)
         self._ws = []
+        torch.cuda.current_stream(self.device).synchronize()  # the buffers are zeros before a pass on any stream
 
     # sequences -----------------------------------------------------------------------------------------------------
 
