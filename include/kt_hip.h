@@ -891,8 +891,8 @@ int kt_hip_dec_kv_read_paged(int dev, const void* kpool_dev, const void* vpool_d
  * sees all. s_j = q . k_j (q of -128, which RoPE never gives, as -127; 4 bits: (m_j (q . c_j) + 4) >> 3),
  * e_j = exp_tab[(max s - s_j + 64) >> 7] with entries clamped to [0, 2^15] and 0 past the 1024th,
  * o = clamp(round_half_away(sum e_j v_j / sum e_j)), 0 where the sum of e is 0.
- * ws_dev: kt_hip_dec_attention_paged_workspace bytes of scratch, 16-byte aligned, needing no contents; calls that may
- * overlap need one each. */
+ * ws_dev: kt_hip_dec_attention_paged_workspace bytes of scratch for the call's own shape (few rows over a wide table need
+ * more than many), 16-byte aligned, needing no contents; calls that may overlap need one each. */
 size_t kt_hip_dec_attention_paged_workspace(int64_t tokens, int64_t seqs, int64_t max_pages, int64_t page, int64_t nh,
                                             int64_t nkv, int64_t hd);
 int kt_hip_dec_attention_paged(int dev, const int8_t* q_dev, int64_t tokens, int64_t q_stride,

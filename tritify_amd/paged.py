@@ -120,7 +120,7 @@ class PagedKV:
             k.data_ptr(), v.data_ptr(), n, B._stream(stream)), "dec paged read")
 
     def workspace_bytes(self, batch: PagedBatch, nh: int) -> int:
-        """Scratch bytes of attend for `nh` q heads over this batch's shape."""
+        """Scratch bytes of attend for `nh` q heads over this batch's shape (a smaller batch may need more)."""
         self._batch(batch)
         n = B.lib().kt_hip_dec_attention_paged_workspace(batch.tokens, batch.seqs, batch.max_pages, self.page, nh,
                                                          self.nkv, self.hd)
