@@ -412,3 +412,33 @@ def test_wrapper_refusals(torch_dev):
         with pytest.raises((ValueError, RuntimeError)):
             bad()
     same(d.attend(), c.attend(0, 0, FILL))
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("row_start", [[0, 90, 40, 60], [90, 0, 90, 30, 90], [0, 90, 89, 88, 87, 90], [-5, 200, -7, 50], [70, 10]])
+def test_row_starts_that_decrease_reach_no_other_memory(torch_dev, row_start, bits):
+    """Outputs between guard rows, pools with pages that no table names: only the batch's rows and its tables' pages change."""
+    from tritify_amd.paged import PagedBatch
+
+    torch = torch_dev
+    say(f"case: row_start={row_start} bits={bits}")
+    seqs, T, G = len(row_start) - 1, 90, 32
+    c = Case(70, [(1, 200)] * seqs, 14, 2, 64, 16, bits, spare=6)
+    d = Dev(torch, c)
+    b = PagedBatch(torch.tensor(row_start, dtype=torch.int32, device="cuda"), d.b.kv_len, d.b.table, T)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    rows = lambda width: torch.randint(-127, 128, (T + 2 * G, width), generator=g, device="cuda").to(torch.int8)  # noqa: E731
+    q, qkv, ws = rows(14 * 64), rows(18 * 64), d.kv.workspace(b, 14)
+    o = torch.full_like(q, FILL)
+    unused = [p for p in range(c.pages) if p not in c.table]
+    assert len(unused) == 6
+    pools = [d.kv.k.clone(), d.kv.v.clone()]
+    cos, sin = rope_tables(220, 64)
+    d.kv.attend(q[G:G + T], b, 14, d.exp, o[G:G + T], ws)
+    assert (o[:G] == FILL).all() and (o[G + T:] == FILL).all()
+    assert torch.equal(pools[0], d.kv.k) and torch.equal(pools[1], d.kv.v)
+    o.fill_(FILL)
+    d.kv.append(qkv[G:G + T], b, 14, torch.from_numpy(cos).cuda(), torch.from_numpy(sin).cuda(), o[G:G + T])
+    assert (o[:G] == FILL).all() and (o[G + T:] == FILL).all()
+    for now, was in ((d.kv.k, pools[0]), (d.kv.v, pools[1])):
+        assert torch.equal(now[unused], was[unused])

@@ -32,8 +32,9 @@ __device__ __forceinline__ PgRows pg_rows(const Paged& a, int b) {
 // Tiles of `step` units, sequence b with rows * mul units: its tiles begin at number floor(t0 mul / step) + per b, which
 // leaves it at least floor(rows mul / step) + per of them, so the grid needs no lengths from the host:
 // tokens mul / step + per seqs tiles in all. Returns the last sequence that begins at or before tile `t` and its first tile,
-// -1 where none does: the wave probes 64 sequences at even distances and goes on between two of them. row_start must not
-// decrease; where it does, some sequence is returned all the same, and its tiles are bounded by its own rows.
+// -1 where none does: the wave probes 64 sequences at even distances and goes on between two of them. Where row_start
+// decreases the probes may end at a sequence that begins past `t`; that counts as none, so that a tile is never before its
+// sequence's first.
 __device__ __forceinline__ int pg_tile_seq(const Paged& a, int t, int mul, int step, int per, int* first) {
     const int lane = threadIdx.x & 63;
     auto begin = [&](int b) { return (int)((int64_t)pg_start(a, b) * mul / step) + per * b; };
@@ -44,7 +45,7 @@ __device__ __forceinline__ int pg_tile_seq(const Paged& a, int t, int mul, int s
         lo += (c - 1) * gap;
         if (gap == 1) {
             *first = begin(lo);
-            return lo;
+            return *first <= t ? lo : -1;
         }
         n = min(gap, n - (c - 1) * gap);
     }
