@@ -241,3 +241,20 @@ def test_captured_steps_of_two_shapes_and_passes_between(model, torch_dev):
             d.run([(other, [1] * (3 * n))])
             del junk
             torch.cuda.synchronize()
+
+
+def test_a_pass_larger_than_the_buffers_is_refused(model, torch_dev):
+    """A caller's own batch of more rows, or of more sequences, than the decoder was made for; a pass within them goes on."""
+    from tritify_amd.paged import PagedBatch, PagedDecoder
+
+    torch = torch_dev
+    d = PagedDecoder(model, 20, max_seqs=2, max_rows=16)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    for rows in ([17], [1, 1, 1], [1, 16]):
+        start = np.concatenate([[0], np.cumsum(rows)])
+        b = PagedBatch(i32(*start), i32(*rows), torch.arange(2 * len(rows), dtype=torch.int32, device="cuda").reshape(-1, 2), int(start[-1]))
+        with pytest.raises(ValueError):
+            d.forward(torch.zeros(b.tokens, dtype=torch.int32, device="cuda"), b, b.row_start[1:].long() - 1, i32(*[0] * b.seqs))
+    p, = prompts([16])
+    s = d.add()
+    assert int(d.run([(s, p)])[0]) == model.generate(p, 1)[0][0]

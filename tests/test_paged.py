@@ -186,3 +186,40 @@ def test_first_maximum_of_ties():
     x[2] = -(2 ** 31)
     assert O.argmax_rows(x, 9).tolist() == [0, 3, 0] and O.argmax_rows(x, 3).tolist() == [0, 0, 0]
     assert exp_table(64)[0] == 32768
+
+
+def _pass(**change):
+    """A decoder of 8 rows and 3 sequences without a model or buffers, and the arguments of a pass of 5 rows: what is not refused
+    fails on the missing model."""
+    import torch
+    from types import SimpleNamespace
+
+    from tritify_amd.paged import PagedDecoder
+
+    d = PagedDecoder.__new__(PagedDecoder)
+    d.torch, d.dev, d.max_rows, d.max_seqs = torch, -1, 8, 3  # torch's number of the CPU
+    a = dict(tokens=5, seqs=3, dev=-1, ids=torch.zeros(5, dtype=torch.int32), last=torch.zeros(3, dtype=torch.int64),
+             out=torch.zeros(3, dtype=torch.int32))
+    a.update({k: v(torch) if callable(v) else v for k, v in change.items()})
+    d.forward(a["ids"], SimpleNamespace(dev=a["dev"], tokens=a["tokens"], seqs=a["seqs"]), a["last"], a["out"])
+
+
+@pytest.mark.parametrize("change", [
+    dict(tokens=9, ids=lambda t: t.zeros(9, dtype=t.int32)), dict(tokens=0), dict(tokens=-1), dict(seqs=0), dict(dev=0),
+    dict(seqs=4, last=lambda t: t.zeros(4, dtype=t.int64), out=lambda t: t.zeros(4, dtype=t.int32)),
+    dict(tokens=2, ids=lambda t: t.zeros(2, dtype=t.int32), last=None), dict(last=None),
+    dict(ids=lambda t: t.zeros(4, dtype=t.int32)), dict(ids=lambda t: t.zeros(5, dtype=t.int64)),
+    dict(ids=lambda t: t.zeros(10, dtype=t.int32)[::2]), dict(ids=lambda t: t.zeros(5, 1, dtype=t.int32)),
+    dict(out=lambda t: t.zeros(2, dtype=t.int32)), dict(out=lambda t: t.zeros(3, dtype=t.int64)),
+    dict(last=lambda t: t.zeros(4, dtype=t.int64)), dict(last=lambda t: t.zeros(3)), dict(last=lambda t: t.zeros(3, 1, dtype=t.int64)),
+])
+def test_passes_past_the_decoders_buffers_are_refused(change):
+    with pytest.raises(ValueError, match="forward"):
+        _pass(**change)
+
+
+@pytest.mark.parametrize("change", [{}, dict(ids=lambda t: t.zeros(9, dtype=t.int32)), dict(last=lambda t: t.zeros(3, dtype=t.int32)),
+                                    dict(tokens=3, last=None)])
+def test_passes_within_the_decoders_buffers_go_on_to_the_model(change):
+    with pytest.raises(AttributeError, match="m"):
+        _pass(**change)

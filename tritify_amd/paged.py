@@ -294,11 +294,30 @@ class PagedDecoder:
             self._ws.append(self.torch.empty(size, dtype=self.torch.int8, device=self.device))
         return self._ws[-1][:n], self._ws[-1][n:]
 
+    def _check_pass(self, tokens_dev, b: PagedBatch, last, out) -> None:
+        """What a pass reads and writes lies within its tensors and the decoder's buffers."""
+        if b.dev != self.dev or not 1 <= b.tokens <= self.max_rows or not 1 <= b.seqs <= self.max_seqs:
+            raise ValueError(f"forward: a batch on GPU {self.dev} of 1 to {self.max_rows} rows and 1 to {self.max_seqs} sequences "
+                             f"is needed, not {b.tokens} rows of {b.seqs} on GPU {b.dev}")
+        i32 = self.torch.int32
+        for t, what, n in ((tokens_dev, "tokens", b.tokens), (out, "out", b.seqs)):
+            if t.dtype is not i32 or t.get_device() != self.dev or t.dim() != 1 or t.shape[0] < n or not t.is_contiguous():
+                raise ValueError(f"forward: {what}: a contiguous vector of at least {n} int32 on GPU {self.dev} is needed, not "
+                                 f"{tuple(t.shape)} {t.dtype} on {t.device}")
+        if last is None:
+            if b.tokens != b.seqs:
+                raise ValueError(f"forward: {b.tokens} rows of {b.seqs} sequences need the indexes of the last rows")
+        elif last.dtype not in (i32, self.torch.int64) or last.get_device() != self.dev or last.shape != (b.seqs,):
+            raise ValueError(f"forward: last: {b.seqs} int32 or int64 on GPU {self.dev} are needed, not {tuple(last.shape)} "
+                             f"{last.dtype} on {last.device}")
+
     def forward(self, tokens_dev, b: PagedBatch, last, out, stream=None) -> None:
-        """The layers over the batch's rows, the logits of each sequence's last row (`last`: their indexes, None where
-        every sequence has one row) to self.logits, the greedy choice of each to out. Asynchronous on `stream`, which
-        torch's current stream has to be; capturable after a call of the batch's shape. Passes of one decoder, captured or
-        not, share its buffers: they follow one another."""
+        """The layers over the batch's rows, whose ids (tokens_dev, int32) are within the vocabulary; the logits of each
+        sequence's last row (`last`: their indexes among the rows, None where every sequence has one row) to self.logits, the
+        greedy choice of each to out (int32). Asynchronous on `stream`, which torch's current stream has to be; capturable
+        after a call of the batch's shape. Passes of one decoder, captured or not, share its buffers: they follow one
+        another."""
+        self._check_pass(tokens_dev, b, last, out)
         m, lib, dev, s, P = self.m, B.lib(), self.dev, B._stream(stream), B._ptr
         T, d, ffn, nh, hd, nq = b.tokens, m.d, m.ffn, m.nh, m.hd, m.nq
         ws, ws_top = self._workspaces(b)
