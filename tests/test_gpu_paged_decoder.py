@@ -46,6 +46,17 @@ def test_generate_equals_the_contiguous_decoder(model, page, chunk):
     assert len(d.free) == free and sorted(d.free) == list(range(free)) and not d.seq
 
 
+@pytest.mark.parametrize("max_rows", [1, 4, 5, 6])
+def test_generate_for_more_prompts_than_a_pass_has_rows(model, max_rows):
+    from tritify_amd.paged import PagedDecoder
+
+    ps = prompts([7, 1, 20, 16, 3, 5])
+    want = np.array([model.generate(p, 4)[0] for p in ps])
+    d = PagedDecoder(model, 40, max_rows=max_rows)
+    assert np.array_equal(d.generate(ps, 4), want)
+    assert len(d.free) == 40 and not d.seq
+
+
 def test_sequences_come_and_go(model, torch_dev):
     """Sequences that join and leave between passes, prompts beside single tokens: logits of every pass as the contiguous
     decoder records them."""

@@ -223,3 +223,33 @@ def test_passes_past_the_decoders_buffers_are_refused(change):
 def test_passes_within_the_decoders_buffers_go_on_to_the_model(change):
     with pytest.raises(AttributeError, match="m"):
         _pass(**change)
+
+
+class Counting:
+    """A PagedDecoder without a model: run notes the rows of its passes and answers with each sequence's length so far."""
+
+    def __new__(cls, max_rows, max_seqs=64):
+        import torch
+
+        from tritify_amd.paged import PagedDecoder
+
+        d = PagedDecoder.__new__(PagedDecoder)
+        d.torch, d.device = torch, torch.device("cpu")
+        d.max_rows, d.max_seqs, d.page, d.sinks, d.seq, d.free, d._next = max_rows, max_seqs, 16, 0, {}, [], 0
+        d.passes = []
+
+        def run(work, stream=None):
+            assert work and sum(len(t) for _, t in work) <= max_rows
+            d.passes.append([len(t) for _, t in work])
+            for s, t in work:
+                d.seq[s]["len"] += len(t)
+            return torch.tensor([d.seq[s]["len"] for s, _ in work], dtype=torch.int32)
+
+        d.run = run
+        return d
+
+
+def test_generates_steps_fit_the_rows_of_a_pass():
+    d = Counting(4)
+    assert d.generate([[5] * n for n in (3, 1, 2, 1, 1, 6)], 3).tolist() == [[n, n + 1, n + 2] for n in (3, 1, 2, 1, 1, 6)]
+    assert d.passes == [[3, 1], [2, 1, 1], [4], [2]] + [[1] * 4, [1] * 2] * 2 and not d.seq

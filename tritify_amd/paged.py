@@ -362,7 +362,7 @@ class PagedDecoder:
     def generate(self, prompts: list, max_new: int, chunk: int | None = None) -> np.ndarray:
         """generate_greedy_by (crates/01-engine/kt-core/src/generate.rs:82-111) for a batch of prompts with no stop
         tokens: max_new tokens each (len(prompts) x max_new). Prompts go in passes of at most `chunk` rows (max_rows by
-        default), shared by as many sequences as fit."""
+        default), shared by as many sequences as fit; a step of more sequences than max_rows takes several passes."""
         chunk = min(chunk or self.max_rows, self.max_rows)
         if max_new < 1 or chunk < 1 or len(prompts) > self.max_seqs or any(len(p) < 1 for p in prompts):
             raise ValueError("generate: at least one token to make, no empty prompt, max_seqs prompts at most")
@@ -385,7 +385,9 @@ class PagedDecoder:
                         out[i, 0] = x
                 todo = left
             for step in range(1, max_new):
-                out[:, step] = self.run([(ids[i], out[i, step - 1:step]) for i in range(len(prompts))]).cpu().numpy()
+                for at in range(0, len(ids), self.max_rows):
+                    now = range(at, min(at + self.max_rows, len(ids)))
+                    out[now.start:now.stop, step] = self.run([(ids[i], out[i, step - 1:step]) for i in now]).cpu().numpy()
         finally:
             for s in ids:
                 self.release(s)
