@@ -174,6 +174,27 @@ def test_passes_and_reads_on_another_stream(model, torch_dev):
     assert torch.equal(k[:62].reshape(-1), model.kc[: 62 * 2 * 64])
 
 
+def test_generate_within_another_stream(model, torch_dev):
+    """The passes, made longer here, are on the null stream, torch's current stream is another: the tokens are read after them."""
+    from tritify_amd.paged import PagedDecoder
+
+    torch = torch_dev
+    ps = prompts([60, 9])
+    want = np.array([model.generate(p, 4)[0] for p in ps])
+    d = PagedDecoder(model, 64, max_rows=100)
+    forward = d.forward
+
+    def late(*a):
+        torch.cuda._sleep(20_000_000)
+        forward(*a)
+
+    d.forward = late
+    with torch.cuda.stream(torch.cuda.Stream()):
+        got = d.generate(ps, 4)
+    torch.cuda.synchronize()
+    assert np.array_equal(got, want)
+
+
 def test_captured_decode_steps(model, torch_dev):
     """A decode step of a batch as one graph: the tables and lengths move on the device arrays between the replays."""
     from tritify_amd.paged import PagedDecoder

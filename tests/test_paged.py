@@ -245,7 +245,7 @@ class Counting:
                 d.seq[s]["len"] += len(t)
             return torch.tensor([d.seq[s]["len"] for s, _ in work], dtype=torch.int32)
 
-        d.run = run
+        d.run, d._torch_stream = run, lambda stream: None
         return d
 
 

@@ -367,6 +367,12 @@ class PagedDecoder:
         if max_new < 1 or chunk < 1 or len(prompts) > self.max_seqs or any(len(p) < 1 for p in prompts):
             raise ValueError("generate: at least one token to make, no empty prompt, max_seqs prompts at most")
         out = np.zeros((len(prompts), max_new), dtype=np.int32)
+
+        def choose(work):
+            t = self.run(work)
+            with self.torch.cuda.stream(self._torch_stream(None)):  # the passes' stream, whatever torch's current one is
+                return t.cpu().numpy()
+
         ids = [self.add() for _ in prompts]
         try:
             todo = [(i, np.asarray(p, dtype=np.int64)) for i, p in enumerate(prompts)]
@@ -379,7 +385,7 @@ class PagedDecoder:
                     if n < len(p):
                         left.append((i, p[n:]))
                     room -= n
-                t = self.run([(ids[i], p) for i, p, _ in work]).cpu().numpy()
+                t = choose([(ids[i], p) for i, p, _ in work])
                 for (i, _, done), x in zip(work, t):
                     if done:
                         out[i, 0] = x
@@ -387,7 +393,7 @@ class PagedDecoder:
             for step in range(1, max_new):
                 for at in range(0, len(ids), self.max_rows):
                     now = range(at, min(at + self.max_rows, len(ids)))
-                    out[now.start:now.stop, step] = self.run([(ids[i], out[i, step - 1:step]) for i in now]).cpu().numpy()
+                    out[now.start:now.stop, step] = choose([(ids[i], out[i, step - 1:step]) for i in now])
         finally:
             for s in ids:
                 self.release(s)
