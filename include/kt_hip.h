@@ -859,6 +859,7 @@ int kt_hip_dec_embed_argmax(int dev, const uint64_t* part_dev, int64_t nparts, c
  * chunk is its 16 int8 values. With 4 bits it is 8 bytes, byte 4 h + r holding code 8 h + r in its low half and code
  * 8 h + 4 + r in its high half, and a part ends with its slots' multipliers (page bytes): a row x of hd values is held as
  * m = ceil(8 max |x| / 7) and the codes c = clamp(round_half_away(8 x / m), +-7) (0 when m is 0), and stands for c m / 8.
+ * (An append writes multipliers up to 147; the read and the attention take any byte, and codes of -8, by the same formulas.)
  *
  * max_pages * page <= KT_PAGED_MAX_POS; nh <= 4096; (tokens + 32 seqs) * nh < 2^27. Pointers and strides (in elements) of int8
  * rows are multiples of 16.

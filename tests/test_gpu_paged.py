@@ -442,3 +442,20 @@ def test_row_starts_that_decrease_reach_no_other_memory(torch_dev, row_start, bi
     assert (o[:G] == FILL).all() and (o[G + T:] == FILL).all()
     for now, was in ((d.kv.k, pools[0]), (d.kv.v, pools[1])):
         assert torch.equal(now[unused], was[unused])
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("what", ["any", "most", "flat"])
+def test_attend_any_byte_in_a_4_bit_pool(torch_dev, what, hd):
+    """A pool is the caller's memory: codes of -8 and multipliers past the 147 that an append writes, to 255 (255 * 2^15 has no
+    three balanced digits, its negative does), by the same formula. In one launch, in split passes and in chunks."""
+    c = Case(71, [(1, 1), (1, 9000), (1, 700), (33, 250)] if what == "any" else [(1, 5000)], 7, 1, hd, 16, 4)
+    n = c.page * hd // 2
+    c.k[:, :n], c.v[:, :n] = (c.g.integers(0, 256, size=(c.pages, n)) for _ in range(2))
+    if what == "any":
+        c.k[:, n:], c.v[:, n:] = (c.g.choice([0, 1, 147, 148, 200, 253, 254, 255], size=(c.pages, c.page)) for _ in range(2))
+    else:
+        c.k[:, n:], c.v[:, n:] = 255, 255
+    if what == "flat":
+        c.exp[:] = 32768
+    check_attend(torch_dev, c)

@@ -22,6 +22,7 @@ namespace kt {
 namespace {
 
 typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+typedef short ss2 __attribute__((ext_vector_type(2)));
 
 struct PgAttend {
     const int8_t* q;
@@ -82,13 +83,13 @@ __device__ __forceinline__ int pg_swz(int n, int r) {
     else return HD == 64 ? n : ((r >> 1) & 1) | (n << 1);
 }
 
-// Four neighbouring dimensions of an output row: clamp(round_half_away(a / b)), a = sum e v and b = sum e as the digits add up (8
-// bits: both negated; 4 bits: v as 16 codes times 1/8 of a multiplier, so 128 sum e), zeros where nothing was seen. The quotient
+// Four neighbouring dimensions of an output row: clamp(round_half_away(a / b)), a = sum e v and b = sum e as the digits add up (both
+// negated; 4 bits: v as 16 codes times 1/8 of a multiplier, so 128 sum e), zeros where nothing was seen. The quotient
 // is a float estimate (relative error below 2^-20, so below 2^-12 for |a / b| < 256); where that is within 2^-12 of a half the
 // exact remainder of 2 |a| + b by 2 b says which side.
 template <int BITS>
 __device__ __forceinline__ void pg_store(int8_t* to, const int64_t (&v)[4], int64_t dn, bool live) {
-    const int64_t b = BITS == 8 ? -dn : 128 * dn;
+    const int64_t b = BITS == 8 ? -dn : -128 * dn;
     auto f = [](uint64_t x) { return __builtin_fmaf((float)(uint32_t)(x >> 32), 4294967296.0f, (float)(uint32_t)x); };
     uint32_t out = 0;
     if (live && b > 0) {
@@ -114,7 +115,7 @@ __device__ __forceinline__ void pg_store(int8_t* to, const int64_t (&v)[4], int6
 #pragma unroll
         for (int r = 0; r < 4; r++) {
             const int x = min(q[r], 127);
-            out |= (uint32_t)(uint8_t)((BITS == 8) != (v[r] < 0) ? -x : x) << (8 * r);
+            out |= (uint32_t)(uint8_t)(v[r] < 0 ? x : -x) << (8 * r);
         }
     }
     *reinterpret_cast<uint32_t*>(to) = out;
@@ -189,8 +190,8 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(W == 8 |
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 e[r] = (uint32_t)min(max(et[i][r], 0), 32768);
-                // 8 bits: the two balanced base-256 digits of -e (2^15 itself has none, -2^15 does); 4 bits: e
-                if constexpr (BITS == 8) e[r] = ((0x8080u - e[r]) ^ 0x8080u) & 0xFFFFu;
+                // 8 bits: the two balanced base-256 digits of -e (2^15 itself has none, -2^15 does); 4 bits: -e
+                e[r] = (BITS == 8 ? (0x8080u - e[r]) ^ 0x8080u : 0u - e[r]) & 0xFFFFu;
             }
             if (NT <= 256 || tid < 256)
                 *reinterpret_cast<v2i*>(sE + 4 * (tid + i * NT)) = v2i{(int)(e[0] | e[1] << 16), (int)(e[2] | e[3] << 16)};
@@ -423,15 +424,15 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(W == 8 |
                 } else {
                     uint32_t f[4];
 #pragma unroll
-                    for (int r = 0; r < 4; r++)  // the balanced digits of e m, below 2^23
-                        f[r] = (__umul24((uint32_t)e[r >> 1][r & 1], ((uint32_t)m[t] >> (8 * r)) & 255) + 0x808080) ^ 0x808080;
+                    for (int r = 0; r < 4; r++)  // the balanced digits of -e m: to -2^15 255 (m is any byte), which e m has not
+                        f[r] = (uint32_t)(__mul24((int)(int16_t)e[r >> 1][r & 1], (int)(((uint32_t)m[t] >> (8 * r)) & 255)) + 0x808080) ^ 0x808080;
                     const uint32_t f01 = __builtin_amdgcn_perm(f[1], f[0], 0x05010400), f23 = __builtin_amdgcn_perm(f[3], f[2], 0x05010400);
                     P[0][t] = (int)__builtin_amdgcn_perm(f23, f01, 0x05040100);
                     P[1][t] = (int)__builtin_amdgcn_perm(f23, f01, 0x07060302);
                     P[ND - 1][t] = (int)__builtin_amdgcn_perm(__builtin_amdgcn_perm(f[3], f[2], 0x0c0c0602),
                                                               __builtin_amdgcn_perm(f[1], f[0], 0x0c0c0602), 0x05040100);
-                    den[0] = (int)__builtin_amdgcn_udot2(e[0], us2{1, 1}, (uint32_t)den[0], false);
-                    den[0] = (int)__builtin_amdgcn_udot2(e[1], us2{1, 1}, (uint32_t)den[0], false);
+                    den[0] = __builtin_amdgcn_sdot2(__builtin_bit_cast(ss2, e[0]), ss2{1, 1}, den[0], false);
+                    den[0] = __builtin_amdgcn_sdot2(__builtin_bit_cast(ss2, e[1]), ss2{1, 1}, den[0], false);
                 }
             }
         };
