@@ -230,11 +230,12 @@ class Counting:
 
     def __new__(cls, max_rows, max_seqs=64):
         import torch
+        from types import SimpleNamespace
 
         from tritify_amd.paged import PagedDecoder
 
         d = PagedDecoder.__new__(PagedDecoder)
-        d.torch, d.device = torch, torch.device("cpu")
+        d.torch, d.device, d.m = torch, torch.device("cpu"), SimpleNamespace(V=1000)
         d.max_rows, d.max_seqs, d.page, d.sinks, d.seq, d.free, d._next = max_rows, max_seqs, 16, 0, {}, [], 0
         d.passes = []
 
@@ -253,3 +254,29 @@ def test_generates_steps_fit_the_rows_of_a_pass():
     d = Counting(4)
     assert d.generate([[5] * n for n in (3, 1, 2, 1, 1, 6)], 3).tolist() == [[n, n + 1, n + 2] for n in (3, 1, 2, 1, 1, 6)]
     assert d.passes == [[3, 1], [2, 1, 1], [4], [2]] + [[1] * 4, [1] * 2] * 2 and not d.seq
+
+
+FLOATS = [[1.5], [2.0], np.array([1.0, 7.9]), [1, float("nan")], ["12"], [None], np.array([[1, 2]]), [1, [2]]]
+
+
+@pytest.mark.parametrize("tokens", FLOATS, ids=repr)
+def test_host_tokens_that_are_not_integers_are_refused(tokens):
+    from tritify_amd.paged import PagedDecoder
+
+    d = Counting(100)
+    s = d.add()
+    with pytest.raises(ValueError, match="integers"):
+        PagedDecoder.run(d, [(s, tokens)])
+    with pytest.raises(ValueError, match="integers"):
+        d.generate([[1, 2], tokens], 2)
+    with pytest.raises(ValueError, match="vocabulary"):
+        d.generate([[1, 2], [3, 1000]], 2)
+    assert d.length(s) == 0 and list(d.seq) == [s] and not d.passes
+
+
+def test_host_tokens_of_any_integer_type():
+    import torch
+
+    d = Counting(100)
+    for ids in ([3, 999], (3, 999), np.array([3, 999], dtype=np.uint16), torch.tensor([3, 999]), [np.int64(3), torch.tensor(999)]):
+        assert d._ids(ids, "") == [3, 999]

@@ -8,6 +8,8 @@ sequence gets the integers that DecoderModel gives it alone. torch allocates the
 """
 from __future__ import annotations
 
+import operator
+
 import numpy as np
 
 from . import backend as B
@@ -254,16 +256,16 @@ class PagedDecoder:
             raise ValueError("run: between 1 and max_seqs sequences, each known and named once")
         if min(rows) < 1 or sum(rows) > self.max_rows:
             raise ValueError(f"run: at least one token each, {self.max_rows} in all at most")
+        ids = []  # of host tokens; a tensor of the device as it is
         for s, t in work:
             if torch.is_tensor(t) and (t.dim() != 1 or t.dtype not in (torch.int32, torch.int64)):
                 raise ValueError(f"run: sequence {s}: tokens are a vector of int32 or int64")
-            if not self._on_gpu(t) and not all(0 <= int(x) < self.m.V for x in t):
-                raise ValueError(f"run: sequence {s} has a token outside the vocabulary")
+            ids.append(t if self._on_gpu(t) else self._ids(t, f"run: sequence {s}"))
         self._reserve([(s, self.seq[s]["len"] + n) for s, n in zip(seqs, rows)])
         with torch.cuda.stream(self._torch_stream(stream)):
             b = self.batch(seqs, rows)
             toks = [t.clamp(0, self.m.V - 1).to(device=self.device, dtype=torch.int32) if self._on_gpu(t) else
-                    torch.tensor([int(x) for x in t], dtype=torch.int32, device=self.device) for _, t in work]
+                    torch.tensor(t, dtype=torch.int32, device=self.device) for t in ids]
             toks = torch.cat(toks) if len(toks) > 1 else toks[0].contiguous()
             last = None
             if b.tokens != b.seqs:
@@ -275,6 +277,16 @@ class PagedDecoder:
             if self.window:
                 self._trim(s)
         return out
+
+    def _ids(self, t, what: str) -> list:
+        """Host tokens as integers of the vocabulary."""
+        try:
+            ids = [operator.index(x) for x in t]
+        except TypeError:
+            raise ValueError(f"{what}: tokens are integers") from None
+        if not all(0 <= x < self.m.V for x in ids):
+            raise ValueError(f"{what} has a token outside the vocabulary")
+        return ids
 
     def _on_gpu(self, t) -> bool:
         return self.torch.is_tensor(t) and t.is_cuda
@@ -366,6 +378,7 @@ class PagedDecoder:
         chunk = min(chunk or self.max_rows, self.max_rows)
         if max_new < 1 or chunk < 1 or len(prompts) > self.max_seqs or any(len(p) < 1 for p in prompts):
             raise ValueError("generate: at least one token to make, no empty prompt, max_seqs prompts at most")
+        todo = [(i, self._ids(p, f"generate: prompt {i}")) for i, p in enumerate(prompts)]
         out = np.zeros((len(prompts), max_new), dtype=np.int32)
 
         def choose(work):
@@ -375,7 +388,6 @@ class PagedDecoder:
 
         ids = [self.add() for _ in prompts]
         try:
-            todo = [(i, np.asarray(p, dtype=np.int64)) for i, p in enumerate(prompts)]
             while todo:
                 room, work, left = chunk, [], []
                 for i, p in todo:
