@@ -459,3 +459,54 @@ def test_attend_any_byte_in_a_4_bit_pool(torch_dev, what, hd):
     if what == "flat":
         c.exp[:] = 32768
     check_attend(torch_dev, c)
+
+
+# sequences of one new token each, positions of the table's width: the positions split over CTAs; 8, 4 and 2 waves at their 65536
+# positions each; and the waves that a wider table asks for where the number of sequences alone would take fewer
+RANGE = [(1, 524288), (70, 524288), (300, 262144), (300, 524288), (1600, 131072), (1600, 262144), (1600, 524288)]
+
+
+@pytest.mark.parametrize("bits,hd", [(8, 64), (4, 64), (8, 128), (4, 128)])
+@pytest.mark.parametrize("seqs,positions", RANGE)
+def test_attend_digit_sums_at_their_bound(torch_dev, seqs, positions, bits, hd):
+    """Tables as wide as a call takes, weights all 2^15, a dimension's value the same at every position: with equal weights a row's
+    answer is that value, and each digit sum is the largest its wave can have. Every page is page 0."""
+    from tritify_amd.paged import PagedBatch, PagedKV, page_bytes
+
+    torch = torch_dev
+    say(f"case: {seqs} sequences, {positions} positions, bits={bits} hd={hd}")
+    page, nh = 256, 7
+    if bits == 8:
+        codes = np.resize([127, -128, -127, 0, 1, -1, 64, -65], hd)
+        value = np.clip(codes, -127, 127)
+        k, v = np.full(page * hd, 127, dtype=np.int8), np.broadcast_to(codes[None, :, None], (page // 16, hd, 16)).astype(np.int8).reshape(-1)
+    else:
+        codes, m = np.resize([7, -8, -7, 0, 1, -1, 3, -4], hd), 255
+        value = np.clip(np.sign(codes) * ((np.abs(codes) * m + 4) // 8), -127, 127)
+        byte = ((codes & 15) | ((codes & 15) << 4))[None, :, None]  # all 16 positions of a dimension alike
+        v = np.concatenate([np.broadcast_to(byte, (page // 16, hd, 8)).astype(np.uint8).reshape(-1), np.full(page, m, dtype=np.uint8)])
+        k = np.concatenate([np.full(page * hd // 2, 0x77, dtype=np.uint8), np.full(page, m, dtype=np.uint8)]).view(np.int8)
+        v = v.view(np.int8)
+    put = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()  # noqa: E731
+    part = page_bytes(page, hd, bits)
+    kv = PagedKV(1, page, 1, hd, bits, k=put(k.reshape(1, 1, part)), v=put(v.reshape(1, 1, part)))
+    rows = np.ones(seqs, dtype=np.int64)
+    kv_len = 1 + (np.arange(seqs) * 37) % 300
+    kv_len[seqs // 2] = positions
+    start = np.concatenate([[0], np.cumsum(rows)]).astype(np.int32)
+    b = PagedBatch(put(start), put(kv_len.astype(np.int32)), torch.zeros(seqs, positions // page, dtype=torch.int32, device="cuda"), seqs)
+    q = torch.full((seqs, nh * hd), 127, dtype=torch.int8, device="cuda")
+    o, exp = torch.full_like(q, FILL), torch.full((1024,), 32768, dtype=torch.int32, device="cuda")
+    kv.attend(q, b, nh, exp, o, kv.workspace(b, nh))
+    same(o.reshape(seqs, nh, hd), np.broadcast_to(value.astype(np.int8), (seqs, nh, hd)))
+
+
+@pytest.mark.parametrize("bits,hd", [(8, 64), (4, 64), (8, 128), (4, 128)])
+def test_attend_the_longest_table(torch_dev, bits, hd):
+    """524288 positions of random values, a single token and the last rows of a chunk, pages named many times over."""
+    c = Case(72, [(1, 30 * 256)], 2, 1, hd, 256, bits, spare=0)
+    c.table = c.g.integers(0, c.pages, size=(2, 524288 // 256)).astype(np.int32)
+    c.max_pages, c.tokens, c.lens = 524288 // 256, 3, [(1, 524288), (2, 400001)]
+    c.kv_len, c.row_start = np.array([524288, 400001], dtype=np.int32), np.array([0, 1, 3], dtype=np.int32)
+    c.q = c.rows8(3, c.width)
+    check_attend(torch_dev, c)
