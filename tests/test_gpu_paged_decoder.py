@@ -57,6 +57,32 @@ def test_generate_for_more_prompts_than_a_pass_has_rows(model, max_rows):
     assert len(d.free) == 40 and not d.seq
 
 
+@pytest.mark.parametrize("seqs", [17, 64, 130])
+def test_many_sequences_in_a_step(model, torch_dev, seqs):
+    """Steps of more rows than the norms are fused for and than the lm_head's one-pass product takes: tokens and logits of each
+    sequence, prompts of a few kinds, are the contiguous decoder's."""
+    from tritify_amd.paged import PagedDecoder
+
+    kinds = prompts([5, 1, 12, 33, 16])
+    ref = [model.generate(p, 4) for p in kinds]
+    of = [(7 * i) % 5 for i in range(seqs)]
+    say(f"case: {seqs} sequences in a step")
+    d = PagedDecoder(model, 6 * seqs, max_seqs=seqs, max_rows=33 * seqs)
+    ids = [d.add() for _ in of]
+    t = d.run([(s, kinds[k]) for s, k in zip(ids, of)])
+    for step in range(4):
+        got = d.logits[:seqs].cpu().numpy()
+        for i, k in enumerate(of):
+            assert np.array_equal(got[i], ref[k][1][step]), (step, i)
+        assert t.cpu().numpy().tolist() == [ref[k][0][step] for k in of], step
+        # host tokens, one tensor of the device a sequence
+        t = d.run([(s, [int(t[i])] if step == 1 else t[i:i + 1]) for i, s in enumerate(ids)])
+    if seqs == 64:
+        d = PagedDecoder(model, 6 * seqs, max_seqs=seqs, max_rows=100)
+        want = np.array([ref[k][0] for k in of])
+        assert np.array_equal(d.generate([kinds[k] for k in of], 4), want)
+
+
 def test_sequences_come_and_go(model, torch_dev):
     """Sequences that join and leave between passes, prompts beside single tokens: logits of every pass as the contiguous
     decoder records them."""
