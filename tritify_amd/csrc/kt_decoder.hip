@@ -176,6 +176,19 @@ __global__ __launch_bounds__(256) void dec_attention_row_kernel(const int8_t* __
     }
 }
 
+// round(a / b) half away from zero clamped to [-127, 127], b > 0: floor((2 |a| + b) / (2 b)) by a double estimate (within
+// one of the exact quotient, which is below 2^8 past the first test) and the exact remainder.
+__device__ __forceinline__ int div_round_q8(int64_t a, int64_t b) {
+    const uint64_t aa = a < 0 ? 0 - (uint64_t)a : (uint64_t)a, n = 2 * aa + (uint64_t)b, d = 2 * (uint64_t)b;
+    if (aa >= 128 * (uint64_t)b) return a < 0 ? -127 : 127;
+    int q = (int)((double)n / (double)d);
+    const int64_t rem = (int64_t)(n - (uint64_t)q * d);
+    if (rem < 0) q--;
+    else if (rem >= (int64_t)d) q++;
+    q = q > 127 ? 127 : q;
+    return a < 0 ? -q : q;
+}
+
 // Prefill attention, hd = 64: a CTA of 8 waves per (q head h, 32 rows), blocks of 32 positions dealt to the waves.
 // Both products run on 32x32x32 int8 MFMAs. S^T = K Q^T puts a row's scores in one lane's registers (lane l: row l % 32;
 // register r of half l / 32: position 8 (r / 4) + 4 (l / 32) + r % 4), which is an operand order of O^T = V^T P^T as it

@@ -108,19 +108,6 @@ __device__ __forceinline__ int tid_now() {
     return t;
 }
 
-// round(a / b) half away from zero clamped to [-127, 127], b > 0: floor((2 |a| + b) / (2 b)) by a double estimate (within
-// one of the exact quotient, which is below 2^8 past the first test) and the exact remainder.
-__device__ __forceinline__ int div_round_q8(int64_t a, int64_t b) {
-    const uint64_t aa = a < 0 ? 0 - (uint64_t)a : (uint64_t)a, n = 2 * aa + (uint64_t)b, d = 2 * (uint64_t)b;
-    if (aa >= 128 * (uint64_t)b) return a < 0 ? -127 : 127;
-    int q = (int)((double)n / (double)d);
-    const int64_t rem = (int64_t)(n - (uint64_t)q * d);
-    if (rem < 0) q--;
-    else if (rem >= (int64_t)d) q++;
-    q = q > 127 ? 127 : q;
-    return a < 0 ? -q : q;
-}
-
 __device__ __forceinline__ int sum4(v4i v) {
     const int ones = 0x01010101;
     int s = __builtin_amdgcn_sdot4(v.x, ones, 0, false);
