@@ -280,3 +280,12 @@ def test_host_tokens_of_any_integer_type():
     d = Counting(100)
     for ids in ([3, 999], (3, 999), np.array([3, 999], dtype=np.uint16), torch.tensor([3, 999]), [np.int64(3), torch.tensor(999)]):
         assert d._ids(ids, "") == [3, 999]
+
+
+def test_generates_bounds():
+    d = Counting(4, max_seqs=3)
+    for bad in (dict(chunk=0), dict(chunk=-1), dict(max_new=0), dict(prompts=[[1]] * 4), dict(prompts=[[1], []])):
+        with pytest.raises(ValueError, match="generate"):
+            d.generate(**{**dict(prompts=[[1, 2]], max_new=2), **bad})
+    assert d.generate([], 3).shape == (0, 3) and not d.passes and not d.seq
+    assert d.generate([[1, 2, 3]], 1, chunk=2).tolist() == [[3]] and d.passes == [[2], [1]]

@@ -375,7 +375,7 @@ class PagedDecoder:
         """generate_greedy_by (crates/01-engine/kt-core/src/generate.rs:82-111) for a batch of prompts with no stop
         tokens: max_new tokens each (len(prompts) x max_new). Prompts go in passes of at most `chunk` rows (max_rows by
         default), shared by as many sequences as fit; a step of more sequences than max_rows takes several passes."""
-        chunk = min(chunk or self.max_rows, self.max_rows)
+        chunk = self.max_rows if chunk is None else min(chunk, self.max_rows)
         if max_new < 1 or chunk < 1 or len(prompts) > self.max_seqs or any(len(p) < 1 for p in prompts):
             raise ValueError("generate: at least one token to make, no empty prompt, max_seqs prompts at most")
         todo = [(i, self._ids(p, f"generate: prompt {i}")) for i, p in enumerate(prompts)]
