@@ -870,8 +870,9 @@ size_t kt_hip_dec_page_bytes(int64_t page, int64_t hd, int bits);
 /* The new rows' RoPE (kt_hip_dec_rope_kv's rule and tables, cos / sin of max_pos positions; 8-byte aligned): row t of
  * qkv_dev (stride qkv_stride; q heads, k heads, v heads; read only) gives its rotated q heads at q_dev + t * q_stride and
  * its rotated k and its v in its position's slot. A row whose position is not below max_pos is as one outside the table:
- * zeros in q_dev, nothing written. Two rows of a call may not share a slot's block of 16 (sequences that share pages
- * share whole pages that no row of the call is in). */
+ * zeros in q_dev, nothing written. A block of 16 slots takes the new rows of at most one block of one sequence's positions;
+ * what a table that gives it those of two leaves in it is undefined (sequences that share pages share whole pages that no
+ * row of the call is in). */
 int kt_hip_dec_rope_kv_paged(int dev, const int8_t* qkv_dev, int64_t tokens, int64_t qkv_stride,
                              const int32_t* row_start_dev, const int32_t* kv_len_dev, const int32_t* table_dev,
                              int64_t seqs, int64_t max_pages, int64_t nh, int64_t nkv, int64_t hd,

@@ -557,21 +557,31 @@ struct Plan {
 };
 
 // From the counts that the host knows. A unit is a column tile of one kv head. Waves: 8 a CTA, one CTA a CU, while the units
-// fit the CUs; else 4, and 2 where that fills the chip by itself (a CTA's waves share its columns, so fewer of them join less).
-// us with 2 / 4 / 8, 14 heads over 2, hd 64: 64 rows behind 4000 positions (56 units) 36.0 / 22.7 / 16.5; 512 behind 4000 (448)
-// 45.9 / 30.9 / 35.3; 1024 alone (896) 15.1 / 12.4 / 23.6; 3 x 1021 alone (2682) 25.5 / 29.0 / 63.5. A wave never has more than
-// 65536 positions: its digit sums stay within 2^14 2^16. Splits, where units leave CUs without one: to 128 CTAs, of at least 8
-// tiles; past that the extra launch, the second reading of K and the sums that meet in memory outweigh it. us with 1 / the
-// rule's / twice its splits: one token behind 131000 (2 units) 353 / 17.8 / 20.2, 4 behind 32000 (8) 92.5 / 18.1 / 21.1, 16 behind
-// 8000 (32) 28.3 / 17.7 / 20.8, 64 (128) 37.1 / 37.1 / 53.8, one behind 5000 17.8 / 11.0 / 10.8; below 64 tiles it gains nothing
-// (behind 2000 10.1 / 11.1 with two).
+// fit the CUs; else 4, and 2 where that fills the chip by itself (a CTA's waves share its columns, so fewer of them join
+// less). us with 2 / 4 / 8, 14 heads over 2, hd 64: 64 rows behind 4000 positions (56 units) 36.0 / 22.7 / 16.5; 512 behind
+// 4000 (448) 45.9 / 30.9 / 35.3; 1024 alone (896) 15.1 / 12.4 / 23.6; 3 x 1021 alone (2682) 25.5 / 29.0 / 63.5. The same
+// rows in 4 bits 53.3 / 29.6 / 21.9, 71.7 / 41.5 / 44.0, 19.1 / 18.0 / 25.6, 37.4 / 37.5 / 68.6. hd 128, 16 heads over 4: 64
+// behind 4000 (68) 47.2 / 31.5 / 22.6, 320 behind 2000 (324) 34.3 / 24.3 / 27.3, 512 behind 4000 (516) 59.9 / 42.4 / 45.6,
+// 1024 alone (1028) 19.1 / 21.0 / 28.2, 1600 alone (1604) 33.4 / 39.5 / 53.3; in 4 bits 64.5 / 38.3 / 28.5, 50.1 / 31.9 /
+// 34.1, 91.9 / 54.5 / 58.2, 25.2 / 25.9 / 32.3, 43.4 / 47.6 / 61.5. So the first border holds for all of them, and at hd
+// 128, with two waves a SIMD, two waves would already do from some 1000 units on, by a tenth. Single tokens differ less: 600
+// behind 1000 (1200 units, hd 64) 36.8 / 41.3 / 54.0, 120 at hd 128 (480) 31.9 / 29.8 / 26.5. A wave never has more than
+// 65536 positions: its digit sums stay within 2^14 2^16. Splits, where units leave CUs without one: to 128 CTAs, of at least
+// 8 tiles; past that the extra launch, the second reading of K and the sums that meet in memory outweigh it. us with 1 / the
+// rule's / twice its splits: one token behind 131000 (2 units) 353 / 17.8 / 20.2, 4 behind 32000 (8) 92.5 / 18.1 / 21.1, 16
+// behind 8000 (32) 28.3 / 17.7 / 20.8, 64 (128) 37.1 / 37.1 / 53.8, one behind 5000 17.8 / 11.0 / 10.8; below 64 tiles it
+// gains nothing (behind 2000 10.1 / 11.1 with two).
 //
-// Kernel times against the bytes and operations that cannot be left out (4 hd a column and visible position): 128 single tokens
-// behind 6100 positions 45.5 us, 199 MB of K and V at 4.4 TB/s (the loads of ragged lengths end unevenly; a plain read of as much
-// reaches 5.9); one token behind 131000 4-bit positions 6 + 14.5 us for 17 MB (two launches, four tiles a wave each, and a join); 1024
-// rows behind 7777 74 us, 30.4 GOP at 0.41 POPS counted once (the scores are formed three times over, weights take two digits);
-// there matrix units, vector units and LDS are busy 25, 50 and 58 % of the time and a wave waits for one of them in turn: 4 waves
-// on 64 columns sharing a tile's K and V in LDS (a third of the reads from the L2) took 87 us against 84 under the profiler.
+// Kernel times against the bytes and operations that cannot be left out (4 hd a column and visible position): 128 single
+// tokens behind 6100 positions 45.5 us, 199 MB of K and V at 4.4 TB/s (the loads of ragged lengths end unevenly; a plain
+// read of as much reaches 5.9); one token behind 131000 4-bit positions 6 + 14.5 us for 17 MB (two launches, four tiles a
+// wave each, and a join; in the second, vector units are busy 45 % of the time and waves wait for half of theirs); 1024 rows
+// behind 7777 74 us, 30.4 GOP at 0.41 POPS counted once (the scores are formed three times over, weights take two digits);
+// there matrix units, vector units and LDS are busy 25, 50 and 58 % of the time and a wave waits for one of them in turn: 4
+// waves on 64 columns sharing a tile's K and V in LDS (a third of the reads from the L2) took 87 us against 84 under the
+// profiler. Two thirds of the LDS time are the turns of K (16 KB a tile over both passes), the rest the look-ups of weights.
+// The same rows over 4-bit pages 123 us, vector units busy 83 %: a score's multiplier and rounding, and three digits of each
+// weight, 465 instructions a tile against 161.
 Plan plan(int64_t tokens, int64_t seqs, int64_t max_pos, int rep, int nkv) {
     const int64_t tiles = seqs + tokens * rep / PG_COLS, steps = max_pos / 64;
     const int64_t units = std::min(tiles, tokens * ((rep + PG_COLS - 1) / PG_COLS)) * nkv;

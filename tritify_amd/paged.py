@@ -362,8 +362,8 @@ class PagedDecoder:
         B.dec_argmax_rows(self.logits, b.seqs, m.V, out, ws_top, stream=stream, dev=dev)
 
     def read(self, s: int, layer: int, max_pos: int | None = None, stream=None):
-        """Sequence s's K and V of a layer as contiguous rows (max_pos x nkv x hd int8, zeros past its length): the caches
-        that DecoderModel continues from. On `stream`, as the passes are."""
+        """Sequence s's K and V of a layer as contiguous rows (max_pos x nkv x hd int8, zeros past its length and where a window
+        has left pages behind): the caches that DecoderModel continues from. On `stream`, as the passes are."""
         torch = self.torch
         n = self.seq[s]["len"] if max_pos is None else max_pos
         with torch.cuda.stream(self._torch_stream(stream)):
