@@ -313,8 +313,8 @@ class PagedDecoder:
                              f"is needed, not {b.tokens} rows of {b.seqs} on GPU {b.dev}")
         i32 = self.torch.int32
         for t, what, n in ((tokens_dev, "tokens", b.tokens), (out, "out", b.seqs)):
-            if t.dtype is not i32 or t.get_device() != self.dev or t.dim() != 1 or t.shape[0] < n or not t.is_contiguous():
-                raise ValueError(f"forward: {what}: a contiguous vector of at least {n} int32 on GPU {self.dev} is needed, not "
+            if t.dtype is not i32 or t.get_device() != self.dev or t.numel() < n or not t.is_contiguous():
+                raise ValueError(f"forward: {what}: a contiguous tensor of at least {n} int32 on GPU {self.dev} is needed, not "
                                  f"{tuple(t.shape)} {t.dtype} on {t.device}")
         if last is None:
             if b.tokens != b.seqs:
