@@ -316,3 +316,27 @@ def test_a_pass_larger_than_the_buffers_is_refused(model, torch_dev):
     p, = prompts([16])
     s = d.add()
     assert int(d.run([(s, p)])[0]) == model.generate(p, 1)[0][0]
+
+
+def test_a_step_padded_with_rows_of_no_sequence(model, torch_dev):
+    """Three sequences of one row each in a pass of five and of twenty rows: the rows behind them change nothing."""
+    from tritify_amd.paged import PagedBatch, PagedDecoder
+
+    torch = torch_dev
+    ps = prompts([9, 30, 4])
+    ref = [model.generate(p, 4) for p in ps]
+    d = PagedDecoder(model, 20, max_rows=64)
+    ids = [d.add() for _ in ps]
+    t = d.run(list(zip(ids, ps)))
+    for step, rows in ((1, 5), (2, 20), (3, 3)):
+        d._reserve([(s, d.length(s) + 1) for s in ids])
+        b = d.batch(ids, [1, 1, 1])
+        x = torch.full((rows,), 5, dtype=torch.int32, device="cuda")
+        x[:3] = t
+        t = torch.full((rows,), -3, dtype=torch.int32, device="cuda")
+        d.forward(x, PagedBatch(b.row_start, b.kv_len, b.table, rows), None, t)
+        assert t.cpu().numpy().tolist() == [r[0][step] for r in ref] + [-3] * (rows - 3)
+        assert np.array_equal(d.logits[:3].cpu().numpy(), [r[1][step] for r in ref])
+        t = t[:3].clone()
+        for s in ids:
+            d.seq[s]["len"] += 1

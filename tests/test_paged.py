@@ -207,7 +207,7 @@ def _pass(**change):
 @pytest.mark.parametrize("change", [
     dict(tokens=9, ids=lambda t: t.zeros(9, dtype=t.int32)), dict(tokens=0), dict(tokens=-1), dict(seqs=0), dict(dev=0),
     dict(seqs=4, last=lambda t: t.zeros(4, dtype=t.int64), out=lambda t: t.zeros(4, dtype=t.int32)),
-    dict(tokens=2, ids=lambda t: t.zeros(2, dtype=t.int32), last=None), dict(last=None),
+    dict(tokens=2, ids=lambda t: t.zeros(2, dtype=t.int32), last=None),
     dict(ids=lambda t: t.zeros(4, dtype=t.int32)), dict(ids=lambda t: t.zeros(5, dtype=t.int64)),
     dict(ids=lambda t: t.zeros(10, dtype=t.int32)[::2]),
     dict(out=lambda t: t.zeros(2, dtype=t.int32)), dict(out=lambda t: t.zeros(3, dtype=t.int64)),
@@ -220,7 +220,7 @@ def test_passes_past_the_decoders_buffers_are_refused(change):
 
 @pytest.mark.parametrize("change", [{}, dict(ids=lambda t: t.zeros(9, dtype=t.int32)),
                                     dict(ids=lambda t: t.zeros(5, 1, dtype=t.int32)), dict(last=lambda t: t.zeros(3, dtype=t.int32)),
-                                    dict(tokens=3, last=None)])
+                                    dict(tokens=3, last=None), dict(last=None)])
 def test_passes_within_the_decoders_buffers_go_on_to_the_model(change):
     with pytest.raises(AttributeError, match="m"):
         _pass(**change)

@@ -317,7 +317,7 @@ class PagedDecoder:
                 raise ValueError(f"forward: {what}: a contiguous tensor of at least {n} int32 on GPU {self.dev} is needed, not "
                                  f"{tuple(t.shape)} {t.dtype} on {t.device}")
         if last is None:
-            if b.tokens != b.seqs:
+            if b.tokens < b.seqs:  # (rows behind the sequences' are a padded batch's)
                 raise ValueError(f"forward: {b.tokens} rows of {b.seqs} sequences need the indexes of the last rows")
         elif last.dtype not in (i32, self.torch.int64) or last.get_device() != self.dev or last.shape != (b.seqs,):
             raise ValueError(f"forward: last: {b.seqs} int32 or int64 on GPU {self.dev} are needed, not {tuple(last.shape)} "
