@@ -14,7 +14,7 @@ position and kv head is held as a multiplier m = ceil(8 max|x| / 7) and codes c 
 norm      V = sum x^2 over a head, R = isqrt(V 2^16 / hd), n = clamp(round(128 x w / R), +-16383) with w at 2^12, then rotate-half by
           the int16 tables of position p + shift[b]: clamp(round((n C - n' S) / 2^20), +-127). v goes as it is.
 weigh     of a row and head, top = max s and R = min(floor(2^40 / sum e), 2^32 - 1) are known; e = T[(top - s + 64) >> 7],
-          s = q . k (4 bits: (m (q . c) + 4) >> 3); W[kv head][position] = sum over rows and heads of (e R) >> 16.
+          s = q . k (4 bits: (m (q . c) + 4) >> 3); W[kv head][position] = sum over rows and heads of e R.
 evict     of more than `budget` positions the first `sinks`, the last `recent` and, of the others, those with the largest W stay (ties: the
           first), in order.
 logprobs  t(d) = (d mant + 2^(shift - 1)) >> shift, in 2^-16 of a power of two. For blocks of 1024 logits with maxima M_B:
@@ -204,7 +204,7 @@ def prepare(case, seed):
         st["stats"] = torch.stack([top, torch.where(R >= 1 << 31, R - (1 << 32), R).to(torch.int32)], dim=-1).contiguous()
     else:
         # sums of weights over many rows: a few positions hold most, many were never looked at
-        w = torch.exp(2.5 * torch.randn(pages, nkv, page, generator=g, device=DEV)).mul_(1 << 22).to(torch.int64)
+        w = torch.exp(2.5 * torch.randn(pages, nkv, page, generator=g, device=DEV)).mul_(1 << 38).to(torch.int64)
         w[torch.rand(pages, nkv, page, generator=g, device=DEV) < 0.2] = 0
         st.update(w=w, to=table_of(after, sum(need)),
                   kept=torch.zeros(seqs, nkv, case["budget"], dtype=torch.int32, device=DEV))
@@ -407,7 +407,7 @@ def _plain_weigh(st):
     x = torch.zeros(c["seqs"], most, nkv, rep, 2, dtype=torch.int64, device=DEV)
     x[b, i] = st["stats"].long().unflatten(1, (nkv, rep))
     top, R = x.permute(0, 2, 1, 3, 4).flatten(2, 3).unbind(dim=-1)
-    w = ((_exp_of(st, top[..., None].to(torch.int32), s).long() * (R & 0xFFFFFFFF)[..., None]) >> 16).sum(dim=2)
+    w = (_exp_of(st, top[..., None].to(torch.int32), s).long() * (R & 0xFFFFFFFF)[..., None]).sum(dim=2)
     live = torch.arange(w.shape[2], device=DEV) < st["kv_len"][:, None]
     sq, j = live.nonzero(as_tuple=True)
     st["w"][st["table"][sq, j // c["page"]].long(), :, j % c["page"]] = w[sq, :, j]
@@ -636,8 +636,8 @@ def exact(case, seed):
                     top, R = st["stats"][at:at + n, h].double().t()
                     R = torch.where(R < 0, R + 4294967296.0, R)
                     i = torch.floor((top[:, None] - s + 64) / 128).clamp(0, 1024).long()
-                    w = torch.floor(T[i] * R[:, None] / 65536)  # exact: below 2^47
-                    total += torch.where(seen, w, 0).sum(dim=0).long()
+                    w = T[i] * R[:, None]  # exact: below 2^47
+                    total += torch.where(seen, w, 0).long().sum(dim=0)
                 st["w"][pid, g, j % page] = total
             at += n
         return st["w"]
