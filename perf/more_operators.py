@@ -19,7 +19,7 @@ evict     of more than `budget` positions the first `sinks`, the last `recent` a
           first), in order.
 logprobs  t(d) = (d mant + 2^(shift - 1)) >> shift, in 2^-16 of a power of two. For blocks of 1024 logits with maxima M_B:
           t = min(t(M_B - x), 31 2^16), e = 2^30 2^(-t / 2^16) (product of two tables, cut), S_B = sum e, W_B = sum e t. Joined to M =
-          max M_B by the same tables, log2 by a table of 1025, outputs in 2^-16 nats.
+          max M_B by the same tables (t at most 41 2^16), log2 by a table of 1025, outputs in 2^-16 nats.
 """
 from __future__ import annotations
 
@@ -459,7 +459,7 @@ def _bits(d, most):
     return ((d.clamp(max=end) * mant + ((1 << shift) >> 1)) >> shift).clamp(max=most)
 
 
-MOST = 31 << 16
+MOST, FAR = 31 << 16, 41 << 16
 LN2 = 5814540  # 2^23 ln 2
 
 
@@ -476,7 +476,7 @@ def _plain_logprobs(st):
     del e, t
     mb = mb[..., 0]
     M = mb.amax(dim=1, keepdim=True)
-    u = _bits(M - mb, MOST)
+    u = _bits(M - mb, FAR)
     m = A[(u & 65535) >> 8] * F[u & 255] >> 32
     W = ((((W + u * S) >> 21) * (m >> 8)) >> (22 + (u >> 16))).sum(dim=1)
     S = (((S >> 8) * m) >> (22 + (u >> 16))).sum(dim=1)
@@ -687,7 +687,7 @@ def _exact_logprobs(st):
         t = torch.where(d < (1 << 22) * 64, (d.clamp(max=1 << 28) * mant + half) >> shift, MOST).clamp(max=MOST)
         e = two[t % 65536] // (2 ** (t // 65536))
         for m_b, s_b, w_b in zip(mb.tolist(), e.sum(dim=1).tolist(), (e * t).sum(dim=1).tolist()):
-            u = power(M - m_b, MOST)
+            u = power(M - m_b, FAR)
             m = A[u % 65536 // 256] * F[u % 256] // 2 ** 32
             S += (s_b // 256 * m) // 2 ** (22 + u // 65536)
             W += ((w_b + u * s_b) // 2 ** 21 * (m // 256)) // 2 ** (22 + u // 65536)
