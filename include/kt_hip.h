@@ -910,6 +910,76 @@ size_t kt_hip_dec_argmax_rows_workspace(int64_t rows, int64_t n);
 int kt_hip_dec_argmax_rows(int dev, const int32_t* logits_dev, int64_t rows, int64_t n, int64_t stride,
                            int32_t* token_dev, void* ws_dev, size_t ws_bytes, void* stream);
 
+/* The append with the heads' norms: kt_hip_dec_rope_kv_paged, where a q head's values go through q_norm_dev and a k head's through
+ * k_norm_dev (hd int16 weights at 2^12, 8-byte aligned; NULL: that head's values are rotated as they are, by the rule above) before the
+ * rotation, in one rounding to a code of 1/32: V = sum x^2 over the head, R = isqrt(V * 2^16 / hd), n = clamp(round_half_away(128 x w / R),
+ * +-16383), 0 where R is 0 (n counts 1/2048 of a unit), a' = clamp(round_half_away((n_a C - n_b S) / 2^20), +-127), b' likewise.
+ * shift_dev (seqs int32, or NULL: zeros): a row at position p of sequence b takes the tables' position p + shift[b] (clamped to
+ * +-2^30 each), which is what a sequence cut down by kt_hip_dec_evict_paged needs: its rows are at the next free position, its
+ * rotations go on counting. A row whose p + shift[b] is not in [0, max_pos) is zeros in q_dev, and nothing of it is written. wpool_dev
+ * (pages x nkv x page int64, 8-byte aligned, or NULL): the accumulated weights of the slots that are written become 0. */
+int kt_hip_dec_norm_rope_kv_paged(int dev, const int8_t* qkv_dev, int64_t tokens, int64_t qkv_stride,
+                                  const int32_t* row_start_dev, const int32_t* kv_len_dev, const int32_t* table_dev,
+                                  int64_t seqs, int64_t max_pages, int64_t nh, int64_t nkv, int64_t hd,
+                                  const int16_t* cos_dev, const int16_t* sin_dev, int64_t max_pos,
+                                  const int16_t* q_norm_dev, const int16_t* k_norm_dev, const int32_t* shift_dev,
+                                  int8_t* q_dev, int64_t q_stride, void* kpool_dev, void* vpool_dev, int64_t* wpool_dev,
+                                  int64_t pages, int64_t page, int bits, void* stream);
+/* kt_hip_dec_attention_paged that also leaves each row's and head's softmax statistics at stats_dev[(t * nh + h) * 2] (tokens x nh x 2
+ * int32, 8-byte aligned): the largest score it sees, and the reciprocal of the sum of its weights, R = min(floor(2^40 / sum e),
+ * 2^32 - 1) as uint32 (0 where the sum is 0; the score is then any). Rows that no sequence has are left as they were. */
+int kt_hip_dec_attention_paged_stats(int dev, const int8_t* q_dev, int64_t tokens, int64_t q_stride,
+                                     const int32_t* row_start_dev, const int32_t* kv_len_dev, const int32_t* table_dev,
+                                     int64_t seqs, int64_t max_pages, int64_t nh, int64_t nkv, int64_t hd,
+                                     const int32_t* exp_tab_dev, int64_t window, int64_t sinks, const void* kpool_dev,
+                                     const void* vpool_dev, int64_t pages, int64_t page, int bits, int8_t* o_dev,
+                                     int64_t o_stride, int32_t* stats_dev, void* ws_dev, size_t ws_bytes, void* stream);
+/* The rows' attention weights added up per position and kv head: for each row, each head of the group and each position that the row
+ * sees (as in the attention, by the same q, table, window and sinks), wpool[page][kv head][slot] += e R, with
+ * e = exp_tab[(top - s + 64) >> 7] as above and (top, R) the row's and head's statistics: 2^40 is one head's whole weight, so a slot has
+ * room for those of 2^23 (past them the sum wraps). With fresh != 0 the sums of the sequences' positions below min(kv_len,
+ * max_pages * page) start from 0. Slots in pages that several of the call's sequences share take the sum over them. Statistics that are
+ * not the rows' own give other sums and reach no other memory. wpool_dev: pages x nkv x page int64, 8-byte aligned. The sums are added
+ * by integer atomics: the same whatever the order. */
+int kt_hip_dec_weigh_paged(int dev, const int8_t* q_dev, int64_t tokens, int64_t q_stride, const int32_t* row_start_dev,
+                           const int32_t* kv_len_dev, const int32_t* table_dev, int64_t seqs, int64_t max_pages,
+                           int64_t nh, int64_t nkv, int64_t hd, const int32_t* exp_tab_dev, int64_t window,
+                           int64_t sinks, const int32_t* stats_dev, int fresh, const void* kpool_dev,
+                           int64_t* wpool_dev, int64_t pages, int64_t page, int bits, void* stream);
+/* Sequences cut down to their heaviest positions: of the L = min(kv_len[b], max_pages * page) positions of sequence b, for each kv
+ * head by itself, all stay where L <= budget; else the first `sinks`, the last `recent` and, of those between, the budget - sinks -
+ * recent with the largest sums in wpool (signed; ties: the lower position; a position without a page is below all others). What stays
+ * goes, in order, to slots 0 .. n - 1 (n = min(L, budget)) of the pages to_dev[b * ceil(budget / page) ..] (an entry outside [0, pages)
+ * drops what goes there): k, v, multipliers and sums; those of a position without a page become zeros. kept_dev (seqs x nkv x budget
+ * int32): the positions that stayed, -1 from n on. The caller then takes to_dev for the sequence's table, n for its length and
+ * L - n more for its shift; the old pages are free. No page may be in to_dev twice, or in both to_dev and table_dev.
+ * 1 <= budget <= KT_PAGED_MAX_POS, sinks + recent <= budget, seqs * ceil(budget / 16) < 2^24 and seqs <= 65535. */
+int kt_hip_dec_evict_paged(int dev, const int32_t* kv_len_dev, const int32_t* table_dev, int64_t seqs, int64_t max_pages,
+                           int64_t nkv, int64_t hd, const int32_t* to_dev, int64_t budget, int64_t recent, int64_t sinks,
+                           int32_t* kept_dev, void* kpool_dev, void* vpool_dev, int64_t* wpool_dev, int64_t pages,
+                           int64_t page, int bits, void* stream);
+/* Log probabilities of rows of n int32 logits (logits_dev + r * stride) under their softmax, in 2^-16 of a natural unit, by integer
+ * rules alone: the same bits whatever the batch. (mant, shift) is the logits' unit: t(d) = (d mant + floor(2^(shift - 1))) >> shift turns a
+ * difference d of logits into 2^-16 of a power of two, 1 <= mant < 2^31, 0 <= shift <= 62; for u codes to the natural unit, mant /
+ * 2^shift = 2^16 log2(e) / u.
+ *   For each block of 1024 neighbouring logits (the last one shorter), M_B its maximum: t = min(t(M_B - x), 31 * 2^16), e = m(t) >>
+ * (t >> 16) with m(t) = (A[(t >> 8) & 255] F[t & 255]) >> 32, A[i] = round(2^31 2^(-i / 2^8)), F[i] = round(2^31 2^(-i / 2^16));
+ * S_B = sum e, W_B = sum e t. With M the row's maximum and u = min(t(M - M_B), 41 * 2^16), k = u >> 16:
+ * S = sum (S_B >> 8) m(u) >> (22 + k), W = sum ((W_B + u S_B) >> 21) (m(u) >> 8) >> (22 + k). L = log2(S / 2^30) at 2^24: a =
+ * floor(log2 S), y = floor(S 2^(31 - a)) - 2^31, i = y >> 21, L = (a - 30) 2^24 + G[i] + ((G[i + 1] - G[i]) (y mod 2^21) >> 21), G[i] =
+ * round(2^24 log2(1 + i / 2^10)). nats(t) = ((t 2^8 + L) 5814540 + 2^30) >> 31 (2^23 ln 2 = 5814539.98).
+ * lp_dev[r] = -nats(min(t(M - x), 2^31 - 1)) of x = the logit of token_dev[r], INT32_MIN for a token outside [0, n). entropy_dev[r] (may be
+ * NULL) = nats(((W << 18) / (S >> 3))). k alternatives (0 <= k <= KT_LOGPROBS_MAX_K; with 0 the arrays may be NULL): top_dev[r * k + i] the
+ * index of the (i + 1)-th largest logit (ties: the lower index first), top_lp_dev its log probability; -1 and INT32_MIN past the n-th.
+ * 0 <= rows <= 65535, 1 <= n <= 2^20. ws_dev: kt_hip_dec_logprobs_rows_workspace bytes (0 for a shape outside these), 8-byte aligned,
+ * needing no contents; calls that may overlap need one each. */
+#define KT_LOGPROBS_MAX_K 32
+size_t kt_hip_dec_logprobs_rows_workspace(int64_t rows, int64_t n, int64_t k);
+int kt_hip_dec_logprobs_rows(int dev, const int32_t* logits_dev, int64_t rows, int64_t n, int64_t stride,
+                             const int32_t* token_dev, int64_t mant, int shift, int32_t* lp_dev, int32_t* entropy_dev,
+                             int64_t k, int32_t* top_dev, int32_t* top_lp_dev, void* ws_dev, size_t ws_bytes,
+                             void* stream);
+
 /* ---------------------------------------------------------------------------------------------------------------
  * Synthetic workload generators (host only, no GPU): the benchmark configs' integer samplers on the reference LCG
  * (apps/kt-demo/src/main.rs:19-22), multithreaded over the host cores. No counterpart in the reference.

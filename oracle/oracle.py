@@ -131,6 +131,11 @@ def _declare(L: C.CDLL) -> None:
         "kt_pg_read": (None, [_P, _P, _P, _L64]),
         "kt_pg_attend": (None, [_P, _P, _L64, _L64, _P, _L64, _L64, _P, _L64]),
         "kt_pg_argmax": (None, [_P, _L64, _L64, _L64, _P]),
+        "kt_pg_norm_rope_append": (None, [_P, _P, _L64, _L64, _P, _P, _L64, _P, _P, _P, _P, _L64, _P]),
+        "kt_pg_stats": (None, [_P, _P, _L64, _L64, _P, _L64, _L64, _P]),
+        "kt_pg_weigh": (None, [_P, _P, _L64, _L64, _P, _L64, _L64, _P, _L64, _P]),
+        "kt_pg_evict": (None, [_P, _P, _L64, _L64, _L64, _P, _P]),
+        "kt_pg_logprobs": (None, [_P, _L64, _L64, _L64, _P, _L64, C.c_int, _P, _P, _P, _P, _P, _L64, _P, _P]),
         "kt_conv2d_i8w16": (None, [_P, _SZ, _SZ, _SZ, _P, _SZ, _SZ, _SZ, _SZ, _SZ, _P, _P, _P, _P, _P, _SZ]),
         "kt_mlp_gelu": (C.c_int, [_P, _SZ, _SZ, _SZ, _P, _P, _P, _P, _P, _P, _P, _P, _P, _SZ]),
         "kt_rd_synthetic": (_P, [C.c_uint64, _SZ, _SZ, _SZ, _SZ, _SZ, _SZ, _SZ, C.c_double, C.c_double, _SZ]),
@@ -801,6 +806,61 @@ def paged_attend(P: Paged, q, nh: int, exp_tab, o, window: int = 0, sinks: int =
     q, exp_tab = _c(q, np.int8), _c(exp_tab, np.int32)
     assert o.dtype == np.int8 and o.flags.c_contiguous
     lib().kt_pg_attend(C.byref(P), _ptr(q), q.shape[1], nh, _ptr(exp_tab), window, sinks, _ptr(o), o.shape[1])
+
+
+def paged_norm_append(P: Paged, qkv, nh: int, cos_t, sin_t, q, q_norm=None, k_norm=None, shift=None, w=None) -> None:
+    """paged_append with the heads' norms (hd int16 each), rotations of position + shift[b], and the sums of written slots made 0."""
+    qkv, cos_t, sin_t = _c(qkv, np.int8), _c(cos_t, np.int16), _c(sin_t, np.int16)
+    q_norm, k_norm = (None if t is None else _c(t, np.int16) for t in (q_norm, k_norm))
+    shift = None if shift is None else _c(shift, np.int32)
+    assert q.dtype == np.int8 and q.flags.c_contiguous and (w is None or (w.dtype == np.int64 and w.flags.c_contiguous))
+    opt = lambda t: None if t is None else _ptr(t)  # noqa: E731
+    lib().kt_pg_norm_rope_append(C.byref(P), _ptr(qkv), qkv.shape[1], nh, _ptr(cos_t), _ptr(sin_t), cos_t.shape[0], opt(q_norm),
+                                 opt(k_norm), opt(shift), _ptr(q), q.shape[1], opt(w))
+
+
+def paged_stats(P: Paged, q, nh: int, exp_tab, window: int = 0, sinks: int = 0) -> np.ndarray:
+    """tokens x nh x 2 int32: the largest score each row and head sees, and the reciprocal of its weights' sum as uint32."""
+    q, exp_tab = _c(q, np.int8), _c(exp_tab, np.int32)
+    stats = np.zeros((P.tokens, nh, 2), dtype=np.int32)
+    lib().kt_pg_stats(C.byref(P), _ptr(q), q.shape[1], nh, _ptr(exp_tab), window, sinks, _ptr(stats))
+    return stats
+
+
+def paged_weigh(P: Paged, q, nh: int, exp_tab, stats, w, window: int = 0, sinks: int = 0, fresh: bool = False) -> None:
+    """The rows' weights added to w (pages x nkv x page int64, in place)."""
+    q, exp_tab, stats = _c(q, np.int8), _c(exp_tab, np.int32), _c(stats, np.int32)
+    assert w.dtype == np.int64 and w.flags.c_contiguous
+    lib().kt_pg_weigh(C.byref(P), _ptr(q), q.shape[1], nh, _ptr(exp_tab), window, sinks, _ptr(stats), int(fresh), _ptr(w))
+
+
+def paged_evict(P: Paged, to, budget: int, recent: int, sinks: int, w) -> np.ndarray:
+    """The positions that stay moved to the pages `to` (seqs x ceil(budget / page)), in P's pools and w; which they are."""
+    T = Paged(P.tokens, P.seqs, to.shape[1], P.pages, P.page, P.nkv, P.hd, P.bits, P.row_start, P.kv_len, 0, P.k, P.v)
+    to = _c(to, np.int32)
+    assert to.shape == (P.seqs, -(-budget // P.page)) and w.dtype == np.int64 and w.flags.c_contiguous
+    T.table = to.ctypes.data
+    kept = np.zeros((P.seqs, P.nkv, budget), dtype=np.int32)
+    lib().kt_pg_evict(C.byref(P), C.byref(T), budget, recent, sinks, _ptr(w), _ptr(kept))
+    return kept
+
+
+def logprob_tables():
+    """2^31 2^(-i / 2^8), 2^31 2^(-i / 2^16), 2^24 log2(1 + i / 2^10), each rounded."""
+    i, j = np.arange(256, dtype=np.float64), np.arange(1025, dtype=np.float64)
+    return tuple(np.round(t).astype(np.int64) for t in (2.0 ** (31 - i / 256), 2.0 ** (31 - i / 65536), 2.0 ** 24 * np.log2(1 + j / 1024)))
+
+
+def logprobs_rows(logits, n: int, tokens, mant: int, shift: int, k: int = 0):
+    """(lp, entropy, top, top_lp) of the first n logits of each row."""
+    logits, tokens = _c(logits, np.int32), _c(tokens, np.int32)
+    rows = logits.shape[0]
+    lp, ent = np.zeros(rows, dtype=np.int32), np.zeros(rows, dtype=np.int32)
+    top, top_lp = np.zeros((rows, k), dtype=np.int32), np.zeros((rows, k), dtype=np.int32)
+    a, f, g = logprob_tables()
+    lib().kt_pg_logprobs(_ptr(logits), rows, n, logits.shape[1], _ptr(tokens), mant, shift, _ptr(a), _ptr(f), _ptr(g), _ptr(lp),
+                         _ptr(ent), k, _ptr(top), _ptr(top_lp))
+    return lp, ent, top, top_lp
 
 
 def argmax_rows(logits, n: int) -> np.ndarray:

@@ -12,6 +12,7 @@ buffers (their data_ptr is passed through the C ABI); torch never computes anyth
 from __future__ import annotations
 
 import ctypes as C
+import math
 import os
 from dataclasses import dataclass
 
@@ -117,6 +118,16 @@ def _declare(L: C.CDLL) -> None:
         "kt_hip_dec_attention_paged_workspace": (_SZ, [_I64] * 7),
         "kt_hip_dec_attention_paged": (_I, [_I, _P, _I64, _I64, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _I64, _I64,
                                             _P, _P, _I64, _I64, _I, _P, _I64, _P, _SZ, _P]),
+        "kt_hip_dec_norm_rope_kv_paged": (_I, [_I, _P, _I64, _I64, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _I64,
+                                               _P, _P, _P, _P, _I64, _P, _P, _P, _I64, _I64, _I, _P]),
+        "kt_hip_dec_attention_paged_stats": (_I, [_I, _P, _I64, _I64, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _I64,
+                                                  _I64, _P, _P, _I64, _I64, _I, _P, _I64, _P, _P, _SZ, _P]),
+        "kt_hip_dec_weigh_paged": (_I, [_I, _P, _I64, _I64, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, _I,
+                                        _P, _P, _I64, _I64, _I, _P]),
+        "kt_hip_dec_evict_paged": (_I, [_I, _P, _P, _I64, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _I64,
+                                        _I, _P]),
+        "kt_hip_dec_logprobs_rows_workspace": (_SZ, [_I64] * 3),
+        "kt_hip_dec_logprobs_rows": (_I, [_I, _P, _I64, _I64, _I64, _P, _I64, _I, _P, _P, _I64, _P, _P, _P, _SZ, _P]),
         "kt_hip_dec_argmax_rows_workspace": (_SZ, [_I64, _I64]),
         "kt_hip_dec_argmax_rows": (_I, [_I, _P, _I64, _I64, _I64, _P, _P, _SZ, _P]),
         "kt_hip_w12_linear_norm": (_I, [_I, _P, _P, _P, _I64, _I64, _I64, _P, _P, _I, _P, _P]),
@@ -1078,3 +1089,38 @@ def dec_argmax_rows(logits_dev, rows: int, n: int, token_dev, ws_dev, stride: in
     check(lib().kt_hip_dec_argmax_rows(dev, _ptr(logits_dev), rows, n, n if stride is None else stride,
                                        _ptr(token_dev), _ptr(ws_dev), ws_dev.nbytes,
                                        _stream(stream)), "dec argmax rows")
+
+
+# log probabilities of a batch's rows
+
+
+def logit_scale(unit: float) -> tuple[int, int]:
+    """(mant, shift) of logits that count `unit` codes to the natural unit: codes to 2^-16 of a power of two."""
+    if not 0 < unit < math.inf:
+        raise ValueError(f"logit_scale: {unit} codes to a natural unit")
+    r = 65536.0 * math.log2(math.e) / unit
+    shift = 30 - math.floor(math.log2(r))
+    mant = round(r * 2.0 ** shift)
+    if mant == 1 << 31:
+        mant, shift = 1 << 30, shift - 1
+    if not 0 <= shift <= 62:
+        raise ValueError(f"logit_scale: {unit} codes to a natural unit")
+    return mant, shift
+
+
+def dec_logprobs_rows_workspace(rows: int, n: int, k: int = 0) -> int:
+    """Bytes of scratch that dec_logprobs_rows of rows x n logits with k alternatives needs."""
+    b = lib().kt_hip_dec_logprobs_rows_workspace(rows, n, k)
+    if b == 0:
+        raise ValueError(f"dec_logprobs_rows: {rows} rows of {n} logits, {k} alternatives")
+    return b
+
+
+def dec_logprobs_rows(logits_dev, rows: int, n: int, tokens_dev, scale, lp_dev, ws_dev, entropy_dev=None, top_dev=None,
+                      top_lp_dev=None, k: int = 0, stride: int | None = None, stream=None, dev: int = 0) -> None:
+    """Log probabilities, in 2^-16 of a natural unit, under each row's softmax (rows `stride` apart, n by default): lp_dev[r] of
+    tokens_dev[r], the entropy, and the k likeliest alternatives (top_dev, top_lp_dev: rows x k). scale: logit_scale(unit)."""
+    mant, shift = scale
+    check(lib().kt_hip_dec_logprobs_rows(dev, _ptr(logits_dev), rows, n, n if stride is None else stride, _ptr(tokens_dev), mant,
+                                         shift, _ptr(lp_dev), _ptr(entropy_dev), k, _ptr(top_dev), _ptr(top_lp_dev), _ptr(ws_dev),
+                                         ws_dev.nbytes, _stream(stream)), "dec logprobs rows")

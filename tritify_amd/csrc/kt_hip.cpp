@@ -1060,25 +1060,39 @@ size_t kt_hip_dec_page_bytes(int64_t page, int64_t hd, int bits) {
     return (size_t)kt::paged_part((int)page, (int)hd, bits);
 }
 
-int kt_hip_dec_rope_kv_paged(int dev, const int8_t* qkv_dev, int64_t tokens, int64_t qkv_stride,
-                             const int32_t* row_start_dev, const int32_t* kv_len_dev, const int32_t* table_dev,
-                             int64_t seqs, int64_t max_pages, int64_t nh, int64_t nkv, int64_t hd,
-                             const int16_t* cos_dev, const int16_t* sin_dev, int64_t max_pos, int8_t* q_dev,
-                             int64_t q_stride, void* kpool_dev, void* vpool_dev, int64_t pages, int64_t page, int bits,
-                             void* stream) {
+int kt_hip_dec_norm_rope_kv_paged(int dev, const int8_t* qkv_dev, int64_t tokens, int64_t qkv_stride,
+                                  const int32_t* row_start_dev, const int32_t* kv_len_dev, const int32_t* table_dev,
+                                  int64_t seqs, int64_t max_pages, int64_t nh, int64_t nkv, int64_t hd,
+                                  const int16_t* cos_dev, const int16_t* sin_dev, int64_t max_pos,
+                                  const int16_t* q_norm_dev, const int16_t* k_norm_dev, const int32_t* shift_dev,
+                                  int8_t* q_dev, int64_t q_stride, void* kpool_dev, void* vpool_dev, int64_t* wpool_dev,
+                                  int64_t pages, int64_t page, int bits, void* stream) {
     if (!paged_ok(tokens, seqs, max_pages, nh, nkv, hd, pages, page, bits) || max_pos < 0 || max_pos > INT_MAX ||
         qkv_stride < (nh + 2 * nkv) * hd || qkv_stride % 16 || q_stride < nh * hd || q_stride % 16)
         return (int)hipErrorInvalidValue;
     if (tokens == 0 || seqs == 0) return 0;
     if (!row_start_dev || !kv_len_dev || !table_dev || !aligned_to(qkv_dev, 16) || !aligned_to(q_dev, 16) ||
         (max_pos > 0 && (!aligned_to(cos_dev, 8) || !aligned_to(sin_dev, 8))) ||
-        (pages > 0 && (!aligned_to(kpool_dev, 16) || !aligned_to(vpool_dev, 16))))
+        (pages > 0 && (!aligned_to(kpool_dev, 16) || !aligned_to(vpool_dev, 16))) ||
+        (q_norm_dev && !aligned_to(q_norm_dev, 8)) || (k_norm_dev && !aligned_to(k_norm_dev, 8)) ||
+        (shift_dev && !aligned_to(shift_dev, 4)) || (wpool_dev && !aligned_to(wpool_dev, 8)))
         return (int)hipErrorInvalidValue;
     KT_TRY(hipSetDevice(dev));
     return (int)kt::launch_pg_append(paged_args(row_start_dev, kv_len_dev, table_dev, kpool_dev, vpool_dev, tokens,
                                                 seqs, max_pages, pages, page, nkv, hd, bits),
-                                     (int)hd, bits, qkv_dev, qkv_stride, (int)nh, cos_dev, sin_dev, (int)max_pos, q_dev,
-                                     q_stride, (hipStream_t)stream);
+                                     (int)hd, bits, qkv_dev, qkv_stride, (int)nh, cos_dev, sin_dev, (int)max_pos,
+                                     q_norm_dev, k_norm_dev, shift_dev, wpool_dev, q_dev, q_stride, (hipStream_t)stream);
+}
+
+int kt_hip_dec_rope_kv_paged(int dev, const int8_t* qkv_dev, int64_t tokens, int64_t qkv_stride,
+                             const int32_t* row_start_dev, const int32_t* kv_len_dev, const int32_t* table_dev,
+                             int64_t seqs, int64_t max_pages, int64_t nh, int64_t nkv, int64_t hd,
+                             const int16_t* cos_dev, const int16_t* sin_dev, int64_t max_pos, int8_t* q_dev,
+                             int64_t q_stride, void* kpool_dev, void* vpool_dev, int64_t pages, int64_t page, int bits,
+                             void* stream) {
+    return kt_hip_dec_norm_rope_kv_paged(dev, qkv_dev, tokens, qkv_stride, row_start_dev, kv_len_dev, table_dev, seqs,
+                                         max_pages, nh, nkv, hd, cos_dev, sin_dev, max_pos, nullptr, nullptr, nullptr,
+                                         q_dev, q_stride, kpool_dev, vpool_dev, nullptr, pages, page, bits, stream);
 }
 
 int kt_hip_dec_kv_read_paged(int dev, const void* kpool_dev, const void* vpool_dev, int64_t pages, int64_t page,
@@ -1104,12 +1118,13 @@ size_t kt_hip_dec_attention_paged_workspace(int64_t tokens, int64_t seqs, int64_
     return kt::pg_attend_workspace((int)tokens, (int)seqs, max_pages * page, (int)nh, (int)nkv, (int)hd);
 }
 
-int kt_hip_dec_attention_paged(int dev, const int8_t* q_dev, int64_t tokens, int64_t q_stride,
-                               const int32_t* row_start_dev, const int32_t* kv_len_dev, const int32_t* table_dev,
-                               int64_t seqs, int64_t max_pages, int64_t nh, int64_t nkv, int64_t hd,
-                               const int32_t* exp_tab_dev, int64_t window, int64_t sinks, const void* kpool_dev,
-                               const void* vpool_dev, int64_t pages, int64_t page, int bits, int8_t* o_dev,
-                               int64_t o_stride, void* ws_dev, size_t ws_bytes, void* stream) {
+// kt_hip_dec_attention_paged and kt_hip_dec_attention_paged_stats (stats_dev non-null).
+static int attention_paged(int dev, const int8_t* q_dev, int64_t tokens, int64_t q_stride, const int32_t* row_start_dev,
+                           const int32_t* kv_len_dev, const int32_t* table_dev, int64_t seqs, int64_t max_pages,
+                           int64_t nh, int64_t nkv, int64_t hd, const int32_t* exp_tab_dev, int64_t window,
+                           int64_t sinks, const void* kpool_dev, const void* vpool_dev, int64_t pages, int64_t page,
+                           int bits, int8_t* o_dev, int64_t o_stride, int32_t* stats_dev, void* ws_dev, size_t ws_bytes,
+                           void* stream) {
     if (!paged_ok(tokens, seqs, max_pages, nh, nkv, hd, pages, page, bits) || window < 0 || sinks < 0 ||
         q_stride < nh * hd || q_stride % 16 || o_stride < nh * hd || o_stride % 16)
         return (int)hipErrorInvalidValue;
@@ -1126,7 +1141,92 @@ int kt_hip_dec_attention_paged(int dev, const int8_t* q_dev, int64_t tokens, int
                                                 seqs, max_pages, pages, page, nkv, hd, bits),
                                      (int)hd, bits, q_dev, q_stride, (int)nh, exp_tab_dev,
                                      (int)(window < most ? window : 0), (int)std::min(sinks, most), o_dev, o_stride,
-                                     ws_dev, (hipStream_t)stream);
+                                     stats_dev, ws_dev, (hipStream_t)stream);
+}
+
+int kt_hip_dec_attention_paged(int dev, const int8_t* q_dev, int64_t tokens, int64_t q_stride,
+                               const int32_t* row_start_dev, const int32_t* kv_len_dev, const int32_t* table_dev,
+                               int64_t seqs, int64_t max_pages, int64_t nh, int64_t nkv, int64_t hd,
+                               const int32_t* exp_tab_dev, int64_t window, int64_t sinks, const void* kpool_dev,
+                               const void* vpool_dev, int64_t pages, int64_t page, int bits, int8_t* o_dev,
+                               int64_t o_stride, void* ws_dev, size_t ws_bytes, void* stream) {
+    return attention_paged(dev, q_dev, tokens, q_stride, row_start_dev, kv_len_dev, table_dev, seqs, max_pages, nh, nkv, hd,
+                           exp_tab_dev, window, sinks, kpool_dev, vpool_dev, pages, page, bits, o_dev, o_stride, nullptr,
+                           ws_dev, ws_bytes, stream);
+}
+
+int kt_hip_dec_attention_paged_stats(int dev, const int8_t* q_dev, int64_t tokens, int64_t q_stride,
+                                     const int32_t* row_start_dev, const int32_t* kv_len_dev, const int32_t* table_dev,
+                                     int64_t seqs, int64_t max_pages, int64_t nh, int64_t nkv, int64_t hd,
+                                     const int32_t* exp_tab_dev, int64_t window, int64_t sinks, const void* kpool_dev,
+                                     const void* vpool_dev, int64_t pages, int64_t page, int bits, int8_t* o_dev,
+                                     int64_t o_stride, int32_t* stats_dev, void* ws_dev, size_t ws_bytes, void* stream) {
+    if (tokens > 0 && seqs > 0 && !aligned_to(stats_dev, 8)) return (int)hipErrorInvalidValue;
+    return attention_paged(dev, q_dev, tokens, q_stride, row_start_dev, kv_len_dev, table_dev, seqs, max_pages, nh, nkv, hd,
+                           exp_tab_dev, window, sinks, kpool_dev, vpool_dev, pages, page, bits, o_dev, o_stride, stats_dev,
+                           ws_dev, ws_bytes, stream);
+}
+
+int kt_hip_dec_weigh_paged(int dev, const int8_t* q_dev, int64_t tokens, int64_t q_stride, const int32_t* row_start_dev,
+                           const int32_t* kv_len_dev, const int32_t* table_dev, int64_t seqs, int64_t max_pages,
+                           int64_t nh, int64_t nkv, int64_t hd, const int32_t* exp_tab_dev, int64_t window,
+                           int64_t sinks, const int32_t* stats_dev, int fresh, const void* kpool_dev,
+                           int64_t* wpool_dev, int64_t pages, int64_t page, int bits, void* stream) {
+    if (!paged_ok(tokens, seqs, max_pages, nh, nkv, hd, pages, page, bits) || seqs > 65535 || window < 0 || sinks < 0 ||
+        q_stride < nh * hd || q_stride % 16)
+        return (int)hipErrorInvalidValue;
+    if (seqs == 0 || pages == 0 || (tokens == 0 && !fresh)) return 0;
+    if (!kv_len_dev || !table_dev || !aligned_to(wpool_dev, 8) || !aligned_to(kpool_dev, 16) ||
+        (tokens > 0 && (!row_start_dev || !exp_tab_dev || !aligned_to(q_dev, 16) || !aligned_to(stats_dev, 8))))
+        return (int)hipErrorInvalidValue;
+    const int64_t most = KT_PAGED_MAX_POS;
+    KT_TRY(hipSetDevice(dev));
+    return (int)kt::launch_pg_weigh(paged_args(row_start_dev, kv_len_dev, table_dev, kpool_dev, nullptr, tokens, seqs,
+                                               max_pages, pages, page, nkv, hd, bits),
+                                    (int)hd, bits, q_dev, q_stride, (int)nh, exp_tab_dev, (int)(window < most ? window : 0),
+                                    (int)std::min(sinks, most), stats_dev, fresh != 0, wpool_dev, (hipStream_t)stream);
+}
+
+int kt_hip_dec_evict_paged(int dev, const int32_t* kv_len_dev, const int32_t* table_dev, int64_t seqs, int64_t max_pages,
+                           int64_t nkv, int64_t hd, const int32_t* to_dev, int64_t budget, int64_t recent, int64_t sinks,
+                           int32_t* kept_dev, void* kpool_dev, void* vpool_dev, int64_t* wpool_dev, int64_t pages,
+                           int64_t page, int bits, void* stream) {
+    if (!paged_ok(0, seqs, max_pages, nkv, nkv, hd, pages, page, bits) || seqs > 65535 || nkv > 65535 || budget < 1 ||
+        budget > KT_PAGED_MAX_POS || recent < 0 || sinks < 0 || recent > budget || sinks > budget - recent ||
+        seqs * ((budget + 15) / 16) >= 1 << 24)
+        return (int)hipErrorInvalidValue;
+    if (seqs == 0) return 0;
+    if (!kv_len_dev || !table_dev || !to_dev || !aligned_to(kept_dev, 4) ||
+        (pages > 0 && (!aligned_to(kpool_dev, 16) || !aligned_to(vpool_dev, 16) || !aligned_to(wpool_dev, 8))))
+        return (int)hipErrorInvalidValue;
+    KT_TRY(hipSetDevice(dev));
+    return (int)kt::launch_pg_evict(paged_args(nullptr, kv_len_dev, table_dev, kpool_dev, vpool_dev, 0, seqs, max_pages,
+                                               pages, page, nkv, hd, bits),
+                                    (int)hd, bits, to_dev, (int)budget, (int)recent, (int)sinks, kept_dev, wpool_dev,
+                                    (hipStream_t)stream);
+}
+
+static bool logprobs_ok(int64_t rows, int64_t n, int64_t k) {
+    return rows >= 0 && rows <= 65535 && n >= 1 && n <= 1 << 20 && k >= 0 && k <= KT_LOGPROBS_MAX_K;
+}
+
+size_t kt_hip_dec_logprobs_rows_workspace(int64_t rows, int64_t n, int64_t k) {
+    return logprobs_ok(rows, n, k) ? kt::lp_workspace(rows, n) : 0;
+}
+
+int kt_hip_dec_logprobs_rows(int dev, const int32_t* logits_dev, int64_t rows, int64_t n, int64_t stride,
+                             const int32_t* token_dev, int64_t mant, int shift, int32_t* lp_dev, int32_t* entropy_dev,
+                             int64_t k, int32_t* top_dev, int32_t* top_lp_dev, void* ws_dev, size_t ws_bytes,
+                             void* stream) {
+    if (!logprobs_ok(rows, n, k) || stride < n || mant < 1 || mant > INT_MAX || shift < 0 || shift > 62)
+        return (int)hipErrorInvalidValue;
+    if (rows == 0) return 0;
+    if (!logits_dev || !token_dev || !lp_dev || (k > 0 && (!top_dev || !top_lp_dev)) || !aligned_to(ws_dev, 8) ||
+        ws_bytes < kt_hip_dec_logprobs_rows_workspace(rows, n, k))
+        return (int)hipErrorInvalidValue;
+    KT_TRY(hipSetDevice(dev));
+    return (int)kt::launch_logprobs(logits_dev, (int)rows, (int)n, stride, token_dev, (uint32_t)mant, shift, lp_dev,
+                                    entropy_dev, (int)k, top_dev, top_lp_dev, ws_dev, (hipStream_t)stream);
 }
 
 size_t kt_hip_dec_argmax_rows_workspace(int64_t rows, int64_t n) {

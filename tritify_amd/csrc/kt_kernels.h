@@ -89,12 +89,22 @@ struct Paged {
 };
 inline int paged_part(int page, int hd, int bits) { return bits == 8 ? page * hd : page * (hd / 2 + 1); }
 hipError_t launch_pg_append(const Paged& a, int hd, int bits, const int8_t* qkv, int64_t stride, int nh,
-                            const int16_t* cosT, const int16_t* sinT, int max_pos, int8_t* q, int64_t q_stride,
+                            const int16_t* cosT, const int16_t* sinT, int max_pos, const int16_t* q_norm,
+                            const int16_t* k_norm, const int32_t* shift, int64_t* w, int8_t* q, int64_t q_stride,
                             hipStream_t s);
 hipError_t launch_pg_read(const Paged& a, int hd, int bits, int8_t* k, int8_t* v, int64_t max_pos, hipStream_t s);
 hipError_t launch_pg_attend(const Paged& a, int hd, int bits, const int8_t* q, int64_t q_stride, int nh,
-                            const int32_t* exp_tab, int window, int sinks, int8_t* o, int64_t o_stride, void* ws,
-                            hipStream_t s);
+                            const int32_t* exp_tab, int window, int sinks, int8_t* o, int64_t o_stride, int32_t* stats,
+                            void* ws, hipStream_t s);
+hipError_t launch_pg_weigh(const Paged& a, int hd, int bits, const int8_t* q, int64_t q_stride, int nh,
+                           const int32_t* exp_tab, int window, int sinks, const int32_t* stats, bool fresh, int64_t* w,
+                           hipStream_t s);
+hipError_t launch_pg_evict(const Paged& a, int hd, int bits, const int32_t* to, int budget, int recent, int sinks,
+                           int32_t* kept, int64_t* w, hipStream_t s);
+size_t lp_workspace(int64_t rows, int64_t n);
+hipError_t launch_logprobs(const int32_t* logits, int rows, int n, int64_t stride, const int32_t* token, uint32_t mant,
+                           int shift, int32_t* lp, int32_t* ent, int k, int32_t* top, int32_t* top_lp, void* ws,
+                           hipStream_t s);
 size_t pg_attend_workspace(int tokens, int seqs, int64_t max_pos, int nh, int nkv, int hd);
 int pg_argmax_parts(int64_t rows, int64_t n);
 hipError_t launch_pg_argmax(const int32_t* logits, int rows, int n, int64_t stride, int32_t* token, uint64_t* part,

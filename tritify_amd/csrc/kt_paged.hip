@@ -16,8 +16,9 @@ namespace kt {
 
 namespace {
 
-__device__ __forceinline__ int rope_round(int v) {  // clamp(round_half_away(v / 2^14)), |v| < 2^30
-    int q = ((v < 0 ? -v : v) + (1 << 13)) >> 14;
+template <int SH = 14>
+__device__ __forceinline__ int rope_round(int v) {  // clamp(round_half_away(v / 2^SH)), |v| <= 2^30
+    int q = ((v < 0 ? -v : v) + (1 << (SH - 1))) >> SH;
     q = q > 127 ? 127 : q;
     return v < 0 ? -q : q;
 }
@@ -47,6 +48,32 @@ __device__ __forceinline__ int value4(int c, int m) {
     return t < 0 ? -q : q;
 }
 
+// What the append with the heads' norms has beside the plain one.
+struct PgNorm {
+    const int16_t *q, *k;  // weights, or null
+    const int32_t* shift;  // or null
+    int64_t* w;            // the sums of weights of a slot, or null
+};
+
+// floor(sqrt(v)), v <= 2^30: the float root is off by less than one.
+__device__ __forceinline__ int isqrt30(int v) {
+    int r = (int)__builtin_amdgcn_sqrtf((float)v);
+    r -= r * r > v;
+    r += (r + 1) * (r + 1) <= v;
+    return r;
+}
+
+// clamp(round_half_away(128 y / R), +-16383), |y| <= 2^22, 1 <= R <= 2^15, inv about 1 / (2 R): floor((256 |y| + R) / (2 R)), a float
+// estimate that is off by one at most below 2^14 (its relative error is below 2^-21), settled by the remainder.
+__device__ __forceinline__ int norm_code(int y, int R, float inv) {
+    const int n = 256 * (y < 0 ? -y : y) + R;
+    int q = (int)__builtin_fminf((float)n * inv, 16384.0f);
+    const int rem = n - q * 2 * R;
+    q += rem < 0 ? -1 : (rem >= 2 * R ? 1 : 0);
+    q = q > 16383 ? 16383 : q;
+    return y < 0 ? -q : q;
+}
+
 // One CTA per (block of 16 positions that a sequence's rows reach, kv head): it rotates the q heads of the group and the k
 // head of the rows in the block, four pairs a thread, stages k and v in LDS and writes the block's bytes. The block is the
 // unit because V's chunk is 16 positions of a dimension, in 4 bits with two positions to a byte: what rows fill goes out in
@@ -57,11 +84,13 @@ __device__ __forceinline__ int value4(int c, int m) {
 // of the busy time; by vector instructions where CTAs fill the CUs: 3 x 4000 rows (hd 64) 12.8 us for 31 MB, 0.74 busy with 19 a
 // value of qkv, and 2048 rows in 4 bits (16 heads over 4, hd 128; two CTAs a CU, one round) 10.2 us for 12 MB, 0.70 with 33.
 // LDS is busy less than a tenth of the time in each.
-template <int HD, int BITS, int NT>
+//
+// NORM: a head's values are in the HH / 4 neighbouring lanes that hold its pairs, so its sum of squares is a few DPP steps.
+template <int HD, int BITS, int NT, bool NORM>
 __global__ __launch_bounds__(NT) void pg_append_kernel(Paged a, const int8_t* __restrict__ qkv, int64_t stride, int nh,
                                                         const int16_t* __restrict__ cosT,
                                                         const int16_t* __restrict__ sinT, int max_pos,
-                                                        int8_t* __restrict__ q, int64_t q_stride) {
+                                                        int8_t* __restrict__ q, int64_t q_stride, PgNorm nm) {
     constexpr int HH = HD / 2, CH = HD / 16;
     __shared__ __attribute__((aligned(16))) int8_t sKV[2][16][HD];
     __shared__ int sM[2][16], sInv[2][16];
@@ -74,7 +103,14 @@ __global__ __launch_bounds__(NT) void pg_append_kernel(Paged a, const int8_t* __
     const int lo = max(16 * blk, s.p0), hi = min(16 * blk + 16, s.p0 + s.n);
     if (lo >= hi) return;
     // the rows whose position the tables and the caches have
-    const int cap = min(max_pos, a.max_pages << a.page_sh), vlo = max(lo, 0), vhi = min(hi, cap);
+    int cap = min(max_pos, a.max_pages << a.page_sh), vlo = max(lo, 0), shift = 0;
+    if constexpr (NORM) {
+        if (nm.shift) shift = max(-(1 << 30), min(nm.shift[b], 1 << 30));
+        cap = (int)min((int64_t)max_pos - shift, (int64_t)(a.max_pages << a.page_sh));
+        vlo = max(vlo, -shift);
+    }
+    vlo = min(vlo, hi);  // (0 <= vhi - vlo <= 16 wherever the block is)
+    const int vhi = max(min(hi, cap), vlo);
     for (int i = tid; i < (vhi - vlo) * CH; i += NT) {
         const int p = vlo + i / CH, c = i % CH;
         const int8_t* src = qkv + (size_t)(s.t0 + (p - s.p0)) * stride + (nh + a.nkv + g) * HD + 16 * c;
@@ -91,14 +127,35 @@ __global__ __launch_bounds__(NT) void pg_append_kernel(Paged a, const int8_t* __
         if (live) {
             const int8_t* src = qkv + t * stride + (hv < rep ? g * rep + hv : nh + g) * HD + 4 * c;
             const int xa = *reinterpret_cast<const int*>(src), xb = *reinterpret_cast<const int*>(src + HH);
-            const v2i C = *reinterpret_cast<const v2i*>(cosT + (size_t)p * HH + 4 * c);
-            const v2i S = *reinterpret_cast<const v2i*>(sinT + (size_t)p * HH + 4 * c);
+            const v2i C = *reinterpret_cast<const v2i*>(cosT + (size_t)(p + shift) * HH + 4 * c);
+            const v2i S = *reinterpret_cast<const v2i*>(sinT + (size_t)(p + shift) * HH + 4 * c);
+            const int16_t* norm = nullptr;
+            if constexpr (NORM) norm = hv < rep ? nm.q : nm.k;
+            if (NORM && norm) {
+                const v2i A = *reinterpret_cast<const v2i*>(norm + 4 * c), B = *reinterpret_cast<const v2i*>(norm + 4 * c + HH);
+                uint32_t V = (uint32_t)__builtin_amdgcn_sdot4(xa, xa, __builtin_amdgcn_sdot4(xb, xb, 0, false), false);
+                V += dpp32<DPP_XOR1>(V);  // (a head's lanes are all here, and all live or none)
+                V += dpp32<DPP_XOR2>(V);
+                V += dpp32<DPP_HALF_MIRROR>(V);
+                if constexpr (HD == 128) V += dpp32<DPP_MIRROR>(V);
+                const int R = max(1, isqrt30((int)(V << (HD == 64 ? 10 : 9))));
+                const float inv = __builtin_amdgcn_rcpf((float)(2 * R));
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int cc = (int)(int16_t)(C[e >> 1] >> (16 * (e & 1))), ss = (int)(int16_t)(S[e >> 1] >> (16 * (e & 1)));
-                const int u = byte_of(xa, e), w = byte_of(xb, e);
-                x |= (rope_round(u * cc - w * ss) & 255) << (8 * e);
-                y |= (rope_round(w * cc + u * ss) & 255) << (8 * e);
+                for (int e = 0; e < 4; e++) {
+                    const int cc = (int)(int16_t)(C[e >> 1] >> (16 * (e & 1))), ss = (int)(int16_t)(S[e >> 1] >> (16 * (e & 1)));
+                    const int u = norm_code(byte_of(xa, e) * (int)(int16_t)(A[e >> 1] >> (16 * (e & 1))), R, inv);
+                    const int w = norm_code(byte_of(xb, e) * (int)(int16_t)(B[e >> 1] >> (16 * (e & 1))), R, inv);
+                    x |= (rope_round<20>(u * cc - w * ss) & 255) << (8 * e);
+                    y |= (rope_round<20>(w * cc + u * ss) & 255) << (8 * e);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int cc = (int)(int16_t)(C[e >> 1] >> (16 * (e & 1))), ss = (int)(int16_t)(S[e >> 1] >> (16 * (e & 1)));
+                    const int u = byte_of(xa, e), w = byte_of(xb, e);
+                    x |= (rope_round(u * cc - w * ss) & 255) << (8 * e);
+                    y |= (rope_round(w * cc + u * ss) & 255) << (8 * e);
+                }
             }
         }
         if (hv < rep) {
@@ -117,6 +174,9 @@ __global__ __launch_bounds__(NT) void pg_append_kernel(Paged a, const int8_t* __
     const int r0 = vlo & 15, r1 = vhi - 16 * blk;  // the block's rows r0 .. r1 - 1
     const size_t part = ((size_t)id * a.nkv + g) * (size_t)a.part;
     const int slot = (16 * blk) & ((1 << a.page_sh) - 1);
+    if constexpr (NORM) {
+        if (nm.w && tid >= r0 && tid < r1) nm.w[(((size_t)id * a.nkv + g) << a.page_sh) + slot + tid] = 0;
+    }
     if constexpr (BITS == 8) {
         uint8_t* kd = a.k + part + slot * HD;
         uint8_t* vd = a.v + part + slot * HD;
@@ -313,23 +373,32 @@ __global__ __launch_bounds__(256) void pg_argmax_join_kernel(const uint64_t* __r
 }  // namespace
 
 hipError_t launch_pg_append(const Paged& a, int hd, int bits, const int8_t* qkv, int64_t stride, int nh,
-                            const int16_t* cosT, const int16_t* sinT, int max_pos, int8_t* q, int64_t q_stride,
+                            const int16_t* cosT, const int16_t* sinT, int max_pos, const int16_t* q_norm,
+                            const int16_t* k_norm, const int32_t* shift, int64_t* w, int8_t* q, int64_t q_stride,
                             hipStream_t s) {
     const dim3 grid((unsigned)(a.tokens / 16 + 2 * a.seqs), (unsigned)a.nkv);
+    const PgNorm nm = {q_norm, k_norm, shift, w};
     // Few CTAs get more threads each, as long as the chip holds them side by side (two of 1024 a CU, some of them empty). us
     // with 256 / 1024: 132 single tokens' CTAs 4-bit 5.0 / 4.6, a chunk of 100 rows 5.0 / 4.2, 512 rows 4-bit 6.7 / 5.6, 498 CTAs
     // 7.2 / 6.8, 520 (hd 128, 4-bit) 13.2 / 10.6; 948 9.8 / 11.1, 1008 (hd 128, 4-bit) 16.0 / 17.1, 1056 of single tokens 4.9 / 7.4.
     const bool wide = (int64_t)grid.x * grid.y <= 768;
     auto go = [&](auto few, auto lots) {
-        if (wide) lots<<<grid, dim3(1024), 0, s>>>(a, qkv, stride, nh, cosT, sinT, max_pos, q, q_stride);
-        else few<<<grid, dim3(256), 0, s>>>(a, qkv, stride, nh, cosT, sinT, max_pos, q, q_stride);
+        if (wide) lots<<<grid, dim3(1024), 0, s>>>(a, qkv, stride, nh, cosT, sinT, max_pos, q, q_stride, nm);
+        else few<<<grid, dim3(256), 0, s>>>(a, qkv, stride, nh, cosT, sinT, max_pos, q, q_stride, nm);
         return hipGetLastError();
     };
+    if (q_norm || k_norm || shift || w) {
+        if (hd == 64)
+            return bits == 8 ? go(pg_append_kernel<64, 8, 256, true>, pg_append_kernel<64, 8, 1024, true>)
+                             : go(pg_append_kernel<64, 4, 256, true>, pg_append_kernel<64, 4, 1024, true>);
+        return bits == 8 ? go(pg_append_kernel<128, 8, 256, true>, pg_append_kernel<128, 8, 1024, true>)
+                         : go(pg_append_kernel<128, 4, 256, true>, pg_append_kernel<128, 4, 1024, true>);
+    }
     if (hd == 64)
-        return bits == 8 ? go(pg_append_kernel<64, 8, 256>, pg_append_kernel<64, 8, 1024>)
-                         : go(pg_append_kernel<64, 4, 256>, pg_append_kernel<64, 4, 1024>);
-    return bits == 8 ? go(pg_append_kernel<128, 8, 256>, pg_append_kernel<128, 8, 1024>)
-                     : go(pg_append_kernel<128, 4, 256>, pg_append_kernel<128, 4, 1024>);
+        return bits == 8 ? go(pg_append_kernel<64, 8, 256, false>, pg_append_kernel<64, 8, 1024, false>)
+                         : go(pg_append_kernel<64, 4, 256, false>, pg_append_kernel<64, 4, 1024, false>);
+    return bits == 8 ? go(pg_append_kernel<128, 8, 256, false>, pg_append_kernel<128, 8, 1024, false>)
+                     : go(pg_append_kernel<128, 4, 256, false>, pg_append_kernel<128, 4, 1024, false>);
 }
 
 hipError_t launch_pg_read(const Paged& a, int hd, int bits, int8_t* k, int8_t* v, int64_t max_pos, hipStream_t s) {

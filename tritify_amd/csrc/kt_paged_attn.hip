@@ -34,6 +34,7 @@ struct PgAttend {
     int32_t* wlow;             // [unit][split][column]: the least negated scores
     unsigned long long* wsum;  // [unit][16 dimensions][register][lane], then the columns' sums of weights
     unsigned* wcnt;            // [unit]: the splits that have added theirs
+    int32_t* stats;            // [row][head]: the largest score, the reciprocal of the weights' sum; or null
 };
 
 // A CTA's part of the work. PG_WHOLE: both passes over all positions; PG_KEEP: the same with pass 1's scores kept in LDS as
@@ -523,6 +524,12 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(W == 8 |
         auto put = [&](int it, const int64_t (&v)[4], int64_t dn) {  // dimensions 16 (it / 64) + 4 (it % 64 / 16) ..
             pg_store<BITS>(out + 16 * (it >> 6) + 4 * ((it & 63) >> 4), v, dn, pos >= 0);
         };
+        auto leave = [&](int64_t dn) {  // by thread tid < cols, whose column is tid: `low` and the sum of its weights, negated
+            const uint64_t R = dn < 0 && pos >= 0 ? (1ull << 40) / (uint64_t)-dn : 0;
+            v2i* to = reinterpret_cast<v2i*>(p.stats + 2 * ((size_t)(s.t0 + row) * (p.rep * a.nkv) + head));
+            *to = v2i{low == INT_MAX || pos < 0 ? 0 : -low, (int)(uint32_t)(R > 0xFFFFFFFFull ? 0xFFFFFFFFull : R)};
+        };
+        if (MODE != PG_SUMS && p.stats && tid < cols) leave(sDen[tid]);
         for (int it = tid; it < DT * 64; it += NT) {
             if ((it & 15) >= cols) continue;
             int64_t v[4];
@@ -540,6 +547,7 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(W == 8 |
         }
         if constexpr (MODE == PG_SUMS) {  // the unit's last CTA has every split's sums (integers: in any order the same)
             if (!split_last(p.wcnt + unit)) return;
+            if (p.stats && tid < cols) leave((int64_t)__hip_atomic_load(sum + PG_COLS * HD + tid, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
             for (int it = tid; it < DT * 64; it += NT) {
                 if ((it & 15) >= cols) continue;
                 int64_t v[4];
@@ -628,8 +636,8 @@ size_t pg_attend_workspace(int tokens, int seqs, int64_t max_pos, int nh, int nk
 }
 
 hipError_t launch_pg_attend(const Paged& a, int hd, int bits, const int8_t* q, int64_t q_stride, int nh,
-                            const int32_t* exp_tab, int window, int sinks, int8_t* o, int64_t o_stride, void* ws,
-                            hipStream_t s) {
+                            const int32_t* exp_tab, int window, int sinks, int8_t* o, int64_t o_stride, int32_t* stats,
+                            void* ws, hipStream_t s) {
     const int64_t max_pos = (int64_t)a.max_pages << a.page_sh;
     const int rep = nh / a.nkv;
     // With a window a column tile's positions are fewer than window + sinks + 256 (15 of other rows, two tiles' ends each), whatever
@@ -642,7 +650,7 @@ hipError_t launch_pg_attend(const Paged& a, int hd, int bits, const int8_t* q, i
     const int64_t cols = a.tokens > a.seqs ? PG_COLS : std::min(rep, PG_COLS), most = (reach / 64 + 8) / 8 * 8 * cols * 256;
     const int64_t room = 163840 - 8 * 64 * (bits == 8 ? hd : hd / 2) - hd * 128 - 4096;
     const PgAttend p = {q, o, q_stride, o_stride, exp_tab, rep, window, sinks, x.splits, (int)std::min(most, room),
-                        (int32_t*)ws, (unsigned long long*)((char*)ws + w.sum), (unsigned*)((char*)ws + w.cnt)};
+                        (int32_t*)ws, (unsigned long long*)((char*)ws + w.sum), (unsigned*)((char*)ws + w.cnt), stats};
     if (hd == 64) return bits == 8 ? attend<64, 8>(a, p, x, s) : attend<64, 4>(a, p, x, s);
     return bits == 8 ? attend<128, 8>(a, p, x, s) : attend<128, 4>(a, p, x, s);
 }

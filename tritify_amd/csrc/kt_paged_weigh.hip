@@ -1,0 +1,284 @@
+// The attention weights of a ragged batch's rows added up per held position and kv head, on gfx950 (kt_hip_dec_weigh_paged, stated
+// in include/kt_hip.h): what an eviction from a paged cache goes by.
+//
+// With each row's largest score and the reciprocal R of its weights' sum in hand, one pass over K does: a wave holds 64 positions of K
+// as B operands and goes through the columns (a row's q heads of one kv head, as in the attention), 64 of them a time. The scores are
+// 16x16x64 int8 MFMAs with the columns as rows, so a lane has one position and 16 columns, whose weights' balanced base-256
+// digits (of -e, two) are the A operand of a second product as they stand; its B operand is R's digits (five, one a column of
+// the result). Sums of e R are so exact in int32 and meet as int64.
+
+#include <algorithm>
+#include <hip/hip_runtime.h>
+#include <limits.h>
+#include <stdint.h>
+#include <type_traits>
+
+#include "kt_paged.h"
+#include "kt_w12_core.h"
+
+namespace kt {
+
+namespace {
+
+typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+
+struct PgWeigh {
+    const int8_t* q;
+    int64_t q_stride;
+    const int32_t* exp_tab;
+    const int32_t* stats;
+    int nh, rep, window, sinks, splits;
+    int64_t* w;
+};
+
+constexpr int WG_GROUP = 64;   // columns a step
+constexpr int WG_UNIT = 512;   // columns of a CTA: each digit sum stays below 2^14 512
+constexpr int WG_WAVES = 4;
+constexpr int WG_DIGITS = 5;   // of R, below 2^32
+
+// -x of 16 int8 values, -128 taken as -127.
+__device__ __forceinline__ v4i negated(v4i x) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t u = (uint32_t)x[i], h = u & 0x80808080u, t = 0x80808080u - (u & 0x7F7F7F7Fu);
+        const uint32_t z = t & 0x80808080u, least = h & z;
+        x[i] = (int)((t & 0x7F7F7F7Fu) | (~(h | z) & 0x80808080u) | (least - (least >> 7)));
+    }
+    return x;
+}
+
+// The sums of the batch's sequences begin from 0.
+__global__ __launch_bounds__(256) void pg_weigh_zero_kernel(Paged a, int64_t* __restrict__ w) {
+    const int b = blockIdx.y, end = min(pg_len(a, b), a.max_pages << a.page_sh), page = 1 << a.page_sh;
+    for (int j = (int)(blockIdx.x * 256 + threadIdx.x); j < end; j += (int)gridDim.x * 256) {
+        const int id = pg_page(a, b, j >> 4);
+        if (id < 0) continue;
+        for (int g = 0; g < a.nkv; g++) w[((((size_t)id * a.nkv + g) << a.page_sh)) + (j & (page - 1))] = 0;
+    }
+}
+
+template <int HD, int BITS>
+__global__ __launch_bounds__(64 * WG_WAVES) void pg_weigh_kernel(Paged a, PgWeigh p) {
+    constexpr int KC = HD / 64, CPR = HD / 16, NT = 64 * WG_WAVES, HH = HD / 2;
+    constexpr int ROWB = BITS == 8 ? HD : HH, CHB = BITS == 8 ? 16 : 8;
+    typedef typename std::conditional<BITS == 8, v4i, v2i>::type Chunk;
+    __shared__ __attribute__((aligned(16))) int8_t sQ[WG_GROUP * HD], sR[WG_DIGITS * WG_GROUP];
+    __shared__ __attribute__((aligned(16))) int sTop[WG_GROUP], sPos[WG_GROUP];
+    __shared__ uint16_t sE[1028];
+    __shared__ int64_t sSum[WG_WAVES][64 * WG_DIGITS];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l16 = lane & 15, gq = lane >> 4;
+
+    // column units 0 .. seqs - 1 are the sequences' first ones, the rest their further ones
+    const int ntiles = (int)gridDim.x / a.nkv, g = (int)blockIdx.x % a.nkv, unit = ntiles - 1 - (int)blockIdx.x / a.nkv;
+    int b = unit, nth = 0;
+    if (unit >= a.seqs) {
+        int first = 0;
+        b = pg_tile_seq(a, unit - a.seqs, p.rep, WG_UNIT, 0, &first);
+        nth = unit - a.seqs - first + 1;
+    }
+    if (b < 0) return;
+    const PgRows s = pg_rows(a, b);
+    const int m0 = nth * WG_UNIT, mrows = s.n * p.rep;
+    if (m0 >= mrows) return;
+    const int cols = min(WG_UNIT, mrows - m0), groups = (cols + WG_GROUP - 1) / WG_GROUP;
+    const int cap = a.max_pages << a.page_sh, nblk = cap >> 4;
+    const int umin = s.p0 + m0 / p.rep, umax = min(s.p0 + (m0 + cols - 1) / p.rep, cap - 1);
+    const int ntile = umax < 0 || a.pages == 0 ? 0 : umax / 64 + 1;
+    int nsink = 0, w0 = 0;
+    if (p.window && ntile) {
+        nsink = min((min(p.sinks, umax + 1) + 63) / 64, ntile);
+        w0 = max(nsink, (max(umin, 0) - min(p.window - 1, max(umin, 0))) / 64);
+    }
+    const int total = nsink + max(0, ntile - w0), step = p.splits * WG_WAVES, start = (int)blockIdx.y * WG_WAVES;
+    const int rounds = start < total ? (total - 1 - start) / step + 1 : 0;  // of the CTA's first wave, which has the most
+    if (rounds == 0) return;
+    auto at = [&](int n) {  // this wave's n-th tile, or -1
+        const int i = start + w + n * step;
+        return i >= total ? -1 : (i < nsink ? i : i - nsink + w0);
+    };
+
+    for (int i = tid; i < 1024; i += NT) {
+        const uint32_t e = (uint32_t)min(max(p.exp_tab[i], 0), 32768);
+        sE[i] = (uint16_t)((0x8080u - e) ^ 0x8080u);  // the two balanced digits of -e
+    }
+    if (tid == 0) sE[1024] = 0;
+
+    // a group's columns: negated q, 2 (top + 64), positions, R's digits
+    int gmin = 0, gmax = 0;
+    auto stage = [&](int grp) {
+        const int first = m0 + grp * WG_GROUP, n = min(WG_GROUP, cols - grp * WG_GROUP);
+        for (int i = tid; i < WG_GROUP * CPR; i += NT) {
+            const int c = i / CPR, ch = i % CPR, m = first + min(c, n - 1), row = m / p.rep, head = g * p.rep + m - row * p.rep;
+            const v4i x = *reinterpret_cast<const v4i*>(p.q + (size_t)(s.t0 + row) * p.q_stride + head * HD + 16 * ch);
+            *reinterpret_cast<v4i*>(sQ + c * HD + 16 * (ch ^ swz<CPR>(c))) = negated(x);
+        }
+        if (tid < WG_GROUP) {
+            const int m = first + min(tid, n - 1), row = m / p.rep, head = g * p.rep + m - row * p.rep;
+            const v2i st = *reinterpret_cast<const v2i*>(p.stats + 2 * ((size_t)(s.t0 + row) * p.nh + head));
+            const bool live = tid < n && s.p0 + row >= 0 && s.p0 + row < cap;
+            sTop[tid] = (int)(128u + 2u * (uint32_t)st.x);
+            sPos[tid] = live ? s.p0 + row : -1;
+            const uint64_t r = (live ? (uint64_t)(uint32_t)st.y : 0) + 0x8080808080ull;
+            // byte 4 t + r of the lanes of quarter q is column 16 t + 4 q + r
+            const int to = ((tid >> 2) & 3) * 16 + (tid >> 4) * 4 + (tid & 3);
+#pragma unroll
+            for (int d = 0; d < WG_DIGITS; d++) sR[d * WG_GROUP + to] = (int8_t)((r >> (8 * d)) ^ 0x80);
+        }
+        gmin = s.p0 + first / p.rep;
+        gmax = s.p0 + (first + n - 1) / p.rep;
+    };
+
+    struct Keys {
+        Chunk x[4][KC];
+        int m[4];  // 4 bits: the multiplier of the lane's position
+        int id[4];
+    };
+    const uint8_t* const kbase = a.k + (size_t)g * a.part;
+    const uint32_t stride = (uint32_t)a.nkv * (uint32_t)a.part;
+    auto load = [&](int T, Keys& k) {
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            const int blk = min(4 * T + t, nblk - 1), slot = (blk << 4) & ((1 << a.page_sh) - 1);
+            const int id = __builtin_amdgcn_readfirstlane(a.table[(size_t)b * a.max_pages + (blk >> (a.page_sh - 4))]);
+            const bool ok = (unsigned)id < (unsigned)a.pages;
+            const uint8_t* from = kbase + (uint64_t)(ok ? (uint32_t)id : 0u) * stride;
+            k.id[t] = ok && 4 * T + t < nblk ? id : -1;
+#pragma unroll
+            for (int c = 0; c < KC; c++)
+                k.x[t][c] = *reinterpret_cast<const Chunk*>(from + (slot + l16) * ROWB + (gq + 4 * c) * CHB);
+            if constexpr (BITS == 4) k.m[t] = from[(HH << a.page_sh) + slot + l16];
+        }
+    };
+    auto widen = [](Chunk x) {  // 4 bits: 16 times the codes
+        if constexpr (BITS == 8) {
+            return x;
+        } else {
+            constexpr int M = (int)0xF0F0F0F0;
+            return v4i{(x.x << 4) & M, x.x & M, (x.y << 4) & M, x.y & M};
+        }
+    };
+    v4i acc[4][2];
+    // the weights of a block's positions and 16 CT columns, times R
+    auto add = [&](auto ct, int T, const Keys& k, bool full) {
+        constexpr int CT = decltype(ct)::value;
+        v4i rd = {0, 0, 0, 0};
+        if (l16 < WG_DIGITS) rd = *reinterpret_cast<const v4i*>(sR + l16 * WG_GROUP + gq * 16);
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            v4i P[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+            const int j = 64 * T + 16 * t + l16;
+#pragma unroll
+            for (int c = 0; c < CT; c++) {
+                const v4i top = *reinterpret_cast<const v4i*>(sTop + 16 * c + 4 * gq);
+                v4i y = BITS == 8 && HD == 64 ? top : v4i{0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < KC; i++) {
+                    const v4i q = *reinterpret_cast<const v4i*>(sQ + (16 * c + l16) * HD + 16 * ((gq + 4 * i) ^ swz<CPR>(l16 + 16 * c)));
+                    y = mfma16(q, widen(k.x[t][i]), y);
+                    if constexpr (BITS == 8 && HD == 64) y = mfma16(q, k.x[t][i], y);
+                }
+                uint32_t u[4];
+#pragma unroll
+                for (int r = 0; r < 4; r++) {  // 2 (top - s + 64)
+                    if constexpr (BITS == 4) y[r] = (__mul24(y[r], k.m[t]) + 63) >> 7;
+                    u[r] = BITS == 8 && HD == 64 ? (uint32_t)y[r] : (uint32_t)y[r] * 2 + (uint32_t)top[r];
+                }
+                if (!full) {
+                    const v4i pos = *reinterpret_cast<const v4i*>(sPos + 16 * c + 4 * gq);
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const bool sees = k.id[t] >= 0 && j <= pos[r] && (p.window == 0 || j > pos[r] - p.window || j < p.sinks);
+                        u[r] = sees ? u[r] : 0x00FFFFFFu;
+                    }
+                }
+                us2 e[2];
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const uint32_t ix = __builtin_bit_cast(uint32_t, __builtin_elementwise_min(
+                        __builtin_bit_cast(us2, __builtin_amdgcn_perm(u[2 * h + 1], u[2 * h], 0x06050201)), us2{1024, 1024}));
+                    e[h] = us2{sE[ix & 0xFFFF], sE[ix >> 16]};
+                }
+                const uint32_t e01 = __builtin_bit_cast(uint32_t, e[0]), e23 = __builtin_bit_cast(uint32_t, e[1]);
+                P[0][c] = (int)__builtin_amdgcn_perm(e23, e01, 0x06040200);
+                P[1][c] = (int)__builtin_amdgcn_perm(e23, e01, 0x07050301);
+            }
+            acc[t][0] = mfma16(P[0], rd, acc[t][0]);
+            acc[t][1] = mfma16(P[1], rd, acc[t][1]);
+        }
+    };
+
+    Keys now, next;
+    if (at(0) >= 0) load(at(0), now);
+    for (int n = 0; n < rounds; n++) {
+        const int T = at(n), T1 = n + 1 < rounds ? at(n + 1) : -1;
+        if (T1 >= 0) load(T1, next);
+#pragma unroll
+        for (int t = 0; t < 4; t++) acc[t][0] = acc[t][1] = v4i{0, 0, 0, 0};
+        for (int grp = 0; grp < groups; grp++) {
+            if (groups > 1 || n == 0) {
+                if (groups > 1) __syncthreads();
+                stage(grp);
+                __syncthreads();
+            }
+            if (T < 0 || 64 * T > gmax) continue;
+            const bool pages = now.id[0] >= 0 && now.id[1] >= 0 && now.id[2] >= 0 && now.id[3] >= 0;
+            const bool full = pages && 64 * T + 63 <= gmin && gmax < cap &&
+                              (p.window == 0 || 64 * T > gmax - p.window || 64 * T + 63 < p.sinks);
+            if (cols - grp * WG_GROUP <= 16) add(std::integral_constant<int, 1>(), T, now, full);
+            else add(std::integral_constant<int, 4>(), T, now, full);
+        }
+        if (T >= 0) {
+            // register r of acc[t], lane l: position 16 t + 4 (l / 16) + r, digit l % 16; turned to a position a lane
+            int64_t* const sum = sSum[w];
+            __builtin_amdgcn_wave_barrier();
+            if (l16 < WG_DIGITS) {
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        sum[(16 * t + 4 * gq + r) * WG_DIGITS + l16] = ((int64_t)acc[t][0][r] + ((int64_t)acc[t][1][r] << 8)) << (8 * l16);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            int64_t v = 0;
+#pragma unroll
+            for (int d = 0; d < WG_DIGITS; d++) v -= sum[lane * WG_DIGITS + d];
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            const int id = gq == 0 ? now.id[0] : (gq == 1 ? now.id[1] : (gq == 2 ? now.id[2] : now.id[3]));
+            if (id >= 0 && v != 0)
+                (void)__hip_atomic_fetch_add(reinterpret_cast<unsigned long long*>(p.w) + ((((size_t)id * a.nkv + g)) << a.page_sh) +
+                                                 ((64 * T + lane) & ((1 << a.page_sh) - 1)),
+                                             (unsigned long long)v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        now = next;
+    }
+}
+
+}  // namespace
+
+hipError_t launch_pg_weigh(const Paged& a, int hd, int bits, const int8_t* q, int64_t q_stride, int nh, const int32_t* exp_tab,
+                           int window, int sinks, const int32_t* stats, bool fresh, int64_t* w, hipStream_t s) {
+    const int64_t max_pos = (int64_t)a.max_pages << a.page_sh;
+    if (fresh) {
+        const int64_t blocks = std::min<int64_t>((max_pos + 255) / 256, std::max<int64_t>(1, 4096 / a.seqs));
+        pg_weigh_zero_kernel<<<dim3((unsigned)blocks, (unsigned)a.seqs), dim3(256), 0, s>>>(a, w);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess || a.tokens == 0) return e;
+    }
+    const int rep = nh / a.nkv;
+    const int64_t reach = window ? std::min<int64_t>(max_pos, (int64_t)window + sinks + WG_UNIT + 128) : max_pos;
+    const int64_t units = (a.seqs + (int64_t)a.tokens * rep / WG_UNIT) * a.nkv;
+    const int64_t rounds = (reach + 64 * WG_WAVES - 1) / (64 * WG_WAVES);
+    const int64_t splits = std::min(rounds, std::max<int64_t>(1, 2048 / units));
+    const PgWeigh p = {q, q_stride, exp_tab, stats, nh, rep, window, sinks, (int)splits, w};
+    auto go = [&](auto kern) {
+        kern<<<dim3((unsigned)units, (unsigned)splits), dim3(64 * WG_WAVES), 0, s>>>(a, p);
+        return hipGetLastError();
+    };
+    if (hd == 64) return bits == 8 ? go(pg_weigh_kernel<64, 8>) : go(pg_weigh_kernel<64, 4>);
+    return bits == 8 ? go(pg_weigh_kernel<128, 8>) : go(pg_weigh_kernel<128, 4>);
+}
+
+}  // namespace kt

@@ -1,5 +1,6 @@
 """The int8 decoder for many sequences at once: KV caches in pages (8 bits, or quantised to 4), attention of chunks and
-single tokens over them, and the greedy choice of a batch, over the C ABI (kt_hip_dec_*_paged, include/kt_hip.h).
+single tokens over them, the greedy choice of a batch and its log probabilities, head norms, and sequences cut down to the
+positions that attention looks at, over the C ABI (kt_hip_dec_*_paged, kt_hip_dec_*_rows, include/kt_hip.h).
 
 The reference decodes one sequence from contiguous caches (crates/01-engine/kt-core/src/model.rs:290-353,
 generate.rs:82-111); `DecoderModel` mirrors that. `PagedKV` holds one layer's pools and offers the operators on them;
@@ -34,10 +35,11 @@ def _need(t, what: str, dtype, dev: int, shape) -> None:
 
 class PagedBatch:
     """A ragged batch on the device: row_start (seqs + 1 int32), kv_len (seqs int32, the new rows counted) and table
-    (seqs x max_pages int32, -1 where a sequence has no page); `tokens` new rows in all. The tensors are read when the
+    (seqs x max_pages int32, -1 where a sequence has no page); `tokens` new rows in all. shift (seqs int32, or None: zeros):
+    how far each sequence's rotations are ahead of its positions, where it has been cut down. The tensors are read when the
     kernels run, so a captured call follows what is copied into them."""
 
-    def __init__(self, row_start, kv_len, table, tokens: int):
+    def __init__(self, row_start, kv_len, table, tokens: int, shift=None):
         import torch
 
         if not table.is_cuda:
@@ -48,16 +50,19 @@ class PagedBatch:
         _need(table, "table", torch.int32, self.dev, table.shape)
         _need(row_start, "row_start", torch.int32, self.dev, (self.seqs + 1,))
         _need(kv_len, "kv_len", torch.int32, self.dev, (self.seqs,))
-        self.row_start, self.kv_len, self.table = row_start, kv_len, table
+        if shift is not None:
+            _need(shift, "shift", torch.int32, self.dev, (self.seqs,))
+        self.row_start, self.kv_len, self.table, self.shift = row_start, kv_len, table, shift
         self.ptrs = (row_start.data_ptr(), kv_len.data_ptr(), table.data_ptr())
 
 
 class PagedKV:
     """One layer's K and V pools: `pages` pages of `page` positions for `nkv` kv heads of `hd` values, in 8 or 4 bits. k
-    and v (pages x nkv x page_bytes int8) are allocated as zeros unless given. Every call is asynchronous on `stream` (None:
-    the null stream)."""
+    and v (pages x nkv x page_bytes int8) are allocated as zeros unless given; w (pages x nkv x page int64), the slots' accumulated
+    attention weights, if given or, as zeros, with `weights`. Every call is asynchronous on `stream` (None: the null stream)."""
 
-    def __init__(self, pages: int, page: int, nkv: int, hd: int, bits: int = 8, k=None, v=None, dev: int = 0):
+    def __init__(self, pages: int, page: int, nkv: int, hd: int, bits: int = 8, k=None, v=None, dev: int = 0, w=None,
+                 weights: bool = False):
         import torch
 
         part = page_bytes(page, hd, bits)
@@ -69,10 +74,13 @@ class PagedKV:
         shape = (pages, nkv, part)
         self.k = torch.zeros(shape, dtype=torch.int8, device=self.device) if k is None else k
         self.v = torch.zeros(shape, dtype=torch.int8, device=self.device) if v is None else v
-        if k is None or v is None:  # zeros before any stream writes
+        self.w = torch.zeros((pages, nkv, page), dtype=torch.int64, device=self.device) if w is None and weights else w
+        if k is None or v is None or (w is None and weights):  # zeros before any stream writes
             torch.cuda.current_stream(self.device).synchronize()
         _need(self.k, "k", torch.int8, dev, shape)
         _need(self.v, "v", torch.int8, dev, shape)
+        if self.w is not None:
+            _need(self.w, "w", torch.int64, dev, (pages, nkv, page))
         self._pools = (self.k.data_ptr(), self.v.data_ptr(), pages, page, bits)  # as every call passes them
 
     def _batch(self, batch: PagedBatch) -> None:
@@ -94,9 +102,11 @@ class PagedKV:
             raise ValueError(f"{what}: rows must start at multiples of 16 bytes")
         return at, stride
 
-    def append(self, qkv, batch: PagedBatch, nh: int, cos, sin, q, stream=None) -> None:
+    def append(self, qkv, batch: PagedBatch, nh: int, cos, sin, q, stream=None, q_norm=None, k_norm=None, shift=None) -> None:
         """The rows of qkv (q heads, k heads, v heads; read only): their rotated q heads to q, their rotated k and their v
-        to the pages. cos / sin: int16 tables of max_pos x hd / 2 at 2^14."""
+        to the pages. cos / sin: int16 tables of max_pos x hd / 2 at 2^14. q_norm / k_norm (hd int16 at 2^12): the heads are brought
+        to a root mean square of 1 (32 codes) and weighted before the rotation. shift (seqs int32; None: the batch's): added to
+        the positions that the tables are read at. The accumulated weights of the written slots, if there are any, become 0."""
         self._batch(batch)
         hd, nkv = self.hd, self.nkv
         shape = cos.shape
@@ -105,9 +115,20 @@ class PagedKV:
         _need(sin, "sin", self._i16, self.dev, shape)
         at, stride = self._rows(qkv, "qkv", batch, (nh + 2 * nkv) * hd)
         to, q_stride = self._rows(q, "q", batch, nh * hd)
-        B.check(B.lib().kt_hip_dec_rope_kv_paged(
+        shift = batch.shift if shift is None else shift
+        if q_norm is None and k_norm is None and shift is None and self.w is None:
+            B.check(B.lib().kt_hip_dec_rope_kv_paged(
+                self.dev, at, batch.tokens, stride, *batch.ptrs, batch.seqs, batch.max_pages, nh, nkv, hd, cos.data_ptr(),
+                sin.data_ptr(), n, to, q_stride, *self._pools, B._stream(stream)), "dec rope + paged append")
+            return
+        for t, what, dtype, size in ((q_norm, "q_norm", self._i16, hd), (k_norm, "k_norm", self._i16, hd),
+                                     (shift, "shift", self._i32, batch.seqs)):
+            if t is not None:
+                _need(t, what, dtype, self.dev, (size,))
+        B.check(B.lib().kt_hip_dec_norm_rope_kv_paged(
             self.dev, at, batch.tokens, stride, *batch.ptrs, batch.seqs, batch.max_pages, nh, nkv, hd, cos.data_ptr(),
-            sin.data_ptr(), n, to, q_stride, *self._pools, B._stream(stream)), "dec rope + paged append")
+            sin.data_ptr(), n, B._ptr(q_norm), B._ptr(k_norm), B._ptr(shift), to, q_stride, *self._pools[:2], B._ptr(self.w),
+            *self._pools[2:], B._stream(stream)), "dec norm + rope + paged append")
 
     def read(self, batch: PagedBatch, k, v, stream=None) -> None:
         """Every sequence's positions as contiguous rows: k / v seqs x max_pos x nkv x hd int8, positions from
@@ -137,19 +158,59 @@ class PagedKV:
         return torch.empty(self.workspace_bytes(batch, nh), dtype=torch.int8, device=self.device)
 
     def attend(self, q, batch: PagedBatch, nh: int, exp_tab, o, ws, window: int = 0, sinks: int = 0,
-               stream=None) -> None:
+               stream=None, stats=None) -> None:
         """The rows' attention over their sequences' pages (after the append of the rows' own k and v), q and o rows of
-        nh * hd. window >= 1: a row at p sees positions past p - window and the first `sinks`; 0: all up to its own."""
+        nh * hd. window >= 1: a row at p sees positions past p - window and the first `sinks`; 0: all up to its own. stats
+        (tokens x nh x 2 int32, or None) takes each row's and head's largest score and the reciprocal of its weights' sum, which
+        weigh needs."""
         self._batch(batch)
         _need(exp_tab, "exp_tab", self._i32, self.dev, (1024,))
         if ws.get_device() != self.dev or not ws.is_contiguous():
             raise ValueError(f"ws: a contiguous tensor on GPU {self.dev} is needed")
         at, q_stride = self._rows(q, "q", batch, nh * self.hd)
         to, o_stride = self._rows(o, "o", batch, nh * self.hd)
-        B.check(B.lib().kt_hip_dec_attention_paged(
+        args = (self.dev, at, batch.tokens, q_stride, *batch.ptrs, batch.seqs, batch.max_pages, nh, self.nkv, self.hd,
+                exp_tab.data_ptr(), window, sinks, *self._pools, to, o_stride)
+        if stats is None:
+            B.check(B.lib().kt_hip_dec_attention_paged(*args, ws.data_ptr(), ws.nbytes, B._stream(stream)), "dec paged attention")
+            return
+        _need(stats, "stats", self._i32, self.dev, (batch.tokens, nh, 2))
+        B.check(B.lib().kt_hip_dec_attention_paged_stats(*args, stats.data_ptr(), ws.data_ptr(), ws.nbytes, B._stream(stream)),
+                "dec paged attention with its statistics")
+
+    def weigh(self, q, batch: PagedBatch, nh: int, exp_tab, stats, window: int = 0, sinks: int = 0, fresh: bool = False,
+              stream=None) -> None:
+        """Each position's share of the rows' attention, per kv head, added to w: 2^40 for a head's whole weight. q, exp_tab, window and
+        sinks as attend took them, stats as it left them. fresh: the sums of the batch's sequences start from 0."""
+        self._batch(batch)
+        if self.w is None:
+            raise ValueError("weigh: the pools were made without accumulated weights")
+        _need(exp_tab, "exp_tab", self._i32, self.dev, (1024,))
+        _need(stats, "stats", self._i32, self.dev, (batch.tokens, nh, 2))
+        at, q_stride = self._rows(q, "q", batch, nh * self.hd)
+        k, _, pages, page, bits = self._pools
+        B.check(B.lib().kt_hip_dec_weigh_paged(
             self.dev, at, batch.tokens, q_stride, *batch.ptrs, batch.seqs, batch.max_pages, nh, self.nkv, self.hd,
-            exp_tab.data_ptr(), window, sinks, *self._pools, to, o_stride, ws.data_ptr(), ws.nbytes, B._stream(stream)),
-            "dec paged attention")
+            exp_tab.data_ptr(), window, sinks, stats.data_ptr(), int(fresh), k, self.w.data_ptr(), pages, page, bits,
+            B._stream(stream)), "dec paged weigh")
+
+    def evict(self, batch: PagedBatch, to, budget: int, kept, recent: int = 0, sinks: int = 0, stream=None) -> None:
+        """The batch's sequences cut down to at most `budget` positions, each kv head by itself: the first `sinks`, the last `recent`
+        and, of the others, those with the largest w (ties: the lower position). They move, in order, to the pages `to`
+        (seqs x ceil(budget / page) int32: pages of no table, each once); kept (seqs x nkv x budget int32) says which they
+        were, -1 past the last. The caller takes `to` for the tables, min(kv_len, budget) for the lengths, and adds what went to the shifts;
+        the old pages are free."""
+        self._batch(batch)
+        if self.w is None:
+            raise ValueError("evict: the pools were made without accumulated weights")
+        if not 1 <= budget <= MAX_POS:
+            raise ValueError(f"evict: a budget of {budget}: 1 to {MAX_POS} positions")
+        _need(to, "to", self._i32, self.dev, (batch.seqs, -(-budget // self.page)))
+        _need(kept, "kept", self._i32, self.dev, (batch.seqs, self.nkv, budget))
+        k, v, pages, page, bits = self._pools
+        B.check(B.lib().kt_hip_dec_evict_paged(
+            self.dev, batch.ptrs[1], batch.ptrs[2], batch.seqs, batch.max_pages, self.nkv, self.hd, to.data_ptr(), budget, recent,
+            sinks, kept.data_ptr(), k, v, self.w.data_ptr(), pages, page, bits, B._stream(stream)), "dec paged evict")
 
 
 class PagedDecoder:
