@@ -222,24 +222,41 @@ class PagedDecoder:
         a, b = d.add(), d.add()
         tokens = d.run([(a, prompt_a), (b, prompt_b)])          # one pass, ragged: the next token of each
         tokens = d.run([(a, tokens[:1]), (b, tokens[1:])])      # a decode step of both
+        lp, entropy, ids, lps = d.logprobs(tokens, unit, k=5)   # of these two, among the likeliest five
         d.release(a)
+
+    q_norm / k_norm (layers x hd int16 at 2^12): the model norms its q and k heads before the rotation. budget >= 1: a sequence that holds
+    more than `most` positions (budget + half of it by default) after a pass is cut down to `budget` of them, in every layer and kv head the
+    first `sinks`, the last `recent` (budget // 2 by default, as far as the sinks leave room) and those that the rows so far have attended to
+    most. The pages for one such cut are set aside.
     """
 
     def __init__(self, model, pages: int, page: int = 16, bits: int = 8, max_seqs: int = 64, max_rows: int = 2048,
-                 window: int = 0, sinks: int = 0):
+                 window: int = 0, sinks: int = 0, q_norm=None, k_norm=None, budget: int = 0, recent: int | None = None,
+                 most: int | None = None):
         import torch
 
         if max_rows < 1 or not 1 <= max_seqs <= 65535 or window < 0 or sinks < 0:
             raise ValueError("PagedDecoder: max_rows >= 1, 1 <= max_seqs <= 65535, window >= 0, sinks >= 0")
+        recent = min(budget // 2, max(0, budget - sinks)) if recent is None else recent
+        most = budget + budget // 2 if most is None else most
+        if budget and (not 1 <= budget <= MAX_POS or window or recent < 0 or sinks + recent > budget or most < budget):
+            raise ValueError(f"PagedDecoder: a budget of {budget} positions (1 to {MAX_POS}) needs no window, sinks + recent within "
+                             f"it (not {sinks} + {recent}) and most not below it (not {most})")
+        spare = -(-budget // page)
+        if budget and pages < spare:
+            raise ValueError(f"PagedDecoder: {pages} pages, {spare} of them set aside to cut a sequence to {budget} positions")
         self.torch, self.m, self.dev, self.device = torch, model, model.dev, model.device
         self.page, self.bits, self.max_seqs, self.max_rows = page, bits, max_seqs, max_rows
-        self.window, self.sinks = window, sinks
-        self.kv = [PagedKV(pages, page, model.nkv, model.hd, bits, dev=model.dev) for _ in range(model.L)]
+        self.window, self.sinks, self.budget, self.recent, self.most = window, sinks, budget, recent, most
+        self.kv = [PagedKV(pages, page, model.nkv, model.hd, bits, dev=model.dev, weights=budget > 0) for _ in range(model.L)]
+        self.q_norm, self.k_norm = (self._norms(t, what) for t, what in ((q_norm, "q_norm"), (k_norm, "k_norm")))
         self.max_pos = min(int(model.rope_cos.shape[0]), MAX_POS)
         self.max_pages = max(1, -(-self.max_pos // page))
         if not window:  # a sequence holds each of its positions; with a window it gives pages back as it goes
             self.max_pages = max(1, min(self.max_pages, pages))
         self.free = list(range(pages - 1, -1, -1))
+        self.spare = [self.free.pop() for _ in range(spare)] if budget else []
         self.seq: dict[int, dict] = {}
         self._next = 0
 
@@ -251,8 +268,18 @@ class PagedDecoder:
         self.qkv, self.q, self.o = zeros(R, m.nq), zeros(R, m.nh * m.hd), zeros(R, m.nh * m.hd)
         self.r_last, self.x_last = zeros(max_seqs, m.d, dt=torch.int32), zeros(max_seqs, m.d)
         self.logits = zeros(max_seqs, m.V, dt=torch.int32)
+        self.stats = zeros(R, m.nh, 2, dt=torch.int32) if budget else None
         self._ws = []
         torch.cuda.current_stream(self.device).synchronize()  # the buffers are zeros before a pass on any stream
+
+    def _norms(self, t, what: str):
+        """The layers' weights on the device, or None."""
+        if t is None:
+            return None
+        t = self.torch.as_tensor(t)
+        if t.dtype is not self.torch.int16 or t.shape != (self.m.L, self.m.hd):
+            raise ValueError(f"PagedDecoder: {what}: {self.m.L} x {self.m.hd} int16 are needed, not {tuple(t.shape)} {t.dtype}")
+        return t.to(self.device).contiguous().clone()
 
     # sequences -----------------------------------------------------------------------------------------------------
 
@@ -260,7 +287,7 @@ class PagedDecoder:
         """A new, empty sequence."""
         s = self._next
         self._next += 1
-        self.seq[s] = dict(len=0, pages=[], gone=-(-self.sinks // self.page))
+        self.seq[s] = dict(len=0, cut=0, pages=[], gone=-(-self.sinks // self.page))
         return s
 
     def release(self, s: int) -> None:
@@ -270,12 +297,17 @@ class PagedDecoder:
     def length(self, s: int) -> int:
         return self.seq[s]["len"]
 
+    def held(self, s: int) -> int:
+        """The positions of s that its pages hold: all, but for those that a budget has cut (a window's are counted)."""
+        return self.seq[s]["len"] - self.seq[s]["cut"]
+
     def _reserve(self, lens: list) -> None:
         """Pages for sequence s up to new positions, all or none."""
-        want = {s: -(-n // self.page) - len(self.seq[s]["pages"]) for s, n in lens}
+        want = {s: -(-(n - self.seq[s]["cut"]) // self.page) - len(self.seq[s]["pages"]) for s, n in lens}
         for s, n in lens:
-            if n > self.max_pos or n > self.max_pages * self.page:
-                raise ValueError(f"sequence {s}: {n} positions, {min(self.max_pos, self.max_pages * self.page)} at most")
+            if n > self.max_pos or n - self.seq[s]["cut"] > self.max_pages * self.page:
+                raise ValueError(f"sequence {s}: {n} positions, {self.seq[s]['cut']} of them cut: {self.max_pos} at most, "
+                                 f"{self.max_pages * self.page} held")
         if sum(max(0, w) for w in want.values()) > len(self.free):
             raise ValueError(f"out of pages: {sum(max(0, w) for w in want.values())} needed, {len(self.free)} free")
         for s, w in want.items():
@@ -290,6 +322,26 @@ class PagedDecoder:
             e["pages"][i] = -1
         e["gone"] = max(e["gone"], gone)
 
+    def _cut(self, seqs: list, stream) -> None:
+        """Those of `seqs` that hold more than `most` positions cut down to the budget, as many at a time as there are pages for. After
+        the pass, on its stream (torch's current one)."""
+        torch = self.torch
+        seqs, need = [s for s in seqs if self.held(s) > self.most], len(self.spare)
+        while seqs:
+            n = min(len(seqs), 1 + len(self.free) // need)
+            now, seqs = seqs[:n], seqs[n:]
+            pages = self.spare + [self.free.pop() for _ in range((n - 1) * need)]
+            to = torch.tensor(pages, dtype=torch.int32).reshape(n, need).to(self.device)
+            b = self.batch(now, [0] * n)
+            kept = torch.empty(n, self.m.nkv, self.budget, dtype=torch.int32, device=self.device)
+            for kv in self.kv:
+                kv.evict(b, to, self.budget, kept, self.recent, self.sinks, stream)
+            for i, s in enumerate(now):
+                e = self.seq[s]
+                self.free += e["pages"]
+                e["pages"], e["cut"] = pages[i * need:(i + 1) * need], e["len"] - self.budget
+            self.spare = [self.free.pop() for _ in range(need)]
+
     # a pass --------------------------------------------------------------------------------------------------------
 
     def batch(self, seqs: list, rows: list) -> PagedBatch:
@@ -301,15 +353,29 @@ class PagedDecoder:
         for i, s in enumerate(seqs):
             table[i, : len(self.seq[s]["pages"])] = self.seq[s]["pages"]
         start = np.concatenate([[0], np.cumsum(rows)]).astype(np.int32)
-        kv = np.array([self.seq[s]["len"] + n for s, n in zip(seqs, rows)], dtype=np.int32)
+        kv = np.array([self.held(s) + n for s, n in zip(seqs, rows)], dtype=np.int32)
         put = lambda a: torch.from_numpy(a).to(self.device)  # noqa: E731
-        return PagedBatch(put(start), put(kv), put(table), int(start[-1]))
+        shift = put(np.array([self.seq[s]["cut"] for s in seqs], dtype=np.int32)) if self.budget else None
+        return PagedBatch(put(start), put(kv), put(table), int(start[-1]), shift)
 
     def run(self, work: list, stream=None):
         """One pass over (sequence, its new tokens) pairs: prompts, chunks of prompts and single tokens alike. Returns the
         greedy next token of each (int32, on the device); their logits are self.logits[: len(work)]. The tokens may be
         host integers, which are checked, or a tensor of the device, whose ids outside the vocabulary count as the nearest
         one inside. Asynchronous on `stream` (None: the null stream); other streams' work is the caller's to order."""
+        seqs, rows, ids = self._work(work)
+        with self.torch.cuda.stream(self._torch_stream(stream)):
+            b, toks = self._tokens(seqs, rows, ids)
+            last = None
+            if b.tokens != b.seqs:
+                last = (b.row_start[1:] - 1).long()
+            out = self.torch.empty(b.seqs, dtype=self.torch.int32, device=self.device)
+            self.forward(toks, b, last, out, stream)
+            self._advance(seqs, rows, stream)
+        return out
+
+    def _work(self, work: list) -> tuple:
+        """The sequences of a pass, their rows, and their tokens checked; their positions are reserved."""
         torch = self.torch
         seqs = [s for s, _ in work]
         rows = [len(t) for _, t in work]
@@ -323,21 +389,24 @@ class PagedDecoder:
                 raise ValueError(f"run: sequence {s}: tokens are a vector of int32 or int64")
             ids.append(t if self._on_gpu(t) else self._ids(t, f"run: sequence {s}"))
         self._reserve([(s, self.seq[s]["len"] + n) for s, n in zip(seqs, rows)])
-        with torch.cuda.stream(self._torch_stream(stream)):
-            b = self.batch(seqs, rows)
-            toks = [t.clamp(0, self.m.V - 1).to(device=self.device, dtype=torch.int32) if self._on_gpu(t) else
-                    torch.tensor(t, dtype=torch.int32, device=self.device) for t in ids]
-            toks = torch.cat(toks) if len(toks) > 1 else toks[0].contiguous()
-            last = None
-            if b.tokens != b.seqs:
-                last = (b.row_start[1:] - 1).long()
-            out = torch.empty(b.seqs, dtype=torch.int32, device=self.device)
-            self.forward(toks, b, last, out, stream)
+        return seqs, rows, ids
+
+    def _tokens(self, seqs: list, rows: list, ids: list) -> tuple:
+        """The batch and its tokens on the device."""
+        torch = self.torch
+        b = self.batch(seqs, rows)
+        toks = [t.clamp(0, self.m.V - 1).to(device=self.device, dtype=torch.int32) if self._on_gpu(t) else
+                torch.tensor(t, dtype=torch.int32, device=self.device) for t in ids]
+        return b, torch.cat(toks) if len(toks) > 1 else toks[0].contiguous()
+
+    def _advance(self, seqs: list, rows: list, stream) -> None:
+        """The sequences after a pass: what a window or a budget leaves of them."""
         for s, n in zip(seqs, rows):
             self.seq[s]["len"] += n
             if self.window:
                 self._trim(s)
-        return out
+        if self.budget:
+            self._cut(seqs, stream)
 
     def _ids(self, t, what: str) -> list:
         """Host tokens as integers of the vocabulary."""
@@ -391,9 +460,21 @@ class PagedDecoder:
         after a call of the batch's shape. Passes of one decoder, captured or not, share its buffers: they follow one
         another."""
         self._check_pass(tokens_dev, b, last, out)
+        vocab = self.m.V
+        self._layers(tokens_dev, b, stream)
+        r = self.r
+        if last is not None:
+            self.torch.index_select(self.r, 0, last, out=self.r_last[: b.seqs])
+            r = self.r_last
+        self._head(r, b.seqs, stream)
+        B.dec_argmax_rows(self.logits, b.seqs, vocab, out, self._workspaces(b)[1], stream=stream, dev=self.dev)
+
+    def _layers(self, tokens_dev, b: PagedBatch, stream) -> None:
+        """The layers over the batch's rows: their residual to self.r."""
         m, lib, dev, s, P = self.m, B.lib(), self.dev, B._stream(stream), B._ptr
         T, d, ffn, nh, hd, nq = b.tokens, m.d, m.ffn, m.nh, m.hd, m.nq
-        ws, ws_top = self._workspaces(b)
+        ws, _ = self._workspaces(b)
+        stats = self.stats[:T] if self.budget else None
         B.check(lib.kt_hip_dec_embed(dev, P(tokens_dev), T, P(m.emb16), d, P(self.r), s), "dec embed")
         fuse = m.fuse_norm and T <= B.NORM_MAX_M
         for l in range(m.L):
@@ -402,8 +483,15 @@ class PagedDecoder:
             else:
                 B.check(lib.kt_hip_dec_rmsnorm(dev, P(self.r), T, d, P(self.xn), d, s), "dec rmsnorm")
                 m._gemm("qkv", l, self.xn, T, nq, d, self.qkv, B.OUT_I8, s)
-            self.kv[l].append(self.qkv, b, nh, m.rope_cos, m.rope_sin, self.q, stream)
-            self.kv[l].attend(self.q, b, nh, m.exp_tab, self.o, ws, self.window, self.sinks, stream)
+            norms = {} if self.q_norm is None else dict(q_norm=self.q_norm[l])
+            if self.k_norm is not None:
+                norms["k_norm"] = self.k_norm[l]
+            self.kv[l].append(self.qkv, b, nh, m.rope_cos, m.rope_sin, self.q, stream, **norms)
+            if self.budget:  # (sinks are what a cut leaves here, not a window's)
+                self.kv[l].attend(self.q, b, nh, m.exp_tab, self.o, ws, 0, 0, stream, stats=stats)
+                self.kv[l].weigh(self.q, b, nh, m.exp_tab, stats, stream=stream)
+            else:
+                self.kv[l].attend(self.q, b, nh, m.exp_tab, self.o, ws, self.window, self.sinks, stream)
             m._gemm("o", l, self.o, T, d, nh * hd, self.r, B.OUT_I32_ADD, s)
             lo, nib, mant, shift = m._layer_ptrs("gu", l, 2 * ffn)
             if fuse:
@@ -414,19 +502,59 @@ class PagedDecoder:
                 B.check(lib.kt_hip_w12_swiglu(dev, P(self.xn), lo, nib, T, ffn, d, mant, shift, P(m.silu), m.h_shift,
                                               P(self.h), ffn, s), "dec gate/up")
             m._gemm("dn", l, self.h, T, d, ffn, self.r, B.OUT_I32_ADD, s)
-        r = self.r
-        if last is not None:
-            self.torch.index_select(self.r, 0, last, out=self.r_last[: b.seqs])
-            r = self.r_last
-        B.check(lib.kt_hip_dec_rmsnorm(dev, P(r), b.seqs, d, P(self.x_last), d, s), "dec rmsnorm")
-        m._gemm("emb", 0, self.x_last, b.seqs, m.V, d, self.logits, B.OUT_I32, s)
-        B.dec_argmax_rows(self.logits, b.seqs, m.V, out, ws_top, stream=stream, dev=dev)
+
+    def _head(self, r, rows: int, stream) -> None:
+        """The logits of the first `rows` rows (at most max_seqs) of the residual r to self.logits."""
+        m, s, P = self.m, B._stream(stream), B._ptr
+        B.check(B.lib().kt_hip_dec_rmsnorm(self.dev, P(r), rows, m.d, P(self.x_last), m.d, s), "dec rmsnorm")
+        m._gemm("emb", 0, self.x_last, rows, m.V, m.d, self.logits, B.OUT_I32, s)
+
+    def logprobs(self, tokens, unit: float, k: int = 0, stream=None):
+        """Of the rows that the last pass left in self.logits, the log probability of tokens[r] in row r (int32 on the device, one for
+        each sequence of the pass, in its order), the entropy, and the k likeliest tokens with theirs (None where k is 0), in
+        2^-16 of a natural unit, which is `unit` codes of a logit. On `stream`, as the pass was."""
+        torch = self.torch
+        n = tokens.numel()
+        if tokens.dtype is not torch.int32 or tokens.get_device() != self.dev or not tokens.is_contiguous() or n > self.max_seqs:
+            raise ValueError(f"logprobs: a contiguous tensor of at most {self.max_seqs} int32 on GPU {self.dev} is needed, not "
+                             f"{tuple(tokens.shape)} {tokens.dtype} on {tokens.device}")
+        with torch.cuda.stream(self._torch_stream(stream)):
+            i32 = lambda *s: torch.empty(*s, dtype=torch.int32, device=self.device)  # noqa: E731
+            out = (i32(n), i32(n), *((i32(n, k), i32(n, k)) if k else (None, None)))
+            ws = torch.empty(B.dec_logprobs_rows_workspace(n, self.m.V, k), dtype=torch.int8, device=self.device)
+            B.dec_logprobs_rows(self.logits, n, self.m.V, tokens, B.logit_scale(unit), out[0], ws, *out[1:], k, stream=stream,
+                                dev=self.dev)
+        return out
+
+    def score(self, work: list, unit: float, k: int = 0, stream=None):
+        """One pass over (sequence, its new tokens) pairs, as run's, for the log probabilities of the tokens themselves: row i of a
+        sequence's tokens gives that of its token i + 1, the last row the entropy and alternatives alone (its log probability is that
+        of no token: -2^31). Returns, for each pair, what logprobs does, one row a token."""
+        torch = self.torch
+        B.logit_scale(unit), B.dec_logprobs_rows_workspace(self.max_seqs, self.m.V, k)  # refused before anything is reserved
+        seqs, rows, ids = self._work(work)
+        with torch.cuda.stream(self._torch_stream(stream)):
+            b, toks = self._tokens(seqs, rows, ids)
+            self._layers(toks, b, stream)
+            want = torch.full_like(toks, -1)
+            want[:-1] = toks[1:]
+            want[(b.row_start[1:] - 1).long()] = -1
+            got = []
+            for at in range(0, b.tokens, self.max_seqs):
+                n = min(self.max_seqs, b.tokens - at)
+                self._head(self.r[at:at + n], n, stream)
+                got.append(self.logprobs(want[at:at + n], unit, k, stream))
+            got = [torch.cat(t) if t[0] is not None else None for t in zip(*got)]
+            self._advance(seqs, rows, stream)
+        parts = [t.split(rows) if t is not None else [None] * len(rows) for t in got]
+        return list(zip(*parts))
 
     def read(self, s: int, layer: int, max_pos: int | None = None, stream=None):
         """Sequence s's K and V of a layer as contiguous rows (max_pos x nkv x hd int8, zeros past its length and where a window
-        has left pages behind): the caches that DecoderModel continues from. On `stream`, as the passes are."""
+        has left pages behind; of a sequence that a budget has cut, what it holds): the caches that DecoderModel continues from. On
+        `stream`, as the passes are."""
         torch = self.torch
-        n = self.seq[s]["len"] if max_pos is None else max_pos
+        n = self.held(s) if max_pos is None else max_pos
         with torch.cuda.stream(self._torch_stream(stream)):
             k, v = (torch.zeros(1, n, self.m.nkv, self.m.hd, dtype=torch.int8, device=self.device) for _ in range(2))
             self.kv[layer].read(self.batch([s], [0]), k, v, stream)
