@@ -31,7 +31,6 @@ struct PgWeigh {
     int64_t* w;
 };
 
-constexpr int WG_GROUP = 64;   // columns a step
 constexpr int WG_UNIT = 512;   // columns of a CTA: each digit sum stays below 2^14 512
 constexpr int WG_WAVES = 4;
 constexpr int WG_DIGITS = 5;   // of R, below 2^32
@@ -57,8 +56,10 @@ __global__ __launch_bounds__(256) void pg_weigh_zero_kernel(Paged a, int64_t* __
     }
 }
 
-template <int HD, int BITS>
-__global__ __launch_bounds__(64 * WG_WAVES) void pg_weigh_kernel(Paged a, PgWeigh p) {
+// CT: 16 columns times CT a step.
+template <int HD, int BITS, int CT>
+__global__ __launch_bounds__(64 * WG_WAVES) __attribute__((amdgpu_waves_per_eu(HD == 64 ? (CT == 4 || BITS == 4 ? 3 : 4) : 2))) void pg_weigh_kernel(Paged a, PgWeigh p) {
+    constexpr int WG_GROUP = 16 * CT, QN = WG_GROUP * HD / 16 > 64 * WG_WAVES ? WG_GROUP * HD / 16 / (64 * WG_WAVES) : 1;
     constexpr int KC = HD / 64, CPR = HD / 16, NT = 64 * WG_WAVES, HH = HD / 2;
     constexpr int ROWB = BITS == 8 ? HD : HH, CHB = BITS == 8 ? 16 : 8;
     typedef typename std::conditional<BITS == 8, v4i, v2i>::type Chunk;
@@ -104,29 +105,42 @@ __global__ __launch_bounds__(64 * WG_WAVES) void pg_weigh_kernel(Paged a, PgWeig
     }
     if (tid == 0) sE[1024] = 0;
 
-    // a group's columns: negated q, 2 (top + 64), positions, R's digits
-    int gmin = 0, gmax = 0;
-    auto stage = [&](int grp) {
+    // a group's columns: negated q, 2 (top + 64), positions, R's digits; on their way while the group before is at work
+    v4i qx[QN];
+    v2i st = {0, 0};
+    int at_row = 0;
+    auto fetch = [&](int grp) {
         const int first = m0 + grp * WG_GROUP, n = min(WG_GROUP, cols - grp * WG_GROUP);
-        for (int i = tid; i < WG_GROUP * CPR; i += NT) {
-            const int c = i / CPR, ch = i % CPR, m = first + min(c, n - 1), row = m / p.rep, head = g * p.rep + m - row * p.rep;
-            const v4i x = *reinterpret_cast<const v4i*>(p.q + (size_t)(s.t0 + row) * p.q_stride + head * HD + 16 * ch);
-            *reinterpret_cast<v4i*>(sQ + c * HD + 16 * (ch ^ swz<CPR>(c))) = negated(x);
+#pragma unroll
+        for (int i = 0; i < QN; i++) {
+            const int it = tid + i * NT, c = it / CPR, ch = it % CPR, m = first + min(c, n - 1), row = m / p.rep;
+            if (QN > 1 || WG_GROUP * CPR >= NT || it < WG_GROUP * CPR)
+                qx[i] = *reinterpret_cast<const v4i*>(p.q + (size_t)(s.t0 + row) * p.q_stride + (g * p.rep + m - row * p.rep) * HD + 16 * ch);
         }
         if (tid < WG_GROUP) {
-            const int m = first + min(tid, n - 1), row = m / p.rep, head = g * p.rep + m - row * p.rep;
-            const v2i st = *reinterpret_cast<const v2i*>(p.stats + 2 * ((size_t)(s.t0 + row) * p.nh + head));
-            const bool live = tid < n && s.p0 + row >= 0 && s.p0 + row < cap;
+            const int m = first + min(tid, n - 1);
+            at_row = m / p.rep;
+            st = *reinterpret_cast<const v2i*>(p.stats + 2 * ((size_t)(s.t0 + at_row) * p.nh + g * p.rep + m - at_row * p.rep));
+        }
+    };
+    auto put = [&](int grp) {
+        const int n = min(WG_GROUP, cols - grp * WG_GROUP);
+#pragma unroll
+        for (int i = 0; i < QN; i++) {
+            const int it = tid + i * NT, c = it / CPR, ch = it % CPR;
+            if (QN > 1 || WG_GROUP * CPR >= NT || it < WG_GROUP * CPR)
+                *reinterpret_cast<v4i*>(sQ + c * HD + 16 * (ch ^ swz<CPR>(c))) = negated(qx[i]);
+        }
+        if (tid < WG_GROUP) {
+            const bool live = tid < n && s.p0 + at_row >= 0 && s.p0 + at_row < cap;
             sTop[tid] = (int)(128u + 2u * (uint32_t)st.x);
-            sPos[tid] = live ? s.p0 + row : -1;
+            sPos[tid] = live ? s.p0 + at_row : -1;
             const uint64_t r = (live ? (uint64_t)(uint32_t)st.y : 0) + 0x8080808080ull;
             // byte 4 t + r of the lanes of quarter q is column 16 t + 4 q + r
-            const int to = ((tid >> 2) & 3) * 16 + (tid >> 4) * 4 + (tid & 3);
+            const int to = ((tid >> 2) & 3) * 4 * CT + (tid >> 4) * 4 + (tid & 3);
 #pragma unroll
             for (int d = 0; d < WG_DIGITS; d++) sR[d * WG_GROUP + to] = (int8_t)((r >> (8 * d)) ^ 0x80);
         }
-        gmin = s.p0 + first / p.rep;
-        gmax = s.p0 + (first + n - 1) / p.rep;
     };
 
     struct Keys {
@@ -159,11 +173,13 @@ __global__ __launch_bounds__(64 * WG_WAVES) void pg_weigh_kernel(Paged a, PgWeig
         }
     };
     v4i acc[4][2];
-    // the weights of a block's positions and 16 CT columns, times R
-    auto add = [&](auto ct, int T, const Keys& k, bool full) {
-        constexpr int CT = decltype(ct)::value;
+    // the weights of the tile's positions and a group's columns, times R
+    auto add = [&](int T, const Keys& k, bool full) {
         v4i rd = {0, 0, 0, 0};
-        if (l16 < WG_DIGITS) rd = *reinterpret_cast<const v4i*>(sR + l16 * WG_GROUP + gq * 16);
+        if (l16 < WG_DIGITS) {
+            if constexpr (CT == 4) rd = *reinterpret_cast<const v4i*>(sR + l16 * WG_GROUP + gq * 16);
+            else rd.x = *reinterpret_cast<const int*>(sR + l16 * WG_GROUP + gq * 4);
+        }
 #pragma unroll
         for (int t = 0; t < 4; t++) {
             v4i P[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
@@ -209,24 +225,31 @@ __global__ __launch_bounds__(64 * WG_WAVES) void pg_weigh_kernel(Paged a, PgWeig
     };
 
     Keys now, next;
-    if (at(0) >= 0) load(at(0), now);
+    if (CT == 1 && at(0) >= 0) load(at(0), now);
+    fetch(0);
     for (int n = 0; n < rounds; n++) {
         const int T = at(n), T1 = n + 1 < rounds ? at(n + 1) : -1;
-        if (T1 >= 0) load(T1, next);
+        if (CT == 1) {
+            if (T1 >= 0) load(T1, next);
+        } else if (T >= 0) {
+            load(T, now);
+        }
 #pragma unroll
         for (int t = 0; t < 4; t++) acc[t][0] = acc[t][1] = v4i{0, 0, 0, 0};
         for (int grp = 0; grp < groups; grp++) {
             if (groups > 1 || n == 0) {
                 if (groups > 1) __syncthreads();
-                stage(grp);
+                put(grp);
                 __syncthreads();
+                if (groups > 1 && (grp + 1 < groups || n + 1 < rounds)) fetch(grp + 1 < groups ? grp + 1 : 0);
             }
+            const int first = m0 + grp * WG_GROUP, gmin = s.p0 + first / p.rep,
+                      gmax = s.p0 + (first + min(WG_GROUP, cols - grp * WG_GROUP) - 1) / p.rep;
             if (T < 0 || 64 * T > gmax) continue;
             const bool pages = now.id[0] >= 0 && now.id[1] >= 0 && now.id[2] >= 0 && now.id[3] >= 0;
             const bool full = pages && 64 * T + 63 <= gmin && gmax < cap &&
                               (p.window == 0 || 64 * T > gmax - p.window || 64 * T + 63 < p.sinks);
-            if (cols - grp * WG_GROUP <= 16) add(std::integral_constant<int, 1>(), T, now, full);
-            else add(std::integral_constant<int, 4>(), T, now, full);
+            add(T, now, full);
         }
         if (T >= 0) {
             // register r of acc[t], lane l: position 16 t + 4 (l / 16) + r, digit l % 16; turned to a position a lane
@@ -252,7 +275,7 @@ __global__ __launch_bounds__(64 * WG_WAVES) void pg_weigh_kernel(Paged a, PgWeig
                                                  ((64 * T + lane) & ((1 << a.page_sh) - 1)),
                                              (unsigned long long)v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
-        now = next;
+        if (CT == 1) now = next;
     }
 }
 
@@ -272,13 +295,16 @@ hipError_t launch_pg_weigh(const Paged& a, int hd, int bits, const int8_t* q, in
     const int64_t units = (a.seqs + (int64_t)a.tokens * rep / WG_UNIT) * a.nkv;
     const int64_t rounds = (reach + 64 * WG_WAVES - 1) / (64 * WG_WAVES);
     const int64_t splits = std::min(rounds, std::max<int64_t>(1, 2048 / units));
+    const bool few = (int64_t)a.tokens * rep <= 16 * (int64_t)a.seqs;  // columns of a sequence, on average
     const PgWeigh p = {q, q_stride, exp_tab, stats, nh, rep, window, sinks, (int)splits, w};
-    auto go = [&](auto kern) {
-        kern<<<dim3((unsigned)units, (unsigned)splits), dim3(64 * WG_WAVES), 0, s>>>(a, p);
+    auto go = [&](auto one, auto four) {
+        if (few) one<<<dim3((unsigned)units, (unsigned)splits), dim3(64 * WG_WAVES), 0, s>>>(a, p);
+        else four<<<dim3((unsigned)units, (unsigned)splits), dim3(64 * WG_WAVES), 0, s>>>(a, p);
         return hipGetLastError();
     };
-    if (hd == 64) return bits == 8 ? go(pg_weigh_kernel<64, 8>) : go(pg_weigh_kernel<64, 4>);
-    return bits == 8 ? go(pg_weigh_kernel<128, 8>) : go(pg_weigh_kernel<128, 4>);
+    if (hd == 64)
+        return bits == 8 ? go(pg_weigh_kernel<64, 8, 1>, pg_weigh_kernel<64, 8, 4>) : go(pg_weigh_kernel<64, 4, 1>, pg_weigh_kernel<64, 4, 4>);
+    return bits == 8 ? go(pg_weigh_kernel<128, 8, 1>, pg_weigh_kernel<128, 8, 4>) : go(pg_weigh_kernel<128, 4, 1>, pg_weigh_kernel<128, 4, 4>);
 }
 
 }  // namespace kt
