@@ -4,8 +4,8 @@
 // With each row's largest score and the reciprocal R of its weights' sum in hand, one pass over K does: a wave holds 64 positions of K
 // as B operands and goes through the columns (a row's q heads of one kv head, as in the attention), 64 of them a time. The scores are
 // 16x16x64 int8 MFMAs with the columns as rows, so a lane has one position and 16 columns, whose weights' balanced base-256
-// digits (of -e, two) are the A operand of a second product as they stand; its B operand is R's digits (five, one a column of
-// the result). Sums of e R are so exact in int32 and meet as int64.
+// digits (of -e, two) are the A operand of a second product as they stand; its B operand is R's digits (five, each in a column of
+// the result, and one further for e's high digit). Sums of e R are so exact in int32 and meet as int64.
 
 #include <algorithm>
 #include <hip/hip_runtime.h>
@@ -31,9 +31,10 @@ struct PgWeigh {
     int64_t* w;
 };
 
-constexpr int WG_UNIT = 512;   // columns of a CTA: each digit sum stays below 2^14 512
+constexpr int WG_UNIT = 256;   // columns of a CTA: each digit sum stays within 2 2^14 256
 constexpr int WG_WAVES = 4;
 constexpr int WG_DIGITS = 5;   // of R, below 2^32
+constexpr int WG_SUMS = 6;     // digits of e R before they carry: e's low one times R's d-th and its high one times the (d - 1)-th
 
 // -x of 16 int8 values, -128 taken as -127.
 __device__ __forceinline__ v4i negated(v4i x) {
@@ -58,17 +59,23 @@ __global__ __launch_bounds__(256) void pg_weigh_zero_kernel(Paged a, int64_t* __
 
 // CT: 16 columns times CT a step.
 template <int HD, int BITS, int CT>
-__global__ __launch_bounds__(64 * WG_WAVES) __attribute__((amdgpu_waves_per_eu(HD == 64 ? (CT == 4 || BITS == 4 ? 3 : 4) : 2))) void pg_weigh_kernel(Paged a, PgWeigh p) {
+__global__ __launch_bounds__(64 * WG_WAVES) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 3 + (BITS == 8 || CT == 1) : 2))) void pg_weigh_kernel(Paged a, PgWeigh p) {
     constexpr int WG_GROUP = 16 * CT, QN = WG_GROUP * HD / 16 > 64 * WG_WAVES ? WG_GROUP * HD / 16 / (64 * WG_WAVES) : 1;
     constexpr int KC = HD / 64, CPR = HD / 16, NT = 64 * WG_WAVES, HH = HD / 2;
     constexpr int ROWB = BITS == 8 ? HD : HH, CHB = BITS == 8 ? 16 : 8;
     typedef typename std::conditional<BITS == 8, v4i, v2i>::type Chunk;
     __shared__ __attribute__((aligned(16))) int8_t sQ[WG_GROUP * HD], sR[WG_DIGITS * WG_GROUP];
     __shared__ __attribute__((aligned(16))) int sTop[WG_GROUP], sPos[WG_GROUP];
-    __shared__ uint16_t sE[1028];
-    __shared__ int64_t sSum[WG_WAVES][64 * WG_DIGITS];
+    __shared__ __attribute__((aligned(8))) uint16_t sE[1028];
+    __shared__ int sSum[WG_WAVES][64 * (WG_SUMS + 1)];
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, gq = lane >> 4;
+    typedef int tab4 __attribute__((ext_vector_type(4), aligned(4)));
+    constexpr int ET = 256 / NT > 1 ? 256 / NT : 1;
+    tab4 et[ET];  // the table is on its way while the batch is looked up
+#pragma unroll
+    for (int i = 0; i < ET; i++)
+        if (NT <= 256 || tid < 256) et[i] = *reinterpret_cast<const tab4*>(p.exp_tab + 4 * (tid + i * NT));
 
     // column units 0 .. seqs - 1 are the sequences' first ones, the rest their further ones
     const int ntiles = (int)gridDim.x / a.nkv, g = (int)blockIdx.x % a.nkv, unit = ntiles - 1 - (int)blockIdx.x / a.nkv;
@@ -83,8 +90,13 @@ __global__ __launch_bounds__(64 * WG_WAVES) __attribute__((amdgpu_waves_per_eu(H
     const int m0 = nth * WG_UNIT, mrows = s.n * p.rep;
     if (m0 >= mrows) return;
     const int cols = min(WG_UNIT, mrows - m0), groups = (cols + WG_GROUP - 1) / WG_GROUP;
-    const int cap = a.max_pages << a.page_sh, nblk = cap >> 4;
-    const int umin = s.p0 + m0 / p.rep, umax = min(s.p0 + (m0 + cols - 1) / p.rep, cap - 1);
+    // column m0 + c is head (rem0 + c) % rep of row row0 + (rem0 + c) / rep; a float quotient of a whole number and a half below 2^13
+    // is nearer to it than to a whole number, so its floor is exact
+    const int row0 = nth ? m0 / p.rep : 0, rem0 = m0 - row0 * p.rep;
+    const float inv = __builtin_amdgcn_rcpf((float)p.rep);
+    auto over = [&](int c) { return (int)(((float)(rem0 + c) + 0.5f) * inv); };
+    const int cap = a.max_pages << a.page_sh, nblk = cap >> 4, pos0 = s.p0 + row0;
+    const int umin = pos0, umax = min(pos0 + __builtin_amdgcn_readfirstlane(over(cols - 1)), cap - 1);
     const int ntile = umax < 0 || a.pages == 0 ? 0 : umax / 64 + 1;
     int nsink = 0, w0 = 0;
     if (p.window && ntile) {
@@ -99,28 +111,51 @@ __global__ __launch_bounds__(64 * WG_WAVES) __attribute__((amdgpu_waves_per_eu(H
         return i >= total ? -1 : (i < nsink ? i : i - nsink + w0);
     };
 
-    for (int i = tid; i < 1024; i += NT) {
-        const uint32_t e = (uint32_t)min(max(p.exp_tab[i], 0), 32768);
-        sE[i] = (uint16_t)((0x8080u - e) ^ 0x8080u);  // the two balanced digits of -e
-    }
-    if (tid == 0) sE[1024] = 0;
+    // A tile's pages (a lane that of its block, lane / 16), read a round before its K is asked for.
+    auto page_of = [&](int T) {
+        const int blk = min(4 * max(T, 0) + gq, nblk - 1);
+        return a.table[(size_t)b * a.max_pages + (blk >> (a.page_sh - 4))];
+    };
+    struct Keys {
+        Chunk x[4][KC];
+        int m[4];     // 4 bits: the multiplier of the lane's position
+        int id;       // the page of the lane's block, or -1
+        uint64_t ok;  // the lanes whose block has a page
+    };
+    const uint8_t* const kbase = a.k + (size_t)g * a.part;
+    const uint32_t stride = (uint32_t)a.nkv * (uint32_t)a.part;
+    const int from_lane = l16 * ROWB + gq * CHB;
+    auto load = [&](int T, int id, Keys& k) {
+        const bool ok = (unsigned)id < (unsigned)a.pages && 4 * T + gq < nblk;
+        k.ok = __ballot(ok);
+        k.id = ok ? id : -1;
+        const int from_id = ok ? id : 0;
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            const int slot = ((4 * T + t) << 4) & ((1 << a.page_sh) - 1);
+            const uint8_t* from = kbase + (uint64_t)(uint32_t)__builtin_amdgcn_readlane(from_id, 16 * t) * stride;
+#pragma unroll
+            for (int c = 0; c < KC; c++) k.x[t][c] = *reinterpret_cast<const Chunk*>(from + (slot * ROWB + 4 * c * CHB) + from_lane);
+            if constexpr (BITS == 4) k.m[t] = from[((HH << a.page_sh) + slot) + l16];
+        }
+    };
 
     // a group's columns: negated q, 2 (top + 64), positions, R's digits; on their way while the group before is at work
     v4i qx[QN];
     v2i st = {0, 0};
     int at_row = 0;
     auto fetch = [&](int grp) {
-        const int first = m0 + grp * WG_GROUP, n = min(WG_GROUP, cols - grp * WG_GROUP);
+        const int n = min(WG_GROUP, cols - grp * WG_GROUP);
 #pragma unroll
         for (int i = 0; i < QN; i++) {
-            const int it = tid + i * NT, c = it / CPR, ch = it % CPR, m = first + min(c, n - 1), row = m / p.rep;
+            const int it = tid + i * NT, c = grp * WG_GROUP + min(it / CPR, n - 1), up = over(c), row = row0 + up;
             if (QN > 1 || WG_GROUP * CPR >= NT || it < WG_GROUP * CPR)
-                qx[i] = *reinterpret_cast<const v4i*>(p.q + (size_t)(s.t0 + row) * p.q_stride + (g * p.rep + m - row * p.rep) * HD + 16 * ch);
+                qx[i] = *reinterpret_cast<const v4i*>(p.q + (size_t)(s.t0 + row) * p.q_stride + (g * p.rep + rem0 + c - up * p.rep) * HD + 16 * (it % CPR));
         }
         if (tid < WG_GROUP) {
-            const int m = first + min(tid, n - 1);
-            at_row = m / p.rep;
-            st = *reinterpret_cast<const v2i*>(p.stats + 2 * ((size_t)(s.t0 + at_row) * p.nh + g * p.rep + m - at_row * p.rep));
+            const int c = grp * WG_GROUP + min(tid, n - 1), up = over(c);
+            at_row = row0 + up;
+            st = *reinterpret_cast<const v2i*>(p.stats + 2 * ((size_t)(s.t0 + at_row) * p.nh + g * p.rep + rem0 + c - up * p.rep));
         }
     };
     auto put = [&](int grp) {
@@ -143,27 +178,19 @@ __global__ __launch_bounds__(64 * WG_WAVES) __attribute__((amdgpu_waves_per_eu(H
         }
     };
 
-    struct Keys {
-        Chunk x[4][KC];
-        int m[4];  // 4 bits: the multiplier of the lane's position
-        int id[4];
-    };
-    const uint8_t* const kbase = a.k + (size_t)g * a.part;
-    const uint32_t stride = (uint32_t)a.nkv * (uint32_t)a.part;
-    auto load = [&](int T, Keys& k) {
+    Keys now, next;
+    int id0 = page_of(at(0)), id1 = rounds > 1 ? page_of(at(1)) : 0;
+    fetch(0);
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
-            const int blk = min(4 * T + t, nblk - 1), slot = (blk << 4) & ((1 << a.page_sh) - 1);
-            const int id = __builtin_amdgcn_readfirstlane(a.table[(size_t)b * a.max_pages + (blk >> (a.page_sh - 4))]);
-            const bool ok = (unsigned)id < (unsigned)a.pages;
-            const uint8_t* from = kbase + (uint64_t)(ok ? (uint32_t)id : 0u) * stride;
-            k.id[t] = ok && 4 * T + t < nblk ? id : -1;
+    for (int i = 0; i < ET; i++) {
+        uint32_t e[4];
 #pragma unroll
-            for (int c = 0; c < KC; c++)
-                k.x[t][c] = *reinterpret_cast<const Chunk*>(from + (slot + l16) * ROWB + (gq + 4 * c) * CHB);
-            if constexpr (BITS == 4) k.m[t] = from[(HH << a.page_sh) + slot + l16];
-        }
-    };
+        for (int r = 0; r < 4; r++) e[r] = ((0x8080u - (uint32_t)min(max(et[i][r], 0), 32768)) ^ 0x8080u) & 0xFFFFu;  // the two balanced digits of -e
+        if (NT <= 256 || tid < 256) *reinterpret_cast<v2i*>(sE + 4 * (tid + i * NT)) = v2i{(int)(e[0] | e[1] << 16), (int)(e[2] | e[3] << 16)};
+    }
+    if (tid == 0) sE[1024] = 0;
+    if (CT == 1 && at(0) >= 0) load(at(0), id0, now);
+
     auto widen = [](Chunk x) {  // 4 bits: 16 times the codes
         if constexpr (BITS == 8) {
             return x;
@@ -172,18 +199,22 @@ __global__ __launch_bounds__(64 * WG_WAVES) __attribute__((amdgpu_waves_per_eu(H
             return v4i{(x.x << 4) & M, x.x & M, (x.y << 4) & M, x.y & M};
         }
     };
-    v4i acc[4][2];
-    // the weights of the tile's positions and a group's columns, times R
-    auto add = [&](int T, const Keys& k, bool full) {
-        v4i rd = {0, 0, 0, 0};
-        if (l16 < WG_DIGITS) {
-            if constexpr (CT == 4) rd = *reinterpret_cast<const v4i*>(sR + l16 * WG_GROUP + gq * 16);
-            else rd.x = *reinterpret_cast<const int*>(sR + l16 * WG_GROUP + gq * 4);
+    v4i acc[4];
+    const int window = p.window ? p.window : 1 << 30;  // (positions lie within +-2^30, those that count below 2^20)
+    // the weights of the tile's positions and a group's columns, times R; `all`: every column sees every position
+    auto add = [&](auto all, int T, const Keys& k) {
+        v4i rd[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+        if constexpr (CT == 4) {
+            if (l16 < WG_DIGITS) rd[0] = *reinterpret_cast<const v4i*>(sR + l16 * WG_GROUP + gq * 16);
+            if (l16 >= 1 && l16 < WG_SUMS) rd[1] = *reinterpret_cast<const v4i*>(sR + (l16 - 1) * WG_GROUP + gq * 16);
+        } else {  // e's two digits side by side in one product
+            if (l16 < WG_DIGITS) rd[0].x = *reinterpret_cast<const int*>(sR + l16 * WG_GROUP + gq * 4);
+            if (l16 >= 1 && l16 < WG_SUMS) rd[0].y = *reinterpret_cast<const int*>(sR + (l16 - 1) * WG_GROUP + gq * 4);
         }
 #pragma unroll
         for (int t = 0; t < 4; t++) {
             v4i P[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-            const int j = 64 * T + 16 * t + l16;
+            const int j = (k.ok >> (16 * t)) & 1 ? 64 * T + 16 * t + l16 : INT_MAX;  // (of no page: past every row)
 #pragma unroll
             for (int c = 0; c < CT; c++) {
                 const v4i top = *reinterpret_cast<const v4i*>(sTop + 16 * c + 4 * gq);
@@ -200,13 +231,11 @@ __global__ __launch_bounds__(64 * WG_WAVES) __attribute__((amdgpu_waves_per_eu(H
                     if constexpr (BITS == 4) y[r] = (__mul24(y[r], k.m[t]) + 63) >> 7;
                     u[r] = BITS == 8 && HD == 64 ? (uint32_t)y[r] : (uint32_t)y[r] * 2 + (uint32_t)top[r];
                 }
-                if (!full) {
+                if constexpr (!all) {
                     const v4i pos = *reinterpret_cast<const v4i*>(sPos + 16 * c + 4 * gq);
 #pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        const bool sees = k.id[t] >= 0 && j <= pos[r] && (p.window == 0 || j > pos[r] - p.window || j < p.sinks);
-                        u[r] = sees ? u[r] : 0x00FFFFFFu;
-                    }
+                    for (int r = 0; r < 4; r++)
+                        u[r] = (j <= pos[r]) & ((j > pos[r] - window) | (j < p.sinks)) ? u[r] : 0x00FFFFFFu;
                 }
                 us2 e[2];
 #pragma unroll
@@ -217,25 +246,25 @@ __global__ __launch_bounds__(64 * WG_WAVES) __attribute__((amdgpu_waves_per_eu(H
                 }
                 const uint32_t e01 = __builtin_bit_cast(uint32_t, e[0]), e23 = __builtin_bit_cast(uint32_t, e[1]);
                 P[0][c] = (int)__builtin_amdgcn_perm(e23, e01, 0x06040200);
-                P[1][c] = (int)__builtin_amdgcn_perm(e23, e01, 0x07050301);
+                P[CT == 4][CT == 4 ? c : 1] = (int)__builtin_amdgcn_perm(e23, e01, 0x07050301);
             }
-            acc[t][0] = mfma16(P[0], rd, acc[t][0]);
-            acc[t][1] = mfma16(P[1], rd, acc[t][1]);
+            acc[t] = mfma16(P[0], rd[0], acc[t]);
+            if constexpr (CT == 4) acc[t] = mfma16(P[1], rd[1], acc[t]);
+            __builtin_amdgcn_sched_barrier(0);  // a block after the other: fewer registers, more waves
         }
     };
 
-    Keys now, next;
-    if (CT == 1 && at(0) >= 0) load(at(0), now);
-    fetch(0);
     for (int n = 0; n < rounds; n++) {
         const int T = at(n), T1 = n + 1 < rounds ? at(n + 1) : -1;
         if (CT == 1) {
-            if (T1 >= 0) load(T1, next);
-        } else if (T >= 0) {
-            load(T, now);
+            if (T1 >= 0) load(T1, id1, next);
+        } else {
+            if (T >= 0) load(T, id0, now);
+            id0 = id1;
         }
+        if (n + 2 < rounds) id1 = page_of(at(n + 2));
 #pragma unroll
-        for (int t = 0; t < 4; t++) acc[t][0] = acc[t][1] = v4i{0, 0, 0, 0};
+        for (int t = 0; t < 4; t++) acc[t] = v4i{0, 0, 0, 0};
         for (int grp = 0; grp < groups; grp++) {
             if (groups > 1 || n == 0) {
                 if (groups > 1) __syncthreads();
@@ -243,35 +272,33 @@ __global__ __launch_bounds__(64 * WG_WAVES) __attribute__((amdgpu_waves_per_eu(H
                 __syncthreads();
                 if (groups > 1 && (grp + 1 < groups || n + 1 < rounds)) fetch(grp + 1 < groups ? grp + 1 : 0);
             }
-            const int first = m0 + grp * WG_GROUP, gmin = s.p0 + first / p.rep,
-                      gmax = s.p0 + (first + min(WG_GROUP, cols - grp * WG_GROUP) - 1) / p.rep;
+            const int gmin = pos0 + __builtin_amdgcn_readfirstlane(over(grp * WG_GROUP)),
+                      gmax = pos0 + __builtin_amdgcn_readfirstlane(over(min(grp * WG_GROUP + WG_GROUP, cols) - 1));
             if (T < 0 || 64 * T > gmax) continue;
-            const bool pages = now.id[0] >= 0 && now.id[1] >= 0 && now.id[2] >= 0 && now.id[3] >= 0;
-            const bool full = pages && 64 * T + 63 <= gmin && gmax < cap &&
-                              (p.window == 0 || 64 * T > gmax - p.window || 64 * T + 63 < p.sinks);
-            add(T, now, full);
+            if (now.ok == ~0ull && 64 * T + 63 <= gmin && gmax < cap &&
+                (p.window == 0 || 64 * T > gmax - p.window || 64 * T + 63 < p.sinks))
+                add(std::true_type(), T, now);
+            else add(std::false_type(), T, now);
         }
         if (T >= 0) {
             // register r of acc[t], lane l: position 16 t + 4 (l / 16) + r, digit l % 16; turned to a position a lane
-            int64_t* const sum = sSum[w];
+            int* const sum = sSum[w];
             __builtin_amdgcn_wave_barrier();
-            if (l16 < WG_DIGITS) {
+            if (l16 < WG_SUMS) {
 #pragma unroll
                 for (int t = 0; t < 4; t++)
 #pragma unroll
-                    for (int r = 0; r < 4; r++)
-                        sum[(16 * t + 4 * gq + r) * WG_DIGITS + l16] = ((int64_t)acc[t][0][r] + ((int64_t)acc[t][1][r] << 8)) << (8 * l16);
+                    for (int r = 0; r < 4; r++) sum[(16 * t + 4 * gq + r) * (WG_SUMS + 1) + l16] = acc[t][r];
             }
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
             __builtin_amdgcn_wave_barrier();
             int64_t v = 0;
 #pragma unroll
-            for (int d = 0; d < WG_DIGITS; d++) v -= sum[lane * WG_DIGITS + d];
+            for (int d = 0; d < WG_SUMS; d++) v -= (int64_t)sum[lane * (WG_SUMS + 1) + d] * (1ll << (8 * d));
             __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
             __builtin_amdgcn_wave_barrier();
-            const int id = gq == 0 ? now.id[0] : (gq == 1 ? now.id[1] : (gq == 2 ? now.id[2] : now.id[3]));
-            if (id >= 0 && v != 0)
-                (void)__hip_atomic_fetch_add(reinterpret_cast<unsigned long long*>(p.w) + ((((size_t)id * a.nkv + g)) << a.page_sh) +
+            if (now.id >= 0 && v != 0)
+                (void)__hip_atomic_fetch_add(reinterpret_cast<unsigned long long*>(p.w) + ((((size_t)now.id * a.nkv + g)) << a.page_sh) +
                                                  ((64 * T + lane) & ((1 << a.page_sh) - 1)),
                                              (unsigned long long)v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
