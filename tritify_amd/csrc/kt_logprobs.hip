@@ -113,38 +113,75 @@ __global__ __launch_bounds__(256) void lp_block_kernel(LpRows p) {
 }
 
 constexpr int LP_CANDS = 1024;  // candidates for alternatives that a CTA keeps
+constexpr int LP_BLOCKS = 1024;  // of a row at most
 
-// A CTA a row: the blocks joined, then the alternatives.
-__global__ __launch_bounds__(256) void lp_join_kernel(LpRows p) {
-    __shared__ uint64_t sKey[LP_CANDS];
+// A CTA a row: the blocks joined, then the alternatives. The k best blocks (of equal maxima the first) stay in registers, 8 fours of
+// logits a thread at most; the least of their maxima is a lower bound of the k-th largest logit that hardly any other logit reaches, so
+// those at or above it are collected and ranked against each other. A row of fewer than k blocks takes a bound from its lanes' maxima.
+template <int NT, bool TOP>
+__global__ __launch_bounds__(NT) void lp_join_kernel(LpRows p) {
+    constexpr int NW = NT / 64, PT = LP_BLOCKS / NT;
     __shared__ uint32_t sT[512];
-    __shared__ int sMax[4], sBlk[KT_LOGPROBS_MAX_K], sCount, sOut[4];
-    __shared__ uint64_t sS[4], sW[4];
+    __shared__ int sMax[NW];
+    __shared__ uint64_t sS[NW], sW[NW];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, row = blockIdx.x;
     const int32_t* x = p.x + (size_t)row * p.stride;
-    const int32_t* bm = p.bm + (size_t)row * p.nb;
-    for (int i = tid; i < 512; i += 256) sT[i] = lp_tables.e[i];
-    int M = INT_MIN;
-    for (int i = tid; i < p.nb; i += 256) M = max(M, bm[i]);
+    const size_t first = (size_t)row * p.nb;
+    int bm[PT], M = INT_MIN;
+    uint64_t bs[PT], bw[PT];
+#pragma unroll
+    for (int i = 0; i < PT; i++) {
+        const int at = tid + i * NT;
+        bm[i] = INT_MIN, bs[i] = bw[i] = 0;
+        if (at < p.nb) bm[i] = p.bm[first + at], bs[i] = p.bs[first + at], bw[i] = p.bw[first + at];
+    }
+    int tok = -1, tok_x = 0;
+    if (tid == 0) {
+        tok = p.token[row];
+        if ((unsigned)tok < (unsigned)p.n) tok_x = x[tok];
+    }
+    for (int i = tid; i < 512; i += NT) sT[i] = lp_tables.e[i];
+#pragma unroll
+    for (int i = 0; i < PT; i++) M = max(M, bm[i]);
     M = wave_max_i32(M);
     if (lane == 0) sMax[w] = M;
-    if (tid == 0) sCount = 0;
+    __shared__ __attribute__((aligned(16))) int sBm[TOP ? LP_BLOCKS : 4];
+    __shared__ int sBlk[KT_LOGPROBS_MAX_K], sBound, sCount;
+    if constexpr (TOP) {
+        sBm[tid] = bm[0];  // (one a thread)
+        if (tid == 0) sCount = 0;
+    }
     __syncthreads();
-    M = max(max(sMax[0], sMax[1]), max(sMax[2], sMax[3]));
+#pragma unroll
+    for (int i = 0; i < NW; i++) M = max(M, sMax[i]);
     uint64_t S = 0, W = 0;
-    for (int i = tid; i < p.nb; i += 256) {
-        const size_t at = (size_t)row * p.nb + i;
+#pragma unroll
+    for (int i = 0; i < PT; i++) {
         const uint32_t u = lp_bits((uint32_t)M - (uint32_t)bm[i], p.mant, p.shift, LP_FAR), k = 22 + (u >> 16);
-        const uint64_t m = __umulhi(sT[(u >> 8) & 255], sT[256 + (u & 255)]), s = p.bs[at];
-        S += ((s >> 8) * m) >> k;
-        W += (((p.bw[at] + u * s) >> 21) * (m >> 8)) >> k;
+        const uint64_t m = __umulhi(sT[(u >> 8) & 255], sT[256 + (u & 255)]);
+        S += ((bs[i] >> 8) * m) >> k;
+        W += (((bw[i] + u * bs[i]) >> 21) * (m >> 8)) >> k;
     }
     S = wave_sum_u64(S);
     W = wave_sum_u64(W);
     if (lane == 0) sS[w] = S, sW[w] = W;
+    const int kb = min(p.k, p.nb);
+    if constexpr (TOP) {
+        if (tid < p.nb) {
+            int rank = 0;
+            for (int j = 0; j < p.nb && rank < kb; j += 4) {
+                const i32x4 o = *reinterpret_cast<const i32x4*>(sBm + j);
+#pragma unroll
+                for (int e = 0; e < 4; e++) rank += (o[e] > bm[0]) | ((o[e] == bm[0]) & (j + e < tid));
+            }
+            if (rank < kb) sBlk[rank] = tid;
+            if (rank == p.k - 1) sBound = bm[0];
+        }
+    }
     __syncthreads();
-    S = sS[0] + sS[1] + sS[2] + sS[3];
-    W = sW[0] + sW[1] + sW[2] + sW[3];
+    S = W = 0;
+#pragma unroll
+    for (int i = 0; i < NW; i++) S += sS[i], W += sW[i];
     const int a = 63 - __clzll((long long)S);
     const uint32_t y = (uint32_t)(a >= 31 ? S >> (a - 31) : S << (31 - a)) & 0x7FFFFFFFu;
     const int gi = (int)(y >> 21);
@@ -152,117 +189,127 @@ __global__ __launch_bounds__(256) void lp_join_kernel(LpRows p) {
                       (((int64_t)(lp_tables.g[gi + 1] - lp_tables.g[gi]) * (y & 0x1FFFFF)) >> 21);
     auto nats = [&](int64_t t) { return (int32_t)(((t * 256 + L) * LP_LN2 + (1 << 30)) >> 31); };
     auto lp_of = [&](int v) { return -nats(lp_bits((uint32_t)M - (uint32_t)v, p.mant, p.shift, INT_MAX)); };
-    if (tid == 0) {
-        const int t = p.token[row];
-        p.lp[row] = (unsigned)t < (unsigned)p.n ? lp_of(x[t]) : INT_MIN;
-        if (p.ent) p.ent[row] = nats((int64_t)((W << 18) / (S >> 3)));
-    }
-    if (p.k == 0) return;
-
-    // the blocks that hold the alternatives, in order of their number
-    const int kb = min(p.k, p.nb);
-    auto key = [](int v, uint32_t i) { return ((uint64_t)((uint32_t)v ^ 0x80000000u) << 32) | (0xFFFFFFFFu - i); };
-    for (int i = tid; i < p.nb; i += 256) {
-        const uint64_t mine = key(bm[i], (uint32_t)i);
-        int rank = 0;
-        for (int j = 0; j < p.nb && rank < kb; j++) rank += key(bm[j], (uint32_t)j) > mine;
-        if (rank < kb) sBlk[rank] = i;
-    }
-    __syncthreads();
-    if (w == 0) {
-        const int mine = lane < kb ? sBlk[lane] : INT_MAX;
-        int rank = 0;
-        for (int j = 0; j < kb; j++) rank += __shfl(mine, j) < mine;
-        if (lane < kb) sBlk[rank] = mine;  // (a wave's reads come before its writes)
-    }
-    __syncthreads();
-    // A lower bound of the k-th largest: of each wave's lanes' maxima the k-th.
-    const int items = kb * 256;  // fours of logits
-    auto each = [&](auto f) {
-        for (int it = tid; it < items; it += 256) {
-            const int i = sBlk[it >> 8] * LP_BLOCK + 4 * (it & 255);
-            if (i + 4 <= p.n) {
-                const i32x4 v = *reinterpret_cast<const i32x4*>(x + i);
+    if constexpr (TOP) {
+        __shared__ uint64_t sKey[LP_CANDS];
+        __shared__ int sOut[NW];
+        constexpr int U = KT_LOGPROBS_MAX_K * (LP_BLOCK / 4) / NT;
+        i32x4 v[U];
+        int at[U];  // the first of four logits; n where there are none
 #pragma unroll
-                for (int e = 0; e < 4; e++) f(v[e], i + e);
+        for (int u = 0; u < U; u++) {
+            const int it = tid + u * NT;
+            at[u] = p.n;
+            if (it < kb * (LP_BLOCK / 4)) at[u] = min(p.n, sBlk[it / (LP_BLOCK / 4)] * LP_BLOCK + 4 * (it % (LP_BLOCK / 4)));
+            if (at[u] + 4 <= p.n) {
+                v[u] = *reinterpret_cast<const i32x4*>(x + at[u]);
             } else {
-                for (int e = 0; i + e < p.n; e++) f(x[i + e], i + e);
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[u][e] = at[u] + e < p.n ? x[at[u] + e] : INT_MIN;
             }
         }
-    };
-    int big = INT_MIN, rank = 0;
-    each([&](int v, int) { big = max(big, v); });
-    for (int j = 0; j < 64; j++) {
-        const int o = __builtin_amdgcn_readlane(big, j);
-        rank += o > big || (o == big && j < lane);
-    }
-    const int kth = __builtin_amdgcn_readlane(big, __ffsll((unsigned long long)__ballot(rank == p.k - 1)) - 1);
-    if (lane == 0) sOut[w] = kth;
-    __syncthreads();
-    int T = max(max(sOut[0], sOut[1]), max(sOut[2], sOut[3]));
-    each([&](int v, int i) {
-        if (v >= T) {
-            const int c = atomicAdd(&sCount, 1);
-            if (c < LP_CANDS) sKey[c] = key(v, (uint32_t)i);
+        if (tid == 0) {
+            p.lp[row] = (unsigned)tok < (unsigned)p.n ? lp_of(tok_x) : INT_MIN;
+            if (p.ent) p.ent[row] = nats((int64_t)((W << 18) / (S >> 3)));
         }
-    });
-    __syncthreads();
-    int cands = sCount;
-    auto count_block = [&](int c) {  // the sum over the CTA
-        __syncthreads();
-        c = wave_sum_i32(c);
-        if (lane == 0) sOut[w] = c;
-        __syncthreads();
-        return sOut[0] + sOut[1] + sOut[2] + sOut[3];
-    };
-    if (cands > LP_CANDS && p.n > p.k) {
-        // Too many at or above the bound, equal ones for the most part: the k-th largest value itself, bit by bit from the first that
-        // the bound and the maximum differ in, then those above it and the first of those equal to it.
-        uint32_t lo = (uint32_t)T ^ 0x80000000u;
-        const uint32_t hi = (uint32_t)M ^ 0x80000000u;
-        if (lo != hi) {
-            const int top = 31 - __clz((int)(lo ^ hi));
-            lo &= ~((2u << top) - 1);
-            for (int b = top; b >= 0; b--) {
-                const uint32_t t = lo | (1u << b);
-                int c = 0;
-                each([&](int v, int) { c += ((uint32_t)v ^ 0x80000000u) >= t; });
-                if (count_block(c) >= p.k) lo = t;
+        auto key = [](int v, uint32_t i) { return ((uint64_t)((uint32_t)v ^ 0x80000000u) << 32) | (0xFFFFFFFFu - i); };
+        auto each = [&](auto f) {
+#pragma unroll
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (at[u] + e < p.n) f(v[u][e], at[u] + e);
+        };
+        auto count = [&](int c) {  // the sum over the CTA
+            __syncthreads();
+            c = wave_sum_i32(c);
+            if (lane == 0) sOut[w] = c;
+            __syncthreads();
+            c = 0;
+#pragma unroll
+            for (int i = 0; i < NW; i++) c += sOut[i];
+            return c;
+        };
+        int T = sBound;
+        if (p.nb < p.k) {  // of each wave's lanes' maxima the k-th
+            int big = INT_MIN, rank = 0;
+            each([&](int v, int) { big = max(big, v); });
+            for (int j = 0; j < 64; j++) {
+                const int o = __builtin_amdgcn_readlane(big, j);
+                rank += (o > big) | ((o == big) & (j < lane));
             }
+            const int kth = __builtin_amdgcn_readlane(big, __ffsll((unsigned long long)__ballot(rank == p.k - 1)) - 1);
+            if (lane == 0) sOut[w] = kth;
+            __syncthreads();
+            T = INT_MIN;
+#pragma unroll
+            for (int i = 0; i < NW; i++) T = max(T, sOut[i]);
         }
-        T = (int)(lo ^ 0x80000000u);
-        __syncthreads();
-        if (tid == 0) sCount = 0;
-        __syncthreads();
         each([&](int v, int i) {
-            if (v > T) sKey[atomicAdd(&sCount, 1)] = key(v, (uint32_t)i);  // fewer than k
+            if (v >= T) {
+                const int c = atomicAdd(&sCount, 1);
+                if (c < LP_CANDS) sKey[c] = key(v, (uint32_t)i);
+            }
         });
         __syncthreads();
-        cands = sCount;
-        __syncthreads();
-        if (w == 0) {  // one wave looks for the first equal ones, in order
-            for (int it = 0; it < kb * LP_BLOCK && cands < p.k; it += 64) {
-                const int i = sBlk[it >> 10] * LP_BLOCK + (it & (LP_BLOCK - 1)) + lane;
-                const bool eq = i < p.n && x[i] == T;
-                const uint64_t all = __ballot(eq);
-                const int before = cands + __popcll(all & ((1ull << lane) - 1));
-                if (eq && before < p.k) sKey[before] = key(T, (uint32_t)i);
-                cands = min(p.k, cands + (int)__popcll(all));
+        int cands = sCount;
+        if (cands > LP_CANDS && p.n > p.k) {
+            // Too many at or above the bound, equal ones for the most part: the k-th largest value itself, bit by bit from the first
+            // that the bound and the maximum differ in, then those above it and the first of those equal to it.
+            uint32_t lo = (uint32_t)T ^ 0x80000000u;
+            const uint32_t hi = (uint32_t)M ^ 0x80000000u;
+            if (lo != hi) {
+                const int top = 31 - __clz((int)(lo ^ hi));
+                lo &= ~((2u << top) - 1);
+                for (int b = top; b >= 0; b--) {
+                    const uint32_t t = lo | (1u << b);
+                    int c = 0;
+                    each([&](int v, int) { c += ((uint32_t)v ^ 0x80000000u) >= t; });
+                    if (count(c) >= p.k) lo = t;
+                }
+            }
+            T = (int)(lo ^ 0x80000000u);
+            __syncthreads();
+            if (tid == 0) sCount = 0;
+            __syncthreads();
+            each([&](int v, int i) {
+                if (v > T) sKey[atomicAdd(&sCount, 1)] = key(v, (uint32_t)i);  // fewer than k
+            });
+            __syncthreads();
+            cands = sCount;
+            __syncthreads();
+            if (w == 0) {  // one wave looks for the first equal ones: the blocks in order of their number, then through each
+                const int mine = lane < kb ? sBlk[lane] : INT_MAX;
+                int rank = 0;
+                for (int j = 0; j < kb; j++) rank += __shfl(mine, j) < mine;
+                for (int q = 0; q < kb && cands < p.k; q++) {
+                    const int blk = __builtin_amdgcn_readlane(mine, __ffsll((unsigned long long)__ballot(lane < kb && rank == q)) - 1);
+                    for (int j = 0; j < LP_BLOCK && cands < p.k; j += 64) {
+                        const int i = blk * LP_BLOCK + j + lane;
+                        const bool eq = i < p.n && x[i] == T;
+                        const uint64_t all = __ballot(eq);
+                        const int before = cands + __popcll(all & ((1ull << lane) - 1));
+                        if (eq && before < p.k) sKey[before] = key(T, (uint32_t)i);
+                        cands = min(p.k, cands + (int)__popcll(all));
+                    }
+                }
+            }
+            cands = p.k;
+            __syncthreads();
+        }
+        if (tid < cands) {
+            const uint64_t mine = sKey[tid];
+            int rank = 0;
+            for (int j = 0; j < cands; j++) rank += sKey[j] > mine;
+            if (rank < p.k) {
+                p.top[(size_t)row * p.k + rank] = (int32_t)(0xFFFFFFFFu - (uint32_t)mine);
+                p.top_lp[(size_t)row * p.k + rank] = lp_of((int)((uint32_t)(mine >> 32) ^ 0x80000000u));
             }
         }
-        cands = p.k;
-        __syncthreads();
+        if (p.n + tid < p.k) p.top[(size_t)row * p.k + p.n + tid] = -1, p.top_lp[(size_t)row * p.k + p.n + tid] = INT_MIN;
+    } else if (tid == 0) {
+        p.lp[row] = (unsigned)tok < (unsigned)p.n ? lp_of(tok_x) : INT_MIN;
+        if (p.ent) p.ent[row] = nats((int64_t)((W << 18) / (S >> 3)));
     }
-    for (int i = tid; i < cands; i += 256) {
-        const uint64_t mine = sKey[i];
-        int rank = 0;
-        for (int j = 0; j < cands; j++) rank += sKey[j] > mine;
-        if (rank < p.k) {
-            p.top[(size_t)row * p.k + rank] = (int32_t)(0xFFFFFFFFu - (uint32_t)mine);
-            p.top_lp[(size_t)row * p.k + rank] = lp_of((int)((uint32_t)(mine >> 32) ^ 0x80000000u));
-        }
-    }
-    for (int i = p.n + tid; i < p.k; i += 256) p.top[(size_t)row * p.k + i] = -1, p.top_lp[(size_t)row * p.k + i] = INT_MIN;
 }
 
 struct LpParts {
@@ -288,7 +335,8 @@ hipError_t launch_logprobs(const int32_t* logits, int rows, int n, int64_t strid
     lp_block_kernel<<<dim3((unsigned)((nb + 3) / 4), (unsigned)rows), dim3(256), 0, s>>>(p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    lp_join_kernel<<<dim3((unsigned)rows), dim3(256), 0, s>>>(p);
+    if (k > 0) lp_join_kernel<1024, true><<<dim3((unsigned)rows), dim3(1024), 0, s>>>(p);
+    else lp_join_kernel<256, false><<<dim3((unsigned)rows), dim3(256), 0, s>>>(p);
     return hipGetLastError();
 }
 

@@ -47,19 +47,24 @@ __device__ __forceinline__ v4i negated(v4i x) {
     return x;
 }
 
-// The sums of the batch's sequences begin from 0.
+// The sums of the batch's sequences begin from 0: two slots a thread, a page's (all its kv heads) side by side.
 __global__ __launch_bounds__(256) void pg_weigh_zero_kernel(Paged a, int64_t* __restrict__ w) {
-    const int b = blockIdx.y, end = min(pg_len(a, b), a.max_pages << a.page_sh), page = 1 << a.page_sh;
-    for (int j = (int)(blockIdx.x * 256 + threadIdx.x); j < end; j += (int)gridDim.x * 256) {
-        const int id = pg_page(a, b, j >> 4);
-        if (id < 0) continue;
-        for (int g = 0; g < a.nkv; g++) w[((((size_t)id * a.nkv + g) << a.page_sh)) + (j & (page - 1))] = 0;
+    typedef long long sums2 __attribute__((ext_vector_type(2)));
+    const int b = blockIdx.y, end = min(pg_len(a, b), a.max_pages << a.page_sh);
+    const int per = a.nkv << (a.page_sh - 1), pages = (max(end, 0) + (1 << a.page_sh) - 1) >> a.page_sh;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (int64_t)pages * per; i += (int64_t)gridDim.x * 256) {
+        const int pg = (int)((uint32_t)i / (uint32_t)per), at = 2 * ((int)i - pg * per);
+        const int id = pg_page(a, b, pg << (a.page_sh - 4)), left = end - (pg << a.page_sh) - (at & ((1 << a.page_sh) - 1));
+        if (id < 0 || left <= 0) continue;
+        int64_t* to = w + ((size_t)id * a.nkv << a.page_sh) + at;
+        if (left > 1 && ((uintptr_t)to & 15) == 0) *reinterpret_cast<sums2*>(to) = sums2{0, 0};
+        else to[0] = 0, to[left > 1] = 0;
     }
 }
 
 // CT: 16 columns times CT a step.
 template <int HD, int BITS, int CT>
-__global__ __launch_bounds__(64 * WG_WAVES) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 3 + (BITS == 8 || CT == 1) : 2))) void pg_weigh_kernel(Paged a, PgWeigh p) {
+__global__ __launch_bounds__(64 * WG_WAVES) __attribute__((amdgpu_waves_per_eu(HD == 64 ? (CT == 1 ? 4 : 3) : 2))) void pg_weigh_kernel(Paged a, PgWeigh p) {
     constexpr int WG_GROUP = 16 * CT, QN = WG_GROUP * HD / 16 > 64 * WG_WAVES ? WG_GROUP * HD / 16 / (64 * WG_WAVES) : 1;
     constexpr int KC = HD / 64, CPR = HD / 16, NT = 64 * WG_WAVES, HH = HD / 2;
     constexpr int ROWB = BITS == 8 ? HD : HH, CHB = BITS == 8 ? 16 : 8;
@@ -211,19 +216,24 @@ __global__ __launch_bounds__(64 * WG_WAVES) __attribute__((amdgpu_waves_per_eu(H
             if (l16 < WG_DIGITS) rd[0].x = *reinterpret_cast<const int*>(sR + l16 * WG_GROUP + gq * 4);
             if (l16 >= 1 && l16 < WG_SUMS) rd[0].y = *reinterpret_cast<const int*>(sR + (l16 - 1) * WG_GROUP + gq * 4);
         }
+        // all blocks of the tile for each 16 columns, whose q and top are read from LDS once (a block after the other, in fewer
+        // registers and with a wave more: 1024 rows behind 7777 50 us against 44)
+        v4i P[4][2] = {};
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
-            v4i P[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-            const int j = (k.ok >> (16 * t)) & 1 ? 64 * T + 16 * t + l16 : INT_MAX;  // (of no page: past every row)
+        for (int c = 0; c < CT; c++) {
+            const v4i top = *reinterpret_cast<const v4i*>(sTop + 16 * c + 4 * gq);
+            v4i q[KC], pos = {0, 0, 0, 0};
 #pragma unroll
-            for (int c = 0; c < CT; c++) {
-                const v4i top = *reinterpret_cast<const v4i*>(sTop + 16 * c + 4 * gq);
+            for (int i = 0; i < KC; i++)
+                q[i] = *reinterpret_cast<const v4i*>(sQ + (16 * c + l16) * HD + 16 * ((gq + 4 * i) ^ swz<CPR>(l16 + 16 * c)));
+            if constexpr (!all) pos = *reinterpret_cast<const v4i*>(sPos + 16 * c + 4 * gq);
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
                 v4i y = BITS == 8 && HD == 64 ? top : v4i{0, 0, 0, 0};
 #pragma unroll
                 for (int i = 0; i < KC; i++) {
-                    const v4i q = *reinterpret_cast<const v4i*>(sQ + (16 * c + l16) * HD + 16 * ((gq + 4 * i) ^ swz<CPR>(l16 + 16 * c)));
-                    y = mfma16(q, widen(k.x[t][i]), y);
-                    if constexpr (BITS == 8 && HD == 64) y = mfma16(q, k.x[t][i], y);
+                    y = mfma16(q[i], widen(k.x[t][i]), y);
+                    if constexpr (BITS == 8 && HD == 64) y = mfma16(q[i], k.x[t][i], y);
                 }
                 uint32_t u[4];
 #pragma unroll
@@ -232,7 +242,7 @@ __global__ __launch_bounds__(64 * WG_WAVES) __attribute__((amdgpu_waves_per_eu(H
                     u[r] = BITS == 8 && HD == 64 ? (uint32_t)y[r] : (uint32_t)y[r] * 2 + (uint32_t)top[r];
                 }
                 if constexpr (!all) {
-                    const v4i pos = *reinterpret_cast<const v4i*>(sPos + 16 * c + 4 * gq);
+                    const int j = (k.ok >> (16 * t)) & 1 ? 64 * T + 16 * t + l16 : INT_MAX;  // (of no page: past every row)
 #pragma unroll
                     for (int r = 0; r < 4; r++)
                         u[r] = (j <= pos[r]) & ((j > pos[r] - window) | (j < p.sinks)) ? u[r] : 0x00FFFFFFu;
@@ -245,12 +255,14 @@ __global__ __launch_bounds__(64 * WG_WAVES) __attribute__((amdgpu_waves_per_eu(H
                     e[h] = us2{sE[ix & 0xFFFF], sE[ix >> 16]};
                 }
                 const uint32_t e01 = __builtin_bit_cast(uint32_t, e[0]), e23 = __builtin_bit_cast(uint32_t, e[1]);
-                P[0][c] = (int)__builtin_amdgcn_perm(e23, e01, 0x06040200);
-                P[CT == 4][CT == 4 ? c : 1] = (int)__builtin_amdgcn_perm(e23, e01, 0x07050301);
+                P[t][0][c] = (int)__builtin_amdgcn_perm(e23, e01, 0x06040200);
+                P[t][CT == 4][CT == 4 ? c : 1] = (int)__builtin_amdgcn_perm(e23, e01, 0x07050301);
             }
-            acc[t] = mfma16(P[0], rd[0], acc[t]);
-            if constexpr (CT == 4) acc[t] = mfma16(P[1], rd[1], acc[t]);
-            __builtin_amdgcn_sched_barrier(0);  // a block after the other: fewer registers, more waves
+        }
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            acc[t] = mfma16(P[t][0], rd[0], acc[t]);
+            if constexpr (CT == 4) acc[t] = mfma16(P[t][1], rd[1], acc[t]);
         }
     };
 
@@ -312,7 +324,7 @@ hipError_t launch_pg_weigh(const Paged& a, int hd, int bits, const int8_t* q, in
                            int window, int sinks, const int32_t* stats, bool fresh, int64_t* w, hipStream_t s) {
     const int64_t max_pos = (int64_t)a.max_pages << a.page_sh;
     if (fresh) {
-        const int64_t blocks = std::min<int64_t>((max_pos + 255) / 256, std::max<int64_t>(1, 4096 / a.seqs));
+        const int64_t blocks = std::min<int64_t>((max_pos * a.nkv + 511) / 512, std::max<int64_t>(1, 4096 / a.seqs));
         pg_weigh_zero_kernel<<<dim3((unsigned)blocks, (unsigned)a.seqs), dim3(256), 0, s>>>(a, w);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess || a.tokens == 0) return e;
