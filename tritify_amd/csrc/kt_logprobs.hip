@@ -8,6 +8,7 @@
 #include <hip/hip_runtime.h>
 #include <limits.h>
 #include <stdint.h>
+#include <type_traits>
 
 #include "kt_dpp.h"
 #include "kt_kernels.h"
@@ -46,12 +47,22 @@ struct LpTables {
 };
 __device__ constexpr LpTables lp_tables{};
 
+// (mant, shift) as the blocks use them: t = (min(d, far) mant + round) >> shift, at most 31 2^16; from the difference `far` on t is there
+// already, and it is less than 31 2^16 + mant there, so 32 bits of the product are enough: its high half from bit sh on (`high`, shift 32
+// or more), or the 32 bits from bit sh.
+struct LpScale {
+    uint32_t mant, far, sh;
+    bool high;
+    uint64_t round;
+};
+
 struct LpRows {
     const int32_t* x;
     int64_t stride;
     int n, nb, k;
     uint32_t mant;
     int shift;
+    LpScale scale;
     int32_t* bm;                  // [row][block]: maximum
     unsigned long long *bs, *bw;  // sums
     const int32_t* token;
@@ -66,13 +77,11 @@ __device__ __forceinline__ uint32_t lp_bits(uint32_t d, uint32_t mant, int shift
     return t > most ? most : (uint32_t)t;
 }
 
-// A wave a block: 16 logits a lane.
+// A wave a block: 16 logits a lane. HIGH: the shift is 32 or more, so t is of the product's high half.
+template <bool HIGH>
 __global__ __launch_bounds__(256) void lp_block_kernel(LpRows p) {
     __shared__ uint32_t sT[512];
-    for (int i = threadIdx.x; i < 512; i += 256) sT[i] = lp_tables.e[i];
-    __syncthreads();
-    const int lane = threadIdx.x & 63, blk = (int)blockIdx.x * 4 + (int)(threadIdx.x >> 6);
-    if (blk >= p.nb) return;
+    const int tid = threadIdx.x, lane = tid & 63, blk = (int)blockIdx.x * 4 + (tid >> 6);
     const int32_t* x = p.x + (size_t)blockIdx.y * p.stride + (size_t)blk * LP_BLOCK;
     const int left = min(LP_BLOCK, p.n - blk * LP_BLOCK);
     int v[16];
@@ -82,26 +91,44 @@ __global__ __launch_bounds__(256) void lp_block_kernel(LpRows p) {
         for (int j = 0; j < 4; j++) {
             const i32x4 y = *reinterpret_cast<const i32x4*>(x + 4 * (lane + 64 * j));
 #pragma unroll
-            for (int e = 0; e < 4; e++) v[4 * j + e] = y[e], top = max(top, y[e]);
+            for (int e = 0; e < 4; e++) v[4 * j + e] = y[e];
         }
     } else {
 #pragma unroll
         for (int j = 0; j < 16; j++) {
             const int i = 4 * (lane + 64 * (j >> 2)) + (j & 3);
             v[j] = i < left ? x[i] : INT_MIN;
-            top = max(top, v[j]);
         }
     }
+    sT[tid] = lp_tables.e[tid];
+    sT[256 + tid] = lp_tables.e[256 + tid];
+    __syncthreads();
+    if (blk >= p.nb) return;
+#pragma unroll
+    for (int j = 0; j < 16; j++) top = max(top, v[j]);
     top = wave_max_i32(top);
     uint64_t S = 0, W = 0;
+    const char* const table = reinterpret_cast<const char*>(sT);
+    auto sums = [&](auto whole) {
 #pragma unroll
-    for (int j = 0; j < 16; j++) {
-        const uint32_t t = lp_bits((uint32_t)top - (uint32_t)v[j], p.mant, p.shift, LP_MOST);
-        uint32_t e = __umulhi(sT[(t >> 8) & 255], sT[256 + (t & 255)]) >> (t >> 16);
-        if (left < LP_BLOCK && 4 * (lane + 64 * (j >> 2)) + (j & 3) >= left) e = 0;
-        S += e;
-        W += (uint64_t)e * t;
-    }
+        for (int j = 0; j < 16; j += 2) {
+            uint32_t e[2];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const uint32_t d = min((uint32_t)top - (uint32_t)v[j + h], p.scale.far);
+                const uint64_t y = (uint64_t)d * p.scale.mant + p.scale.round;
+                const uint32_t hi = (uint32_t)(y >> 32), lo = (uint32_t)y;
+                const uint32_t t = min(HIGH ? hi >> p.scale.sh : __builtin_amdgcn_alignbit(hi, lo, p.scale.sh), (uint32_t)LP_MOST);
+                e[h] = __umulhi(*reinterpret_cast<const uint32_t*>(table + ((t >> 6) & 0x3FC)),
+                                *reinterpret_cast<const uint32_t*>(table + 1024 + ((t << 2) & 0x3FC))) >> (t >> 16);
+                if (!whole && 4 * (lane + 64 * (j >> 2)) + (j & 3) + h >= left) e[h] = 0;
+                W += (uint64_t)e[h] * t;
+            }
+            S += e[0] + e[1];  // (at most 2^31)
+        }
+    };
+    if (left == LP_BLOCK) sums(std::true_type());
+    else sums(std::false_type());
     S = wave_sum_u64(S);
     W = wave_sum_u64(W);
     if (lane == 0) {
@@ -127,6 +154,7 @@ __global__ __launch_bounds__(NT) void lp_join_kernel(LpRows p) {
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, row = blockIdx.x;
     const int32_t* x = p.x + (size_t)row * p.stride;
     const size_t first = (size_t)row * p.nb;
+    auto key = [](int v, uint32_t i) { return ((uint64_t)((uint32_t)v ^ 0x80000000u) << 32) | (0xFFFFFFFFu - i); };  // (value, then the lower index)
     int bm[PT], M = INT_MIN;
     uint64_t bs[PT], bw[PT];
 #pragma unroll
@@ -140,15 +168,19 @@ __global__ __launch_bounds__(NT) void lp_join_kernel(LpRows p) {
         tok = p.token[row];
         if ((unsigned)tok < (unsigned)p.n) tok_x = x[tok];
     }
+    __shared__ int sG[TOP ? 1025 : 1];
+    const int* const g = TOP ? sG : lp_tables.g;  // (with alternatives it is on its way early, for all that wait for L)
     for (int i = tid; i < 512; i += NT) sT[i] = lp_tables.e[i];
+    if constexpr (TOP)
+        for (int i = tid; i < 1025; i += NT) sG[i] = lp_tables.g[i];
 #pragma unroll
     for (int i = 0; i < PT; i++) M = max(M, bm[i]);
     M = wave_max_i32(M);
     if (lane == 0) sMax[w] = M;
-    __shared__ __attribute__((aligned(16))) int sBm[TOP ? LP_BLOCKS : 4];
+    __shared__ uint64_t sBm[TOP ? LP_BLOCKS : 1];
     __shared__ int sBlk[KT_LOGPROBS_MAX_K], sBound, sCount;
     if constexpr (TOP) {
-        sBm[tid] = bm[0];  // (one a thread)
+        sBm[tid] = tid < p.nb ? key(bm[0], (uint32_t)tid) : 0;  // (one a thread)
         if (tid == 0) sCount = 0;
     }
     __syncthreads();
@@ -167,15 +199,16 @@ __global__ __launch_bounds__(NT) void lp_join_kernel(LpRows p) {
     if (lane == 0) sS[w] = S, sW[w] = W;
     const int kb = min(p.k, p.nb);
     if constexpr (TOP) {
-        if (tid < p.nb) {
-            int rank = 0;
-            for (int j = 0; j < p.nb && rank < kb; j += 4) {
-                const i32x4 o = *reinterpret_cast<const i32x4*>(sBm + j);
-#pragma unroll
-                for (int e = 0; e < 4; e++) rank += (o[e] > bm[0]) | ((o[e] == bm[0]) & (j + e < tid));
-            }
-            if (rank < kb) sBlk[rank] = tid;
-            if (rank == p.k - 1) sBound = bm[0];
+        // each block's rank among the others: a few lanes a block, as many as there are threads for
+        const int lg = min(6, 31 - __clz(NT / p.nb)), per = 1 << lg, i = tid >> lg;
+        const uint64_t mine = sBm[min(i, LP_BLOCKS - 1)];
+        int rank = 0;
+#pragma unroll 8
+        for (int j = tid & (per - 1); j < p.nb; j += per) rank += sBm[j] > mine;
+        for (int o = 1; o < per; o <<= 1) rank += __shfl_xor(rank, o);
+        if (i < p.nb && rank < kb && (tid & (per - 1)) == 0) {
+            sBlk[rank] = i;
+            if (rank == p.k - 1) sBound = (int)((uint32_t)(mine >> 32) ^ 0x80000000u);
         }
     }
     __syncthreads();
@@ -185,8 +218,7 @@ __global__ __launch_bounds__(NT) void lp_join_kernel(LpRows p) {
     const int a = 63 - __clzll((long long)S);
     const uint32_t y = (uint32_t)(a >= 31 ? S >> (a - 31) : S << (31 - a)) & 0x7FFFFFFFu;
     const int gi = (int)(y >> 21);
-    const int64_t L = (int64_t)(a - 30) * (1 << 24) + lp_tables.g[gi] +
-                      (((int64_t)(lp_tables.g[gi + 1] - lp_tables.g[gi]) * (y & 0x1FFFFF)) >> 21);
+    const int64_t L = (int64_t)(a - 30) * (1 << 24) + g[gi] + (((int64_t)(g[gi + 1] - g[gi]) * (y & 0x1FFFFF)) >> 21);
     auto nats = [&](int64_t t) { return (int32_t)(((t * 256 + L) * LP_LN2 + (1 << 30)) >> 31); };
     auto lp_of = [&](int v) { return -nats(lp_bits((uint32_t)M - (uint32_t)v, p.mant, p.shift, INT_MAX)); };
     if constexpr (TOP) {
@@ -211,7 +243,6 @@ __global__ __launch_bounds__(NT) void lp_join_kernel(LpRows p) {
             p.lp[row] = (unsigned)tok < (unsigned)p.n ? lp_of(tok_x) : INT_MIN;
             if (p.ent) p.ent[row] = nats((int64_t)((W << 18) / (S >> 3)));
         }
-        auto key = [](int v, uint32_t i) { return ((uint64_t)((uint32_t)v ^ 0x80000000u) << 32) | (0xFFFFFFFFu - i); };
         auto each = [&](auto f) {
 #pragma unroll
             for (int u = 0; u < U; u++)
@@ -244,12 +275,16 @@ __global__ __launch_bounds__(NT) void lp_join_kernel(LpRows p) {
 #pragma unroll
             for (int i = 0; i < NW; i++) T = max(T, sOut[i]);
         }
-        each([&](int v, int i) {
-            if (v >= T) {
-                const int c = atomicAdd(&sCount, 1);
-                if (c < LP_CANDS) sKey[c] = key(v, (uint32_t)i);
-            }
-        });
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (max(max(v[u].x, v[u].y), max(v[u].z, v[u].w)) < T) continue;
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (v[u][e] >= T && at[u] + e < p.n) {
+                    const int c = atomicAdd(&sCount, 1);
+                    if (c < LP_CANDS) sKey[c] = key(v[u][e], (uint32_t)(at[u] + e));
+                }
+        }
         __syncthreads();
         int cands = sCount;
         if (cands > LP_CANDS && p.n > p.k) {
@@ -323,6 +358,21 @@ LpParts lp_parts(int64_t rows, int64_t n) {
 
 }  // namespace
 
+namespace {
+
+LpScale lp_scale(uint32_t mant, int shift) {
+    auto t = [&](uint64_t d) { return ((unsigned __int128)d * mant + ((1ull << shift) >> 1)) >> shift; };
+    uint64_t lo = 0, hi = 0xFFFFFFFFu;  // the least difference whose t is past the bound, if there is one
+    while (lo < hi) {
+        const uint64_t mid = (lo + hi) / 2;
+        if (t(mid) >= (unsigned)LP_MOST) hi = mid;
+        else lo = mid + 1;
+    }
+    return {mant, (uint32_t)lo, (uint32_t)(shift >= 32 ? shift - 32 : shift), shift >= 32, (1ull << shift) >> 1};
+}
+
+}  // namespace
+
 size_t lp_workspace(int64_t rows, int64_t n) { return lp_parts(rows, n).bytes; }
 
 hipError_t launch_logprobs(const int32_t* logits, int rows, int n, int64_t stride, const int32_t* token, uint32_t mant,
@@ -330,9 +380,12 @@ hipError_t launch_logprobs(const int32_t* logits, int rows, int n, int64_t strid
                            hipStream_t s) {
     const LpParts w = lp_parts(rows, n);
     const int nb = (n + LP_BLOCK - 1) / LP_BLOCK;
-    const LpRows p = {logits, stride, n, nb, k, mant, shift, (int32_t*)ws, (unsigned long long*)((char*)ws + w.bs),
+    const LpScale sc = lp_scale(mant, shift);
+    const LpRows p = {logits, stride, n, nb, k, mant, shift, sc, (int32_t*)ws, (unsigned long long*)((char*)ws + w.bs),
                       (unsigned long long*)((char*)ws + w.bw), token, lp, ent, top, top_lp};
-    lp_block_kernel<<<dim3((unsigned)((nb + 3) / 4), (unsigned)rows), dim3(256), 0, s>>>(p);
+    const dim3 blocks((unsigned)((nb + 3) / 4), (unsigned)rows);
+    if (sc.high) lp_block_kernel<true><<<blocks, dim3(256), 0, s>>>(p);
+    else lp_block_kernel<false><<<blocks, dim3(256), 0, s>>>(p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     if (k > 0) lp_join_kernel<1024, true><<<dim3((unsigned)rows), dim3(1024), 0, s>>>(p);

@@ -106,7 +106,8 @@ __global__ __launch_bounds__(NT) void pg_append_kernel(Paged a, const int8_t* __
     int cap = min(max_pos, a.max_pages << a.page_sh), vlo = max(lo, 0), shift = 0;
     if constexpr (NORM) {
         if (nm.shift) shift = max(-(1 << 30), min(nm.shift[b], 1 << 30));
-        cap = (int)min((int64_t)max_pos - shift, (int64_t)(a.max_pages << a.page_sh));
+        const int64_t left = (int64_t)max_pos - shift;
+        cap = left < (a.max_pages << a.page_sh) ? (int)left : a.max_pages << a.page_sh;
         vlo = max(vlo, -shift);
     }
     vlo = min(vlo, hi);  // (0 <= vhi - vlo <= 16 wherever the block is)
