@@ -953,11 +953,14 @@ int kt_hip_dec_weigh_paged(int dev, const int8_t* q_dev, int64_t tokens, int64_t
  * drops what goes there): k, v, multipliers and sums; those of a position without a page become zeros. kept_dev (seqs x nkv x budget
  * int32): the positions that stayed, -1 from n on. The caller then takes to_dev for the sequence's table, n for its length and
  * L - n more for its shift; the old pages are free. No page may be in to_dev twice, or in both to_dev and table_dev.
- * 1 <= budget <= KT_PAGED_MAX_POS, sinks + recent <= budget, seqs * ceil(budget / 16) < 2^24 and seqs <= 65535. */
+ * 1 <= budget <= KT_PAGED_MAX_POS, sinks + recent <= budget, seqs * ceil(budget / 16) < 2^24 and seqs <= 65535. ws_dev:
+ * kt_hip_dec_evict_paged_workspace bytes (0 for a shape outside these), 8-byte aligned, needing no contents; calls that may overlap need
+ * one each. */
+size_t kt_hip_dec_evict_paged_workspace(int64_t seqs, int64_t max_pages, int64_t page, int64_t nkv);
 int kt_hip_dec_evict_paged(int dev, const int32_t* kv_len_dev, const int32_t* table_dev, int64_t seqs, int64_t max_pages,
                            int64_t nkv, int64_t hd, const int32_t* to_dev, int64_t budget, int64_t recent, int64_t sinks,
                            int32_t* kept_dev, void* kpool_dev, void* vpool_dev, int64_t* wpool_dev, int64_t pages,
-                           int64_t page, int bits, void* stream);
+                           int64_t page, int bits, void* ws_dev, size_t ws_bytes, void* stream);
 /* Log probabilities of rows of n int32 logits (logits_dev + r * stride) under their softmax, in 2^-16 of a natural unit, by integer
  * rules alone: the same bits whatever the batch. (mant, shift) is the logits' unit: t(d) = (d mant + floor(2^(shift - 1))) >> shift turns a
  * difference d of logits into 2^-16 of a power of two, 1 <= mant < 2^31, 0 <= shift <= 62; for u codes to the natural unit, mant /

@@ -232,7 +232,7 @@ STATS = {**{k: v for k, v in ATTEND.items() if k not in ("ws", "ws_bytes", "stre
 WEIGH = dict(dev=0, q=P, tokens=3, q_stride=256, row_start=P, kv_len=P, table=P, seqs=2, max_pages=4, nh=4, nkv=2, hd=64, exp=P, window=0,
              sinks=0, stats=P, fresh=0, k=P, w=P, pages=8, page=16, bits=8, stream=None)
 EVICT = dict(dev=0, kv_len=P, table=P, seqs=2, max_pages=4, nkv=2, hd=64, to=P, budget=32, recent=3, sinks=2, kept=P, k=P, v=P, w=P, pages=8,
-             page=16, bits=8, stream=None)
+             page=16, bits=8, ws=P, ws_bytes=1 << 40, stream=None)
 LOGPROBS = dict(dev=0, logits=P, rows=3, n=1000, stride=1000, token=P, mant=1 << 30, shift=30, lp=P, ent=P, k=5, top=P, top_lp=P, ws=P,
                 ws_bytes=1 << 40, stream=None)
 
@@ -259,7 +259,8 @@ REFUSED = (
         dict(stats=P + 4), dict(w=None), dict(w=P + 4), dict(seqs=65536)]]
     + [("kt_hip_dec_evict_paged", EVICT, x) for x in [*of(EVICT, GEOMETRY)] + [
         dict(to=None), dict(kept=None), dict(kept=P + 2), dict(w=None), dict(w=P + 4), dict(budget=0), dict(budget=524289), dict(recent=-1),
-        dict(sinks=-1), dict(recent=31), dict(sinks=30), dict(recent=1 << 62, sinks=1 << 62), dict(seqs=65536), dict(seqs=60000, budget=8192)]]
+        dict(sinks=-1), dict(recent=31), dict(sinks=30), dict(recent=1 << 62, sinks=1 << 62), dict(seqs=65536), dict(seqs=60000, budget=8192),
+        dict(ws=None), dict(ws=P + 4), dict(ws_bytes=255)]]
     + [("kt_hip_dec_logprobs_rows", LOGPROBS, x) for x in [
         dict(rows=-1), dict(rows=65536), dict(n=0), dict(n=(1 << 20) + 1, stride=1 << 21), dict(stride=999), dict(k=-1), dict(k=33),
         dict(mant=0), dict(mant=-5), dict(mant=1 << 31), dict(shift=-1), dict(shift=63), dict(logits=None), dict(token=None), dict(lp=None),
@@ -293,6 +294,9 @@ def test_empty_calls_do_nothing():
     assert L.kt_hip_dec_logprobs_rows_workspace(0, 5, 0) > 0
     for bad in ((-1, 5, 0), (65536, 5, 0), (1, 0, 0), (1, (1 << 20) + 1, 0), (1, 5, 33), (1, 5, -1)):
         assert L.kt_hip_dec_logprobs_rows_workspace(*bad) == 0
+    assert L.kt_hip_dec_evict_paged_workspace(1, 4, 16, 2) > 0 and L.kt_hip_dec_evict_paged_workspace(0, 4, 16, 2) > 0
+    for bad in ((-1, 4, 16, 2), (65536, 4, 16, 2), (1, 0, 16, 2), (1, 4, 17, 2), (1, 4, 16, 0), (1, 524288 // 16 + 1, 16, 2)):
+        assert L.kt_hip_dec_evict_paged_workspace(*bad) == 0
     from tritify_amd import backend as B
 
     with pytest.raises(ValueError):

@@ -125,7 +125,8 @@ def _declare(L: C.CDLL) -> None:
         "kt_hip_dec_weigh_paged": (_I, [_I, _P, _I64, _I64, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, _I,
                                         _P, _P, _I64, _I64, _I, _P]),
         "kt_hip_dec_evict_paged": (_I, [_I, _P, _P, _I64, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _I64,
-                                        _I, _P]),
+                                        _I, _P, _SZ, _P]),
+        "kt_hip_dec_evict_paged_workspace": (_SZ, [_I64] * 4),
         "kt_hip_dec_logprobs_rows_workspace": (_SZ, [_I64] * 3),
         "kt_hip_dec_logprobs_rows": (_I, [_I, _P, _I64, _I64, _I64, _P, _I64, _I, _P, _P, _I64, _P, _P, _P, _SZ, _P]),
         "kt_hip_dec_argmax_rows_workspace": (_SZ, [_I64, _I64]),

@@ -1187,23 +1187,29 @@ int kt_hip_dec_weigh_paged(int dev, const int8_t* q_dev, int64_t tokens, int64_t
                                     (int)std::min(sinks, most), stats_dev, fresh != 0, wpool_dev, (hipStream_t)stream);
 }
 
+size_t kt_hip_dec_evict_paged_workspace(int64_t seqs, int64_t max_pages, int64_t page, int64_t nkv) {
+    if (!paged_ok(0, seqs, max_pages, nkv, nkv, 64, 0, page, 8) || seqs > 65535) return 0;
+    return kt::pg_evict_workspace(seqs, nkv, max_pages * page);
+}
+
 int kt_hip_dec_evict_paged(int dev, const int32_t* kv_len_dev, const int32_t* table_dev, int64_t seqs, int64_t max_pages,
                            int64_t nkv, int64_t hd, const int32_t* to_dev, int64_t budget, int64_t recent, int64_t sinks,
                            int32_t* kept_dev, void* kpool_dev, void* vpool_dev, int64_t* wpool_dev, int64_t pages,
-                           int64_t page, int bits, void* stream) {
+                           int64_t page, int bits, void* ws_dev, size_t ws_bytes, void* stream) {
     if (!paged_ok(0, seqs, max_pages, nkv, nkv, hd, pages, page, bits) || seqs > 65535 || nkv > 65535 || budget < 1 ||
         budget > KT_PAGED_MAX_POS || recent < 0 || sinks < 0 || recent > budget || sinks > budget - recent ||
         seqs * ((budget + 15) / 16) >= 1 << 24)
         return (int)hipErrorInvalidValue;
     if (seqs == 0) return 0;
-    if (!kv_len_dev || !table_dev || !to_dev || !aligned_to(kept_dev, 4) ||
+    if (!kv_len_dev || !table_dev || !to_dev || !aligned_to(kept_dev, 4) || !aligned_to(ws_dev, 8) ||
+        ws_bytes < kt_hip_dec_evict_paged_workspace(seqs, max_pages, page, nkv) ||
         (pages > 0 && (!aligned_to(kpool_dev, 16) || !aligned_to(vpool_dev, 16) || !aligned_to(wpool_dev, 8))))
         return (int)hipErrorInvalidValue;
     KT_TRY(hipSetDevice(dev));
     return (int)kt::launch_pg_evict(paged_args(nullptr, kv_len_dev, table_dev, kpool_dev, vpool_dev, 0, seqs, max_pages,
                                                pages, page, nkv, hd, bits),
                                     (int)hd, bits, to_dev, (int)budget, (int)recent, (int)sinks, kept_dev, wpool_dev,
-                                    (hipStream_t)stream);
+                                    ws_dev, (hipStream_t)stream);
 }
 
 static bool logprobs_ok(int64_t rows, int64_t n, int64_t k) {

@@ -100,7 +100,8 @@ hipError_t launch_pg_weigh(const Paged& a, int hd, int bits, const int8_t* q, in
                            const int32_t* exp_tab, int window, int sinks, const int32_t* stats, bool fresh, int64_t* w,
                            hipStream_t s);
 hipError_t launch_pg_evict(const Paged& a, int hd, int bits, const int32_t* to, int budget, int recent, int sinks,
-                           int32_t* kept, int64_t* w, hipStream_t s);
+                           int32_t* kept, int64_t* w, void* ws, hipStream_t s);
+size_t pg_evict_workspace(int64_t seqs, int64_t nkv, int64_t max_pos);
 size_t lp_workspace(int64_t rows, int64_t n);
 hipError_t launch_logprobs(const int32_t* logits, int rows, int n, int64_t stride, const int32_t* token, uint32_t mant,
                            int shift, int32_t* lp, int32_t* ent, int k, int32_t* top, int32_t* top_lp, void* ws,

@@ -22,17 +22,20 @@ struct PgEvict {
 };
 
 constexpr int EV_NT = 1024, EV_WAVES = EV_NT / 64;
-constexpr int EV_BINS = 4096;   // of sums
+constexpr int EV_BINS = 2048;   // of sums
 constexpr int EV_CANDS = 1024;  // positions of one bin that are ranked against each other
-constexpr int EV_U = 8;         // positions of a lane in flight
+#ifndef EVL
+#define EVL 16384
+#endif
+constexpr int64_t EV_LONG = EVL;
+constexpr int EV_U = 8;         // words of a wave in flight: 64 positions each
 
-// The bin of a sum: the values below 64 one each, from there on 32 to a power of two, mirrored for negative ones; bin 0 for a position
-// without a page (no sum has it).
-__device__ __forceinline__ int weight_bin(int64_t w) {
-    const uint64_t m = (uint64_t)(w < 0 ? ~w : w);
+// The bin of a sum: the values below 64 one each, from there on 32 to a power of two; bin 0 for negative ones, which only a caller's own
+// sums hold, and for positions without a page.
+__device__ __forceinline__ int weight_bin(int64_t w, bool page) {
+    const uint64_t m = (uint64_t)w;
     const int sh = max(0, 58 - __clzll((long long)(m | 1)));
-    const int b = 32 * sh + (int)(m >> sh);
-    return w < 0 ? 2047 - b : 2048 + b;
+    return page && w >= 0 ? 1 + 32 * sh + (int)(m >> sh) : 0;
 }
 // The order of sums as unsigned numbers, 0 for a position without a page.
 __device__ __forceinline__ uint64_t weight_key(int64_t w, bool page) {
@@ -40,117 +43,215 @@ __device__ __forceinline__ uint64_t weight_key(int64_t w, bool page) {
     return page ? (k ? k : 1) : 0;
 }
 
-// A CTA a sequence and kv head. Which positions stay: the sums' histogram says in which bin the least that stays lies and how many of the
-// bin do; a second sweep notes a bit for each position above that bin, and its members are ranked against each other (their sums, then
-// their positions). The bits give the order. Each wave sweeps neighbouring positions, 64 a step.
-//
-// Two sweeps of the sums, whatever the length: 131001 positions (2 kv heads, two CTAs at work) XX us; 64 sequences of up to 2200, 2 kv
-// heads, YY us.
-__global__ __launch_bounds__(EV_NT) void pg_select_kernel(Paged a, PgEvict p) {
+// What several CTAs of a sequence and kv head share where its positions are too many for one: in the workspace, for each.
+struct EvShared {
+    int* hist;       // [EV_BINS], then the count of candidates
+    uint64_t* key;   // [EV_CANDS]
+    int* at;         // [EV_CANDS]
+    uint64_t* bits;  // a word for 64 positions
+};
+struct EvSpace {
+    char* base;
+    size_t stride, key, at, bits;
+    __host__ __device__ EvShared of(size_t i) const {
+        char* const x = base + i * stride;
+        return {(int*)x, (uint64_t*)(x + key), (int*)(x + at), (uint64_t*)(x + bits)};
+    }
+};
+
+// The positions that a sequence and kv head choose from, and the words of 64 that a wave of a CTA reads, eight at a time.
+struct EvSweep {
+    const Paged& a;
+    const int32_t* table;
+    const int64_t* sums;
+    uint32_t stride;
+    int lo, hi, lane;
+    int64_t x[EV_U];
+    uint32_t page;  // bit u: the position of word u has a page
+    __device__ EvSweep(const Paged& a, const PgEvict& p, int b, int g, int lo, int hi)
+        : a(a), table(a.table + (size_t)b * a.max_pages), sums(p.w + ((size_t)g << a.page_sh)),
+          stride((uint32_t)a.nkv << a.page_sh), lo(lo), hi(hi), lane(threadIdx.x & 63), page(0) {}
+    __device__ void load(int word, int end) {
+        int id[EV_U];
+        page = 0;
+#pragma unroll
+        for (int u = 0; u < EV_U; u++) {
+            const int j = lo + 64 * (word + u) + lane;
+            id[u] = -1;
+            if (word + u < end && j < hi) id[u] = table[j >> a.page_sh];
+        }
+#pragma unroll
+        for (int u = 0; u < EV_U; u++) {
+            const int j = lo + 64 * (word + u) + lane;
+            const bool ok = (unsigned)id[u] < (unsigned)a.pages;
+            page |= (uint32_t)ok << u;
+            x[u] = 0;
+            if (ok) x[u] = sums[(uint64_t)(uint32_t)id[u] * stride + (uint32_t)(j & ((1 << a.page_sh) - 1))];
+        }
+    }
+    // f(word, position or -1, sum, whether it has a page) for the loaded words below `end`, all lanes at work
+    template <class F>
+    __device__ void each(int word, int end, F f) {
+#pragma unroll
+        for (int u = 0; u < EV_U; u++) {
+            const int j = lo + 64 * (word + u) + lane;
+            if (word + u < end) f(word + u, j < hi ? j : -1, x[u], (bool)((page >> u) & 1));
+        }
+    }
+    template <class F>
+    __device__ void all(int w0, int w1, F f) {
+        for (int w = w0; w < w1; w += EV_U) load(w, w1), each(w, w1, f);
+    }
+};
+
+// A position's bin counted. Lanes with the first lane's bin are counted together: one bin may have most positions (zeros).
+__device__ __forceinline__ void count_bin(int* hist, int bin) {
+    const int one = __builtin_amdgcn_readfirstlane(bin), same = (int)__popcll(__ballot(bin == one));
+    if ((threadIdx.x & 63) == 0 && one >= 0) atomicAdd(&hist[one], same);
+    if (bin != one && bin >= 0) atomicAdd(&hist[bin], 1);
+}
+
+// Of a histogram, from the largest bin: the bin that the most-th position is in, and how many of the bin those are. By the whole CTA.
+struct EvBin {
+    int bin, need, members;
+};
+__device__ __forceinline__ EvBin find_bin(const int* hist, int most) {
+    __shared__ int sWave[EV_WAVES];
+    __shared__ EvBin sOut;
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    constexpr int N = EV_BINS / EV_NT;
+    int c[N], sum = 0;
+#pragma unroll
+    for (int i = 0; i < N; i++) c[i] = hist[EV_BINS - 1 - N * tid - i], sum += c[i];
+    int above = sum;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int v = __shfl_up(above, o);
+        above += lane >= o ? v : 0;
+    }
+    if (lane == 63) sWave[wv] = above;
+    above -= sum;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < EV_WAVES; i++) above += i < wv ? sWave[i] : 0;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        if (above < most && above + c[i] >= most) sOut = {EV_BINS - 1 - N * tid - i, most - above, c[i]};
+        above += c[i];
+    }
+    __syncthreads();
+    return sOut;
+}
+
+// Several CTAs a sequence and kv head: the histogram cleared, its parts added, and the positions above its bin noted, the bin's own listed.
+__global__ __launch_bounds__(256) void pg_select_clear_kernel(EvSpace sp) {
+    int* const hist = sp.of(blockIdx.x).hist;
+    for (int i = threadIdx.x; i <= EV_BINS; i += 256) hist[i] = 0;
+}
+
+constexpr int EV_PART = EV_WAVES * EV_U;  // words of a CTA
+
+template <bool MARK>
+__global__ __launch_bounds__(EV_NT) void pg_select_part_kernel(Paged a, PgEvict p, EvSpace sp) {
+    __shared__ int sHist[MARK ? 1 : EV_BINS];
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), g = blockIdx.y, b = blockIdx.z;
+    const int L = max(0, min(pg_len(a, b), a.max_pages << a.page_sh));
+    const int lo = p.sinks, hi = L - p.recent, most = p.budget - p.sinks - p.recent;
+    const int words = (hi - lo + 63) / 64, w0 = (int)blockIdx.x * EV_PART + wv * EV_U, w1 = min(w0 + EV_U, words);
+    if (L <= p.budget || most == 0 || (int)blockIdx.x * EV_PART >= words) return;
+    EvSweep s(a, p, b, g, lo, hi);
+    s.load(w0, w1);
+    const EvShared sh = sp.of((size_t)b * a.nkv + g);
+    if constexpr (!MARK) {
+        for (int i = tid; i < EV_BINS; i += EV_NT) sHist[i] = 0;
+        __syncthreads();
+        s.each(w0, w1, [&](int, int j, int64_t x, bool page) { count_bin(sHist, j < 0 ? -1 : weight_bin(x, page)); });
+        __syncthreads();
+        for (int i = tid; i < EV_BINS; i += EV_NT)
+            if (sHist[i]) atomicAdd(&sh.hist[i], sHist[i]);
+    } else {
+        const EvBin e = find_bin(sh.hist, most);
+        s.each(w0, w1, [&](int word, int j, int64_t x, bool page) {
+            const int bin = j < 0 ? -1 : weight_bin(x, page);
+            const uint64_t stay = __ballot(bin > e.bin || (e.need == e.members && bin == e.bin));
+            if (lane == 0) sh.bits[word] = stay;
+            if (bin == e.bin && e.need < e.members && e.members <= EV_CANDS) {
+                const int c = atomicAdd(&sh.hist[EV_BINS], 1);
+                if (c < EV_CANDS) sh.key[c] = weight_key(x, page), sh.at[c] = j;  // (more only if the sums change under the call)
+            }
+        });
+    }
+}
+
+// Which positions stay, a CTA a sequence and kv head: the sums' histogram says in which bin the least that stays lies and how many of
+// the bin do; a bit is noted for each position above that bin, and its members are ranked against each other (their sums, then their
+// positions). The bits give the order. SHARED: histogram, bits and members are in the workspace, and each of the CTAs (grid x) writes its
+// share of the positions.
+template <bool SHARED>
+__global__ __launch_bounds__(EV_NT) void pg_select_kernel(Paged a, PgEvict p, EvSpace sp) {
     extern __shared__ uint64_t sBits[];  // a word for 64 positions
     __shared__ int sHist[EV_BINS];
     __shared__ uint64_t sKey[EV_CANDS], sAnd[EV_WAVES], sOr[EV_WAVES];
     __shared__ int sAt[EV_CANDS], sWave[EV_WAVES], sBin, sNeed, sCount;
-    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), g = blockIdx.x, b = blockIdx.y;
-    const int L = max(0, min(pg_len(a, b), a.max_pages << a.page_sh));
-    int32_t* kept = p.kept + ((size_t)b * a.nkv + g) * p.budget;
+    const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), g = blockIdx.y, b = blockIdx.z;
+    const int L = max(0, min(pg_len(a, b), a.max_pages << a.page_sh)), part = (int)blockIdx.x, parts = (int)gridDim.x;
+    int32_t* const kept = p.kept + ((size_t)b * a.nkv + g) * p.budget;
     if (L <= p.budget) {
-        for (int i = tid; i < p.budget; i += EV_NT) kept[i] = i < L ? i : -1;
+        for (int i = part * EV_NT + tid; i < p.budget; i += parts * EV_NT) kept[i] = i < L ? i : -1;
         return;
     }
     const int lo = p.sinks, hi = L - p.recent, most = p.budget - p.sinks - p.recent;
-    for (int i = tid; i < p.sinks; i += EV_NT) kept[i] = i;
-    for (int i = tid; i < p.recent; i += EV_NT) kept[p.budget - p.recent + i] = hi + i;
+    for (int i = part * EV_NT + tid; i < p.sinks; i += parts * EV_NT) kept[i] = i;
+    for (int i = part * EV_NT + tid; i < p.recent; i += parts * EV_NT) kept[p.budget - p.recent + i] = hi + i;
     if (most == 0) return;
-    for (int i = tid; i < EV_BINS; i += EV_NT) sHist[i] = 0;
-    if (tid == 0) sCount = 0;
-
-    // the wave's words, and f(word, position or -1, sum, whether it has a page) for each of them, all lanes at work
+    // each wave's neighbouring words
     const int words = (hi - lo + 63) / 64, seg = (words + EV_WAVES - 1) / EV_WAVES, w0 = min(wv * seg, words), w1 = min(w0 + seg, words);
-    auto sweep = [&](auto f) {
-        for (int wd = w0; wd < w1; wd += EV_U) {
-            int id[EV_U];
-            int64_t x[EV_U];
-#pragma unroll
-            for (int u = 0; u < EV_U; u++) {
-                const int j = lo + 64 * (wd + u) + lane;
-                id[u] = wd + u < w1 && j < hi ? pg_page(a, b, j >> 4) : -1;
-            }
-#pragma unroll
-            for (int u = 0; u < EV_U; u++) {
-                const int j = lo + 64 * (wd + u) + lane;
-                x[u] = 0;
-                if (id[u] >= 0) x[u] = p.w[(((size_t)id[u] * a.nkv + g) << a.page_sh) + (j & ((1 << a.page_sh) - 1))];
-            }
-#pragma unroll
-            for (int u = 0; u < EV_U; u++) {
-                const int j = lo + 64 * (wd + u) + lane;
-                if (wd + u < w1) f(wd + u, j < hi ? j : -1, x[u], id[u] >= 0);
-            }
-        }
-    };
-    __syncthreads();
-    sweep([&](int, int j, int64_t x, bool page) {
-        // lanes with the first lane's bin are counted together: one bin may have most positions (zeros)
-        const int bin = j < 0 ? -1 : (page ? weight_bin(x) : 0), one = __builtin_amdgcn_readfirstlane(bin);
-        const int same = (int)__popcll(__ballot(bin == one));
-        if (lane == 0 && one >= 0) atomicAdd(&sHist[one], same);
-        if (bin != one && bin >= 0) atomicAdd(&sHist[bin], 1);
-    });
-    __syncthreads();
-    {  // from the largest bin: thread t has bins 4095 - 4 t and the three below
-        int c[4], sum = 0;
-#pragma unroll
-        for (int i = 0; i < 4; i++) c[i] = sHist[EV_BINS - 1 - 4 * tid - i], sum += c[i];
-        int above = sum;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int v = __shfl_up(above, o);
-            above += lane >= o ? v : 0;
-        }
-        if (lane == 63) sWave[wv] = above;
-        above -= sum;
+    EvSweep s(a, p, b, g, lo, hi);
+    EvBin e;
+    if constexpr (SHARED) {
+        const EvShared sh = sp.of((size_t)b * a.nkv + g);
+        e = find_bin(sh.hist, most);
+        for (int i = tid; i < words; i += EV_NT) sBits[i] = sh.bits[i];
+        if (e.need < e.members && tid < min(e.members, EV_CANDS)) sKey[tid] = sh.key[tid], sAt[tid] = sh.at[tid];
+    } else {
+        s.load(w0, w1);
+        for (int i = tid; i < EV_BINS; i += EV_NT) sHist[i] = 0;
+        if (tid == 0) sCount = 0;
         __syncthreads();
-        for (int i = 0; i < wv; i++) above += sWave[i];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if (above < most && above + c[i] >= most) sBin = EV_BINS - 1 - 4 * tid - i, sNeed = most - above;
-            above += c[i];
-        }
+        auto count = [&](int, int j, int64_t x, bool page) { count_bin(sHist, j < 0 ? -1 : weight_bin(x, page)); };
+        s.each(w0, w1, count);
+        if (seg > EV_U) s.all(w0 + EV_U, w1, count);
+        __syncthreads();
+        e = find_bin(sHist, most);
+        auto mark = [&](int word, int j, int64_t x, bool page) {
+            const int bin = j < 0 ? -1 : weight_bin(x, page);
+            const uint64_t stay = __ballot(bin > e.bin || (e.need == e.members && bin == e.bin));
+            if (lane == 0) sBits[word] = stay;
+            if (bin == e.bin && e.need < e.members && e.members <= EV_CANDS) {
+                const int c = atomicAdd(&sCount, 1);
+                if (c < EV_CANDS) sKey[c] = weight_key(x, page), sAt[c] = j;  // (more only if the sums change under the call)
+            }
+        };
+        if (seg > EV_U) s.all(w0, w1, mark);
+        else s.each(w0, w1, mark);  // (still in registers)
     }
     __syncthreads();
-    const int bin = sBin, members = sHist[bin];
-    int need = sNeed;  // of the bin's members
-    const bool all = need == members, few = members <= EV_CANDS;
-    sweep([&](int word, int j, int64_t x, bool page) {
-        const int mine = j < 0 ? -1 : (page ? weight_bin(x) : 0);
-        const uint64_t stay = __ballot(mine > bin || (all && mine == bin));
-        if (lane == 0) sBits[word] = stay;
-        if (mine == bin && few && !all) {
-            const int c = atomicAdd(&sCount, 1);
-            sKey[c] = weight_key(x, page);
-            sAt[c] = j;
-        }
-    });
-    __syncthreads();
-    if (!all && few) {
-        if (tid < members) {
+    int need = e.need;
+    if (need < e.members && e.members <= EV_CANDS) {
+        if (tid < e.members) {
             const uint64_t mine = sKey[tid];
             const int at = sAt[tid];
             int rank = 0;
-            for (int i = 0; i < members; i++) rank += (sKey[i] > mine) | ((sKey[i] == mine) & (sAt[i] < at));
+            for (int i = 0; i < e.members; i++) rank += (sKey[i] > mine) | ((sKey[i] == mine) & (sAt[i] < at));
             if (rank < need) atomicOr(reinterpret_cast<unsigned long long*>(&sBits[(at - lo) >> 6]), 1ull << ((at - lo) & 63));
         }
         __syncthreads();
-    } else if (!all) {
+    } else if (need < e.members) {
         // More members than that, equal ones for the most part: the least sum that stays, eight bits at a time from the first that the
         // members differ in; then those above it and the first of those equal to it.
         uint64_t both = ~0ull, any = 0;
         auto members_of = [&](auto f) {
-            sweep([&](int word, int j, int64_t x, bool page) {
-                const bool in = j >= 0 && (page ? weight_bin(x) : 0) == bin;
-                f(word, in, weight_key(x, page));
-            });
+            s.all(w0, w1, [&](int word, int j, int64_t x, bool page) { f(word, j >= 0 && weight_bin(x, page) == e.bin, weight_key(x, page)); });
         };
         members_of([&](int, bool in, uint64_t k) {
             if (in) both &= k, any |= k;
@@ -211,19 +312,32 @@ __global__ __launch_bounds__(EV_NT) void pg_select_kernel(Paged a, PgEvict p) {
         });
         __syncthreads();
     }
-    // each wave its words, after the bits of the waves before
-    int mine = 0;
-    for (int wd = w0 + lane; wd < w1; wd += 64) mine += (int)__popcll(sBits[wd]);
+    // each wave its words (of the CTA's share), after the bits of all words before
+    const int share = (words + parts - 1) / parts, s0 = min(part * share, words), s1 = min(s0 + share, words);
+    const int sseg = (s1 - s0 + EV_WAVES - 1) / EV_WAVES, v0 = min(s0 + wv * sseg, s1), v1 = min(v0 + sseg, s1);
+    int bits_before = 0, mine = 0;
+    if constexpr (SHARED)
+        for (int i = tid; i < s0; i += EV_NT) bits_before += (int)__popcll(sBits[i]);
+    for (int i = v0 + lane; i < v1; i += 64) mine += (int)__popcll(sBits[i]);
     mine = wave_sum_i32(mine);
     __syncthreads();  // (the counts of the ties are read)
     if (lane == 0) sWave[wv] = mine;
+    if constexpr (SHARED) {
+        bits_before = wave_sum_i32(bits_before);
+        if (lane == 0) sAnd[wv] = (uint64_t)bits_before;
+    }
     __syncthreads();
     int at = p.sinks;
-    for (int i = 0; i < wv; i++) at += sWave[i];
+#pragma unroll
+    for (int i = 0; i < EV_WAVES; i++) {
+        at += i < wv ? sWave[i] : 0;
+        if constexpr (SHARED) at += (int)sAnd[i];
+    }
 #pragma unroll 4
-    for (int wd = w0; wd < w1; wd++) {
-        const uint64_t bits = sBits[wd];
-        if ((bits >> lane) & 1) kept[at + (int)__popcll(bits & ((1ull << lane) - 1))] = lo + 64 * wd + lane;
+    for (int i = v0; i < v1; i++) {
+        const uint64_t bits = sBits[i];
+        const int to = at + (int)__popcll(bits & ((1ull << lane) - 1));
+        if (((bits >> lane) & 1) && to < p.budget - p.recent) kept[to] = lo + 64 * i + lane;
         at += (int)__popcll(bits);
     }
 }
@@ -305,14 +419,39 @@ __global__ __launch_bounds__(256) void pg_move_kernel(Paged a, PgEvict p, int nb
     }
 }
 
+EvSpace ev_space(int64_t max_pos) {
+    const size_t key = (EV_BINS + 2) * 4, at = key + EV_CANDS * 8, bits = at + EV_CANDS * 4;
+    return {nullptr, (bits + (size_t)(max_pos + 63) / 64 * 8 + 255) / 256 * 256, key, at, bits};
+}
+
+// One CTA a sequence and kv head does it in one launch, and reads and orders a long one's sums alone. 
+bool ev_shared(int64_t max_pos) { return max_pos > EV_LONG; }
+
 }  // namespace
 
+size_t pg_evict_workspace(int64_t seqs, int64_t nkv, int64_t max_pos) {
+    return ev_shared(max_pos) ? (size_t)seqs * nkv * ev_space(max_pos).stride : 256;
+}
+
 hipError_t launch_pg_evict(const Paged& a, int hd, int bits, const int32_t* to, int budget, int recent, int sinks, int32_t* kept,
-                           int64_t* w, hipStream_t s) {
+                           int64_t* w, void* ws, hipStream_t s) {
     const int page = 1 << a.page_sh, nblk = (budget + EV_MOVE - 1) / EV_MOVE;
+    const int64_t max_pos = (int64_t)a.max_pages * page;
     const PgEvict p = {to, (budget + page - 1) / page, budget, recent, sinks, kept, w};
-    const size_t words = ((size_t)a.max_pages * page + 63) / 64 * 8;  // at most 64 KB
-    pg_select_kernel<<<dim3((unsigned)a.nkv, (unsigned)a.seqs), dim3(EV_NT), words, s>>>(a, p);
+    const size_t lds = (size_t)(max_pos + 63) / 64 * 8;  // the bits: at most 64 KB
+    EvSpace sp = ev_space(max_pos);
+    sp.base = (char*)ws;
+    if (ev_shared(max_pos)) {
+        const dim3 grid((unsigned)((max_pos + 64 * EV_PART - 1) / (64 * EV_PART)), (unsigned)a.nkv, (unsigned)a.seqs);
+        pg_select_clear_kernel<<<dim3((unsigned)(a.seqs * a.nkv)), dim3(256), 0, s>>>(sp);
+        pg_select_part_kernel<false><<<grid, dim3(EV_NT), 0, s>>>(a, p, sp);
+        pg_select_part_kernel<true><<<grid, dim3(EV_NT), 0, s>>>(a, p, sp);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        pg_select_kernel<true><<<grid, dim3(EV_NT), lds, s>>>(a, p, sp);
+    } else {
+        pg_select_kernel<false><<<dim3(1, (unsigned)a.nkv, (unsigned)a.seqs), dim3(EV_NT), lds, s>>>(a, p, sp);
+    }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     auto go = [&](auto kern) {

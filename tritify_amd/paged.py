@@ -33,6 +33,15 @@ def _need(t, what: str, dtype, dev: int, shape) -> None:
                          f"{tuple(t.shape)} {t.dtype} on {t.device}")
 
 
+def _torch_stream(stream, device):
+    """torch's name for `stream` (None: the null stream)."""
+    import torch
+
+    if stream is None or stream == 0:
+        return torch.cuda.default_stream(device)
+    return torch.cuda.ExternalStream(stream, device=device) if isinstance(stream, int) else stream
+
+
 class PagedBatch:
     """A ragged batch on the device: row_start (seqs + 1 int32), kv_len (seqs int32, the new rows counted) and table
     (seqs x max_pages int32, -1 where a sequence has no page); `tokens` new rows in all. shift (seqs int32, or None: zeros):
@@ -81,6 +90,7 @@ class PagedKV:
         _need(self.v, "v", torch.int8, dev, shape)
         if self.w is not None:
             _need(self.w, "w", torch.int64, dev, (pages, nkv, page))
+            self._no_ws = torch.empty(256, dtype=torch.int8, device=self.device)  # of calls that need none
         self._pools = (self.k.data_ptr(), self.v.data_ptr(), pages, page, bits)  # as every call passes them
 
     def _batch(self, batch: PagedBatch) -> None:
@@ -194,23 +204,44 @@ class PagedKV:
             exp_tab.data_ptr(), window, sinks, stats.data_ptr(), int(fresh), k, self.w.data_ptr(), pages, page, bits,
             B._stream(stream)), "dec paged weigh")
 
-    def evict(self, batch: PagedBatch, to, budget: int, kept, recent: int = 0, sinks: int = 0, stream=None) -> None:
+    def evict_workspace_bytes(self, batch: PagedBatch) -> int:
+        """Scratch bytes of evict for this batch's shape; 256 where it needs none."""
+        self._batch(batch)
+        n = B.lib().kt_hip_dec_evict_paged_workspace(batch.seqs, batch.max_pages, self.page, self.nkv)
+        if n == 0:
+            raise ValueError(f"evict: {batch.seqs} sequences")
+        return n
+
+    def evict(self, batch: PagedBatch, to, budget: int, kept, recent: int = 0, sinks: int = 0, stream=None, ws=None) -> None:
         """The batch's sequences cut down to at most `budget` positions, each kv head by itself: the first `sinks`, the last `recent`
         and, of the others, those with the largest w (ties: the lower position). They move, in order, to the pages `to`
         (seqs x ceil(budget / page) int32: pages of no table, each once); kept (seqs x nkv x budget int32) says which they
         were, -1 past the last. The caller takes `to` for the tables, min(kv_len, budget) for the lengths, and adds what went to the shifts;
-        the old pages are free."""
-        self._batch(batch)
+        the old pages are free. ws: scratch of evict_workspace_bytes, one for each call that may overlap; None: of the call's own, from torch's
+        allocator for `stream`."""
+        n = self.evict_workspace_bytes(batch)
         if self.w is None:
             raise ValueError("evict: the pools were made without accumulated weights")
         if not 1 <= budget <= MAX_POS:
             raise ValueError(f"evict: a budget of {budget}: 1 to {MAX_POS} positions")
         _need(to, "to", self._i32, self.dev, (batch.seqs, -(-budget // self.page)))
         _need(kept, "kept", self._i32, self.dev, (batch.seqs, self.nkv, budget))
+        if ws is None:
+            ws = self._no_ws if n <= 256 else self._scratch(n, stream)
+        elif ws.get_device() != self.dev or not ws.is_contiguous():
+            raise ValueError(f"ws: a contiguous tensor on GPU {self.dev} is needed")
         k, v, pages, page, bits = self._pools
         B.check(B.lib().kt_hip_dec_evict_paged(
             self.dev, batch.ptrs[1], batch.ptrs[2], batch.seqs, batch.max_pages, self.nkv, self.hd, to.data_ptr(), budget, recent,
-            sinks, kept.data_ptr(), k, v, self.w.data_ptr(), pages, page, bits, B._stream(stream)), "dec paged evict")
+            sinks, kept.data_ptr(), k, v, self.w.data_ptr(), pages, page, bits, ws.data_ptr(), ws.nbytes, B._stream(stream)),
+            "dec paged evict")
+
+    def _scratch(self, n: int, stream):
+        """n bytes that are this stream's until what it has been given is done."""
+        import torch
+
+        with torch.cuda.stream(_torch_stream(stream, self.device)):
+            return torch.empty(n, dtype=torch.int8, device=self.device)
 
 
 class PagedDecoder:
@@ -422,10 +453,7 @@ class PagedDecoder:
         return self.torch.is_tensor(t) and t.is_cuda
 
     def _torch_stream(self, stream):
-        torch = self.torch
-        if stream is None or stream == 0:
-            return torch.cuda.default_stream(self.device)
-        return torch.cuda.ExternalStream(stream, device=self.device) if isinstance(stream, int) else stream
+        return _torch_stream(stream, self.device)
 
     def _workspaces(self, b: PagedBatch) -> tuple:
         """Scratch of the attention and of the choice. What a captured pass may hold is kept when a larger one is made."""
