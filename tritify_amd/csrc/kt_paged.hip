@@ -63,14 +63,13 @@ __device__ __forceinline__ int isqrt30(int v) {
     return r;
 }
 
-// clamp(round_half_away(128 y / R), +-16383), |y| <= 2^22, 1 <= R <= 2^15, inv about 1 / (2 R): floor((256 |y| + R) / (2 R)), a float
-// estimate that is off by one at most below 2^14 (its relative error is below 2^-21), settled by the remainder.
+// clamp(round_half_away(128 y / R), +-16383), |y| <= 2^22, 1 <= R <= 2^15: floor(min(256 |y| + R, 2^14 2 R - 1) / (2 R)) with y's sign. inv is
+// 1 / (2 R) short of it by 2^-21 to 2^-20 of itself, more than what rounding adds, so the float quotient's floor (below 2^14) is the whole
+// one or one less, which the remainder says.
 __device__ __forceinline__ int norm_code(int y, int R, float inv) {
-    const int n = 256 * (y < 0 ? -y : y) + R;
-    int q = (int)__builtin_fminf((float)n * inv, 16384.0f);
-    const int rem = n - q * 2 * R;
-    q += rem < 0 ? -1 : (rem >= 2 * R ? 1 : 0);
-    q = q > 16383 ? 16383 : q;
+    const int n = min(256 * (y < 0 ? -y : y) + R, 32768 * R - 1);
+    int q = (int)((float)n * inv);
+    q += n - __mul24(q, 2 * R) >= 2 * R;
     return y < 0 ? -q : q;
 }
 
@@ -140,7 +139,7 @@ __global__ __launch_bounds__(NT) void pg_append_kernel(Paged a, const int8_t* __
                 V += dpp32<DPP_HALF_MIRROR>(V);
                 if constexpr (HD == 128) V += dpp32<DPP_MIRROR>(V);
                 const int R = max(1, isqrt30((int)(V << (HD == 64 ? 10 : 9))));
-                const float inv = __builtin_amdgcn_rcpf((float)(2 * R));
+                const float inv = __builtin_amdgcn_rcpf((float)(2 * R)) * (1 - 0x1.8p-21f);
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const int cc = (int)(int16_t)(C[e >> 1] >> (16 * (e & 1))), ss = (int)(int16_t)(S[e >> 1] >> (16 * (e & 1)));

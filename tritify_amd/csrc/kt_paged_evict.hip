@@ -24,10 +24,6 @@ struct PgEvict {
 constexpr int EV_NT = 1024, EV_WAVES = EV_NT / 64;
 constexpr int EV_BINS = 2048;   // of sums
 constexpr int EV_CANDS = 1024;  // positions of one bin that are ranked against each other
-#ifndef EVL
-#define EVL 16384
-#endif
-constexpr int64_t EV_LONG = EVL;
 constexpr int EV_U = 8;         // words of a wave in flight: 64 positions each
 
 // The bin of a sum: the values below 64 one each, from there on 32 to a power of two; bin 0 for negative ones, which only a caller's own
@@ -424,8 +420,10 @@ EvSpace ev_space(int64_t max_pos) {
     return {nullptr, (bits + (size_t)(max_pos + 63) / 64 * 8 + 255) / 256 * 256, key, at, bits};
 }
 
-// One CTA a sequence and kv head does it in one launch, and reads and orders a long one's sums alone. 
-bool ev_shared(int64_t max_pos) { return max_pos > EV_LONG; }
+// One CTA a sequence and kv head takes one launch, and a long one's sums alone; several take four. us of the launches, one / several: one
+// sequence of 4000 positions (2 kv heads) 8.4 / 18.4, 8000 11.3 / 20.5, 16000 19.2 / 22, 24000 25.3 / 23, 32000 31 / 20.4, 131000 114 / 27; 64
+// of 4000 9.2 / 22, of 16000 21.1 / 26; and each further launch costs the caller some 3.
+bool ev_shared(int64_t max_pos) { return max_pos > 24576; }
 
 }  // namespace
 
