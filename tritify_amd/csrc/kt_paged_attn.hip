@@ -34,7 +34,7 @@ struct PgAttend {
     int32_t* wlow;             // [unit][split][column]: the least negated scores
     unsigned long long* wsum;  // [unit][16 dimensions][register][lane], then the columns' sums of weights
     unsigned* wcnt;            // [unit]: the splits that have added theirs
-    int32_t* stats;            // [row][head]: the largest score, the reciprocal of the weights' sum; or null
+    int32_t* stats;            // STATS: [row][head]: the largest score, the reciprocal of the weights' sum
 };
 
 // A CTA's part of the work. PG_WHOLE: both passes over all positions; PG_KEEP: the same with pass 1's scores kept in LDS as
@@ -122,7 +122,8 @@ __device__ __forceinline__ void pg_store(int8_t* to, const int64_t (&v)[4], int6
     *reinterpret_cast<uint32_t*>(to) = out;
 }
 
-template <int HD, int BITS, int W, int MODE>
+// STATS: the columns' statistics too (a kernel of its own: what it keeps of them costs 128 single tokens behind 6100 a fiftieth).
+template <int HD, int BITS, int W, int MODE, bool STATS>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(W == 8 || HD == 128 ? 2 : (BITS == 8 ? 4 : 3)))) void pg_attend_kernel(
     Paged a, PgAttend p) {
     constexpr int HH = HD / 2, KC = HD / 64, DT = HD / 16, ND = BITS == 8 ? 2 : 3;
@@ -524,12 +525,14 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(W == 8 |
         auto put = [&](int it, const int64_t (&v)[4], int64_t dn) {  // dimensions 16 (it / 64) + 4 (it % 64 / 16) ..
             pg_store<BITS>(out + 16 * (it >> 6) + 4 * ((it & 63) >> 4), v, dn, pos >= 0);
         };
-        auto leave = [&](int64_t dn) {  // by thread tid < cols, whose column is tid: `low` and the sum of its weights, negated
+        [[maybe_unused]] auto leave = [&](int64_t dn) {  // by thread tid < cols, whose column is tid: `low` and the sum of its weights, negated
             const uint64_t R = dn < 0 && pos >= 0 ? (1ull << 40) / (uint64_t)-dn : 0;
             v2i* to = reinterpret_cast<v2i*>(p.stats + 2 * ((size_t)(s.t0 + row) * (p.rep * a.nkv) + head));
             *to = v2i{low == INT_MAX || pos < 0 ? 0 : -low, (int)(uint32_t)(R > 0xFFFFFFFFull ? 0xFFFFFFFFull : R)};
         };
-        if (MODE != PG_SUMS && p.stats && tid < cols) leave(sDen[tid]);
+        if constexpr (STATS && MODE != PG_SUMS) {
+            if (tid < cols) leave(sDen[tid]);
+        }
         for (int it = tid; it < DT * 64; it += NT) {
             if ((it & 15) >= cols) continue;
             int64_t v[4];
@@ -547,7 +550,9 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(W == 8 |
         }
         if constexpr (MODE == PG_SUMS) {  // the unit's last CTA has every split's sums (integers: in any order the same)
             if (!split_last(p.wcnt + unit)) return;
-            if (p.stats && tid < cols) leave((int64_t)__hip_atomic_load(sum + PG_COLS * HD + tid, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+            if constexpr (STATS) {
+                if (tid < cols) leave((int64_t)__hip_atomic_load(sum + PG_COLS * HD + tid, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+            }
             for (int it = tid; it < DT * 64; it += NT) {
                 if ((it & 15) >= cols) continue;
                 int64_t v[4];
@@ -611,20 +616,20 @@ Parts parts(const Plan& x, int nkv, int hd) {
     return {sum, cnt, cnt + (units * 4 + 255) / 256 * 256};
 }
 
-template <int HD, int BITS>
+template <int HD, int BITS, bool STATS>
 hipError_t attend(const Paged& a, const PgAttend& p, const Plan& x, hipStream_t s) {
     const dim3 grid((unsigned)(x.tiles * a.nkv), (unsigned)x.splits), block(64 * x.w);
     if (x.w == 2) {
-        pg_attend_kernel<HD, BITS, 2, PG_WHOLE><<<grid, block, 0, s>>>(a, p);
+        pg_attend_kernel<HD, BITS, 2, PG_WHOLE, STATS><<<grid, block, 0, s>>>(a, p);
     } else if (x.w == 4) {
-        pg_attend_kernel<HD, BITS, 4, PG_WHOLE><<<grid, block, 0, s>>>(a, p);
+        pg_attend_kernel<HD, BITS, 4, PG_WHOLE, STATS><<<grid, block, 0, s>>>(a, p);
     } else if (x.splits == 1) {
-        pg_attend_kernel<HD, BITS, 8, PG_KEEP><<<grid, block, (size_t)p.keep, s>>>(a, p);
+        pg_attend_kernel<HD, BITS, 8, PG_KEEP, STATS><<<grid, block, (size_t)p.keep, s>>>(a, p);
     } else {
-        pg_attend_kernel<HD, BITS, 8, PG_MAX><<<grid, block, 0, s>>>(a, p);
+        pg_attend_kernel<HD, BITS, 8, PG_MAX, false><<<grid, block, 0, s>>>(a, p);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
-        pg_attend_kernel<HD, BITS, 8, PG_SUMS><<<grid, block, 0, s>>>(a, p);
+        pg_attend_kernel<HD, BITS, 8, PG_SUMS, STATS><<<grid, block, 0, s>>>(a, p);
     }
     return hipGetLastError();
 }
@@ -651,8 +656,12 @@ hipError_t launch_pg_attend(const Paged& a, int hd, int bits, const int8_t* q, i
     const int64_t room = 163840 - 8 * 64 * (bits == 8 ? hd : hd / 2) - hd * 128 - 4096;
     const PgAttend p = {q, o, q_stride, o_stride, exp_tab, rep, window, sinks, x.splits, (int)std::min(most, room),
                         (int32_t*)ws, (unsigned long long*)((char*)ws + w.sum), (unsigned*)((char*)ws + w.cnt), stats};
-    if (hd == 64) return bits == 8 ? attend<64, 8>(a, p, x, s) : attend<64, 4>(a, p, x, s);
-    return bits == 8 ? attend<128, 8>(a, p, x, s) : attend<128, 4>(a, p, x, s);
+    if (stats) {
+        if (hd == 64) return bits == 8 ? attend<64, 8, true>(a, p, x, s) : attend<64, 4, true>(a, p, x, s);
+        return bits == 8 ? attend<128, 8, true>(a, p, x, s) : attend<128, 4, true>(a, p, x, s);
+    }
+    if (hd == 64) return bits == 8 ? attend<64, 8, false>(a, p, x, s) : attend<64, 4, false>(a, p, x, s);
+    return bits == 8 ? attend<128, 8, false>(a, p, x, s) : attend<128, 4, false>(a, p, x, s);
 }
 
 }  // namespace kt

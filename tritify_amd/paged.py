@@ -125,7 +125,8 @@ class PagedKV:
         _need(sin, "sin", self._i16, self.dev, shape)
         at, stride = self._rows(qkv, "qkv", batch, (nh + 2 * nkv) * hd)
         to, q_stride = self._rows(q, "q", batch, nh * hd)
-        shift = batch.shift if shift is None else shift
+        if shift is None:
+            shift = batch.shift
         if q_norm is None and k_norm is None and shift is None and self.w is None:
             B.check(B.lib().kt_hip_dec_rope_kv_paged(
                 self.dev, at, batch.tokens, stride, *batch.ptrs, batch.seqs, batch.max_pages, nh, nkv, hd, cos.data_ptr(),
