@@ -234,13 +234,16 @@ __global__ __launch_bounds__(EV_NT) void pg_select_kernel(Paged a, PgEvict p, Ev
     __syncthreads();
     int need = e.need;
     if (need < e.members && e.members <= EV_CANDS) {
-        if (tid < e.members) {
-            const uint64_t mine = sKey[tid];
-            const int at = sAt[tid];
-            int rank = 0;
-            for (int i = 0; i < e.members; i++) rank += (sKey[i] > mine) | ((sKey[i] == mine) & (sAt[i] < at));
-            if (rank < need) atomicOr(reinterpret_cast<unsigned long long*>(&sBits[(at - lo) >> 6]), 1ull << ((at - lo) & 63));
-        }
+        // a few lanes a member, as many as there are threads for
+        const int lg = min(6, 31 - __clz(EV_NT / e.members)), per = 1 << lg, m = tid >> lg;
+        const uint64_t mine = sKey[m];
+        const int at = sAt[m];
+        int rank = 0;
+#pragma unroll 8
+        for (int i = tid & (per - 1); i < e.members; i += per) rank += (sKey[i] > mine) | ((sKey[i] == mine) & (sAt[i] < at));
+        for (int o = 1; o < per; o <<= 1) rank += __shfl_xor(rank, o);
+        if (m < e.members && rank < need && (tid & (per - 1)) == 0)
+            atomicOr(reinterpret_cast<unsigned long long*>(&sBits[(at - lo) >> 6]), 1ull << ((at - lo) & 63));
         __syncthreads();
     } else if (need < e.members) {
         // More members than that, equal ones for the most part: the least sum that stays, eight bits at a time from the first that the

@@ -324,7 +324,7 @@ hipError_t launch_pg_weigh(const Paged& a, int hd, int bits, const int8_t* q, in
                            int window, int sinks, const int32_t* stats, bool fresh, int64_t* w, hipStream_t s) {
     const int64_t max_pos = (int64_t)a.max_pages << a.page_sh;
     if (fresh) {
-        const int64_t blocks = std::min<int64_t>((max_pos * a.nkv + 511) / 512, std::max<int64_t>(1, 4096 / a.seqs));
+        const int64_t blocks = std::min<int64_t>((max_pos * a.nkv + 511) / 512, std::max<int64_t>(1, 1024 / a.seqs));
         pg_weigh_zero_kernel<<<dim3((unsigned)blocks, (unsigned)a.seqs), dim3(256), 0, s>>>(a, w);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess || a.tokens == 0) return e;
