@@ -27,7 +27,7 @@ struct PgWeigh {
     int64_t q_stride;
     const int32_t* exp_tab;
     const int32_t* stats;
-    int nh, rep, window, sinks, splits;
+    int nh, rep, unit, window, sinks, splits;  // unit: columns of a CTA, at most WG_UNIT
     int64_t* w;
 };
 
@@ -87,14 +87,14 @@ __global__ __launch_bounds__(64 * WG_WAVES) __attribute__((amdgpu_waves_per_eu(H
     int b = unit, nth = 0;
     if (unit >= a.seqs) {
         int first = 0;
-        b = pg_tile_seq(a, unit - a.seqs, p.rep, WG_UNIT, 0, &first);
+        b = pg_tile_seq(a, unit - a.seqs, p.rep, p.unit, 0, &first);
         nth = unit - a.seqs - first + 1;
     }
     if (b < 0) return;
     const PgRows s = pg_rows(a, b);
-    const int m0 = nth * WG_UNIT, mrows = s.n * p.rep;
+    const int m0 = nth * p.unit, mrows = s.n * p.rep;
     if (m0 >= mrows) return;
-    const int cols = min(WG_UNIT, mrows - m0), groups = (cols + WG_GROUP - 1) / WG_GROUP;
+    const int cols = min(p.unit, mrows - m0), groups = (cols + WG_GROUP - 1) / WG_GROUP;
     // column m0 + c is head (rem0 + c) % rep of row row0 + (rem0 + c) / rep; a float quotient of a whole number and a half below 2^13
     // is nearer to it than to a whole number, so its floor is exact
     const int row0 = nth ? m0 / p.rep : 0, rem0 = m0 - row0 * p.rep;
@@ -329,13 +329,16 @@ hipError_t launch_pg_weigh(const Paged& a, int hd, int bits, const int8_t* q, in
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess || a.tokens == 0) return e;
     }
+    // A CTA's columns: 256, fewer where that leaves CUs without a CTA; its positions: all that leaves some 2048 CTAs.
     const int rep = nh / a.nkv;
     const int64_t reach = window ? std::min<int64_t>(max_pos, (int64_t)window + sinks + WG_UNIT + 128) : max_pos;
-    const int64_t units = (a.seqs + (int64_t)a.tokens * rep / WG_UNIT) * a.nkv;
     const int64_t rounds = (reach + 64 * WG_WAVES - 1) / (64 * WG_WAVES);
-    const int64_t splits = std::min(rounds, std::max<int64_t>(1, 2048 / units));
-    const bool few = (int64_t)a.tokens * rep <= 16 * (int64_t)a.seqs;  // columns of a sequence, on average
-    const PgWeigh p = {q, q_stride, exp_tab, stats, nh, rep, window, sinks, (int)splits, w};
+    auto units_of = [&](int unit) { return (a.seqs + (int64_t)a.tokens * rep / unit) * a.nkv; };
+    int unit = WG_UNIT;
+    while (unit > 64 && units_of(unit) * rounds < 1024) unit /= 2;
+    const int64_t units = units_of(unit), splits = std::min(rounds, std::max<int64_t>(1, 2048 / units));
+    const bool few = (int64_t)a.tokens * rep <= 24 * (int64_t)a.seqs;  // columns of a sequence, on average
+    const PgWeigh p = {q, q_stride, exp_tab, stats, nh, rep, unit, window, sinks, (int)splits, w};
     auto go = [&](auto one, auto four) {
         if (few) one<<<dim3((unsigned)units, (unsigned)splits), dim3(64 * WG_WAVES), 0, s>>>(a, p);
         else four<<<dim3((unsigned)units, (unsigned)splits), dim3(64 * WG_WAVES), 0, s>>>(a, p);
