@@ -224,6 +224,31 @@ def test_weigh_pages_left_out_and_positions_outside(torch_dev, bits):
     check_weigh(torch_dev, c)
 
 
+@pytest.mark.parametrize("bits,hd", HD_BITS)
+def test_weigh_of_a_chunk_is_that_of_its_parts(torch_dev, bits, hd):
+    """Chunks large enough that a CTA takes 256 columns, against calls of a few rows each, whose CTAs take 64: the same sums."""
+    from tritify_amd.paged import PagedBatch
+
+    torch = torch_dev
+    c = Case(15, [(900, 4000), (1, 3000)], 16, 4, hd, 64, bits)
+    say(f"case: weigh in parts bits={bits} hd={hd}")
+    d = More(torch, c)
+    for window, sinks in ((0, 0), (1500, 70)):
+        d.attend(window, sinks)
+        whole = d.weigh(window, sinks, fresh=True).clone()
+        d.kv.w[:] = torch.where(whole == put(torch, d.w0), d.kv.w, 0)  # the slots that no position has keep what they had
+        d.kv.weigh(d.q, d.b, 16, d.exp, d.stats, window, sinks, fresh=True)
+        assert torch.equal(d.kv.w, whole)
+        d.kv.weigh(d.q[:0], PagedBatch(d.b.row_start * 0, d.b.kv_len, d.b.table, 0), 16, d.exp, d.stats[:0], window, sinks, fresh=True)
+        for at in list(range(0, 900, 61)) + [900]:
+            n = 1 if at == 900 else min(61, 900 - at)
+            one = 1 if at == 900 else 0
+            lens = torch.tensor([3000 if one else 3100 + at + n], dtype=torch.int32, device="cuda")
+            b = PagedBatch(torch.tensor([0, n], dtype=torch.int32, device="cuda"), lens, d.b.table[one:one + 1], n)
+            d.kv.weigh(d.q[at:at + n], b, 16, d.exp, d.stats[at:at + n], window, sinks)
+        assert torch.equal(d.kv.w, whole)
+
+
 def test_weigh_shared_pages(torch_dev):
     """A common prompt's pages in several tables: each slot has the sum over the sequences."""
     c = Case(14, [(1, 100), (3, 90), (1, 100)], 6, 2, 64, 16, 8)
@@ -369,6 +394,17 @@ def test_evict_long(torch_dev, L, budget):
     check_evict(torch_dev, c, budget, 0, 0, c.g.integers(0, 50, size=(c.pages, 2, 64)))
 
 
+def test_evict_from_the_widest_table(torch_dev):
+    """524288 positions in pages that are named many times over: sums of 64 to a page, so 8192 positions have each."""
+    c = spare_case(8, [64 * 256], 1, 64, 256, 8, 1000)
+    table = np.resize(c.table[0, :64], 2048)
+    c.table, c.max_pages = table[None].astype(np.int32), 2048
+    c.kv_len = np.array([524288], dtype=np.int32)
+    check_evict(torch_dev, c, 1000, 100, 7)
+    c.kv_len = np.array([524288 - 1000], dtype=np.int32)
+    check_evict(torch_dev, c, 1000, 0, 0, c.g.integers(0, 1 << 45, size=(c.pages, 1, 256)))
+
+
 @pytest.mark.parametrize("bits", [8, 4])
 def test_evict_many_sequences(torch_dev, bits):
     c = spare_case(5, [(i * 37) % 200 for i in range(300)], 2, 64, 16, bits, 60)
@@ -464,6 +500,16 @@ def test_logprobs_many_rows_and_tokens_outside(torch_dev):
     tokens[:4] = [-(2 ** 31), 2 ** 31 - 1, 300, -1]
     lp = check_logprobs(torch_dev, x, 300, tokens, 30000, 4)[0]
     assert ((lp == -(2 ** 31)) == ((tokens < 0) | (tokens >= 300))).all()
+
+
+@pytest.mark.parametrize("k", [1, 8, 9])
+def test_logprobs_many_rows_of_many_blocks(torch_dev, k):
+    g = np.random.default_rng(7)
+    x = np.round(g.normal(0, 1 << 18, size=(260, 40001))).astype(np.int32)
+    x[3], x[4] = -5, g.integers(0, 3, size=40001)
+    x[5, ::1024] += 1 << 22  # every block's maximum far above its others
+    x[6] = np.sort(x[6])
+    check_logprobs(torch_dev, x, 40000, g.integers(0, 40000, size=260), 87381, k)
 
 
 def test_logprobs_of_a_batch_are_those_of_each_row(torch_dev):

@@ -59,7 +59,7 @@ struct LpScale {
 struct LpRows {
     const int32_t* x;
     int64_t stride;
-    int n, nb, k;
+    int rows, n, nb, k;
     uint32_t mant;
     int shift;
     LpScale scale;
@@ -81,9 +81,12 @@ __device__ __forceinline__ uint32_t lp_bits(uint32_t d, uint32_t mant, int shift
 template <bool HIGH>
 __global__ __launch_bounds__(256) void lp_block_kernel(LpRows p) {
     __shared__ uint32_t sT[512];
-    const int tid = threadIdx.x, lane = tid & 63, blk = (int)blockIdx.x * 4 + (tid >> 6);
-    const int32_t* x = p.x + (size_t)blockIdx.y * p.stride + (size_t)blk * LP_BLOCK;
-    const int left = min(LP_BLOCK, p.n - blk * LP_BLOCK);
+    const int tid = threadIdx.x, lane = tid & 63;
+    const uint32_t unit = blockIdx.x * 4 + (uint32_t)__builtin_amdgcn_readfirstlane(tid >> 6), row = unit / (uint32_t)p.nb;
+    const int blk = (int)(unit - row * (uint32_t)p.nb);
+    const bool in = row < (uint32_t)p.rows;
+    const int32_t* x = p.x + (size_t)row * p.stride + (size_t)blk * LP_BLOCK;
+    const int left = in ? min(LP_BLOCK, p.n - blk * LP_BLOCK) : 0;
     int v[16];
     int top = INT_MIN;
     if (left == LP_BLOCK) {
@@ -103,7 +106,7 @@ __global__ __launch_bounds__(256) void lp_block_kernel(LpRows p) {
     sT[tid] = lp_tables.e[tid];
     sT[256 + tid] = lp_tables.e[256 + tid];
     __syncthreads();
-    if (blk >= p.nb) return;
+    if (!in) return;
 #pragma unroll
     for (int j = 0; j < 16; j++) top = max(top, v[j]);
     top = wave_max_i32(top);
@@ -132,10 +135,9 @@ __global__ __launch_bounds__(256) void lp_block_kernel(LpRows p) {
     S = wave_sum_u64(S);
     W = wave_sum_u64(W);
     if (lane == 0) {
-        const size_t at = (size_t)blockIdx.y * p.nb + blk;
-        p.bm[at] = top;
-        p.bs[at] = S;
-        p.bw[at] = W;
+        p.bm[unit] = top;
+        p.bs[unit] = S;
+        p.bw[unit] = W;
     }
 }
 
@@ -145,7 +147,8 @@ constexpr int LP_BLOCKS = 1024;  // of a row at most
 // A CTA a row: the blocks joined, then the alternatives. The k best blocks (of equal maxima the first) stay in registers, 8 fours of
 // logits a thread at most; the least of their maxima is a lower bound of the k-th largest logit that hardly any other logit reaches, so
 // those at or above it are collected and ranked against each other. A row of fewer than k blocks takes a bound from its lanes' maxima.
-template <int NT, bool TOP>
+// BEST: how many of the best blocks there is room for.
+template <int NT, bool TOP, int BEST>
 __global__ __launch_bounds__(NT) void lp_join_kernel(LpRows p) {
     constexpr int NW = NT / 64, PT = LP_BLOCKS / NT;
     __shared__ uint32_t sT[512];
@@ -180,7 +183,9 @@ __global__ __launch_bounds__(NT) void lp_join_kernel(LpRows p) {
     __shared__ uint64_t sBm[TOP ? LP_BLOCKS : 1];
     __shared__ int sBlk[KT_LOGPROBS_MAX_K], sBound, sCount;
     if constexpr (TOP) {
-        sBm[tid] = tid < p.nb ? key(bm[0], (uint32_t)tid) : 0;  // (one a thread)
+#pragma unroll
+        for (int i = 0; i < PT; i++)
+            if (tid + i * NT < p.nb) sBm[tid + i * NT] = key(bm[i], (uint32_t)(tid + i * NT));
         if (tid == 0) sCount = 0;
     }
     __syncthreads();
@@ -200,15 +205,17 @@ __global__ __launch_bounds__(NT) void lp_join_kernel(LpRows p) {
     const int kb = min(p.k, p.nb);
     if constexpr (TOP) {
         // each block's rank among the others: a few lanes a block, as many as there are threads for
-        const int lg = min(6, 31 - __clz(NT / p.nb)), per = 1 << lg, i = tid >> lg;
-        const uint64_t mine = sBm[min(i, LP_BLOCKS - 1)];
-        int rank = 0;
+        const int lg = p.nb >= NT ? 0 : min(6, 31 - __clz(NT / p.nb)), per = 1 << lg;
+        for (int i = tid >> lg; i < p.nb; i += NT >> lg) {
+            const uint64_t mine = sBm[i];
+            int rank = 0;
 #pragma unroll 8
-        for (int j = tid & (per - 1); j < p.nb; j += per) rank += sBm[j] > mine;
-        for (int o = 1; o < per; o <<= 1) rank += __shfl_xor(rank, o);
-        if (i < p.nb && rank < kb && (tid & (per - 1)) == 0) {
-            sBlk[rank] = i;
-            if (rank == p.k - 1) sBound = (int)((uint32_t)(mine >> 32) ^ 0x80000000u);
+            for (int j = tid & (per - 1); j < p.nb; j += per) rank += sBm[j] > mine;
+            for (int o = 1; o < per; o <<= 1) rank += __shfl_xor(rank, o);
+            if (rank < kb && (tid & (per - 1)) == 0) {
+                sBlk[rank] = i;
+                if (rank == p.k - 1) sBound = (int)((uint32_t)(mine >> 32) ^ 0x80000000u);
+            }
         }
     }
     __syncthreads();
@@ -224,7 +231,7 @@ __global__ __launch_bounds__(NT) void lp_join_kernel(LpRows p) {
     if constexpr (TOP) {
         __shared__ uint64_t sKey[LP_CANDS];
         __shared__ int sOut[NW];
-        constexpr int U = KT_LOGPROBS_MAX_K * (LP_BLOCK / 4) / NT;
+        constexpr int U = BEST * (LP_BLOCK / 4) / NT;
         i32x4 v[U];
         int at[U];  // the first of four logits; n where there are none
 #pragma unroll
@@ -331,9 +338,10 @@ __global__ __launch_bounds__(NT) void lp_join_kernel(LpRows p) {
             cands = p.k;
             __syncthreads();
         }
-        if (tid < cands) {
-            const uint64_t mine = sKey[tid];
+        for (int i = tid; i < cands; i += NT) {
+            const uint64_t mine = sKey[i];
             int rank = 0;
+#pragma unroll 8
             for (int j = 0; j < cands; j++) rank += sKey[j] > mine;
             if (rank < p.k) {
                 p.top[(size_t)row * p.k + rank] = (int32_t)(0xFFFFFFFFu - (uint32_t)mine);
@@ -381,15 +389,20 @@ hipError_t launch_logprobs(const int32_t* logits, int rows, int n, int64_t strid
     const LpParts w = lp_parts(rows, n);
     const int nb = (n + LP_BLOCK - 1) / LP_BLOCK;
     const LpScale sc = lp_scale(mant, shift);
-    const LpRows p = {logits, stride, n, nb, k, mant, shift, sc, (int32_t*)ws, (unsigned long long*)((char*)ws + w.bs),
+    const LpRows p = {logits, stride, rows, n, nb, k, mant, shift, sc, (int32_t*)ws, (unsigned long long*)((char*)ws + w.bs),
                       (unsigned long long*)((char*)ws + w.bw), token, lp, ent, top, top_lp};
-    const dim3 blocks((unsigned)((nb + 3) / 4), (unsigned)rows);
+    const dim3 blocks((unsigned)(((int64_t)rows * nb + 3) / 4));  // (at most 2^24 - 256)
     if (sc.high) lp_block_kernel<true><<<blocks, dim3(256), 0, s>>>(p);
     else lp_block_kernel<false><<<blocks, dim3(256), 0, s>>>(p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    if (k > 0) lp_join_kernel<1024, true><<<dim3((unsigned)rows), dim3(1024), 0, s>>>(p);
-    else lp_join_kernel<256, false><<<dim3((unsigned)rows), dim3(256), 0, s>>>(p);
+    // Where eight blocks hold the alternatives 256 threads will do, in more CTAs at a time: us of the join with 256 / 1024 threads, 700 rows of
+    // 300 logits 11.5 / 29.9, of 5000 14.7 / 36.4, of 151936 14.2 / 25; 300 of 50000 8.1 / 13.4; 128 of 30000 7.5 / 8.0; but few rows of many
+    // blocks rank them faster with more: 64 of 151936 10.2 / 8.0, one 7.9 / 7.0.
+    const bool small = std::min(k, nb) <= 8 && (rows > 256 || nb <= 32);
+    if (k == 0) lp_join_kernel<256, false, 0><<<dim3((unsigned)rows), dim3(256), 0, s>>>(p);
+    else if (small) lp_join_kernel<256, true, 8><<<dim3((unsigned)rows), dim3(256), 0, s>>>(p);
+    else lp_join_kernel<1024, true, KT_LOGPROBS_MAX_K><<<dim3((unsigned)rows), dim3(1024), 0, s>>>(p);
     return hipGetLastError();
 }
 
