@@ -648,6 +648,60 @@ def test_together_captured(torch_dev):
             assert np.array_equal(got.cpu().numpy(), want)
 
 
+@pytest.mark.parametrize("own", [True, False])
+def test_a_long_table_captured(torch_dev, own):
+    """Attention in splits with its statistics, the weights from 0 and a cut by several CTAs captured once, with the cut's scratch
+    given or of its own; between the replays eager calls of the same pools."""
+    torch = torch_dev
+    c = Case(95, [(1, 30000), (3, 260)], 4, 2, 64, 64, 4, spare=14)
+    d = More(torch, c)
+    kept = torch.zeros(2, 2, 400, dtype=torch.int32, device="cuda")
+    to = np.setdiff1d(np.arange(c.pages), c.table)[:14].reshape(2, 7).astype(np.int32)
+    to_dev = put(torch, to)
+    ws = None if own else torch.empty(d.kv.evict_workspace_bytes(d.b), dtype=torch.int8, device="cuda")
+    assert d.kv.evict_workspace_bytes(d.b) > 256
+
+    def step(s):
+        d.kv.attend(d.q, d.b, 4, d.exp, d.o, d.ws, 0, 0, s, stats=d.stats)
+        d.kv.weigh(d.q, d.b, 4, d.exp, d.stats, 0, 0, True, s)
+        d.kv.evict(d.b, to_dev, 400, kept, 50, 4, s, ws)
+
+    s, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        g.capture_begin()
+        step(s)
+        g.capture_end()
+    torch.cuda.synchronize()
+    k, v, w = c.k.copy(), c.v.copy(), d.w0.copy()
+
+    def want():
+        stats = O.paged_stats(c.oracle(k, v), c.q, 4, c.exp)
+        for b in range(2):  # fresh
+            for j in range(int(c.kv_len[b])):
+                w[c.table[b, j // 64], :, j % 64] = 0
+        O.paged_weigh(c.oracle(k, v), c.q, 4, c.exp, stats, w)
+        return O.paged_evict(c.oracle(k, v), to, 400, 50, 4, w)
+
+    for i in range(3):
+        say(f"case: replay {i}")
+        c.kv_len = np.array([30000 - 777 * i, 260 - 60 * i], dtype=np.int32)
+        c.q = c.rows8(*c.q.shape)
+        d.b.kv_len.copy_(torch.from_numpy(c.kv_len))
+        d.q.copy_(torch.from_numpy(c.q))
+        torch.cuda.synchronize()
+        for by in (g.replay, lambda: step(None)):
+            kept.fill_(FILL)
+            torch.cuda.synchronize()
+            by()
+            torch.cuda.synchronize()
+            chosen = want()
+            same(kept, chosen, "kept")
+            same(d.kv.w, w, "sums")
+            same(d.kv.k, k.view(np.int8), "k")
+            same(d.kv.v, v.view(np.int8), "v")
+
+
 def test_two_streams_at_once(torch_dev):
     """Two chains and two batches of logits on two streams side by side, each with its own buffers."""
     import tritify_amd as TA

@@ -242,7 +242,7 @@ __global__ __launch_bounds__(EV_NT) void pg_select_kernel(Paged a, PgEvict p, Ev
 #pragma unroll 8
         for (int i = tid & (per - 1); i < e.members; i += per) rank += (sKey[i] > mine) | ((sKey[i] == mine) & (sAt[i] < at));
         for (int o = 1; o < per; o <<= 1) rank += __shfl_xor(rank, o);
-        if (m < e.members && rank < need && (tid & (per - 1)) == 0)
+        if (m < e.members && rank < need && (tid & (per - 1)) == 0 && (unsigned)(at - lo) < (unsigned)(hi - lo))  // (fewer if they change)
             atomicOr(reinterpret_cast<unsigned long long*>(&sBits[(at - lo) >> 6]), 1ull << ((at - lo) & 63));
         __syncthreads();
     } else if (need < e.members) {
@@ -359,7 +359,7 @@ __global__ __launch_bounds__(256) void pg_move_kernel(Paged a, PgEvict p, int nb
     if (tid < EV_MOVE) {
         const int j = tid < n ? p.kept[((size_t)b * a.nkv + g) * p.budget + first + tid] : -1;
         const int id = tid < n ? p.to[(size_t)b * p.to_pages + ((first + tid) >> a.page_sh)] : -1;
-        const int from = j < 0 ? -1 : pg_page(a, b, j >> 4), sl = j & mask, to_sl = (first + tid) & mask;
+        const int from = (unsigned)j < (unsigned)L ? pg_page(a, b, j >> 4) : -1, sl = j & mask, to_sl = (first + tid) & mask;
         const bool there = (unsigned)id < (unsigned)a.pages;
         const size_t part = ((size_t)max(from, 0) * a.nkv + g) * (size_t)a.part;
         sK[tid] = from < 0 ? nullptr : a.k + part + sl * ROWB;
