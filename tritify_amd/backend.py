@@ -1100,6 +1100,8 @@ def logit_scale(unit: float) -> tuple[int, int]:
     if not 0 < unit < math.inf:
         raise ValueError(f"logit_scale: {unit} codes to a natural unit")
     r = 65536.0 * math.log2(math.e) / unit
+    if not 2.0 ** -40 < r < 2.0 ** 40:
+        raise ValueError(f"logit_scale: {unit} codes to a natural unit")
     shift = 30 - math.floor(math.log2(r))
     mant = round(r * 2.0 ** shift)
     if mant == 1 << 31:
