@@ -179,6 +179,59 @@ def test_budget_on_another_stream(model):  # noqa: F811
     assert got == want
 
 
+def test_captured_steps_under_a_budget(model):  # noqa: F811
+    """A sequence that has been cut, decoded by replays of one captured pass: tokens and accumulated weights as by eager passes."""
+    import torch
+    from tritify_amd.paged import PagedDecoder
+
+    p, (qn, kn) = prompts([90])[0], norms(5)
+    made = [PagedDecoder(model, 30, q_norm=qn, k_norm=kn, budget=40, recent=10, sinks=2, most=50) for _ in range(2)]
+    (d, a), (e, _) = [(d, d.add()) for d in made]
+    toks = [d.run([(a, p)]) for d in made]
+    assert d.held(a) == 40 and d.length(a) == 90
+    d._reserve([(a, 98)])
+    b = d.batch([a], [1])
+    x, out = toks[0].clone(), torch.empty_like(toks[0])
+    s, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        before = [kv.w.clone() for kv in d.kv]
+        d.forward(x, b, None, out, s)  # the shape's workspace; what it adds to the weights is taken back
+        for kv, w in zip(d.kv, before):
+            kv.w.copy_(w)
+        torch.cuda.synchronize()
+        g.capture_begin()
+        d.forward(x, b, None, out, s)
+        g.capture_end()
+    torch.cuda.synchronize()
+    t = toks[1]
+    for step in range(8):
+        say(f"case: replay {step}")
+        g.replay()
+        torch.cuda.synchronize()
+        t = e.run([(a, t)])
+        torch.cuda.synchronize()
+        assert torch.equal(out, t)
+        for l in range(model.L):
+            assert torch.equal(d.kv[l].w, e.kv[l].w) and torch.equal(d.kv[l].k, e.kv[l].k) and torch.equal(d.kv[l].v, e.kv[l].v)
+        x.copy_(out)
+        b.kv_len.add_(1)
+        torch.cuda.synchronize()
+
+
+def test_a_batch_without_shifts_under_a_budget(model):  # noqa: F811
+    import torch
+    from tritify_amd.paged import PagedBatch, PagedDecoder
+
+    d = PagedDecoder(model, 30, budget=40)
+    a = d.add()
+    t = d.run([(a, prompts([20])[0])])
+    d._reserve([(a, 21)])
+    b = d.batch([a], [1])
+    with pytest.raises(ValueError, match="shifts"):
+        d.forward(t, PagedBatch(b.row_start, b.kv_len, b.table, 1), None, torch.empty_like(t))
+
+
 @pytest.mark.parametrize("k", [0, 5])
 def test_logprobs_of_a_pass(model, k):  # noqa: F811
     import torch

@@ -223,6 +223,69 @@ def test_logit_scale():
             logit_scale(bad)
 
 
+@pytest.mark.parametrize("unit", [5e-324, 1e-300, 1e300, 1.7e308])
+def test_logit_scale_of_units_past_all_powers(unit):
+    from tritify_amd.backend import logit_scale
+
+    with pytest.raises(ValueError, match="logit_scale"):
+        logit_scale(unit)
+
+
+# -- the decoder's own checks, without a model or buffers -------------------------------------------------------------
+
+
+@pytest.mark.parametrize("nh,nkv,positions", [(64, 1, 131072), (16, 1, 524288), (128, 4, 300000)])
+def test_a_budget_whose_sums_may_not_hold_is_refused(nh, nkv, positions):
+    from types import SimpleNamespace
+
+    from tritify_amd.paged import PagedDecoder
+
+    m = SimpleNamespace(nh=nh, nkv=nkv, rope_cos=np.zeros((positions, 0)))
+    with pytest.raises(ValueError, match="2.23 heads"):
+        PagedDecoder(m, 100, budget=64)
+
+
+def test_a_pass_under_a_budget_needs_the_shifts():
+    import torch
+    from types import SimpleNamespace
+
+    from tritify_amd.paged import PagedDecoder
+
+    d = PagedDecoder.__new__(PagedDecoder)
+    d.torch, d.dev, d.max_rows, d.max_seqs, d.budget, d.m = torch, -1, 8, 3, 32, SimpleNamespace(V=10)  # -1: torch's number of the CPU
+    i32 = torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="shifts"):
+        d.forward(i32, SimpleNamespace(dev=-1, tokens=2, seqs=2, shift=None), None, i32)
+
+
+def test_cuts_of_many_sequences_at_a_time_are_within_what_evict_takes():
+    import torch
+
+    from tritify_amd.paged import PagedDecoder
+
+    page, budget, n = 256, 524288 - 16, 520
+    need, calls = -(-budget // page), []
+
+    class Evict:
+        def evict(self, b, to, budget, kept, recent, sinks, stream):
+            calls.append(to.shape[0])
+            assert to.shape == (len(b), need) and to.shape[0] * (budget // 16) < 1 << 24 and len(set(to.flatten().tolist())) == to.numel()
+
+    class M:
+        nkv = 1
+
+    d = PagedDecoder.__new__(PagedDecoder)
+    d.torch, d.device, d.m, d.page, d.budget, d.recent, d.sinks, d.most = torch, "cpu", M, page, budget, 0, 0, budget
+    d.kv, d.batch = [Evict()], lambda seqs, rows: seqs
+    own = 2048
+    d.seq = {s: dict(len=budget + 1, cut=0, pages=list(range(s * own, (s + 1) * own)), gone=0) for s in range(n)}
+    d.free, d.spare = list(range(n * own, 2 * n * own)), list(range(2 * n * own, 2 * n * own + need))
+    d._cut(list(d.seq), None)
+    assert sum(calls) == n and max(calls) == 512 and all(d.held(s) == budget for s in d.seq)
+    pages = d.free + d.spare + [p for e in d.seq.values() for p in e["pages"]]
+    assert len(pages) == len(set(pages)) == 2 * n * own + need
+
+
 # -- refusals --------------------------------------------------------------------------------------------------------
 
 P = 1 << 20  # an aligned address that no call here dereferences

@@ -275,6 +275,9 @@ class PagedDecoder:
         if budget and (not 1 <= budget <= MAX_POS or window or recent < 0 or sinks + recent > budget or most < budget):
             raise ValueError(f"PagedDecoder: a budget of {budget} positions (1 to {MAX_POS}) needs no window, sinks + recent within "
                              f"it (not {sinks} + {recent}) and most not below it (not {most})")
+        if budget and min(int(model.rope_cos.shape[0]), MAX_POS) * (model.nh // model.nkv) >= 1 << 23:
+            raise ValueError(f"PagedDecoder: a budget: {model.rope_cos.shape[0]} positions of {model.nh // model.nkv} q heads to a kv head may "
+                             "put more weight on one position than its sum holds, that of 2^23 heads")
         spare = -(-budget // page)
         if budget and pages < spare:
             raise ValueError(f"PagedDecoder: {pages} pages, {spare} of them set aside to cut a sequence to {budget} positions")
@@ -360,7 +363,7 @@ class PagedDecoder:
         torch = self.torch
         seqs, need = [s for s in seqs if self.held(s) > self.most], len(self.spare)
         while seqs:
-            n = min(len(seqs), 1 + len(self.free) // need)
+            n = min(len(seqs), 1 + len(self.free) // need, ((1 << 24) - 1) // -(-self.budget // 16))
             now, seqs = seqs[:n], seqs[n:]
             pages = self.spare + [self.free.pop() for _ in range((n - 1) * need)]
             to = torch.tensor(pages, dtype=torch.int32).reshape(n, need).to(self.device)
@@ -487,9 +490,12 @@ class PagedDecoder:
         sequence's last row (`last`: their indexes among the rows, None where every sequence has one row) to self.logits, the
         greedy choice of each to out (int32). Asynchronous on `stream`, which torch's current stream has to be; capturable
         after a call of the batch's shape. Passes of one decoder, captured or not, share its buffers: they follow one
-        another."""
+        another. Under a budget the batch has its sequences' shifts, as `batch` gives them; the weights that the rows attend with are
+        added up, but no sequence is cut."""
         self._check_pass(tokens_dev, b, last, out)
         vocab = self.m.V
+        if self.budget and b.shift is None:
+            raise ValueError("forward: a decoder with a budget needs the batch's shifts")
         self._layers(tokens_dev, b, stream)
         r = self.r
         if last is not None:
