@@ -16,11 +16,15 @@ namespace kt {
 
 namespace {
 
+// The low bytes of four ints.
+__device__ __forceinline__ int pack4(const int (&v)[4]) {
+    return (int)__builtin_amdgcn_perm(__builtin_amdgcn_perm((uint32_t)v[3], (uint32_t)v[2], 0x0C0C0400),
+                                      __builtin_amdgcn_perm((uint32_t)v[1], (uint32_t)v[0], 0x0C0C0400), 0x05040100);
+}
+
 template <int SH = 14>
 __device__ __forceinline__ int rope_round(int v) {  // clamp(round_half_away(v / 2^SH)), |v| <= 2^30
-    int q = ((v < 0 ? -v : v) + (1 << (SH - 1))) >> SH;
-    q = q > 127 ? 127 : q;
-    return v < 0 ? -q : q;
+    return max(-127, min((v + (1 << (SH - 1)) + (v >> 31)) >> SH, 127));
 }
 
 __device__ __forceinline__ int byte_of(int w, int i) { return (int)(int8_t)(w >> (8 * i)); }
@@ -63,14 +67,14 @@ __device__ __forceinline__ int isqrt30(int v) {
     return r;
 }
 
-// clamp(round_half_away(128 y / R), +-16383), |y| <= 2^22, 1 <= R <= 2^15: floor(min(256 |y| + R, 2^14 2 R - 1) / (2 R)) with y's sign. inv is
-// 1 / (2 R) short of it by 2^-21 to 2^-20 of itself, more than what rounding adds, so the float quotient's floor (below 2^14) is the whole
-// one or one less, which the remainder says.
-__device__ __forceinline__ int norm_code(int y, int R, float inv) {
-    const int n = min(256 * (y < 0 ? -y : y) + R, 32768 * R - 1);
-    int q = (int)((float)n * inv);
-    q += n - __mul24(q, 2 * R) >= 2 * R;
-    return y < 0 ? -q : q;
+// clamp(round_half_away(128 y / R), +-16383), |y| <= 2^22, 1 <= R <= 2^15, in floats: c is 128 / R short of it by 2^-21 to 2^-20 of itself,
+// more than what the product's rounding adds, so the floor (below 2^14) is the whole one or one less, which the remainder, exact in an
+// fma, says. r = R / 128.
+__device__ __forceinline__ int norm_code(int y, float r, float c) {
+    const float a = __builtin_fabsf((float)y);
+    float q = __builtin_floorf(__builtin_fmaf(a, c, 0.5f));
+    q += __builtin_fmaf(-q, r, a) >= 0.5f * r ? 1.0f : 0.0f;
+    return (int)__builtin_copysignf(__builtin_fminf(q, 16383.0f), (float)y);
 }
 
 // One CTA per (block of 16 positions that a sequence's rows reach, kv head): it rotates the q heads of the group and the k
@@ -123,7 +127,7 @@ __global__ __launch_bounds__(NT) void pg_append_kernel(Paged a, const int8_t* __
         const int hv = x4 - r * (rep + 1), p = lo + r;
         const size_t t = (size_t)(s.t0 + (p - s.p0));
         const bool live = p >= vlo && p < vhi;
-        int x = 0, y = 0;
+        int xs[4] = {}, ys[4] = {};
         if (live) {
             const int8_t* src = qkv + t * stride + (hv < rep ? g * rep + hv : nh + g) * HD + 4 * c;
             const int xa = *reinterpret_cast<const int*>(src), xb = *reinterpret_cast<const int*>(src + HH);
@@ -139,25 +143,26 @@ __global__ __launch_bounds__(NT) void pg_append_kernel(Paged a, const int8_t* __
                 V += dpp32<DPP_HALF_MIRROR>(V);
                 if constexpr (HD == 128) V += dpp32<DPP_MIRROR>(V);
                 const int R = max(1, isqrt30((int)(V << (HD == 64 ? 10 : 9))));
-                const float inv = __builtin_amdgcn_rcpf((float)(2 * R)) * (1 - 0x1.8p-21f);
+                const float r = (float)R * 0x1p-7f, inv = __builtin_amdgcn_rcpf(r) * (1 - 0x1.8p-21f);
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const int cc = (int)(int16_t)(C[e >> 1] >> (16 * (e & 1))), ss = (int)(int16_t)(S[e >> 1] >> (16 * (e & 1)));
-                    const int u = norm_code(byte_of(xa, e) * (int)(int16_t)(A[e >> 1] >> (16 * (e & 1))), R, inv);
-                    const int w = norm_code(byte_of(xb, e) * (int)(int16_t)(B[e >> 1] >> (16 * (e & 1))), R, inv);
-                    x |= (rope_round<20>(u * cc - w * ss) & 255) << (8 * e);
-                    y |= (rope_round<20>(w * cc + u * ss) & 255) << (8 * e);
+                    const int u = norm_code(byte_of(xa, e) * (int)(int16_t)(A[e >> 1] >> (16 * (e & 1))), r, inv);
+                    const int w = norm_code(byte_of(xb, e) * (int)(int16_t)(B[e >> 1] >> (16 * (e & 1))), r, inv);
+                    xs[e] = rope_round<20>(__mul24(u, cc) - __mul24(w, ss));
+                    ys[e] = rope_round<20>(__mul24(w, cc) + __mul24(u, ss));
                 }
             } else {
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const int cc = (int)(int16_t)(C[e >> 1] >> (16 * (e & 1))), ss = (int)(int16_t)(S[e >> 1] >> (16 * (e & 1)));
                     const int u = byte_of(xa, e), w = byte_of(xb, e);
-                    x |= (rope_round(u * cc - w * ss) & 255) << (8 * e);
-                    y |= (rope_round(w * cc + u * ss) & 255) << (8 * e);
+                    xs[e] = rope_round(u * cc - w * ss);
+                    ys[e] = rope_round(w * cc + u * ss);
                 }
             }
         }
+        const int x = pack4(xs), y = pack4(ys);
         if (hv < rep) {
             int8_t* to = q + t * q_stride + (g * rep + hv) * HD + 4 * c;
             *reinterpret_cast<int*>(to) = x;
