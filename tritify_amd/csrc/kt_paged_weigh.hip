@@ -64,7 +64,7 @@ __global__ __launch_bounds__(256) void pg_weigh_zero_kernel(Paged a, int64_t* __
 
 // CT: 16 columns times CT a step.
 template <int HD, int BITS, int CT>
-__global__ __launch_bounds__(64 * WG_WAVES) __attribute__((amdgpu_waves_per_eu(HD == 64 ? (CT == 1 ? 4 : 3) : 2))) void pg_weigh_kernel(Paged a, PgWeigh p) {
+__global__ __launch_bounds__(64 * WG_WAVES) __attribute__((amdgpu_waves_per_eu(HD == 64 ? (CT == 1 || BITS == 8 ? 4 : 3) : 2))) void pg_weigh_kernel(Paged a, PgWeigh p) {
     constexpr int WG_GROUP = 16 * CT, QN = WG_GROUP * HD / 16 > 64 * WG_WAVES ? WG_GROUP * HD / 16 / (64 * WG_WAVES) : 1;
     constexpr int KC = HD / 64, CPR = HD / 16, NT = 64 * WG_WAVES, HH = HD / 2;
     constexpr int ROWB = BITS == 8 ? HD : HH, CHB = BITS == 8 ? 16 : 8;
