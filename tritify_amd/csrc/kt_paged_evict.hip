@@ -145,7 +145,9 @@ __global__ __launch_bounds__(256) void pg_select_clear_kernel(EvSpace sp) {
     for (int i = threadIdx.x; i <= EV_BINS; i += 256) hist[i] = 0;
 }
 
-constexpr int EV_PART = EV_WAVES * EV_U;  // words of a CTA
+// Words of a wave here, four: us of the two kernels with two / four / eight for one sequence of 131000 (2 kv heads) 10.8 / 12.0 / 14.3, 16 of
+// them 33.4 / 25.0 / 24.5, 64 of 32000 32.0 / 24.4 / 23.9.
+constexpr int EV_PU = 4, EV_PART = EV_WAVES * EV_PU;
 
 template <bool MARK>
 __global__ __launch_bounds__(EV_NT) void pg_select_part_kernel(Paged a, PgEvict p, EvSpace sp) {
@@ -153,7 +155,7 @@ __global__ __launch_bounds__(EV_NT) void pg_select_part_kernel(Paged a, PgEvict 
     const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), g = blockIdx.y, b = blockIdx.z;
     const int L = max(0, min(pg_len(a, b), a.max_pages << a.page_sh));
     const int lo = p.sinks, hi = L - p.recent, most = p.budget - p.sinks - p.recent;
-    const int words = (hi - lo + 63) / 64, w0 = (int)blockIdx.x * EV_PART + wv * EV_U, w1 = min(w0 + EV_U, words);
+    const int words = (hi - lo + 63) / 64, w0 = (int)blockIdx.x * EV_PART + wv * EV_PU, w1 = min(w0 + EV_PU, words);
     if (L <= p.budget || most == 0 || (int)blockIdx.x * EV_PART >= words) return;
     EvSweep s(a, p, b, g, lo, hi);
     s.load(w0, w1);
@@ -423,10 +425,10 @@ EvSpace ev_space(int64_t max_pos) {
     return {nullptr, (bits + (size_t)(max_pos + 63) / 64 * 8 + 255) / 256 * 256, key, at, bits};
 }
 
-// One CTA a sequence and kv head takes one launch, and a long one's sums alone; several take four. us of the launches, one / several: one
-// sequence of 4000 positions (2 kv heads) 8.4 / 18.4, 8000 11.3 / 20.5, 16000 19.2 / 22, 24000 25.3 / 23, 32000 31 / 20.4, 131000 114 / 27; 64
-// of 4000 9.2 / 22, of 16000 21.1 / 26; and each further launch costs the caller some 3.
-bool ev_shared(int64_t max_pos) { return max_pos > 24576; }
+// One CTA a sequence and kv head takes one launch, and a long one's sums alone: us for one sequence of 4000 positions (2 kv heads) 8.4, of 8000
+// 11.3, 16000 19.2, 24000 25, 32000 31, 131000 114, for 64 of 4000 9.2, of 16000 21.1. Several take four launches (and of the caller 10 us
+// more): one of 25000 17.9, 32000 17.8, 131000 18.2, 64 of 32000 36.6.
+bool ev_shared(int64_t max_pos) { return max_pos > 16384; }
 
 }  // namespace
 
@@ -449,7 +451,10 @@ hipError_t launch_pg_evict(const Paged& a, int hd, int bits, const int32_t* to, 
         pg_select_part_kernel<true><<<grid, dim3(EV_NT), 0, s>>>(a, p, sp);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
-        pg_select_kernel<true><<<grid, dim3(EV_NT), lds, s>>>(a, p, sp);
+        // a CTA a CU: each repeats the choice among the bin's members (16 sequences of 131000 with 8 / 16 / 32 CTAs each 9.3 / 14.5 / 25 us, 64
+        // of 32000 with 1 / 2 / 4 / 8 9.8 / 8.4 / 13 / 22.4)
+        const unsigned parts = (unsigned)std::min<int64_t>(64, std::max<int64_t>(1, 256 / ((int64_t)a.seqs * a.nkv)));
+        pg_select_kernel<true><<<dim3(parts, grid.y, grid.z), dim3(EV_NT), lds, s>>>(a, p, sp);
     } else {
         pg_select_kernel<false><<<dim3(1, (unsigned)a.nkv, (unsigned)a.seqs), dim3(EV_NT), lds, s>>>(a, p, sp);
     }
