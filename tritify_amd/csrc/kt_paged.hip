@@ -82,13 +82,15 @@ __device__ __forceinline__ int norm_code(int y, float r, float c) {
 // unit because V's chunk is 16 positions of a dimension, in 4 bits with two positions to a byte: what rows fill goes out in
 // dwords, what only some of them belong to byte by byte (4 bits: read, merged and written back by its only owner).
 //
-// Bound by the chain of one block (batch, rows, RoPE, LDS, pages) while few are at work: 64 single tokens 3.9 us for 0.15 MB,
-// 4 x 512 rows (14 heads over 2, hd 64) 6.2 us for 4.8 MB, where waves wait 56 % of their time and vector instructions take 0.41
-// of the busy time; by vector instructions where CTAs fill the CUs: 3 x 4000 rows (hd 64) 12.8 us for 31 MB, 0.74 busy with 19 a
-// value of qkv, and 2048 rows in 4 bits (16 heads over 4, hd 128; two CTAs a CU, one round) 10.2 us for 12 MB, 0.70 with 33.
+// Bound by the chain of one block (batch, rows, RoPE, LDS, pages) while few are at work: 64 single tokens 4.0 us for 0.15 MB,
+// 4 x 512 rows (14 heads over 2, hd 64) 5.9 us for 4.8 MB, where waves wait 60 % of their time and vector instructions take 0.36
+// of the busy time; by vector instructions where CTAs fill the CUs: 3 x 4000 rows (hd 64) 11.3 us for 31 MB, 0.69 busy with 16 a
+// value of qkv, and 2048 rows in 4 bits (16 heads over 4, hd 128; two CTAs a CU, one round) 9.8 us for 12 MB, 0.66 with 30.
 // LDS is busy less than a tenth of the time in each.
 //
-// NORM: a head's values are in the HH / 4 neighbouring lanes that hold its pairs, so its sum of squares is a few DPP steps.
+// NORM: a head's values are in the HH / 4 neighbouring lanes that hold its pairs, so its sum of squares is a few DPP steps. Its quotients and
+// the wider products make it vector instructions again: 4 x 512 rows (16 heads over 4, hd 128) 11.5 us for 13 MB, 0.69 busy with 31 a value of
+// qkv; a chunk of 2048 in 4 bits 12.0 us, 0.73 with 43; 64 single tokens 4.6 us.
 template <int HD, int BITS, int NT, bool NORM>
 __global__ __launch_bounds__(NT) void pg_append_kernel(Paged a, const int8_t* __restrict__ qkv, int64_t stride, int nh,
                                                         const int16_t* __restrict__ cosT,
@@ -385,7 +387,8 @@ hipError_t launch_pg_append(const Paged& a, int hd, int bits, const int8_t* qkv,
     const PgNorm nm = {q_norm, k_norm, shift, w};
     // Few CTAs get more threads each, as long as the chip holds them side by side (two of 1024 a CU, some of them empty). us
     // with 256 / 1024: 132 single tokens' CTAs 4-bit 5.0 / 4.6, a chunk of 100 rows 5.0 / 4.2, 512 rows 4-bit 6.7 / 5.6, 498 CTAs
-    // 7.2 / 6.8, 520 (hd 128, 4-bit) 13.2 / 10.6; 948 9.8 / 11.1, 1008 (hd 128, 4-bit) 16.0 / 17.1, 1056 of single tokens 4.9 / 7.4.
+    // 7.2 / 6.8, 520 (hd 128, 4-bit) 13.2 / 10.6; 948 9.8 / 11.1, 1008 (hd 128, 4-bit) 16.0 / 17.1, 1056 of single tokens 4.9 / 7.4. With norms:
+    // 132 single tokens' 4.4 / 4.6, 544 (hd 128) 12.0 / 11.5, 520 (hd 128, 4-bit) 15.8 / 12.0.
     const bool wide = (int64_t)grid.x * grid.y <= 768;
     auto go = [&](auto few, auto lots) {
         if (wide) lots<<<grid, dim3(1024), 0, s>>>(a, qkv, stride, nh, cosT, sinT, max_pos, q, q_stride, nm);
