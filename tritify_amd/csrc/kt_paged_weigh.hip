@@ -311,13 +311,13 @@ __global__ __launch_bounds__(64 * WG_WAVES) __attribute__((amdgpu_waves_per_eu(H
             }
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
             __builtin_amdgcn_wave_barrier();
-            int64_t v = 0;
+            int64_t v = 0;  // of -e R
 #pragma unroll
-            for (int d = 0; d < WG_SUMS; d++) v -= (int64_t)sum[lane * (WG_SUMS + 1) + d] * (1ll << (8 * d));
+            for (int d = 0; d < WG_SUMS; d++) v += (int64_t)sum[lane * (WG_SUMS + 1) + d] * (1ll << (8 * d));
             __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
             __builtin_amdgcn_wave_barrier();
             if (now.id >= 0 && v != 0)
-                (void)__hip_atomic_fetch_add(reinterpret_cast<unsigned long long*>(p.w) + ((((size_t)now.id * a.nkv + g)) << a.page_sh) +
+                (void)__hip_atomic_fetch_sub(reinterpret_cast<unsigned long long*>(p.w) + ((((size_t)now.id * a.nkv + g)) << a.page_sh) +
                                                  ((64 * T + lane) & ((1 << a.page_sh) - 1)),
                                              (unsigned long long)v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
