@@ -2,9 +2,9 @@
 // (kt_hip_dec_logprobs_rows, stated in include/kt_hip.h). The softmax's sums are taken per block of 1024 logits against the block's own
 // maximum, in integers, so one pass over the logits does and no order of waves or CTAs changes a bit; a block is what one wave
 // holds in registers. A second launch joins a row's blocks (24 bytes each) and looks its alternatives up: the k largest logits lie in the
-// k blocks with the largest maxima (of equal ones the first). 1021 rows of 151936 logits: 105 us at 5.9 TB/s, which is what a read of this card's
-// memory reaches (vector units 0.77 busy with 18 instructions a logit), and 6.6 to join; 64 rows 10.3 and 8.2 us, one row 3.4 and 6.9: the join's
-// chain of blocks, ranks, candidates and ranks again.
+// k blocks with the largest maxima (of equal ones the first). 1021 rows of 151936 logits: 110 us in all, 5.65 TB/s, near what a read of this
+// card's memory reaches (vector units 0.77 busy with 18 instructions a logit; the join 6.6 us of it); 64 rows 10.3 and 8.2 us, one row 3.4 and 6.9:
+// the join's chain of blocks, ranks, candidates and ranks again.
 
 #include <algorithm>
 #include <hip/hip_runtime.h>

@@ -90,7 +90,7 @@ __device__ __forceinline__ int norm_code(int y, float r, float c) {
 //
 // NORM: a head's values are in the HH / 4 neighbouring lanes that hold its pairs, so its sum of squares is a few DPP steps. Its quotients and
 // the wider products make it vector instructions again: 4 x 512 rows (16 heads over 4, hd 128) 11.5 us for 13 MB, 0.69 busy with 31 a value of
-// qkv; a chunk of 2048 in 4 bits 12.0 us, 0.73 with 43; 64 single tokens 4.6 us.
+// qkv; a chunk of 2048 in 4 bits 12.0 us, 0.72 with 43; 64 single tokens 4.6 us.
 template <int HD, int BITS, int NT, bool NORM>
 __global__ __launch_bounds__(NT) void pg_append_kernel(Paged a, const int8_t* __restrict__ qkv, int64_t stride, int nh,
                                                         const int16_t* __restrict__ cosT,
