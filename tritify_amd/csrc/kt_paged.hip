@@ -122,6 +122,13 @@ __global__ __launch_bounds__(NT) void pg_append_kernel(Paged a, const int8_t* __
         const int8_t* src = qkv + (size_t)(s.t0 + (p - s.p0)) * stride + (nh + a.nkv + g) * HD + 16 * c;
         *reinterpret_cast<v4i*>(&sKV[1][p & 15][16 * c]) = *reinterpret_cast<const v4i*>(src);
     }
+    // a thread's dimensions are the same ones in all of its turns, and so are their norms' weights
+    [[maybe_unused]] v2i wq[2], wk[2];
+    if constexpr (NORM) {
+        const int d = 4 * (tid % (HH / 4));
+        if (nm.q) wq[0] = *reinterpret_cast<const v2i*>(nm.q + d), wq[1] = *reinterpret_cast<const v2i*>(nm.q + d + HH);
+        if (nm.k) wk[0] = *reinterpret_cast<const v2i*>(nm.k + d), wk[1] = *reinterpret_cast<const v2i*>(nm.k + d + HH);
+    }
     const int items = (hi - lo) * (rep + 1) * (HH / 4);
     const uint32_t inv = 0xFFFFFFFFu / (uint32_t)(rep + 1) + 1;  // x / (rep + 1) = x inv >> 32 while x (rep + 1) < 2^32
     for (int i = tid; i < items; i += NT) {
@@ -135,10 +142,8 @@ __global__ __launch_bounds__(NT) void pg_append_kernel(Paged a, const int8_t* __
             const int xa = *reinterpret_cast<const int*>(src), xb = *reinterpret_cast<const int*>(src + HH);
             const v2i C = *reinterpret_cast<const v2i*>(cosT + (size_t)(p + shift) * HH + 4 * c);
             const v2i S = *reinterpret_cast<const v2i*>(sinT + (size_t)(p + shift) * HH + 4 * c);
-            const int16_t* norm = nullptr;
-            if constexpr (NORM) norm = hv < rep ? nm.q : nm.k;
-            if (NORM && norm) {
-                const v2i A = *reinterpret_cast<const v2i*>(norm + 4 * c), B = *reinterpret_cast<const v2i*>(norm + 4 * c + HH);
+            if (NORM && (hv < rep ? nm.q : nm.k)) {
+                const v2i A = hv < rep ? wq[0] : wk[0], B = hv < rep ? wq[1] : wk[1];
                 uint32_t V = (uint32_t)__builtin_amdgcn_sdot4(xa, xa, __builtin_amdgcn_sdot4(xb, xb, 0, false), false);
                 V += dpp32<DPP_XOR1>(V);  // (a head's lanes are all here, and all live or none)
                 V += dpp32<DPP_XOR2>(V);
