@@ -90,7 +90,7 @@ __device__ __forceinline__ int norm_code(int y, float r, float c) {
 //
 // NORM: a head's values are in the HH / 4 neighbouring lanes that hold its pairs, so its sum of squares is a few DPP steps. Its quotients and
 // the wider products make it vector instructions again: 4 x 512 rows (16 heads over 4, hd 128) 11.5 us for 13 MB, 0.69 busy with 31 a value of
-// qkv; a chunk of 2048 in 4 bits 12.0 us, 0.72 with 43; 64 single tokens 4.6 us.
+// qkv; a chunk of 2048 in 4 bits 12.0 us, 0.72 with 43; 64 single tokens 4.4 us.
 template <int HD, int BITS, int NT, bool NORM>
 __global__ __launch_bounds__(NT) void pg_append_kernel(Paged a, const int8_t* __restrict__ qkv, int64_t stride, int nh,
                                                         const int16_t* __restrict__ cosT,
@@ -393,7 +393,7 @@ hipError_t launch_pg_append(const Paged& a, int hd, int bits, const int8_t* qkv,
     // Few CTAs get more threads each, as long as the chip holds them side by side (two of 1024 a CU, some of them empty). us
     // with 256 / 1024: 132 single tokens' CTAs 4-bit 5.0 / 4.6, a chunk of 100 rows 5.0 / 4.2, 512 rows 4-bit 6.7 / 5.6, 498 CTAs
     // 7.2 / 6.8, 520 (hd 128, 4-bit) 13.2 / 10.6; 948 9.8 / 11.1, 1008 (hd 128, 4-bit) 16.0 / 17.1, 1056 of single tokens 4.9 / 7.4. With norms:
-    // 132 single tokens' 4.4 / 4.6, 544 (hd 128) 12.0 / 11.5, 520 (hd 128, 4-bit) 15.8 / 12.0.
+    // 132 single tokens 4.3 / 4.4, 544 (hd 128) 12.0 / 11.5, 520 (hd 128, 4-bit) 15.8 / 12.0.
     const bool wide = (int64_t)grid.x * grid.y <= 768;
     auto go = [&](auto few, auto lots) {
         if (wide) lots<<<grid, dim3(1024), 0, s>>>(a, qkv, stride, nh, cosT, sinT, max_pos, q, q_stride, nm);

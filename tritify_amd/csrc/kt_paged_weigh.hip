@@ -71,7 +71,8 @@ __global__ __launch_bounds__(256) void pg_weigh_zero_kernel(Paged a, int64_t* __
 // CT: 16 columns times CT a step. Waves a SIMD: with three instead of four the chunk of 1024 rows takes 45.5 us instead of 42.5, four spill some
 // registers outside the loop over columns; in 4 bits, whose multipliers need more, four take 83 us and three 55.
 template <int HD, int BITS, int CT>
-__global__ __launch_bounds__(64 * WG_WAVES) __attribute__((amdgpu_waves_per_eu(HD == 64 ? (CT == 1 || BITS == 8 ? 4 : 3) : 2))) void pg_weigh_kernel(Paged a, PgWeigh p) {
+__global__ __launch_bounds__(64 * WG_WAVES) __attribute__((amdgpu_waves_per_eu(HD == 64 ? (CT == 1 || BITS == 8 ? 4 : 3) : 2))) void
+pg_weigh_kernel(Paged a, PgWeigh p) {
     constexpr int WG_GROUP = 16 * CT, QN = WG_GROUP * HD / 16 > 64 * WG_WAVES ? WG_GROUP * HD / 16 / (64 * WG_WAVES) : 1;
     constexpr int KC = HD / 64, CPR = HD / 16, NT = 64 * WG_WAVES, HH = HD / 2;
     constexpr int ROWB = BITS == 8 ? HD : HH, CHB = BITS == 8 ? 16 : 8;
@@ -162,7 +163,8 @@ __global__ __launch_bounds__(64 * WG_WAVES) __attribute__((amdgpu_waves_per_eu(H
         for (int i = 0; i < QN; i++) {
             const int it = tid + i * NT, c = grp * WG_GROUP + min(it / CPR, n - 1), up = over(c), row = row0 + up;
             if (QN > 1 || WG_GROUP * CPR >= NT || it < WG_GROUP * CPR)
-                qx[i] = *reinterpret_cast<const v4i*>(p.q + (size_t)(s.t0 + row) * p.q_stride + (g * p.rep + rem0 + c - up * p.rep) * HD + 16 * (it % CPR));
+                qx[i] = *reinterpret_cast<const v4i*>(p.q + (size_t)(s.t0 + row) * p.q_stride +
+                                                      (g * p.rep + rem0 + c - up * p.rep) * HD + 16 * (it % CPR));
         }
         if (tid < WG_GROUP) {
             const int c = grp * WG_GROUP + min(tid, n - 1), up = over(c);

@@ -132,14 +132,22 @@ class PagedKV:
                 self.dev, at, batch.tokens, stride, *batch.ptrs, batch.seqs, batch.max_pages, nh, nkv, hd, cos.data_ptr(),
                 sin.data_ptr(), n, to, q_stride, *self._pools, B._stream(stream)), "dec rope + paged append")
             return
-        for t, what, dtype, size in ((q_norm, "q_norm", self._i16, hd), (k_norm, "k_norm", self._i16, hd),
-                                     (shift, "shift", self._i32, batch.seqs)):
-            if t is not None:
-                _need(t, what, dtype, self.dev, (size,))
+        qn = kn = ahead = 0
+        if q_norm is not None:
+            _need(q_norm, "q_norm", self._i16, self.dev, (hd,))
+            qn = q_norm.data_ptr()
+        if k_norm is not None:
+            _need(k_norm, "k_norm", self._i16, self.dev, (hd,))
+            kn = k_norm.data_ptr()
+        if shift is not None:
+            if shift is not batch.shift:  # (which was looked at)
+                _need(shift, "shift", self._i32, self.dev, (batch.seqs,))
+            ahead = shift.data_ptr()
+        k, v, pages, page, bits = self._pools
         B.check(B.lib().kt_hip_dec_norm_rope_kv_paged(
             self.dev, at, batch.tokens, stride, *batch.ptrs, batch.seqs, batch.max_pages, nh, nkv, hd, cos.data_ptr(),
-            sin.data_ptr(), n, B._ptr(q_norm), B._ptr(k_norm), B._ptr(shift), to, q_stride, *self._pools[:2], B._ptr(self.w),
-            *self._pools[2:], B._stream(stream)), "dec norm + rope + paged append")
+            sin.data_ptr(), n, qn, kn, ahead, to, q_stride, k, v, 0 if self.w is None else self.w.data_ptr(), pages, page, bits,
+            B._stream(stream)), "dec norm + rope + paged append")
 
     def read(self, batch: PagedBatch, k, v, stream=None) -> None:
         """Every sequence's positions as contiguous rows: k / v seqs x max_pos x nkv x hd int8, positions from
