@@ -357,7 +357,7 @@ __global__ __launch_bounds__(256) void pg_move_kernel(Paged a, PgEvict p, int nb
     __shared__ int sOdd[EV_MOVE], sTo[EV_MOVE / 16];
     const int b = (int)blockIdx.x / nblk, first = ((int)blockIdx.x - b * nblk) * EV_MOVE, g = blockIdx.y, tid = threadIdx.x;
     const int L = max(0, min(pg_len(a, b), a.max_pages << a.page_sh)), n = min(EV_MOVE, min(L, p.budget) - first);
-    if (n <= 0) return;
+    if (n <= 0 || a.pages == 0) return;
     const int mask = (1 << a.page_sh) - 1;
     const size_t mult = (size_t)(HH << a.page_sh);
     if (tid < EV_MOVE) {
@@ -382,26 +382,34 @@ __global__ __launch_bounds__(256) void pg_move_kernel(Paged a, PgEvict p, int nb
     }
     __syncthreads();
     auto to_of = [&](int r) { return ((size_t)sTo[r >> 4] * a.nkv + g) * (size_t)a.part; };
+    constexpr int U = HD / 64;
+    Chunk k[U];
+    uint32_t v[U][16];
 #pragma unroll
-    for (int i = 0; i < HD / 64; i++) {
-        const int it = tid + 256 * i, r = it / CH, c = it % CH;
-        if (r >= n || sTo[r >> 4] < 0) continue;
-        Chunk x = {};
-        if (sK[r]) x = *reinterpret_cast<const Chunk*>(sK[r] + c * CHB);
-        *reinterpret_cast<Chunk*>(a.k + to_of(r) + ((first + r) & mask) * ROWB + c * CHB) = x;
+    for (int i = 0; i < U; i++) {  // all loads in flight together: what is not there is read from the pool's start
+        const int it = tid + 256 * i, d = it % HD, r0 = 16 * (it / HD);
+        const uint8_t* from = sK[it / CH];
+        k[i] = *reinterpret_cast<const Chunk*>(from ? from + it % CH * CHB : a.k);
+#pragma unroll
+        for (int r = 0; r < 16; r++) from = sV[r0 + r], v[i][r] = from ? from[d * CHB] : *a.v;
     }
 #pragma unroll
-    for (int i = 0; i < HD / 64; i++) {
+    for (int i = 0; i < U; i++) {
+        const int it = tid + 256 * i, r = it / CH, c = it % CH;
+        if (r < n && sTo[r >> 4] >= 0)
+            *reinterpret_cast<Chunk*>(a.k + to_of(r) + ((first + r) & mask) * ROWB + c * CHB) = sK[r] ? k[i] : Chunk{};
+    }
+#pragma unroll
+    for (int i = 0; i < U; i++) {
         const int it = tid + 256 * i, d = it % HD, r0 = 16 * (it / HD), left = n - r0;
         if (left <= 0 || sTo[r0 >> 4] < 0) continue;
-        uint32_t v[16];
 #pragma unroll
-        for (int r = 0; r < 16; r++) v[r] = sV[r0 + r] ? sV[r0 + r][d * CHB] : 0;
+        for (int r = 0; r < 16; r++) v[i][r] = sV[r0 + r] ? v[i][r] : 0;
         uint8_t* const out = a.v + to_of(r0) + (size_t)(((first + r0) & mask) >> 4) * 16 * ROWB + d * CHB;
         if constexpr (BITS == 8) {
             v4i x = {0, 0, 0, 0};
 #pragma unroll
-            for (int r = 0; r < 16; r++) x[r >> 2] |= (int)(v[r] << (8 * (r & 3)));
+            for (int r = 0; r < 16; r++) x[r >> 2] |= (int)(v[i][r] << (8 * (r & 3)));
             if (left >= 16) {
                 *reinterpret_cast<v4i*>(out) = x;
             } else {
@@ -412,7 +420,7 @@ __global__ __launch_bounds__(256) void pg_move_kernel(Paged a, PgEvict p, int nb
 #pragma unroll
             for (int r = 0; r < 16; r++) {
                 const int sh = 8 * (r & 3) + 4 * ((r >> 2) & 1);
-                x[r >> 3] |= ((v[r] >> sOdd[r0 + r]) & 15) << sh;
+                x[r >> 3] |= ((v[i][r] >> sOdd[r0 + r]) & 15) << sh;
                 if (r >= left) keep[r >> 3] |= 15u << sh;
             }
             uint32_t* const to = reinterpret_cast<uint32_t*>(out);
