@@ -1,7 +1,9 @@
 // Eviction from paged KV caches by accumulated attention weight on gfx950 (kt_hip_dec_evict_paged, stated in include/kt_hip.h): for
 // each sequence and kv head the heaviest positions are chosen, then their k, v, multipliers and sums go to other pages. 64 sequences of about
 // 2200 cut to 1024 (2 kv heads of 64): 10.1 us to choose, a chain of two passes over the sums (in registers), a histogram and a ranking with
-// a CTA to two CUs; 14.0 us to move 34 MB, waves waiting 0.87 of their time. One of 131000 to 16384 in 4 bits: 24 us to choose, 5.4 to move.
+// a CTA to two CUs; 13.1 us to move 34 MB, waves waiting for most of it; 64 of 8000 cut to 4096 48.7 us for 142 MB, with the rest of the
+// lines that kept bytes lie in some 210 at 4.3 TB/s (128 or 256 slots a CTA: no change; V's chunks of 16 positions read whole, once for
+// neighbouring slots: 54.8, in 4 bits 38.5 against 42.9). One of 131000 to 16384 in 4 bits: 24 us to choose, 5.5 to move.
 
 #include <algorithm>
 #include <hip/hip_runtime.h>
