@@ -148,7 +148,8 @@ constexpr int LP_BLOCKS = 1024;  // of a row at most
 
 // A CTA a row: the blocks joined, then the alternatives. The k best blocks (of equal maxima the first) stay in registers, 8 fours of
 // logits a thread at most; the least of their maxima is a lower bound of the k-th largest logit that hardly any other logit reaches, so
-// those at or above it are collected and ranked against each other. A row of fewer than k blocks takes a bound from its lanes' maxima.
+// those at or above it are collected and ranked against each other. A row of fewer than k blocks takes the k-th of its 64 lanes' maxima: of
+// G lanes, all waves' logits dealt to them, some G ln(G / (G - k)) logits reach it, 24 for 20 alternatives.
 // BEST: how many of the best blocks there is room for.
 template <int NT, bool TOP, int BEST>
 __global__ __launch_bounds__(NT) void lp_join_kernel(LpRows p) {
@@ -183,12 +184,13 @@ __global__ __launch_bounds__(NT) void lp_join_kernel(LpRows p) {
     M = wave_max_i32(M);
     if (lane == 0) sMax[w] = M;
     __shared__ uint64_t sBm[TOP ? LP_BLOCKS : 1];
-    __shared__ int sBlk[KT_LOGPROBS_MAX_K], sBound, sCount;
+    __shared__ int sBlk[KT_LOGPROBS_MAX_K], sRank[64], sBound, sCount;
     if constexpr (TOP) {
 #pragma unroll
         for (int i = 0; i < PT; i++)
             if (tid + i * NT < p.nb) sBm[tid + i * NT] = key(bm[i], (uint32_t)(tid + i * NT));
         if (tid == 0) sCount = 0;
+        if (tid < 64) sRank[tid] = 0;
     }
     __syncthreads();
 #pragma unroll
@@ -232,7 +234,7 @@ __global__ __launch_bounds__(NT) void lp_join_kernel(LpRows p) {
     auto lp_of = [&](int v) { return -nats(lp_bits((uint32_t)M - (uint32_t)v, p.mant, p.shift, INT_MAX)); };
     if constexpr (TOP) {
         __shared__ uint64_t sKey[LP_CANDS];
-        __shared__ int sOut[NW];
+        __shared__ int sOut[NW], sLane[NT];
         constexpr int U = BEST * (LP_BLOCK / 4) / NT;
         i32x4 v[U];
         int at[U];  // the first of four logits; n where there are none
@@ -270,19 +272,22 @@ __global__ __launch_bounds__(NT) void lp_join_kernel(LpRows p) {
             return c;
         };
         int T = sBound;
-        if (p.nb < p.k) {  // of each wave's lanes' maxima the k-th
+        if (p.nb < p.k) {  // the k-th of the lanes' maxima over all waves
             int big = INT_MIN, rank = 0;
             each([&](int v, int) { big = max(big, v); });
-            for (int j = 0; j < 64; j++) {
-                const int o = __builtin_amdgcn_readlane(big, j);
+            sLane[tid] = big;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < NW; i++) big = max(big, sLane[64 * i + lane]);
+#pragma unroll
+            for (int i = 0; i < 64 / NW; i++) {  // each wave counts against its share of the lanes
+                const int j = 64 / NW * __builtin_amdgcn_readfirstlane(w) + i, o = __builtin_amdgcn_readlane(big, j);
                 rank += (o > big) | ((o == big) & (j < lane));
             }
-            const int kth = __builtin_amdgcn_readlane(big, __ffsll((unsigned long long)__ballot(rank == p.k - 1)) - 1);
-            if (lane == 0) sOut[w] = kth;
+            atomicAdd(&sRank[lane], rank);
             __syncthreads();
-            T = INT_MIN;
-#pragma unroll
-            for (int i = 0; i < NW; i++) T = max(T, sOut[i]);
+            rank = sRank[lane];
+            T = __builtin_amdgcn_readlane(big, __ffsll((unsigned long long)__ballot(rank == p.k - 1)) - 1);
         }
 #pragma unroll
         for (int u = 0; u < U; u++) {
