@@ -404,8 +404,8 @@ hipError_t launch_logprobs(const int32_t* logits, int rows, int n, int64_t strid
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     // Where eight blocks hold the alternatives 256 threads will do, in more CTAs at a time: us of the join with 256 / 1024 threads, 700 rows of
-    // 300 logits 11.5 / 29.9, of 5000 14.7 / 36.4, of 151936 14.2 / 25; 300 of 50000 8.1 / 13.4; 128 of 30000 7.5 / 8.0; but few rows of many
-    // blocks rank them faster with more: 64 of 151936 10.2 / 8.0, one 7.9 / 7.0.
+    // 300 logits 9.8 / 22, of 5000 11.7 / 23.4, of 151936 13.5 / 22.2; 300 of 50000 8.3 / 13.4; 128 of 30000 7.5 / 8.0; but few rows of many blocks
+    // rank them faster with more: 64 of 151936 10.8 / 7.9, one 8.0 / 7.0.
     const bool small = std::min(k, nb) <= 8 && (rows > 256 || nb <= 32);
     if (k == 0) lp_join_kernel<256, false, 0><<<dim3((unsigned)rows), dim3(256), 0, s>>>(p);
     else if (small) lp_join_kernel<256, true, 8><<<dim3((unsigned)rows), dim3(256), 0, s>>>(p);
