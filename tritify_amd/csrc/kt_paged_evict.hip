@@ -1,9 +1,8 @@
 // Eviction from paged KV caches by accumulated attention weight on gfx950 (kt_hip_dec_evict_paged, stated in include/kt_hip.h): for
 // each sequence and kv head the heaviest positions are chosen, then their k, v, multipliers and sums go to other pages. 64 sequences of about
 // 2200 cut to 1024 (2 kv heads of 64): 10.1 us to choose, a chain of two passes over the sums (in registers), a histogram and a ranking with
-// a CTA to two CUs; 13.1 us to move 34 MB, waves waiting for most of it; 64 of 8000 cut to 4096 48.7 us for 142 MB, with the rest of the
-// lines that kept bytes lie in some 210 at 4.3 TB/s (128 or 256 slots a CTA: no change; V's chunks of 16 positions read whole, once for
-// neighbouring slots: 54.8, in 4 bits 38.5 against 42.9). One of 131000 to 16384 in 4 bits: 24 us to choose, 5.5 to move.
+// a CTA to two CUs; 9.7 us to move 34 MB; 64 of 8000 cut to 4096 41.8 us for 142 MB, with the rest of the lines that kept bytes lie in some
+// 210 at 5 TB/s (128 or 256 slots a CTA: no change). One of 131000 to 16384 in 4 bits: 24 us to choose, 5.6 to move.
 
 #include <algorithm>
 #include <hip/hip_runtime.h>
@@ -347,17 +346,23 @@ __global__ __launch_bounds__(EV_NT) void pg_select_kernel(Paged a, PgEvict p, Ev
     }
 }
 
-constexpr int EV_MOVE = 64;  // slots of a CTA
+constexpr int EV_MOVE = 64;   // slots of a CTA
+constexpr int EV_CHUNKS = 4;  // chunks' rows of V that a wave holds in LDS
 
-// A CTA 64 slots of a sequence's and kv head's new pages: where each comes from, then all at once K's chunks, a thread each, and V's, whose
-// 16 positions of a dimension come from as many chunks (their bytes, or halves of them, one by one: neighbours lie in the same few lines).
+// A CTA 64 slots of a sequence's and kv head's new pages: where each comes from, then K's chunks, a thread each, and V's, by a wave the 16
+// slots of 64 dimensions. What these come from are chunks of 16 positions: of a few, where most positions stay, the rows go to LDS whole
+// and a lane picks its dimension's bytes (or halves of them) there; of more, each slot's bytes are loaded, neighbours in the same lines. us
+// with up to 4 chunks in LDS / bytes alone (up to 6: within a tenth, or more): 64 sequences of 8000 to their last 4096 34.6 / 48.8, to the
+// heaviest 4096 41.8 / 48.7 (4 bits 35.6 / 43.7), to 2000 30.1 / 30.4, to 1000 19.1 / 18.8; of 2200 to 1024 9.8 / 13.6.
 template <int HD, int BITS>
 __global__ __launch_bounds__(256) void pg_move_kernel(Paged a, PgEvict p, int nblk) {
-    constexpr int HH = HD / 2, CH = HD / 16, ROWB = BITS == 8 ? HD : HH, CHB = BITS == 8 ? 16 : 8;
+    constexpr int HH = HD / 2, CH = HD / 16, ROWB = BITS == 8 ? HD : HH, CHB = BITS == 8 ? 16 : 8, U = HD / 64;
     typedef typename std::conditional<BITS == 8, v4i, v2i>::type Chunk;
-    __shared__ const uint8_t *sK[EV_MOVE], *sV[EV_MOVE];  // the slot's row in K, its first byte in V; null without a page
-    __shared__ int sOdd[EV_MOVE], sTo[EV_MOVE / 16];
+    __shared__ const uint8_t *sK[EV_MOVE], *sV[EV_MOVE];  // the slot's row in K, its chunks' row in V; null without a page
+    __shared__ int sE[EV_MOVE], sTo[EV_MOVE / 16];        // its byte of a chunk, with 4 bits and 4 more where it is the high half
+    __shared__ __attribute__((aligned(16))) int8_t sChunk[4][EV_CHUNKS * 64 * CHB];
     const int b = (int)blockIdx.x / nblk, first = ((int)blockIdx.x - b * nblk) * EV_MOVE, g = blockIdx.y, tid = threadIdx.x;
+    const int lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int L = max(0, min(pg_len(a, b), a.max_pages << a.page_sh)), n = min(EV_MOVE, min(L, p.budget) - first);
     if (n <= 0 || a.pages == 0) return;
     const int mask = (1 << a.page_sh) - 1;
@@ -370,8 +375,8 @@ __global__ __launch_bounds__(256) void pg_move_kernel(Paged a, PgEvict p, int nb
         const size_t part = ((size_t)max(from, 0) * a.nkv + g) * (size_t)a.part;
         sK[tid] = from < 0 ? nullptr : a.k + part + sl * ROWB;
         const int e = sl & 15;
-        sV[tid] = from < 0 ? nullptr : a.v + part + (size_t)(sl >> 4) * 16 * ROWB + (BITS == 8 ? e : 4 * (e >> 3) + (e & 3));
-        sOdd[tid] = BITS == 8 ? 0 : 4 * ((e >> 2) & 1);
+        sV[tid] = from < 0 ? nullptr : a.v + part + (size_t)(sl >> 4) * 16 * ROWB;
+        sE[tid] = BITS == 8 ? e : (4 * (e >> 3) + (e & 3)) | ((e & 4) << 4);
         if ((tid & 15) == 0) sTo[tid >> 4] = there ? id : -1;
         if (there) {
             p.w[(((size_t)id * a.nkv + g) << a.page_sh) + to_sl] = from < 0 ? 0 : p.w[(((size_t)from * a.nkv + g) << a.page_sh) + sl];
@@ -384,34 +389,60 @@ __global__ __launch_bounds__(256) void pg_move_kernel(Paged a, PgEvict p, int nb
     }
     __syncthreads();
     auto to_of = [&](int r) { return ((size_t)sTo[r >> 4] * a.nkv + g) * (size_t)a.part; };
-    constexpr int U = HD / 64;
     Chunk k[U];
-    uint32_t v[U][16];
 #pragma unroll
-    for (int i = 0; i < U; i++) {  // all loads in flight together: what is not there is read from the pool's start
-        const int it = tid + 256 * i, d = it % HD, r0 = 16 * (it / HD);
-        const uint8_t* from = sK[it / CH];
+    for (int i = 0; i < U; i++) {  // (what is not there is read from the pool's start)
+        const int it = tid + 256 * i;
+        const uint8_t* const from = sK[it / CH];
         k[i] = *reinterpret_cast<const Chunk*>(from ? from + it % CH * CHB : a.k);
-#pragma unroll
-        for (int r = 0; r < 16; r++) from = sV[r0 + r], v[i][r] = from ? from[d * CHB] : *a.v;
     }
-#pragma unroll
+    int8_t* const lds = sChunk[w];
+#pragma unroll 1
     for (int i = 0; i < U; i++) {
-        const int it = tid + 256 * i, r = it / CH, c = it % CH;
-        if (r < n && sTo[r >> 4] >= 0)
-            *reinterpret_cast<Chunk*>(a.k + to_of(r) + ((first + r) & mask) * ROWB + c * CHB) = sK[r] ? k[i] : Chunk{};
-    }
+        const int r0 = 16 * ((w + 4 * i) / U), d0 = 64 * ((w + 4 * i) % U), left = n - r0;
+        // the 16 slots' chunks and bytes, a lane each; the slots whose chunk is not that of the slot before
+        const uint64_t from = (uint64_t)sV[r0 + (lane & 15)], before = __shfl_up(from, 1);
+        const int e = sE[r0 + (lane & 15)];
+        const uint32_t news = ((uint32_t)__ballot(from != before) & 0xFFFF) | 1, there = (uint32_t)__ballot(from != 0) & 0xFFFF;
+        auto base = [&](int r) {
+            return reinterpret_cast<const uint8_t*>((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)from, r) |
+                                                    (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(from >> 32), r) << 32);
+        };
+        uint32_t v[16];
+        if (__builtin_popcount(news) <= EV_CHUNKS) {
+            uint32_t more = news;
 #pragma unroll
-    for (int i = 0; i < U; i++) {
-        const int it = tid + 256 * i, d = it % HD, r0 = 16 * (it / HD), left = n - r0;
+            for (int c = 0; c < EV_CHUNKS; c++) {
+                if (more == 0) break;
+                const int r = __builtin_ctz(more);
+                more &= more - 1;
+                if (((there >> r) & 1) && (BITS == 8 || lane < 32)) dma16(make_rsrc(base(r) + d0 * CHB, 64 * CHB), lds + c * 64 * CHB, 16 * lane, 0);
+            }
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+            for (int r = 0; r < 16; r++)
+                v[r] = (uint8_t)lds[(__builtin_popcount(news & ((2u << r) - 1)) - 1) * 64 * CHB + (__builtin_amdgcn_readlane(e, r) & 15) + CHB * lane];
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // before a wave's next chunks take their place
+        } else {
+#pragma unroll
+            for (int r = 0; r < 16; r++) v[r] = ((there >> r) & 1 ? base(r) : a.v)[(d0 + lane) * CHB + (__builtin_amdgcn_readlane(e, r) & 15)];
+        }
+#pragma unroll
+        for (int r = 0; r < 16; r++) v[r] = (there >> r) & 1 ? v[r] : 0;
+        if (i == 0) {
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int it = tid + 256 * u, r = it / CH, c = it % CH;
+                if (r < n && sTo[r >> 4] >= 0)
+                    *reinterpret_cast<Chunk*>(a.k + to_of(r) + ((first + r) & mask) * ROWB + c * CHB) = sK[r] ? k[u] : Chunk{};
+            }
+        }
         if (left <= 0 || sTo[r0 >> 4] < 0) continue;
-#pragma unroll
-        for (int r = 0; r < 16; r++) v[i][r] = sV[r0 + r] ? v[i][r] : 0;
-        uint8_t* const out = a.v + to_of(r0) + (size_t)(((first + r0) & mask) >> 4) * 16 * ROWB + d * CHB;
+        uint8_t* const out = a.v + to_of(r0) + (size_t)(((first + r0) & mask) >> 4) * 16 * ROWB + (d0 + lane) * CHB;
         if constexpr (BITS == 8) {
             v4i x = {0, 0, 0, 0};
 #pragma unroll
-            for (int r = 0; r < 16; r++) x[r >> 2] |= (int)(v[i][r] << (8 * (r & 3)));
+            for (int r = 0; r < 16; r++) x[r >> 2] |= (int)(v[r] << (8 * (r & 3)));
             if (left >= 16) {
                 *reinterpret_cast<v4i*>(out) = x;
             } else {
@@ -422,7 +453,7 @@ __global__ __launch_bounds__(256) void pg_move_kernel(Paged a, PgEvict p, int nb
 #pragma unroll
             for (int r = 0; r < 16; r++) {
                 const int sh = 8 * (r & 3) + 4 * ((r >> 2) & 1);
-                x[r >> 3] |= ((v[i][r] >> sOdd[r0 + r]) & 15) << sh;
+                x[r >> 3] |= ((v[r] >> (__builtin_amdgcn_readlane(e, r) >> 4)) & 15) << sh;
                 if (r >= left) keep[r >> 3] |= 15u << sh;
             }
             uint32_t* const to = reinterpret_cast<uint32_t*>(out);
