@@ -1,8 +1,8 @@
 // Eviction from paged KV caches by accumulated attention weight on gfx950 (kt_hip_dec_evict_paged, stated in include/kt_hip.h): for
 // each sequence and kv head the heaviest positions are chosen, then their k, v, multipliers and sums go to other pages. 64 sequences of about
-// 2200 cut to 1024 (2 kv heads of 64): 10.1 us to choose, a chain of two passes over the sums (in registers), a histogram and a ranking with
+// 2200 cut to 1024 (2 kv heads of 64): 10 to 11 us to choose, a chain of two passes over the sums (in registers), a histogram and a ranking with
 // a CTA to two CUs; 9.7 us to move 34 MB; 64 of 8000 cut to 4096 41.8 us for 142 MB, with the rest of the lines that kept bytes lie in some
-// 210 at 5 TB/s (128 or 256 slots a CTA: no change). One of 131000 to 16384 in 4 bits: 24 us to choose, 5.6 to move.
+// 210 at 5 TB/s (128 or 256 slots a CTA: no change). One of 131000 to 16384 in 4 bits: 21 us to choose, 5.6 to move.
 
 #include <algorithm>
 #include <hip/hip_runtime.h>
@@ -25,16 +25,17 @@ struct PgEvict {
 };
 
 constexpr int EV_NT = 1024, EV_WAVES = EV_NT / 64;
-constexpr int EV_BINS = 2048;   // of sums
+constexpr int EV_BINS = 4096;   // of sums
 constexpr int EV_CANDS = 1024;  // positions of one bin that are ranked against each other
 constexpr int EV_U = 8;         // words of a wave in flight: 64 positions each
 
-// The bin of a sum: the values below 64 one each, from there on 32 to a power of two; bin 0 for negative ones, which only a caller's own
-// sums hold, and for positions without a page.
+// The bin of a sum: the values below 128 one each, from there on 64 to a power of two; bin 0 for negative ones, which only a caller's own
+// sums hold, and for positions without a page. (With 32 to a power of two a bin of 131000 positions has twice the members to rank: to 16384
+// 16.9 us for the last two steps against 13.9; of 64 x 2200, in one CTA each, no change.)
 __device__ __forceinline__ int weight_bin(int64_t w, bool page) {
     const uint64_t m = (uint64_t)w;
-    const int sh = max(0, 58 - __clzll((long long)(m | 1)));
-    return page && w >= 0 ? 1 + 32 * sh + (int)(m >> sh) : 0;
+    const int sh = max(0, 57 - __clzll((long long)(m | 1)));
+    return page && w >= 0 ? 1 + 64 * sh + (int)(m >> sh) : 0;
 }
 // The order of sums as unsigned numbers, 0 for a position without a page.
 __device__ __forceinline__ uint64_t weight_key(int64_t w, bool page) {
@@ -470,7 +471,7 @@ EvSpace ev_space(int64_t max_pos) {
 
 // One CTA a sequence and kv head takes one launch, and a long one's sums alone: us for one sequence of 4000 positions (2 kv heads) 8.4, of 8000
 // 11.3, 16000 19.2, 24000 25, 32000 31, 131000 114, for 64 of 4000 9.2, of 16000 21.1. Several take four launches (and of the caller 10 us
-// more): one of 25000 17.9, 32000 17.8, 131000 18.2, 64 of 32000 36.6.
+// more): one of 25000 17.9, 32000 17.8, 131000 18.2 (19.0 with the bins as they are now), 64 of 32000 36.6 (39.2).
 bool ev_shared(int64_t max_pos) { return max_pos > 16384; }
 
 }  // namespace
