@@ -428,6 +428,20 @@ def test_evict_pages_left_out(torch_dev, bits):
     check_evict(torch_dev, c, 48, 0, 0, w, to)
 
 
+@pytest.mark.parametrize("L,many", [(300, True), (5000, True), (20000, True), (5000, False), (20000, False)])
+def test_evict_the_least_sums(torch_dev, L, many):
+    """The least of 64 bits is below the next one, whichever has the lower position, and above a position without a page: with cuts among
+    the negative sums and, where most are negative, among the positions without a page (more than a bin's candidates, or fewer)."""
+    c = spare_case(12, [L, L - 7], 2, 64, 16, 8, L - L // 5 if many else L - 100)
+    gone = L // 50 if many else 1
+    for b in range(2):
+        c.table[b, c.g.permutation(L // 16)[:gone]] = -1
+    least = -(2 ** 63) + c.g.integers(0, 3, size=(c.pages, 2, 16))
+    w = least if many else np.where(c.g.random(least.shape) < 300 / L, least, c.g.integers(0, 1 << 45, size=least.shape))
+    for budget in (L // 2, L - L // 5) if many else (L - 100,):
+        check_evict(torch_dev, c, budget, 10, 4, w)
+
+
 # -- log probabilities -----------------------------------------------------------------------------------------------
 
 

@@ -29,19 +29,16 @@ constexpr int EV_BINS = 4096;   // of sums
 constexpr int EV_CANDS = 1024;  // positions of one bin that are ranked against each other
 constexpr int EV_U = 8;         // words of a wave in flight: 64 positions each
 
-// The bin of a sum: the values below 128 one each, from there on 64 to a power of two; bin 0 for negative ones, which only a caller's own
-// sums hold, and for positions without a page. (With 32 to a power of two a bin of 131000 positions has twice the members to rank: to 16384
-// 16.9 us for the last two steps against 13.9; of 64 x 2200, in one CTA each, no change.)
+// The bin of a sum: the values below 128 one each, from there on 64 to a power of two; bin 1 for negative ones, which only a caller's own
+// sums hold, and bin 0 for positions without a page, below them all. (With 32 to a power of two a bin of 131000 positions has twice the
+// members to rank: to 16384 16.9 us for the last two steps against 13.9; of 64 x 2200, in one CTA each, no change.)
 __device__ __forceinline__ int weight_bin(int64_t w, bool page) {
     const uint64_t m = (uint64_t)w;
     const int sh = max(0, 57 - __clzll((long long)(m | 1)));
-    return page && w >= 0 ? 1 + 64 * sh + (int)(m >> sh) : 0;
+    return page ? (w >= 0 ? 2 + 64 * sh + (int)(m >> sh) : 1) : 0;
 }
-// The order of sums as unsigned numbers, 0 for a position without a page.
-__device__ __forceinline__ uint64_t weight_key(int64_t w, bool page) {
-    const uint64_t k = (uint64_t)w ^ (1ull << 63);
-    return page ? (k ? k : 1) : 0;
-}
+// The order of a bin's sums as unsigned numbers (those of positions without a page, which are read as 0, are equal).
+__device__ __forceinline__ uint64_t weight_key(int64_t w) { return (uint64_t)w ^ (1ull << 63); }
 
 // What several CTAs of a sequence and kv head share where its positions are too many for one: in the workspace, for each.
 struct EvShared {
@@ -179,7 +176,7 @@ __global__ __launch_bounds__(EV_NT) void pg_select_part_kernel(Paged a, PgEvict 
             if (lane == 0) sh.bits[word] = stay;
             if (bin == e.bin && e.need < e.members && e.members <= EV_CANDS) {
                 const int c = atomicAdd(&sh.hist[EV_BINS], 1);
-                if (c < EV_CANDS) sh.key[c] = weight_key(x, page), sh.at[c] = j;  // (more only if the sums change under the call)
+                if (c < EV_CANDS) sh.key[c] = weight_key(x), sh.at[c] = j;  // (more only if the sums change under the call)
             }
         });
     }
@@ -231,7 +228,7 @@ __global__ __launch_bounds__(EV_NT) void pg_select_kernel(Paged a, PgEvict p, Ev
             if (lane == 0) sBits[word] = stay;
             if (bin == e.bin && e.need < e.members && e.members <= EV_CANDS) {
                 const int c = atomicAdd(&sCount, 1);
-                if (c < EV_CANDS) sKey[c] = weight_key(x, page), sAt[c] = j;  // (more only if the sums change under the call)
+                if (c < EV_CANDS) sKey[c] = weight_key(x), sAt[c] = j;  // (more only if the sums change under the call)
             }
         };
         if (seg > EV_U) s.all(w0, w1, mark);
@@ -256,7 +253,7 @@ __global__ __launch_bounds__(EV_NT) void pg_select_kernel(Paged a, PgEvict p, Ev
         // members differ in; then those above it and the first of those equal to it.
         uint64_t both = ~0ull, any = 0;
         auto members_of = [&](auto f) {
-            s.all(w0, w1, [&](int word, int j, int64_t x, bool page) { f(word, j >= 0 && weight_bin(x, page) == e.bin, weight_key(x, page)); });
+            s.all(w0, w1, [&](int word, int j, int64_t x, bool page) { f(word, j >= 0 && weight_bin(x, page) == e.bin, weight_key(x)); });
         };
         members_of([&](int, bool in, uint64_t k) {
             if (in) both &= k, any |= k;
