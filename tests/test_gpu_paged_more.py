@@ -442,6 +442,19 @@ def test_evict_the_least_sums(torch_dev, L, many):
         check_evict(torch_dev, c, budget, 10, 4, w)
 
 
+@pytest.mark.parametrize("width", [4, 2048])
+def test_evict_of_no_sequences(torch_dev, width):
+    from tritify_amd.paged import PagedBatch, PagedKV
+
+    torch = torch_dev
+    z = lambda *s: torch.zeros(s, dtype=torch.int32, device="cuda")  # noqa: E731
+    kv, b = PagedKV(5, 16, 2, 64, weights=True), PagedBatch(z(1), z(0), z(0, width), 0)
+    assert kv.evict_workspace_bytes(b) > 0
+    kv.evict(b, z(0, 3), 40, z(0, 2, 40), recent=3)
+    torch.cuda.synchronize()
+    assert not kv.k.any() and not kv.v.any() and not kv.w.any()
+
+
 # -- log probabilities -----------------------------------------------------------------------------------------------
 
 

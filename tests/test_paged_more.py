@@ -364,3 +364,12 @@ def test_empty_calls_do_nothing():
 
     with pytest.raises(ValueError):
         B.dec_logprobs_rows_workspace(1, 5, 40)
+
+
+@pytest.mark.parametrize("page", [16, 256])
+def test_no_sequences_over_a_wide_table(page):
+    """A shape that the eviction takes has scratch of some bytes, whatever the table's width."""
+    L, wide = _lib(), 524288 // page
+    n = L.kt_hip_dec_evict_paged_workspace(0, wide, page, 2)
+    assert 0 < n <= L.kt_hip_dec_evict_paged_workspace(1, wide, page, 2)
+    assert L.kt_hip_dec_evict_paged(*{**EVICT, "seqs": 0, "max_pages": wide, "page": page, "ws_bytes": n}.values()) == 0

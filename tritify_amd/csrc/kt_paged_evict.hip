@@ -474,7 +474,7 @@ bool ev_shared(int64_t max_pos) { return max_pos > 16384; }
 }  // namespace
 
 size_t pg_evict_workspace(int64_t seqs, int64_t nkv, int64_t max_pos) {
-    return ev_shared(max_pos) ? (size_t)seqs * nkv * ev_space(max_pos).stride : 256;
+    return ev_shared(max_pos) ? std::max<size_t>(256, (size_t)seqs * nkv * ev_space(max_pos).stride) : 256;  // (0 says a shape refused)
 }
 
 hipError_t launch_pg_evict(const Paged& a, int hd, int bits, const int32_t* to, int budget, int recent, int sinks, int32_t* kept,
