@@ -373,3 +373,13 @@ def test_no_sequences_over_a_wide_table(page):
     n = L.kt_hip_dec_evict_paged_workspace(0, wide, page, 2)
     assert 0 < n <= L.kt_hip_dec_evict_paged_workspace(1, wide, page, 2)
     assert L.kt_hip_dec_evict_paged(*{**EVICT, "seqs": 0, "max_pages": wide, "page": page, "ws_bytes": n}.values()) == 0
+
+
+@pytest.mark.parametrize("tokens", [0, 5])
+@pytest.mark.parametrize("page", [16, 256])
+def test_no_sequences_attend_over_a_wide_table(page, tokens):
+    L, wide = _lib(), 524288 // page
+    n = L.kt_hip_dec_attention_paged_workspace(tokens, 0, wide, page, 14, 2, 64)
+    assert n > 0
+    empty = {**STATS, "tokens": tokens, "seqs": 0, "max_pages": wide, "page": page, "ws_bytes": n}
+    assert L.kt_hip_dec_attention_paged_stats(*empty.values()) == 0

@@ -613,7 +613,7 @@ Parts parts(const Plan& x, int nkv, int hd) {
     if (x.splits == 1) return {0, 0, 256};
     const size_t units = (size_t)x.tiles * nkv;
     const size_t sum = (units * x.splits * PG_COLS * 4 + 255) / 256 * 256, cnt = sum + units * PG_COLS * (hd + 1) * 8;
-    return {sum, cnt, cnt + (units * 4 + 255) / 256 * 256};
+    return {sum, cnt, std::max<size_t>(256, cnt + (units * 4 + 255) / 256 * 256)};  // (0 says a shape refused)
 }
 
 template <int HD, int BITS, bool STATS>
