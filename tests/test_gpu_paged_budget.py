@@ -219,6 +219,54 @@ def test_captured_steps_under_a_budget(model):  # noqa: F811
         torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("bits", [8, 4])
+def test_captured_steps_by_the_documented_calls(model, bits):  # noqa: F811
+    """Scratch reserved, a step captured and replayed, nothing taken back by hand: tokens, caches and accumulated weights as by eager
+    passes, and after the cuts that follow the same positions are held."""
+    import torch
+    from tritify_amd.paged import PagedDecoder
+
+    p = prompts([90])[0]
+    made = [PagedDecoder(model, 30, bits=bits, budget=40, recent=10, sinks=2, most=50) for _ in range(2)]
+    (d, a), (e, _) = [(d, d.add()) for d in made]
+    toks = [d.run([(a, p)]) for d in made]
+    d._reserve([(a, 98)])
+    b = d.batch([a], [1])
+    x, out = toks[0].clone(), torch.empty_like(toks[0])
+    s, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        d.reserve_scratch(b)
+        held = len(d._ws)
+        torch.cuda.synchronize()
+        g.capture_begin()
+        d.forward(x, b, None, out, s)
+        g.capture_end()
+    torch.cuda.synchronize()
+    assert len(d._ws) == held
+    t = toks[1]
+    for step in range(8):
+        say(f"case: replay {step} bits={bits}")
+        g.replay()
+        torch.cuda.synchronize()
+        t = e.run([(a, t)])
+        torch.cuda.synchronize()
+        assert torch.equal(out, t)
+        for l in range(model.L):
+            assert torch.equal(d.kv[l].w, e.kv[l].w) and torch.equal(d.kv[l].k, e.kv[l].k) and torch.equal(d.kv[l].v, e.kv[l].v)
+        x.copy_(out)
+        b.kv_len.add_(1)
+        torch.cuda.synchronize()
+    d.seq[a]["len"] += 8  # the replays' tokens; two more passes cut both sequences
+    for _ in range(3):
+        x, t = d.run([(a, x)]), e.run([(a, t)])
+        assert torch.equal(x, t) and d.held(a) == e.held(a)
+    assert d.length(a) == e.length(a) == 101 and d.held(a) == 40
+    for l in range(model.L):
+        for u, v in zip(d.read(a, l), e.read(a, l)):
+            assert torch.equal(u, v)
+
+
 def test_a_batch_without_shifts_under_a_budget(model):  # noqa: F811
     import torch
     from tritify_amd.paged import PagedBatch, PagedDecoder

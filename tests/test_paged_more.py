@@ -286,6 +286,34 @@ def test_cuts_of_many_sequences_at_a_time_are_within_what_evict_takes():
     assert len(pages) == len(set(pages)) == 2 * n * own + need
 
 
+def test_scratch_is_reserved_without_a_pass():
+    """No operator runs, so no weight is added; what the pass then asks for is there, and smaller shapes take it too."""
+    import torch
+    from types import SimpleNamespace
+
+    from tritify_amd.paged import PagedDecoder
+
+    class Scratch:  # no other operator to call
+        def workspace_bytes(self, b, nh):
+            return b.tokens * 1000 + 7
+
+    d = PagedDecoder.__new__(PagedDecoder)
+    d.torch, d.dev, d.device, d.max_rows, d.max_seqs, d.m = torch, -1, "cpu", 4096, 64, SimpleNamespace(V=200000, nh=14)
+    d.kv, d._ws = [Scratch()], []
+    batch = lambda tokens, seqs: SimpleNamespace(dev=-1, tokens=tokens, seqs=seqs)  # noqa: E731
+    assert d.reserve_scratch(batch(2048, 64)) is None
+    held = d._ws[-1].data_ptr()
+    for tokens, seqs in ((2048, 64), (64, 64), (1, 1)):
+        d.reserve_scratch(batch(tokens, seqs))
+        ws, top = d._workspaces(batch(tokens, seqs))
+        assert ws.data_ptr() == held and ws.numel() >= tokens * 1000 + 7 and top.numel() > 0 and len(d._ws) == 1
+    d.reserve_scratch(batch(4096, 64))
+    assert len(d._ws) == 2 and d._ws[0].data_ptr() == held  # a captured pass may hold it
+    for bad in (batch(0, 1), batch(4097, 1), batch(1, 0), batch(65, 65), SimpleNamespace(dev=0, tokens=1, seqs=1)):
+        with pytest.raises(ValueError, match="reserve_scratch"):
+            d.reserve_scratch(bad)
+
+
 # -- refusals --------------------------------------------------------------------------------------------------------
 
 P = 1 << 20  # an aligned address that no call here dereferences

@@ -478,11 +478,20 @@ class PagedDecoder:
             self._ws.append(self.torch.empty(size, dtype=self.torch.int8, device=self.device))
         return self._ws[-1][:n], self._ws[-1][n:]
 
+    def reserve_scratch(self, b: PagedBatch) -> None:
+        """Scratch for `forward` of batches of b's shape (rows, sequences, table width), so that the pass can be captured. Nothing runs
+        and nothing of the decoder changes. On the stream of the passes, which torch's current one has to be, before the capture."""
+        self._check_batch(b, "reserve_scratch")
+        self._workspaces(b)
+
+    def _check_batch(self, b: PagedBatch, what: str) -> None:
+        if b.dev != self.dev or not 1 <= b.tokens <= self.max_rows or not 1 <= b.seqs <= self.max_seqs:
+            raise ValueError(f"{what}: a batch on GPU {self.dev} of 1 to {self.max_rows} rows and 1 to {self.max_seqs} sequences "
+                             f"is needed, not {b.tokens} rows of {b.seqs} on GPU {b.dev}")
+
     def _check_pass(self, tokens_dev, b: PagedBatch, last, out) -> None:
         """What a pass reads and writes lies within its tensors and the decoder's buffers."""
-        if b.dev != self.dev or not 1 <= b.tokens <= self.max_rows or not 1 <= b.seqs <= self.max_seqs:
-            raise ValueError(f"forward: a batch on GPU {self.dev} of 1 to {self.max_rows} rows and 1 to {self.max_seqs} sequences "
-                             f"is needed, not {b.tokens} rows of {b.seqs} on GPU {b.dev}")
+        self._check_batch(b, "forward")
         i32 = self.torch.int32
         for t, what, n in ((tokens_dev, "tokens", b.tokens), (out, "out", b.seqs)):
             if t.dtype is not i32 or t.get_device() != self.dev or t.numel() < n or not t.is_contiguous():
@@ -499,9 +508,10 @@ class PagedDecoder:
         """The layers over the batch's rows, whose ids (tokens_dev, int32) are within the vocabulary; the logits of each
         sequence's last row (`last`: their indexes among the rows, None where every sequence has one row) to self.logits, the
         greedy choice of each to out (int32). Asynchronous on `stream`, which torch's current stream has to be; capturable
-        after a call of the batch's shape. Passes of one decoder, captured or not, share its buffers: they follow one
-        another. Under a budget the batch has its sequences' shifts, as `batch` gives them; the weights that the rows attend with are
-        added up, but no sequence is cut."""
+        after reserve_scratch of the batch's shape. Passes of one decoder, captured or not, share its buffers: they follow one
+        another. Under a budget the batch has its sequences' shifts, as `batch` gives them, and no sequence is cut. Each pass then adds
+        the weights that its rows attend with to those held: the same rows passed twice (a trial before a capture, say) count
+        twice in the cuts that follow, where without a budget the second pass leaves everything as the first did."""
         self._check_pass(tokens_dev, b, last, out)
         vocab = self.m.V
         if self.budget and b.shift is None:
