@@ -286,6 +286,42 @@ def test_cuts_of_many_sequences_at_a_time_are_within_what_evict_takes():
     assert len(pages) == len(set(pages)) == 2 * n * own + need
 
 
+@pytest.mark.parametrize("fails", [0, 1, 2])
+def test_a_cut_that_fails_loses_no_pages(fails):
+    """Where a layer's eviction cannot run (no memory for its scratch, say), the sequences are as they were and the next pass cuts them."""
+    import torch
+
+    from tritify_amd.paged import PagedDecoder
+
+    state = dict(calls=0, broken=True, to=[])
+
+    class Evict:
+        def evict(self, b, to, budget, kept, recent, sinks, stream):
+            state["calls"] += 1
+            if state["broken"] and state["calls"] > fails:
+                raise RuntimeError("no memory")
+            state["to"].append(to.flatten().tolist())
+
+    class M:
+        nkv = 2
+
+    d = PagedDecoder.__new__(PagedDecoder)
+    d.torch, d.device, d.m, d.page, d.budget, d.recent, d.sinks, d.most = torch, "cpu", M, 16, 40, 8, 2, 50
+    d.kv, d.batch = [Evict()] * 3, lambda seqs, rows: seqs
+    d.seq = {s: dict(len=60 + s, cut=0, pages=list(range(4 * s, 4 * s + 4)), gone=0) for s in range(5)}
+    d.free, d.spare = list(range(40, 20, -1)), [20, 41, 42]
+    before = [dict(e, pages=list(e["pages"])) for e in d.seq.values()], list(d.free), list(d.spare)
+    with pytest.raises(RuntimeError, match="no memory"):
+        d._cut(list(d.seq), None)
+    assert (list(d.seq.values()), d.free, d.spare) == before
+    state.update(broken=False, to=[])
+    d._cut(list(d.seq), None)
+    assert all(d.held(s) == 40 and len(d.seq[s]["pages"]) == 3 for s in d.seq) and len(state["to"]) == 3
+    pages = d.free + d.spare + [p for e in d.seq.values() for p in e["pages"]]
+    assert sorted(pages) == list(range(43)) and len(d.spare) == 3
+    assert state["to"][0] == [20, 41, 42] + list(range(21, 33))  # the spare pages, then the free ones from the list's end
+
+
 def test_scratch_is_reserved_without_a_pass():
     """No operator runs, so no weight is added; what the pass then asks for is there, and smaller shapes take it too."""
     import torch

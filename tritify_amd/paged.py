@@ -375,12 +375,14 @@ class PagedDecoder:
         while seqs:
             n = min(len(seqs), 1 + len(self.free) // need, ((1 << 24) - 1) // -(-self.budget // 16))
             now, seqs = seqs[:n], seqs[n:]
-            pages = self.spare + [self.free.pop() for _ in range((n - 1) * need)]
+            more = (n - 1) * need  # from the list's end, and off it once all layers have been cut
+            pages = self.spare + self.free[-1:-1 - more:-1]
             to = torch.tensor(pages, dtype=torch.int32).reshape(n, need).to(self.device)
             b = self.batch(now, [0] * n)
             kept = torch.empty(n, self.m.nkv, self.budget, dtype=torch.int32, device=self.device)
             for kv in self.kv:
                 kv.evict(b, to, self.budget, kept, self.recent, self.sinks, stream)
+            del self.free[len(self.free) - more:]
             for i, s in enumerate(now):
                 e = self.seq[s]
                 self.free += e["pages"]
