@@ -3,6 +3,12 @@
 // 2200 cut to 1024 (2 kv heads of 64): 10 to 11 us to choose, a chain of two passes over the sums (in registers), a histogram and a ranking with
 // a CTA to two CUs; 9.7 us to move 34 MB; 64 of 8000 cut to 4096 41.8 us for 142 MB, with the rest of the lines that kept bytes lie in some
 // 210 at 5 TB/s (128 or 256 slots a CTA: no change). One of 131000 to 16384 in 4 bits: 21 us to choose, 5.6 to move.
+//
+// These are sums spread as attention leaves them. Many positions in the bin of the least sum that stays cost more: up to EV_CANDS of
+// them are ranked by as few lanes as there are left for each (64 x 2200 to 1024, seven in ten sums 0 and the cut among them: 63 us to choose
+// against 11), past that the sums are read again for each step (64 x 8000 to 4096 of the same kind 22.6 us against 13.1), and by each of
+// several CTAs (one of 131000 to 16384, 95 in 100 sums 0: 136 us in the last of the four launches against 7.9; all sums within one power
+// of two: 312).
 
 #include <algorithm>
 #include <hip/hip_runtime.h>
@@ -31,7 +37,8 @@ constexpr int EV_U = 8;         // words of a wave in flight: 64 positions each
 
 // The bin of a sum: the values below 128 one each, from there on 64 to a power of two; bin 1 for negative ones, which only a caller's own
 // sums hold, and bin 0 for positions without a page, below them all. (With 32 to a power of two a bin of 131000 positions has twice the
-// members to rank: to 16384 16.9 us for the last two steps against 13.9; of 64 x 2200, in one CTA each, no change.)
+// members to rank: to 16384 16.9 us for the last two steps against 13.9; of 64 x 2200, in one CTA each, no change. Where few members are to be
+// ranked the wider histogram only costs: the figures in brackets above ev_shared.)
 __device__ __forceinline__ int weight_bin(int64_t w, bool page) {
     const uint64_t m = (uint64_t)w;
     const int sh = max(0, 57 - __clzll((long long)(m | 1)));
@@ -468,7 +475,9 @@ EvSpace ev_space(int64_t max_pos) {
 
 // One CTA a sequence and kv head takes one launch, and a long one's sums alone: us for one sequence of 4000 positions (2 kv heads) 8.4, of 8000
 // 11.3, 16000 19.2, 24000 25, 32000 31, 131000 114, for 64 of 4000 9.2, of 16000 21.1. Several take four launches (and of the caller 10 us
-// more): one of 25000 17.9, 32000 17.8, 131000 18.2 (19.0 with the bins as they are now), 64 of 32000 36.6 (39.2).
+// more): one of 25000 17.9, 32000 17.8, 131000 18.2 (19.0 with the bins as they are now), 64 of 32000 36.6 (39.2). The rule goes by the
+// table's width, which is all that the host knows: 63 sequences of 1000 beside one of 17000 take the four launches too, 21 us against 7.9
+// for 64 of 1000.
 bool ev_shared(int64_t max_pos) { return max_pos > 16384; }
 
 }  // namespace

@@ -7,11 +7,13 @@
 // digits (of -e, two) are the A operand of a second product as they stand; its B operand is R's digits (five, each in a column of
 // the result, and one further for e's high digit). Sums of e R are so exact in int32 and meet as int64.
 //
-// What it takes: 128 single tokens behind about 6100 (14 heads over 2 of 64) 28.7 us, K at 3.5 TB/s (vector units 0.42 busy, LDS 0.28, waves
-// waiting for K 0.6 of their time), and 6.0 us for the zeros of a fresh start; one token behind 131000 in 4 bits 7.5 us, behind 640 4.8; 1024
-// rows behind 7777 (15 GOP) 42.5 us: the table's look-ups have LDS busy 0.62 of the time, over half of it with bank conflicts, vector
-// units 0.60, a third of that for what each CTA begins and ends with, MFMAs 0.22. (Eight and sixteen copies of the table side by side, fewer
-// conflicts: 49 to 51 us against 45.7, what the copies take to fill; 32, none, in a CTA of 16 waves a CU: 47 to 59 against 42.8.)
+// What it takes: 128 single tokens behind about 6100 (14 heads over 2 of 64) 28.7 us, K at 3.5 TB/s (vector units 0.42 busy, LDS 0.28,
+// waves waiting for K 0.6 of their time), behind 6.0 us for the zeros of a fresh start, and 26.2 where the sums go on, as a decoder's do;
+// 24.6 of that for equal lengths, as a sequence's tiles are dealt to a number of CTAs that the table's width gives and the longest decide;
+// one token behind 131000 in 4 bits 7.5 us, behind 640 4.8; 1024 rows behind 7777 (15 GOP) 42.5 us: the table's look-ups have LDS busy 0.62
+// of the time, over half of it with bank conflicts, vector units 0.60, a third of that for what each CTA begins and ends with, MFMAs 0.22.
+// (Eight and sixteen copies of the table side by side, fewer conflicts: 49 to 51 us against 45.7, what the copies take to fill; 32, none,
+// in a CTA of 16 waves a CU: 47 to 59 against 42.8.)
 
 #include <algorithm>
 #include <hip/hip_runtime.h>
@@ -69,7 +71,7 @@ __global__ __launch_bounds__(256) void pg_weigh_zero_kernel(Paged a, int64_t* __
 }
 
 // CT: 16 columns times CT a step. Waves a SIMD: with three instead of four the chunk of 1024 rows takes 45.5 us instead of 42.5, four spill some
-// registers outside the loop over columns; in 4 bits, whose multipliers need more, four take 83 us and three 55.
+// registers outside the loop over columns; in 4 bits, whose multipliers need more, four take 83 us and three 54.
 template <int HD, int BITS, int CT>
 __global__ __launch_bounds__(64 * WG_WAVES) __attribute__((amdgpu_waves_per_eu(HD == 64 ? (CT == 1 || BITS == 8 ? 4 : 3) : 2))) void
 pg_weigh_kernel(Paged a, PgWeigh p) {
@@ -350,7 +352,8 @@ hipError_t launch_pg_weigh(const Paged& a, int hd, int bits, const int8_t* q, in
     const int64_t units = units_of(unit), splits = std::min(rounds, std::max<int64_t>(1, 2048 / units));
     const bool few = (int64_t)a.tokens * rep <= 24 * (int64_t)a.seqs;  // columns of a sequence, on average
     // 16 or 64 columns a step, us with 16 / 64 (7 heads a kv head): 64 sequences of 2 rows 6.3 / 8.5, of 3 7.9 / 8.6, of 5 9.4 /
-    // 8.6; 64 of one row behind 4000 12.0 / 16.3, in heads of 128 17.1 / 26.1; one of 40 rows behind 2000 21.0 / 14.3.
+    // 8.6; 64 of one row behind 4000 12.0 / 16.3, in heads of 128 17.1 / 26.1; one of 40 rows behind 2000 21.0 / 14.3. The average hides one
+    // chunk beside many tokens: 64 single tokens and 150 rows take 16 columns, behind 1000 10.5 / 9.7, behind 4000 41.6 / 30.4.
     const PgWeigh p = {q, q_stride, exp_tab, stats, nh, rep, unit, window, sinks, (int)splits, w};
     auto go = [&](auto one, auto four) {
         if (few) one<<<dim3((unsigned)units, (unsigned)splits), dim3(64 * WG_WAVES), 0, s>>>(a, p);
