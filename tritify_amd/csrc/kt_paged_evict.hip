@@ -5,7 +5,7 @@
 // 210 at 5 TB/s (128 or 256 slots a CTA: no change). One of 131000 to 16384 in 4 bits: 21 us to choose, 5.6 to move.
 //
 // These are sums spread as attention leaves them. Many positions in the bin of the least sum that stays cost more: up to EV_CANDS of
-// them are ranked by as few lanes as there are left for each (64 x 2200 to 1024, seven in ten sums 0 and the cut among them: 63 us to choose
+// them are compared with each other, by one lane each where they are over 512 (64 x 2200 to 1024, seven in ten sums 0 and the cut among them: 63 us to choose
 // against 11), past that the sums are read again for each step (64 x 8000 to 4096 of the same kind 22.6 us against 13.1), and by each of
 // several CTAs (one of 131000 to 16384, 95 in 100 sums 0: 136 us in the last of the four launches against 7.9; all sums within one power
 // of two: 312).
